@@ -100,8 +100,8 @@ typedef struct lact_scan_io {
  * ends with shadow_dump.  A caller compiled against 1000 that uses one of these must be compiled again.  1002: new entries
  * lact_swiglu_ffn_hidden_bytes, lact_swa_fwd_cache_bytes and lact_swa_fwd_cache; larger workspaces (asked for as before):
  * programs of many short steps by up to 128 MB for weights and 58 MB for hidden activations, fp32 programs by their
- * operands in bf16 pieces (6 bytes a value: an update and apply of D = H take 30 H bytes per token, 12 H before).  No
- * counterpart in the reference. */
+ * operands in bf16 pieces (6 bytes a value: an update and apply of D = H take 30 H bytes per token, 12 H before).  1003: new
+ * entries lact_linear_attention_* and lact_group_norm_*.  No counterpart in the reference. */
 int lact_version(void);
 
 /* Human-readable text for a return code.  No counterpart in the reference. */
@@ -334,6 +334,37 @@ int lact_swa_bwd(const void *q, const void *k, const void *v, const void *o, con
                  int64_t q_bs, int64_t k_ts, int64_t k_bs, int64_t v_ts, int64_t v_bs, int64_t o_ts, int64_t o_bs,
                  int64_t do_ts, int64_t do_bs, int64_t window, float softmax_scale, const int32_t *seq_start,
                  int32_t *status_word, void *stream);
+
+/* Linear attention with a decay per head: per batch entry (or packed sequence) and head, with a state S [dk, dv] in fp32,
+ *   S_t = exp(log_decay[head]) S_(t-1) + k_t v_t^T,   o_t = scale q_t^T S_t .
+ * q [batch, tokens, heads, dk], k and v [batch, tokens, kv_heads, dk or dv] bf16, heads adjacent within a token, token / batch
+ * strides in elements (multiples of 8), bases 16-byte aligned; dk, dv 64 or 128 each; kv_heads divides heads (consecutive heads
+ * share).  log_decay: fp32 [heads], meant to be <= 0 (-inf: no memory).  states fp32, contiguous [sequences, heads, dk, dv].  No counterpart in the
+ * reference, whose recurrences have nonlinear memories. */
+typedef struct lact_linear_config {
+  int64_t batch, tokens, heads, kv_heads, dk, dv;
+  int64_t sequences; /* with cu_seqlens: packed sequences within the one batch entry; else 0 */
+  int64_t q_ts, q_bs, k_ts, k_bs, v_ts, v_bs;
+  int64_t do_ts, do_bs; /* of dout (lact_linear_attention_bwd) */
+  float scale;          /* finite, not zero */
+} lact_linear_config;
+/* Scratch of one forward (backward = 0) or backward call, 256-byte aligned. */
+int lact_linear_attention_workspace_bytes(const lact_linear_config *cfg, int32_t backward, size_t *bytes_out);
+/* o [batch, tokens, heads, dv] bf16, contiguous.  cu_seqlens: NULL, or int32 [sequences + 1] on the device for a batch of one:
+ * sequences back to back, empty ones allowed; tokens outside of them have zero outputs.  state_in, state_out: NULL or
+ * [batch or sequences, heads, dk, dv]; they may not overlap. */
+int lact_linear_attention_fwd(const lact_linear_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
+                              const int32_t *cu_seqlens, const float *state_in, float *state_out, void *o, void *workspace,
+                              size_t workspace_bytes, int32_t *status_word, void *stream);
+/* Gradients dq [batch, tokens, heads, dk], dk and dv [batch, tokens, kv_heads, dk or dv] (bf16, contiguous, written; shared heads
+ * added up) and dstate_in (NULL or fp32), from dout (bf16) and dstate_out (the gradient of state_out, NULL: zeros). */
+int lact_linear_attention_bwd(const lact_linear_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
+                              const int32_t *cu_seqlens, const float *state_in, const void *dout, const float *dstate_out, void *dq,
+                              void *dk, void *dv, float *dstate_in, void *workspace, size_t workspace_bytes,
+                              int32_t *status_word, void *stream);
+/* One token of every entry (tokens = 1): reads state_in, writes state_out, which may be the same array. */
+int lact_linear_attention_step(const lact_linear_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
+                               const float *state_in, float *state_out, void *o, void *stream);
 
 /* Backward of lact_qkv_prologue / lact_qkv_prologue_rope on the saved projections (same strides): dq, dk, dv are the
  * gradients of the head-major outputs ([(b n_heads), s, d] bf16, NULL = none), dxq, dxk, dxv the gradients of the

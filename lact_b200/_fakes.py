@@ -114,6 +114,25 @@ def _(q, k, v, o, lse, dout, window, softmax_scale, seq_start=None):
     return [q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)]
 
 
+@_fake("linear_attention_fwd")
+def _(q, k, v, log_decay, scale, state, cu_seqlens, want_state):
+    b, l, h, dk = q.shape
+    n = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    outs = [q.new_empty((b, l, h, v.shape[3]))]
+    return outs + [q.new_empty((n, h, dk, v.shape[3]), dtype=F32)] if want_state else outs
+
+
+@_fake("linear_attention_bwd")
+def _(q, k, v, log_decay, scale, state, cu_seqlens, dout, dlast):
+    outs = [t.new_empty(t.shape) for t in (q, k, v)]
+    return outs + [state.new_empty(state.shape)] if state is not None else outs
+
+
+@_fake("linear_attention_step")
+def _(q, k, v, log_decay, scale, state, new_state):
+    return q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
+
+
 @_fake("seq_start")
 def _(cu_seqlens, n_tokens):
     return cu_seqlens.new_empty((n_tokens,), dtype=torch.int32)

@@ -23,6 +23,7 @@
 #include "grad_fused.cuh"
 #include "swa_bwd.cuh"
 #include "swa_pairs.cuh"
+#include "linear_steps.cuh"
 
 namespace lact {
 namespace {
@@ -2046,6 +2047,46 @@ int scan_fwd_f32(const lact_scan_config& c, const lact_scan_io& io, int32_t n_st
   return store_state(c, io, W02, W1, p.G02, p.G1, stream);
 }
 
+// ------------------------------------------------------------------------------------------ linear attention
+int linear_check(const lact_linear_config* c, const void* cu) {
+  if (c == nullptr) return LACT_ERR_NULL;
+  if ((c->dk != 64 && c->dk != 128) || (c->dv != 64 && c->dv != 128)) return LACT_ERR_SHAPE;
+  if (c->batch < 1 || c->tokens < 1 || c->heads < 1 || c->kv_heads < 1 || c->heads % c->kv_heads != 0) return LACT_ERR_SHAPE;
+  if (c->batch > 65535 || c->heads > 65535 || c->tokens > (1ll << 30) || c->sequences < 0 || c->sequences > (1ll << 24)) return LACT_ERR_SHAPE;
+  if ((c->sequences > 0) != (cu != nullptr) || (cu != nullptr && c->batch != 1)) return LACT_ERR_CONFIG;
+  if ((c->sequences > 0 ? c->sequences : c->batch) * c->heads > (1ll << 30)) return LACT_ERR_SHAPE;
+  if (!(c->scale > -INFINITY && c->scale < INFINITY) || c->scale == 0.f) return LACT_ERR_CONFIG;
+  return LACT_OK;
+}
+int linear_operand(const void* p, int64_t ts, int64_t bs, int64_t row) {
+  if (p == nullptr) return LACT_ERR_NULL;
+  return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || ts % 8 != 0 || bs % 8 != 0 || ts < row ? LACT_ERR_SHAPE : LACT_OK;
+}
+
+template <int A, int B>
+int launch_linear_steps(const LinearArgs& a, cudaStream_t st) {
+  KernelScope scope(kClsOther, st);
+  LACT_CUDA(launch_pdl(linear_steps_kernel<A, B>, dim3(static_cast<unsigned>(a.sequences) * a.heads, B / 32), dim3(256), 0, st, a));
+  return LACT_OK;
+}
+int linear_run(const LinearArgs& a, int64_t A, int64_t B, cudaStream_t st) {
+  if (A == 64) return B == 64 ? launch_linear_steps<64, 64>(a, st) : launch_linear_steps<64, 128>(a, st);
+  return B == 64 ? launch_linear_steps<128, 64>(a, st) : launch_linear_steps<128, 128>(a, st);
+}
+LinearArgs linear_args(const lact_linear_config* c, const float* log_decay, const int32_t* cu) {
+  LinearArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.x_share = a.y_share = a.z_share = 1;
+  a.log_decay = log_decay;
+  a.cu = cu;
+  a.sequences = static_cast<int32_t>(cu != nullptr ? c->sequences : c->batch);
+  a.L = static_cast<int32_t>(c->tokens);
+  a.heads = static_cast<int32_t>(c->heads);
+  a.scale = c->scale;
+  a.in_mul = a.out_mul = 1.f;
+  return a;
+}
+
 }  // namespace
 }  // namespace lact
 
@@ -2056,7 +2097,7 @@ using namespace lact;
 
 extern "C" {
 
-int lact_version(void) { return 1002; }
+int lact_version(void) { return 1003; }
 
 const char* lact_error_string(int code) {
   switch (code) {
@@ -3163,6 +3204,121 @@ int lact_swa_bwd(const void* q, const void* k, const void* v, const void* o, con
   a.o_bs = l * n_heads * d;
   const int64_t ctas = b * n_heads * q_tiles;
   return d == 64 ? launch_swa_bwd<64, 1>(a, ctas, st) : launch_swa_bwd<128, 1>(a, ctas, st);
+}
+
+// ------------------------------------------------------------------------------------------ linear attention
+int lact_linear_attention_workspace_bytes(const lact_linear_config* c, int32_t backward, size_t* bytes_out) {
+  if (c == nullptr || bytes_out == nullptr) return LACT_ERR_NULL;
+  LACT_TRY(linear_check(c, c->sequences > 0 ? c : nullptr));
+  *bytes_out = 0;
+  // shared heads: the gradients of every head in fp32, before they are added up
+  if (backward && c->kv_heads != c->heads) *bytes_out = static_cast<size_t>(c->batch * c->tokens * c->heads * std::max(c->dk, c->dv)) * 4;
+  return LACT_OK;
+}
+
+int lact_linear_attention_fwd(const lact_linear_config* c, const void* q, const void* k, const void* v, const float* log_decay,
+                              const int32_t* cu, const float* state_in, float* state_out, void* o, void* workspace,
+                              size_t workspace_bytes, int32_t* status_word, void* stream) {
+  LACT_TRY(linear_check(c, cu));
+  if (!log_decay || !o || !status_word) return LACT_ERR_NULL;
+  LACT_TRY(linear_operand(q, c->q_ts, c->q_bs, c->heads * c->dk));
+  LACT_TRY(linear_operand(k, c->k_ts, c->k_bs, c->kv_heads * c->dk));
+  LACT_TRY(linear_operand(v, c->v_ts, c->v_bs, c->kv_heads * c->dv));
+  if ((reinterpret_cast<uintptr_t>(o) & 31) != 0) return LACT_ERR_SHAPE;
+  LACT_TRY(check_device());
+  size_t need = 0;
+  LACT_TRY(lact_linear_attention_workspace_bytes(c, 0, &need));
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return LACT_ERR_WORKSPACE;
+  LinearArgs a = linear_args(c, log_decay, cu);
+  a.x = static_cast<const bf16*>(q); a.x_ts = c->q_ts; a.x_bs = c->q_bs;
+  a.y = static_cast<const bf16*>(k); a.y_ts = c->k_ts; a.y_bs = c->k_bs;
+  a.z = static_cast<const bf16*>(v); a.z_ts = c->v_ts; a.z_bs = c->v_bs;
+  a.y_share = a.z_share = static_cast<int32_t>(c->heads / c->kv_heads);
+  a.out = o;
+  a.s_in = state_in;
+  a.s_out = state_out;
+  return linear_run(a, c->dk, c->dv, static_cast<cudaStream_t>(stream));
+}
+
+int lact_linear_attention_step(const lact_linear_config* c, const void* q, const void* k, const void* v, const float* log_decay,
+                               const float* state_in, float* state_out, void* o, void* stream) {
+  LACT_TRY(linear_check(c, nullptr));
+  if (c->tokens != 1) return LACT_ERR_SHAPE;
+  if (!log_decay || !o || !state_in || !state_out) return LACT_ERR_NULL;
+  LACT_TRY(linear_operand(q, c->q_ts, c->q_bs, c->heads * c->dk));
+  LACT_TRY(linear_operand(k, c->k_ts, c->k_bs, c->kv_heads * c->dk));
+  LACT_TRY(linear_operand(v, c->v_ts, c->v_bs, c->kv_heads * c->dv));
+  LACT_TRY(check_device());
+  LinearArgs a = linear_args(c, log_decay, nullptr);
+  a.x = static_cast<const bf16*>(q); a.x_ts = c->q_ts; a.x_bs = c->q_bs;
+  a.y = static_cast<const bf16*>(k); a.y_ts = c->k_ts; a.y_bs = c->k_bs;
+  a.z = static_cast<const bf16*>(v); a.z_ts = c->v_ts; a.z_bs = c->v_bs;
+  a.y_share = a.z_share = static_cast<int32_t>(c->heads / c->kv_heads);
+  a.out = o;
+  a.s_in = state_in;
+  a.s_out = state_out;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (c->dk == 64) return c->dv == 64 ? launch_linear_steps<64, 64>(a, st) : launch_linear_steps<64, 128>(a, st);
+  return c->dv == 64 ? launch_linear_steps<128, 64>(a, st) : launch_linear_steps<128, 128>(a, st);
+}
+
+int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const void* k, const void* v, const float* log_decay,
+                              const int32_t* cu, const float* state_in, const void* dout, const float* dstate_out, void* dq, void* dk,
+                              void* dv, float* dstate_in, void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream) {
+  LACT_TRY(linear_check(c, cu));
+  if (!log_decay || !dq || !dk || !dv || !status_word) return LACT_ERR_NULL;
+  LACT_TRY(linear_operand(q, c->q_ts, c->q_bs, c->heads * c->dk));
+  LACT_TRY(linear_operand(k, c->k_ts, c->k_bs, c->kv_heads * c->dk));
+  LACT_TRY(linear_operand(v, c->v_ts, c->v_bs, c->kv_heads * c->dv));
+  LACT_TRY(linear_operand(dout, c->do_ts, c->do_bs, c->heads * c->dv));
+  for (const void* p : {dq, dk, dv})
+    if ((reinterpret_cast<uintptr_t>(p) & 31) != 0) return LACT_ERR_SHAPE;
+  LACT_TRY(check_device());
+  size_t need = 0;
+  LACT_TRY(lact_linear_attention_workspace_bytes(c, 1, &need));
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 31) != 0)) return LACT_ERR_WORKSPACE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int32_t share = static_cast<int32_t>(c->heads / c->kv_heads);
+  struct Operand { const void* p; int64_t ts, bs; int32_t share; };
+  const Operand Q{q, c->q_ts, c->q_bs, 1}, K{k, c->k_ts, c->k_bs, share}, V{v, c->v_ts, c->v_bs, share}, DO{dout, c->do_ts, c->do_bs, 1};
+  auto with = [&](const Operand& x, const Operand& y, const Operand& z, void* out, bool reverse) {
+    LinearArgs a = linear_args(c, log_decay, cu);
+    a.x = static_cast<const bf16*>(x.p); a.x_ts = x.ts; a.x_bs = x.bs; a.x_share = x.share;
+    a.y = static_cast<const bf16*>(y.p); a.y_ts = y.ts; a.y_bs = y.bs; a.y_share = y.share;
+    a.z = static_cast<const bf16*>(z.p); a.z_ts = z.ts; a.z_bs = z.bs; a.z_share = z.share;
+    a.out = out;
+    a.reverse = reverse;
+    if (reverse) {
+      a.in_mul = 1.f / c->scale;
+      a.out_mul = c->scale;
+      a.s_in = dstate_out;
+      if (share > 1) {
+        a.out = workspace;
+        a.out_f32 = 1;
+      }
+    }
+    return a;
+  };
+  auto add_up = [&](void* out, int64_t d) -> int {
+    if (share == 1) return LACT_OK;
+    const int64_t n4 = c->batch * c->tokens * c->kv_heads * d / 4;
+    KernelScope scope(kClsOther, st);
+    LACT_CUDA(launch_pdl(linear_sum_heads_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((n4 + 255) / 256, sm_count() * 8))), dim3(256), 0, st,
+                         static_cast<const float*>(workspace), static_cast<bf16*>(out), n4, share, static_cast<int32_t>(d / 4)));
+    return LACT_OK;
+  };
+  LinearArgs a = with(DO, V, K, dq, false);
+  a.s_in = state_in;
+  a.s_in_t = 1;
+  LACT_TRY(linear_run(a, c->dv, c->dk, st));
+  a = with(K, Q, DO, dv, true);
+  a.s_out = dstate_in;
+  LACT_TRY(linear_run(a, c->dk, c->dv, st));
+  LACT_TRY(add_up(dv, c->dv));
+  a = with(V, DO, Q, dk, true);
+  a.s_in_t = 1;
+  LACT_TRY(linear_run(a, c->dv, c->dk, st));
+  return add_up(dk, c->dk);
 }
 
 int lact_l2_norm_add(const void* x, int32_t x_dtype, const void* x_add, int32_t add_dtype, const void* scale, void* y,

@@ -101,6 +101,89 @@ def out_epilogue(fw_x: torch.Tensor, norm_weight: torch.Tensor, num_heads: int, 
     return L.call(_op("out_epilogue"), fw_x, norm_weight, scale_proj, o, num_heads, float(eps))
 
 
+# ------------------------------------------------------------------------------------------ linear attention
+def _linear_heads(what, q, k, v, log_decay, dims):
+    """Checks shared by the prompt and the token form (`dims` axes, heads and features last); returns heads, dk, dv."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != dims:
+            raise ValueError(f"{name} must have {dims} axes")
+        if t.dtype != BF16:
+            raise TypeError(f"{name}: bf16 activations")
+    h, hk, dk, dv = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
+    if q.shape[:-2] != k.shape[:-2] or k.shape[:-1] != v.shape[:-1] or k.shape[-1] != dk:
+        raise ValueError("q [..., h, dk], k [..., h_kv, dk], v [..., h_kv, dv] of the same batch and tokens")
+    if dk not in (64, 128) or dv not in (64, 128):
+        raise ValueError("dk and dv must be 64 or 128")
+    if h == 0 or hk == 0 or h % hk:
+        raise ValueError("the heads of k and v must divide those of q")
+    if log_decay.shape != (h,) or log_decay.dtype != torch.float32:
+        raise ValueError("log_decay: [heads] in float32")
+    if any(t.device != q.device for t in (k, v, log_decay)):
+        raise ValueError("all tensors must be on the same device")
+    if not q.is_cuda:
+        raise ValueError(f"{what} needs CUDA tensors (there is no CPU implementation)")
+    return h, dk, dv
+
+
+def _linear_scale(scale, dk):
+    scale = float(scale) if scale is not None else dk ** -0.5
+    if not math.isfinite(scale) or abs(scale) < 1e-30 or abs(scale) > 1e30:
+        raise ValueError("scale must be finite and not zero")
+    return scale
+
+
+def _linear_state(name, state, shape, device):
+    if tuple(state.shape) != shape or state.dtype != torch.float32 or state.device != device:
+        raise ValueError(f"{name}: a float32 {list(shape)} tensor on the device of q")
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: Optional[float] = None,
+                     initial_state: Optional[torch.Tensor] = None, output_final_state: bool = False,
+                     cu_seqlens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Causal linear attention with a decay per head, the recurrence with a linear memory beside this package's fast weights:
+    `S_t = exp(log_decay[h]) S_(t-1) + k_t v_t^T`, `o_t = scale q_t^T S_t` with S [dk, dv] in float32.
+
+    q [b, l, h, dk], k [b, l, h_kv, dk], v [b, l, h_kv, dv] bf16 (dk, dv 64 or 128; h a multiple of h_kv: consecutive heads share a
+    key and value head; views of a fused projection are read where they lie), log_decay [h] float32, not above 0 (-inf: a head
+    without memory); it gets no gradient.  `scale`: dk ** -0.5 by default.  initial_state [b, h, dk, dv] float32 or None (zeros).
+    `cu_seqlens` (int32 [n + 1] on the device, b must be 1): n sequences packed back to back, empty ones allowed, each with its
+    own state ([n, h, dk, dv]); tokens outside of them have zero outputs.  Returns o [b, l, h, dv] bf16 and the state behind the
+    last token (None without `output_final_state`).  Differentiable with respect to q, k, v and initial_state, through both.
+    Products take q, k, v as they are and round the weights of a tile's tokens and its incoming state to bf16; sums and the state
+    itself are kept in float32.  A NaN or an infinity in k, v reaches the outputs of its whole tile of 128 tokens (counted from
+    the start of its sequence) and, as the formula has it, all later ones."""
+    h, dk, dv = _linear_heads("linear_attention", q, k, v, log_decay, 4)
+    n = q.shape[0]
+    if cu_seqlens is not None:
+        if q.shape[0] != 1:
+            raise ValueError("packed sequences (cu_seqlens) need a batch of one")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise ValueError("cu_seqlens: whole numbers [n + 1]")
+        cu_seqlens = cu_seqlens.to(device=q.device, dtype=torch.int32).contiguous()
+        n = cu_seqlens.numel() - 1
+    if initial_state is not None:
+        _linear_state("initial_state", initial_state, (n, h, dk, dv), q.device)
+    r = L.call(_op("linear_attention_fwd"), q, k, v, log_decay, _linear_scale(scale, dk), initial_state, cu_seqlens,
+               bool(output_final_state))
+    return r[0], r[1] if output_final_state else None
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
+                          scale: Optional[float] = None, new_state: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One new token of every sequence (generation): `linear_attention` in its recurrent form.  q [b, h, dk], k [b, h_kv, dk],
+    v [b, h_kv, dv] bf16, state [b, h, dk, dv] float32, contiguous: read, and written in place, or to `new_state` (an array apart
+    from it).  Returns o [b, h, dv] bf16.  No backward: a call with gradients raises."""
+    h, dk, dv = _linear_heads("linear_attention_step", q, k, v, log_decay, 3)
+    for name, t in (("state", state), ("new_state", state if new_state is None else new_state)):
+        _linear_state(name, t, (q.shape[0], h, dk, dv), q.device)
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous: it is written where it lies")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, state, new_state)):
+        raise NotImplementedError("linear_attention_step has no backward: use linear_attention")
+    return L.call(_op("linear_attention_step"), q, k, v, log_decay, _linear_scale(scale, dk), state,
+                  state if new_state is None else new_state)
+
+
 # ------------------------------------------------------------------------------------------ sliding-window attention
 def sliding_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window_size: Optional[int] = None,
                              softmax_scale: Optional[float] = None,

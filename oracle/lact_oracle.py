@@ -847,3 +847,28 @@ def ar_block_visibility(l, mini_batch_size, update_every, num_chunks, kv_cache_s
         else:
             vis[s + mb:s + ue, s + mb - kv_cache_size:min(s + ue, s + 2 * mb)] = True
     return vis
+
+
+# --------------------------------------------------------------------------- linear attention with a decay per head
+def linear_attention(q, k, v, log_decay, scale=None, state=None, cu=None):
+    """Token by token in 64 bits (differentiable): q [b, l, h, dk], k, v [b, l, h_kv, .]; returns o [b, l, h, dv] and the
+    states behind the last token.  `cu`: bounds of packed sequences (list), batch of one, a state each."""
+    b, l, h, dk = q.shape
+    scale = dk ** -0.5 if scale is None else scale
+    share = h // k.shape[2]
+    q, k, v = q.double(), k.double().repeat_interleave(share, 2), v.double().repeat_interleave(share, 2)
+    lam = torch.exp(log_decay.double())[None, :, None, None]
+    cu_ = [0, l] if cu is None else [int(x) for x in cu]
+    outs, last = [q.new_zeros(b, cu_[0], h, v.shape[3])], []
+    for n in range(len(cu_) - 1):
+        S = q.new_zeros(b, h, dk, v.shape[3])
+        if state is not None:
+            S = state.double() if cu is None else state[n:n + 1].double()
+        rows = [q.new_zeros(b, 0, h, v.shape[3])]
+        for t in range(cu_[n], cu_[n + 1]):
+            S = lam * S + k[:, t, :, :, None] * v[:, t, :, None, :]
+            rows.append(scale * torch.einsum("bhk,bhkv->bhv", q[:, t], S)[:, None])
+        outs.append(torch.cat(rows, 1))
+        last.append(S)
+    outs.append(q.new_zeros(b, l - cu_[-1], h, v.shape[3]))
+    return torch.cat(outs, 1), torch.cat(last)
