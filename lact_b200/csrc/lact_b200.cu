@@ -23,7 +23,7 @@
 #include "grad_fused.cuh"
 #include "swa_bwd.cuh"
 #include "swa_pairs.cuh"
-#include "linear_steps.cuh"
+#include "linear_chunks.cuh"
 
 namespace lact {
 namespace {
@@ -2069,9 +2069,82 @@ int launch_linear_steps(const LinearArgs& a, cudaStream_t st) {
   LACT_CUDA(launch_pdl(linear_steps_kernel<A, B>, dim3(static_cast<unsigned>(a.sequences) * a.heads, B / 32), dim3(256), 0, st, a));
   return LACT_OK;
 }
-int linear_run(const LinearArgs& a, int64_t A, int64_t B, cudaStream_t st) {
+int linear_steps(const LinearArgs& a, int64_t A, int64_t B, cudaStream_t st) {
   if (A == 64) return B == 64 ? launch_linear_steps<64, 64>(a, st) : launch_linear_steps<64, 128>(a, st);
   return B == 64 ? launch_linear_steps<128, 64>(a, st) : launch_linear_steps<128, 128>(a, st);
+}
+
+// How a call's tiles are dealt to CTAs.
+struct LinearPlan {
+  bool steps;      // token by token
+  bool cut;        // sequences are cut: a pass over the shares of the states comes first
+  int ctas;
+  int64_t per;     // tiles a CTA takes (0: the kernel works it out)
+};
+LinearPlan linear_plan(const lact_linear_config* c) {
+  const int64_t sms = std::min(sm_count(), kLinearMaxCtas);
+  if (c->sequences > 0) {
+    const int64_t most = c->heads * (c->tokens / 128 + std::min(c->sequences, c->tokens));
+    const int ctas = static_cast<int>(std::min(sms, most));
+    return {false, ctas > 1, ctas, 0};
+  }
+  const int64_t tiles = ceil_div(c->tokens, 128), chains = c->batch * c->heads, total = tiles * chains;
+  if (c->tokens <= 8) return {true, false, 0, 0};
+  const int64_t whole = tiles * ((chains + sms - 1) / sms), even = (total + sms - 1) / sms;
+  const bool cut = 3 * whole > 4 * even + 10;
+  const int64_t per = cut ? even : whole;
+  return {false, cut, static_cast<int>((total + per - 1) / per), per};
+}
+size_t linear_slots(const LinearPlan& p, int64_t dk, int64_t dv) { return p.cut ? static_cast<size_t>(p.ctas) * (dk * dv * 4 + sizeof(LinearPiece)) : 0; }
+
+template <int A, int B, bool PIECE>
+int launch_linear_chunks(const LinearChunkArgs& a, int ctas, cudaStream_t st) {
+  auto kernel = linear_chunks_kernel<A, B, PIECE>;
+  constexpr uint32_t smem = LinearSmem<A, B>::kBytes;
+  static_assert(smem <= 232448, "shared memory budget exceeded");
+  static std::mutex mu;
+  static bool configured[64] = {false};
+  int dev = 0;
+  LACT_CUDA(cudaGetDevice(&dev));
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 64 || !configured[dev]) {
+      LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      if (dev < 64) configured[dev] = true;
+    }
+  }
+  KernelScope scope(kClsOther, st);
+  LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kLinearThreads), smem, st, a));
+  return LACT_OK;
+}
+// `carried`: the slots hold what the CTAs begin with already
+template <int A, int B>
+int linear_chunks(const LinearChunkArgs& a, const LinearPlan& p, bool carried, cudaStream_t st) {
+  if (p.cut && !carried) {
+    LACT_TRY((launch_linear_chunks<A, B, true>(a, p.ctas, st)));
+    KernelScope scope(kClsOther, st);
+    LACT_CUDA(launch_pdl(linear_carry_kernel, dim3(A * B / 128), dim3(128), 0, st, a.a.s_in, a.a.s_in_t, a.a.in_mul, a.slots, a.pieces,
+                         p.ctas, A, B));
+  }
+  return launch_linear_chunks<A, B, false>(a, p.ctas, st);
+}
+int linear_run(const lact_linear_config* c, const LinearArgs& a, int64_t A, int64_t B, void* slots, bool carried, int32_t* status,
+               cudaStream_t st) {
+  const LinearPlan p = linear_plan(c);
+  if (p.steps) return linear_steps(a, A, B, st);
+  LinearChunkArgs k;
+  std::memset(&k, 0, sizeof(k));
+  k.a = a;
+  LACT_TRY(encode_map_heads(&k.x, a.x, c->batch, c->tokens, c->heads / a.x_share, A, a.x_ts, a.x_bs));
+  LACT_TRY(encode_map_heads(&k.y, a.y, c->batch, c->tokens, c->heads / a.y_share, A, a.y_ts, a.y_bs));
+  LACT_TRY(encode_map_heads(&k.z, a.z, c->batch, c->tokens, c->heads / a.z_share, B, a.z_ts, a.z_bs));
+  k.per = p.per;
+  k.slots = static_cast<float*>(slots);
+  k.pieces = reinterpret_cast<LinearPiece*>(static_cast<uint8_t*>(slots) + static_cast<size_t>(p.ctas) * A * B * 4);
+  k.slots_t = carried;
+  k.status = status;
+  if (A == 64) return B == 64 ? linear_chunks<64, 64>(k, p, carried, st) : linear_chunks<64, 128>(k, p, carried, st);
+  return B == 64 ? linear_chunks<128, 64>(k, p, carried, st) : linear_chunks<128, 128>(k, p, carried, st);
 }
 LinearArgs linear_args(const lact_linear_config* c, const float* log_decay, const int32_t* cu) {
   LinearArgs a;
@@ -3210,9 +3283,9 @@ int lact_swa_bwd(const void* q, const void* k, const void* v, const void* o, con
 int lact_linear_attention_workspace_bytes(const lact_linear_config* c, int32_t backward, size_t* bytes_out) {
   if (c == nullptr || bytes_out == nullptr) return LACT_ERR_NULL;
   LACT_TRY(linear_check(c, c->sequences > 0 ? c : nullptr));
-  *bytes_out = 0;
+  *bytes_out = (linear_slots(linear_plan(c), c->dk, c->dv) + 255) / 256 * 256;
   // shared heads: the gradients of every head in fp32, before they are added up
-  if (backward && c->kv_heads != c->heads) *bytes_out = static_cast<size_t>(c->batch * c->tokens * c->heads * std::max(c->dk, c->dv)) * 4;
+  if (backward && c->kv_heads != c->heads) *bytes_out += static_cast<size_t>(c->batch * c->tokens * c->heads * std::max(c->dk, c->dv)) * 4;
   return LACT_OK;
 }
 
@@ -3228,7 +3301,7 @@ int lact_linear_attention_fwd(const lact_linear_config* c, const void* q, const 
   LACT_TRY(check_device());
   size_t need = 0;
   LACT_TRY(lact_linear_attention_workspace_bytes(c, 0, &need));
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return LACT_ERR_WORKSPACE;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return LACT_ERR_WORKSPACE;
   LinearArgs a = linear_args(c, log_decay, cu);
   a.x = static_cast<const bf16*>(q); a.x_ts = c->q_ts; a.x_bs = c->q_bs;
   a.y = static_cast<const bf16*>(k); a.y_ts = c->k_ts; a.y_bs = c->k_bs;
@@ -3237,7 +3310,7 @@ int lact_linear_attention_fwd(const lact_linear_config* c, const void* q, const 
   a.out = o;
   a.s_in = state_in;
   a.s_out = state_out;
-  return linear_run(a, c->dk, c->dv, static_cast<cudaStream_t>(stream));
+  return linear_run(c, a, c->dk, c->dv, workspace, false, status_word, static_cast<cudaStream_t>(stream));
 }
 
 int lact_linear_attention_step(const lact_linear_config* c, const void* q, const void* k, const void* v, const float* log_decay,
@@ -3257,9 +3330,7 @@ int lact_linear_attention_step(const lact_linear_config* c, const void* q, const
   a.out = o;
   a.s_in = state_in;
   a.s_out = state_out;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (c->dk == 64) return c->dv == 64 ? launch_linear_steps<64, 64>(a, st) : launch_linear_steps<64, 128>(a, st);
-  return c->dv == 64 ? launch_linear_steps<128, 64>(a, st) : launch_linear_steps<128, 128>(a, st);
+  return linear_steps(a, c->dk, c->dv, static_cast<cudaStream_t>(stream));
 }
 
 int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const void* k, const void* v, const float* log_decay,
@@ -3276,7 +3347,8 @@ int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const 
   LACT_TRY(check_device());
   size_t need = 0;
   LACT_TRY(lact_linear_attention_workspace_bytes(c, 1, &need));
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 31) != 0)) return LACT_ERR_WORKSPACE;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return LACT_ERR_WORKSPACE;
+  float* const each_head = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (linear_slots(linear_plan(c), c->dk, c->dv) + 255) / 256 * 256);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int32_t share = static_cast<int32_t>(c->heads / c->kv_heads);
   struct Operand { const void* p; int64_t ts, bs; int32_t share; };
@@ -3293,7 +3365,7 @@ int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const 
       a.out_mul = c->scale;
       a.s_in = dstate_out;
       if (share > 1) {
-        a.out = workspace;
+        a.out = each_head;
         a.out_f32 = 1;
       }
     }
@@ -3304,20 +3376,20 @@ int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const 
     const int64_t n4 = c->batch * c->tokens * c->kv_heads * d / 4;
     KernelScope scope(kClsOther, st);
     LACT_CUDA(launch_pdl(linear_sum_heads_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((n4 + 255) / 256, sm_count() * 8))), dim3(256), 0, st,
-                         static_cast<const float*>(workspace), static_cast<bf16*>(out), n4, share, static_cast<int32_t>(d / 4)));
+                         static_cast<const float*>(each_head), static_cast<bf16*>(out), n4, share, static_cast<int32_t>(d / 4)));
     return LACT_OK;
   };
   LinearArgs a = with(DO, V, K, dq, false);
   a.s_in = state_in;
   a.s_in_t = 1;
-  LACT_TRY(linear_run(a, c->dv, c->dk, st));
+  LACT_TRY(linear_run(c, a, c->dv, c->dk, workspace, false, status_word, st));
   a = with(K, Q, DO, dv, true);
   a.s_out = dstate_in;
-  LACT_TRY(linear_run(a, c->dk, c->dv, st));
+  LACT_TRY(linear_run(c, a, c->dk, c->dv, workspace, false, status_word, st));
   LACT_TRY(add_up(dv, c->dv));
   a = with(V, DO, Q, dk, true);
   a.s_in_t = 1;
-  LACT_TRY(linear_run(a, c->dv, c->dk, st));
+  LACT_TRY(linear_run(c, a, c->dv, c->dk, workspace, true, status_word, st));   // the CTAs begin with the states of dv, transposed
   return add_up(dk, c->dk);
 }
 
