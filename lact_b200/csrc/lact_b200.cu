@@ -2123,7 +2123,7 @@ int linear_chunks(const LinearChunkArgs& a, const LinearPlan& p, bool carried, c
   if (p.cut && !carried) {
     LACT_TRY((launch_linear_chunks<A, B, true>(a, p.ctas, st)));
     KernelScope scope(kClsOther, st);
-    LACT_CUDA(launch_pdl(linear_carry_kernel, dim3(A * B / 128), dim3(128), 0, st, a.a.s_in, a.a.s_in_t, a.a.in_mul, a.slots, a.pieces,
+    LACT_CUDA(launch_pdl(linear_carry_kernel, dim3(A * B / 512, p.ctas), dim3(128), 0, st, a.a.s_in, a.a.s_in_t, a.a.in_mul, a.slots, a.pieces,
                          p.ctas, A, B));
   }
   return launch_linear_chunks<A, B, false>(a, p.ctas, st);

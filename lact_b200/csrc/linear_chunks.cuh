@@ -1,17 +1,19 @@
 // Linear attention with a decay per head (linear_steps.cuh has the formulas), tiles of 128 tokens on the tensor cores:
 //   G = X Y^T,  P_ij = G_ij lambda^(i-j) (j <= i),  out = scale (P Z + diag(lambda^(i+1)) X S),
-//   S <- lambda^n S + (diag(lambda^(n-1-j)) Y)^T Z                                     (backwards in time: the mirror image).
-// A CTA takes a run of tiles of consecutive (sequence, head)s, keeps S in tensor memory over them and reads every tile once:
+//   S <- lambda^n S + D,  D = (diag(lambda^(n-1-j)) Y)^T Z                             (backwards in time: the mirror image).
+// A CTA takes a run of tiles of consecutive (sequence, head)s and reads every tile once:
 //   warp 0       loads the tiles of X, Y, Z through a ring of stages;
 //   warp 1       issues the products: G(t + 1) as soon as P(t) has been used and the tile is there;
-//   warps 2-9    ("rows") G -> P (to tensor memory, the first operand of P Z from there), later both parts of the output -> memory;
-//   warps 10-17  ("state") S -> bf16 in shared memory for X S, S * lambda^n back to tensor memory, then Y -> Y lambda^(n-1-j) in bf16
-//                pieces, in place and into the tile's X and the copy of S, which X S has used by then.
-// Roundings: P and the copy of S to bf16, as operands of products whose sum is rounded to bf16 in the end.  S itself stays in fp32:
-// decayed rows of Y are two bf16 pieces (16 bits of the product; what is lost, 2^-17, is far below the copy's rounding), three
-// (24 bits) where the last state is an output.
+//   warps 4-11   ("rows") G -> P (to tensor memory, the first operand of P Z from there), later both parts of the output -> memory;
+//   warps 12-19  ("state") keep S in registers: S <- lambda^n S + D, its copy in bf16 to shared memory for X S, then
+//                Y -> diag(lambda^(n-1-j)) Y in bf16 pieces, the first in place.
+// Roundings: P and the copy of S to bf16, as operands of products whose sum is rounded to bf16 in the end.  S itself is added up in
+// fp32 (D alone is summed by the tensor core, which truncates: over a long sequence that would show): the decayed rows of Y are two
+// bf16 pieces (16 bits of the product; what is lost, 2^-17, is far below the copy's rounding), three (24 bits) where the last state
+// is an output.
 // Long sequences of few heads: `per` tiles a CTA may begin within a sequence.  linear_chunks_kernel<..., PIECE> first leaves every CTA's
-// share of the state of the sequence that goes on behind it, linear_carry_kernel adds the shares up in order.
+// share of the state of the sequence that goes on behind it, linear_carry_kernel adds the shares up in order.  The shares are taken
+// from the last tile to the first, so that the tiles the CTA begins with afterwards have been read last and are still in L2.
 #pragma once
 #include "linear_steps.cuh"
 #include "umma_gemm.cuh"
@@ -37,11 +39,22 @@ struct LinearChunkArgs {
 
 template <int A, int B>
 struct LinearSmem {
-  static constexpr int kStages = A == 128 ? 2 : B == 128 ? 3 : 4;
-  static constexpr uint32_t kXY = 128 * A * 2, kZ = 128 * B * 2, kStage = 2 * kXY + kZ;   // X, Y, Z of one tile
-  static constexpr uint32_t kS = kStages * kStage;                                         // copy of S, third piece of Y
+  static constexpr bool kRing5 = A == 128 && B == 128;   // no room for two whole stages beside the rest: five tiles of 32 KB in a ring
+  static constexpr int kStages = kRing5 || A == 128 ? 2 : B == 128 ? 3 : 4;
+  static constexpr int kPieceStages = kRing5 ? 2 : A == 128 ? 3 : 4;                     // of Y and Z alone
+  static constexpr uint32_t kXY = 128 * A * 2, kZ = 128 * B * 2;
+  static constexpr uint32_t kTiles = kRing5 ? 5 * kXY : kStages * (2 * kXY + kZ);
+  static constexpr uint32_t kLow = kTiles;          // second piece of Y
+  static constexpr uint32_t kS = kLow + kXY;        // copy of S; third piece of Y
   static constexpr uint32_t kBars = kS + kXY;
-  static constexpr uint32_t kBytes = kBars + 256;
+  static constexpr uint32_t kFactors = kBars + 256; // a table of 32 decays per row warp
+  static constexpr uint32_t kBytes = kFactors + 8 * 128;
+  static_assert(kPieceStages * (kXY + kZ) <= kTiles, "the stages of the shares fit");
+  // where X, Y, Z of the CTA's tile t lie
+  static __device__ __forceinline__ uint32_t x(int t) { return kRing5 ? 3 * t % 5 * kXY : t % kStages * (2 * kXY + kZ); }
+  static __device__ __forceinline__ uint32_t y(int t) { return kRing5 ? (3 * t + 1) % 5 * kXY : x(t) + kXY; }
+  static __device__ __forceinline__ uint32_t z(int t) { return kRing5 ? (3 * t + 2) % 5 * kXY : x(t) + 2 * kXY; }
+  static __device__ __forceinline__ uint32_t piece_y(int t) { return t % kPieceStages * (kXY + kZ); }
 };
 
 // The tiles of a launch in order: sequence, head, tile (backwards in time: from the last).
@@ -127,32 +140,79 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-constexpr int kLinearRowWarps = 8, kLinearStateWarps = 8;
-constexpr int kLinearThreads = 64 + 32 * (kLinearRowWarps + kLinearStateWarps);
+// Rows 32 * quarter + lane of a tile of Y times the decay until the tile's end, as bf16 pieces: the first in place, the second to `low`,
+// a third to `lowest` (0: none).  Two threads a row; rows past the sequence become zeros.
+template <int A>
+__device__ __forceinline__ void linear_decay_rows(uint32_t y, uint32_t low, uint32_t lowest, int tid, float f, bool real) {
+  constexpr uint32_t kBox = 128 * 128;
+  const int j = tid & 127, part = tid >> 7;
+  const F32x2 ff = f32x2(f, f), minus = f32x2(-1.f, -1.f);
+#pragma unroll 4
+  for (int i = 0; i < A / 16; ++i) {
+    const int unit = part * (A / 16) + i;
+    const uint32_t off = (unit >> 3) * kBox + j * 128 + (((unit & 7) ^ (j & 7)) << 4);
+    uint32_t u[4], w[4], l[4], m[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(y + off));
+    auto pair = [](uint32_t b) { return f32x2(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)); };
+    auto round = [](F32x2 p) {
+      float p0, p1;
+      f32x2_split(p, p0, p1);
+      return pack_bf16x2(p0, p1);
+    };
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      F32x2 p = f32x2_mul(pair(real ? u[e] : 0u), ff);
+      w[e] = round(p);
+      p = f32x2_fma(pair(w[e]), minus, p);
+      l[e] = round(p);
+      if (lowest != 0) m[e] = round(f32x2_fma(pair(l[e]), minus, p));
+    }
+    auto put = [&](uint32_t to, const uint32_t (&v)[4]) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + off), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+    };
+    put(y, w);
+    put(low, l);
+    if (lowest != 0) put(lowest, m);
+  }
+}
+// Rows `from` to 127 of a tile of Z become zeros (256 threads).
+template <int B>
+__device__ __forceinline__ void linear_clear_rows(uint32_t z, int from, int tid) {
+  for (int i = tid; i < (128 - from) * (B / 8); i += 256) {
+    const int row = from + i / (B / 8), u = i % (B / 8);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(z + (u >> 3) * (128 * 128) + row * 128 + (u & 7) * 16), "r"(0) : "memory");
+  }
+}
+
+constexpr int kLinearThreads = 640;   // a warpgroup for loads and products, two for the rows, two for the state
+// registers per thread of each: 128 x 64 + 256 x 80 + 256 x 128 = 640 x 96
+constexpr int kLinearIssueRegs = 64, kLinearRowRegs = 80, kLinearStateRegs = 128, kLinearLaunchRegs = 96;
+static_assert(kLinearIssueRegs + 2 * kLinearRowRegs + 2 * kLinearStateRegs <= 5 * kLinearLaunchRegs, "the shares of the registers");
 
 template <int A, int B, bool PIECE>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const __grid_constant__ LinearChunkArgs args) {
   static_assert((A == 64 || A == 128) && (B == 64 || B == 128), "64 or 128 features");
   using SM = LinearSmem<A, B>;
-  constexpr int NS = SM::kStages;
+  constexpr int NS = PIECE ? SM::kPieceStages : SM::kStages;
   constexpr uint32_t kBox = 128 * 128;       // [128 rows][64 features] box of a tile
   constexpr uint32_t kSBox = B * 128;        // [B rows][64 columns] box of the copy of S
-  constexpr uint32_t kTmemCols = 512, kG = 128, kO = 256, kOx = 384;   // S at 0, G and P, P Z, X S
+  constexpr uint32_t kTmemCols = 512, kG = 128, kO = 256, kOx = 384;   // D at 0, G and P (PIECE: a second D), P Z, X S
   extern __shared__ __align__(1024) uint8_t linear_smem[];
   const uint32_t base = smem_u32(linear_smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(linear_smem + SM::kBars);
   uint64_t* xy_full = bars;             // [NS]
   uint64_t* z_full = bars + 4;          // [NS]
-  uint64_t* stage_empty = bars + 8;     // [NS]
+  uint64_t* stage_empty = bars + 8;     // [NS] Y and Z (and, the ring of five aside, X) have been used
   uint64_t* g_full = bars + 12;         // G is in tensor memory
   uint64_t* p_full = bars + 13;         // an arrival per row warp: P is there (and Z is clean)
-  uint64_t* s_ready = bars + 14;        // an arrival per state warp: the copy of S is there, S is decayed
+  uint64_t* s_ready = bars + 14;        // an arrival per state warp: D has been read, the copy of S is there
   uint64_t* x_done = bars + 15;         // X and the copy of S have been used
   uint64_t* o_full = bars + 16;         // both parts of the output are there
   uint64_t* o_empty = bars + 17;        // an arrival per row warp: they have been read
-  uint64_t* y_ready = bars + 18;        // an arrival per state warp: the pieces of Y are there
-  uint64_t* s_full = bars + 19;         // S has taken the tile in
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* y_ready = bars + 18;        // an arrival per warp that makes them: the pieces of Y are there
+  uint64_t* d_full = bars + 19;         // [2] D is there (PIECE: two of them in turn)
+  uint64_t* d_read = bars + 21;         // [2] PIECE: an arrival per state warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   const LinearArgs& a = args.a;
 
@@ -160,13 +220,13 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) { mbar_init(&xy_full[s], 1); mbar_init(&z_full[s], 1); mbar_init(&stage_empty[s], 1); }
     mbar_init(g_full, 1);
-    mbar_init(p_full, kLinearRowWarps);
-    mbar_init(s_ready, kLinearStateWarps);
+    mbar_init(p_full, 8);
+    mbar_init(s_ready, 8);
     mbar_init(x_done, 1);
     mbar_init(o_full, 1);
-    mbar_init(o_empty, kLinearRowWarps);
-    mbar_init(y_ready, kLinearStateWarps);
-    mbar_init(s_full, 1);
+    mbar_init(o_empty, 8);
+    mbar_init(y_ready, 8);
+    for (int s = 0; s < 2; ++s) { mbar_init(&d_full[s], 1); mbar_init(&d_read[s], 8); }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -189,17 +249,18 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   LinearTiles it;
   bool mid = false;       // the first tile goes on with a sequence that the CTA before this one has begun
   if (count > 0) {
-    if (PIECE) {
+    if (PIECE) {   // the tiles of the last one's sequence, from the last to the first
       it.seek(a, end - 1);
       const bool goes_on = it.c + 1 < it.tiles;
-      const int back = min(it.c, count - 1);   // tiles of the last one's sequence before it
-      it.c -= back;
-      mid = it.c > 0;
+      const int back = min(it.c, count - 1);
+      mid = it.c - back > 0;
       if (threadIdx.x == 0) {
-        // tokens of tiles c .. c + back: all whole, but for the first of a walk backwards
-        const int tokens = (back + 1) * 128 - (a.reverse && !mid ? 128 - it.valid(it.place(a)) : 0);
+        LinearTiles at = it;
+        at.c -= back;
+        // tokens of these tiles: all whole, but for the first of a walk backwards
+        const int tokens = (back + 1) * 128 - (a.reverse && !mid ? 128 - at.valid(at.place(a)) : 0);
         args.pieces[blockIdx.x] = {goes_on, mid, it.n * a.heads + it.head,
-                                   exp2f(decay_log2(a, it.head) * static_cast<float>(tokens - 1 + it.first_decay(a)))};
+                                   exp2f(decay_log2(a, it.head) * static_cast<float>(tokens - 1 + at.first_decay(a)))};
       }
       count = goes_on ? back + 1 : 0;
     } else {
@@ -209,111 +270,149 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   } else if (PIECE && threadIdx.x == 0) {
     args.pieces[blockIdx.x] = {0, 0, 0, 0.f};
   }
+  auto advance = [&]() {
+    if (PIECE) --it.c;
+    else it.next(a);
+  };
   // (swizzled tiles need the alignment asked for above)
   bool failed = uniform(static_cast<uint32_t>(*reinterpret_cast<volatile int32_t*>(args.status))) != kStatusOk || (base & 1023u) != 0;
-  const int pieces = !PIECE && a.s_out == nullptr ? 2 : 3;
+  const bool three = a.s_out != nullptr;
+  auto y_of = [&](int t) { return base + (PIECE ? SM::piece_y(t) : SM::y(t)); };
+  auto z_of = [&](int t) { return PIECE ? y_of(t) + SM::kXY : base + SM::z(t); };
 
-  if (warp == 0) {
-    const uint32_t leader = elect_leader();
-    for (int t = 0; t < count && !failed; ++t, it.next(a)) {
-      const int st = t % NS, row = it.s.first + it.place(a);
-      const uint32_t dst = base + st * SM::kStage;
-      if (t >= NS && !mbar_wait_warp(&stage_empty[st], (t / NS - 1) & 1, abort_flag)) { failed = true; break; }
-      mbar_expect_tx_if(leader, &xy_full[st], PIECE ? SM::kXY : 2 * SM::kXY);
-      for (int j = 0; j < A / 64; ++j) {
-        if (!PIECE) tma_load_4d_if(leader, dst + j * kBox, &args.x, &xy_full[st], 64 * j, row, it.head / a.x_share, it.s.entry);
-        tma_load_4d_if(leader, dst + SM::kXY + j * kBox, &args.y, &xy_full[st], 64 * j, row, it.head / a.y_share, it.s.entry);
+  if (warp < 4) {
+    registers_shrink<kLinearIssueRegs>();
+    if (warp == 0) {
+      const uint32_t leader = elect_leader();
+      for (int t = 0; t < count && !failed; ++t, advance()) {
+        const int st = t % NS, row = it.s.first + it.place(a);
+        if (t >= NS && !mbar_wait_warp(&stage_empty[st], (t / NS - 1) & 1, abort_flag)) { failed = true; break; }
+        mbar_expect_tx_if(leader, &xy_full[st], PIECE ? SM::kXY : 2 * SM::kXY);
+        for (int j = 0; j < A / 64; ++j) {
+          if (!PIECE) tma_load_4d_if(leader, base + SM::x(t) + j * kBox, &args.x, &xy_full[st], 64 * j, row, it.head / a.x_share, it.s.entry);
+          tma_load_4d_if(leader, y_of(t) + j * kBox, &args.y, &xy_full[st], 64 * j, row, it.head / a.y_share, it.s.entry);
+        }
+        // (ring of five: Z comes to where X of the tile before was)
+        if (!PIECE && SM::kRing5 && t >= 1 && !mbar_wait_warp(x_done, (t - 1) & 1, abort_flag)) { failed = true; break; }
+        mbar_expect_tx_if(leader, &z_full[st], SM::kZ);
+        for (int j = 0; j < B / 64; ++j)
+          tma_load_4d_if(leader, z_of(t) + j * kBox, &args.z, &z_full[st], 64 * j, row, it.head / a.z_share, it.s.entry);
       }
-      mbar_expect_tx_if(leader, &z_full[st], SM::kZ);
-      for (int j = 0; j < B / 64; ++j)
-        tma_load_4d_if(leader, dst + 2 * SM::kXY + j * kBox, &args.z, &z_full[st], 64 * j, row, it.head / a.z_share, it.s.entry);
-    }
-  } else if (warp == 1) {
-    const uint32_t leader = elect_leader();
-    const uint32_t idesc_g = make_idesc_bf16(128, 128, 0, 0);   // X Y^T, both K-major
-    const uint32_t idesc_ox = make_idesc_bf16(128, B, 0, 0);    // X S: the copy of S is [B][A], K-major
-    const uint32_t idesc_o = make_idesc_bf16(128, B, 0, 1);     // P Z: P in tensor memory, Z MN-major
-    const uint32_t idesc_s = make_idesc_bf16(128, A, 1, 1);     // Z^T Y, both MN-major (64 features: the upper lanes take what follows Z)
-    const SmemDescBase desc(kBox);
-    auto stage = [&](int64_t t) { return base + static_cast<uint32_t>(t % NS) * SM::kStage; };
-    auto phase = [&](int64_t t) { return (t / NS) & 1; };
-    auto issue_g = [&](int64_t t) {
-      const uint32_t x = stage(t), y = x + SM::kXY;
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < A / 64; ++kk)
-#pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4)
-          umma_bf16_if(leader, tmem + kG, desc.at((x + kk * kBox + k4 * 32) >> 4), desc.at((y + kk * kBox + k4 * 32) >> 4), idesc_g,
-                       (kk | k4) != 0);
-      umma_commit_if(leader, g_full);
-    };
-    if (!PIECE && count > 0 && !failed) {
-      if (mbar_wait_warp(&xy_full[0], 0, abort_flag)) issue_g(0);
-      else failed = true;
-    }
-    for (int t = 0; t < count && !failed; ++t) {
-      const uint32_t par = t & 1, x = stage(t), y = x + SM::kXY, z = y + SM::kXY, s = base + SM::kS;
-      bool g_next = true;
-      if (!PIECE) {
-        if (!mbar_wait_warp(s_ready, par, abort_flag) || (t >= 1 && !mbar_wait_warp(o_empty, par ^ 1, abort_flag))) { failed = true; break; }
+    } else if (warp == 1) {
+      const uint32_t leader = elect_leader();
+      const uint32_t idesc_g = make_idesc_bf16(128, 128, 0, 0);   // X Y^T, both K-major
+      const uint32_t idesc_ox = make_idesc_bf16(128, B, 0, 0);    // X S: the copy of S is [B][A], K-major
+      const uint32_t idesc_o = make_idesc_bf16(128, B, 0, 1);     // P Z: P in tensor memory, Z MN-major
+      const uint32_t idesc_d = make_idesc_bf16(128, A, 1, 1);     // Z^T Y, both MN-major (64 features: the upper lanes take what follows Z)
+      const SmemDescBase desc(kBox);
+      auto issue_g = [&](int t) {
+        const uint32_t x = base + SM::x(t), y = y_of(t);
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < A / 64; ++kk)
 #pragma unroll
           for (int k4 = 0; k4 < 4; ++k4)
-            umma_bf16_if(leader, tmem + kOx, desc.at((x + kk * kBox + k4 * 32) >> 4), desc.at((s + kk * kSBox + k4 * 32) >> 4), idesc_ox,
+            umma_bf16_if(leader, tmem + kG, desc.at((x + kk * kBox + k4 * 32) >> 4), desc.at((y + kk * kBox + k4 * 32) >> 4), idesc_g,
                          (kk | k4) != 0);
-        umma_commit_if(leader, x_done);
-        if (!mbar_wait_warp(p_full, par, abort_flag) || !mbar_wait_warp(&z_full[t % NS], phase(t), abort_flag)) { failed = true; break; }
-        tc_fence_after();
+        umma_commit_if(leader, g_full);
+      };
+      if (!PIECE && count > 0 && !failed) {
+        if (mbar_wait_warp(&xy_full[0], 0, abort_flag)) issue_g(0);
+        else failed = true;
+      }
+      for (int t = 0; t < count && !failed; ++t) {
+        const uint32_t par = t & 1, x = base + SM::x(t), y = y_of(t), z = z_of(t);
+        bool g_next = false;
+        if (!PIECE) {
+          if (!mbar_wait_warp(s_ready, par, abort_flag) || (t >= 1 && !mbar_wait_warp(o_empty, par ^ 1, abort_flag))) { failed = true; break; }
+          tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_bf16_ta_if(leader, tmem + kO, tmem + kG + (k >> 1) * 32 + (k & 1) * 8, desc.at((z + k * 2048) >> 4), idesc_o, k != 0);
-        umma_commit_if(leader, o_full);
-        g_next = t + 1 < count;
-        if (g_next && __all_sync(0xFFFFFFFFu, mbar_test(&xy_full[(t + 1) % NS], phase(t + 1)))) {
-          issue_g(t + 1);
-          g_next = false;
+          for (int kk = 0; kk < A / 64; ++kk)
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4)
+              umma_bf16_if(leader, tmem + kOx, desc.at((x + kk * kBox + k4 * 32) >> 4),
+                           desc.at((base + SM::kS + kk * kSBox + k4 * 32) >> 4), idesc_ox, (kk | k4) != 0);
+          umma_commit_if(leader, x_done);
+          if (!mbar_wait_warp(p_full, par, abort_flag) || !mbar_wait_warp(&z_full[t % NS], (t / NS) & 1, abort_flag)) { failed = true; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            umma_bf16_ta_if(leader, tmem + kO, tmem + kG + (k >> 1) * 32 + (k & 1) * 8, desc.at((z + k * 2048) >> 4), idesc_o, k != 0);
+          umma_commit_if(leader, o_full);
+          g_next = t + 1 < count;
+          if (g_next && __all_sync(0xFFFFFFFFu, mbar_test(&xy_full[(t + 1) % NS], ((t + 1) / NS) & 1))) {
+            issue_g(t + 1);
+            g_next = false;
+          }
         }
-      }
-      if (!mbar_wait_warp(y_ready, par, abort_flag) || (PIECE && !mbar_wait_warp(&z_full[t % NS], phase(t), abort_flag))) { failed = true; break; }
-      tc_fence_after();
-      for (int p = 0; p < pieces; ++p) {
-        const uint32_t yp = p == 0 ? y : p == 1 ? x : s;
+        if (!mbar_wait_warp(y_ready, par, abort_flag)) { failed = true; break; }
+        if (PIECE && (!mbar_wait_warp(&z_full[t % NS], (t / NS) & 1, abort_flag) ||
+                      (t >= 2 && !mbar_wait_warp(&d_read[t & 1], ((t >> 1) - 1) & 1, abort_flag)))) { failed = true; break; }
+        tc_fence_after();
+        const uint32_t d = tmem + (PIECE ? par * kG : 0);
+        const uint32_t low = base + (PIECE && !three && par ? SM::kS : SM::kLow);
+        for (int p = 0; p < (three ? 3 : 2); ++p) {
+          const uint32_t yp = p == 0 ? y : p == 1 ? low : base + SM::kS;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_bf16_if(leader, tmem, desc.at((z + k * 2048) >> 4), desc.at((yp + k * 2048) >> 4), idesc_s, 1);
-      }
-      umma_commit_if(leader, s_full);
-      umma_commit_if(leader, &stage_empty[t % NS]);
-      if (!PIECE && g_next) {
-        if (!mbar_wait_warp(&xy_full[(t + 1) % NS], phase(t + 1), abort_flag)) { failed = true; break; }
-        issue_g(t + 1);
+          for (int k = 0; k < 8; ++k)
+            umma_bf16_if(leader, d, desc.at((z + k * 2048) >> 4), desc.at((yp + k * 2048) >> 4), idesc_d, (p | k) != 0);
+        }
+        umma_commit_if(leader, &d_full[PIECE ? par : 0]);
+        umma_commit_if(leader, &stage_empty[t % NS]);
+        if (g_next) {
+          if (!mbar_wait_warp(&xy_full[(t + 1) % NS], ((t + 1) / NS) & 1, abort_flag)) { failed = true; break; }
+          issue_g(t + 1);
+        }
       }
     }
-  } else if (warp < 2 + kLinearRowWarps) {
+  } else if (warp < 12) {
+    registers_shrink<kLinearRowRegs>();
     // ---------------- rows: two threads per row of the tile (tensor-memory lane), 64 columns of G and half of the output each
-    if constexpr (!PIECE) {
-      const int quarter = warp & 3, half = (warp - 2) >> 2, r = quarter * 32 + lane;
-      const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-      const int tid = threadIdx.x - 64;
-      linear_zero_rest<B>(a, static_cast<int64_t>(blockIdx.x) * 256 + tid, static_cast<int64_t>(gridDim.x) * 256);
-      if (a.cu != nullptr && a.s_out != nullptr) {   // empty sequences keep their states
-        for (int n = blockIdx.x; n < a.sequences; n += gridDim.x) {
-          if (linear_span(a, n).len != 0) continue;
-          const int64_t size = static_cast<int64_t>(a.heads) * (A * B), at = n * size;
-          for (int64_t i = tid; i < size; i += 256) a.s_out[at + i] = a.s_in != nullptr ? a.s_in[at + i] : 0.f;
-        }
-      }
-      int head = -1;
-      float g2 = 0.f;
-      for (int t = 0; t < count && !failed; ++t, it.next(a)) {
-        const uint32_t par = t & 1;
-        const int place = it.place(a), nv = it.valid(place);
+    const int quarter = warp & 3, half = (warp - 4) >> 2, r = quarter * 32 + lane, tid = threadIdx.x - 128;
+    int head = -1;
+    float g2 = 0.f;
+    if constexpr (PIECE) {   // the pieces of Y; the tiles' own end is where their decays count from
+      for (int t = 0; t < count && !failed; ++t, advance()) {
+        const int st = t % NS, nv = it.valid(it.place(a)), used = three ? t - 1 : t - 2;   // (the tile that used this place last)
         if (it.head != head) {
           head = it.head;
           g2 = decay_log2(a, head);
+        }
+        const int j = tid & 127;
+        const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
+        if (!mbar_wait_warp(&xy_full[st], (t / NS) & 1, abort_flag) ||
+            (used >= 0 && !mbar_wait_warp(&d_full[used & 1], (used >> 1) & 1, abort_flag))) { failed = true; break; }
+        linear_decay_rows<A>(y_of(t), base + (!three && (t & 1) ? SM::kS : SM::kLow), three ? base + SM::kS : 0, tid, f, j < nv);
+        if (nv < 128 && a.cu != nullptr) {
+          if (!mbar_wait_warp(&z_full[st], (t / NS) & 1, abort_flag)) { failed = true; break; }
+          linear_clear_rows<B>(z_of(t), nv, tid);
+        }
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(y_ready);
+      }
+    } else {
+      const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+      linear_zero_rest<B>(a, static_cast<int64_t>(blockIdx.x) * 256 + tid, static_cast<int64_t>(gridDim.x) * 256);
+      if (a.cu != nullptr && a.s_out != nullptr) {   // empty sequences keep their states
+        const int64_t size = static_cast<int64_t>(a.heads) * (A * B / 4);
+        for (int n = 0; n < a.sequences; ++n) {
+          if (linear_span(a, n).len != 0) continue;
+          for (int64_t i = blockIdx.x * 256ll + tid; i < size; i += gridDim.x * 256ll)
+            reinterpret_cast<float4*>(a.s_out)[n * size + i] =
+                a.s_in != nullptr ? reinterpret_cast<const float4*>(a.s_in)[n * size + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      float* const factors = reinterpret_cast<float*>(linear_smem + SM::kFactors) + (warp - 4) * 32;
+      for (int t = 0; t < count && !failed; ++t, advance()) {
+        const uint32_t par = t & 1;
+        const int place = it.place(a), nv = it.valid(place);
+        if (it.head != head) {   // the decays of 32 columns among themselves
+          head = it.head;
+          g2 = decay_log2(a, head);
+          __syncwarp();
+          factors[lane] = exp2f(g2 * static_cast<float>(a.reverse ? lane : 31 - lane));
+          __syncwarp();
         }
         if (!mbar_wait_warp(g_full, par, abort_flag)) { failed = true; break; }
         tc_fence_after();
@@ -327,32 +426,50 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           } else {
             uint32_t bits[32];
             tmem_ld32(tmem + lane_off + kG + c0, bits);
-            // exponents of columns j: |r - c0 - j| tokens
-            const float step = a.reverse ? g2 : -g2, from = (a.reverse ? c0 - r : r - c0) * g2;
-            const int lo = a.reverse ? r - c0 : 0, hi = a.reverse ? nv - 1 - c0 : r - c0;   // visible columns
-            tmem_ld_wait();
-            float p[32];
+            if (cb != quarter) {
+              // lambda^(distance to the column nearest to the diagonal) * lambda^(from there)
+              const float f = exp2_ftz(g2 * static_cast<float>(a.reverse ? c0 - r : r - c0 - 31));
+              const F32x2 ff = f32x2(f, f);
+              const int hi = a.reverse ? nv - 1 - c0 : 31;
+              tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) p[j] = __uint_as_float(bits[j]) * exp2_ftz(fmaf(static_cast<float>(j), step, from));
-            if (cb == quarter || hi < 31) {
+              for (int j = 0; j < 32; j += 4) {
+                const float4 c = *reinterpret_cast<const float4*>(factors + j);
+                const F32x2 p01 = f32x2_mul(f32x2(__uint_as_float(bits[j]), __uint_as_float(bits[j + 1])), f32x2_mul(f32x2(c.x, c.y), ff));
+                const F32x2 p23 = f32x2_mul(f32x2(__uint_as_float(bits[j + 2]), __uint_as_float(bits[j + 3])), f32x2_mul(f32x2(c.z, c.w), ff));
+                float p0, p1, p2, p3;
+                f32x2_split(p01, p0, p1);
+                f32x2_split(p23, p2, p3);
+                if (hi < 31) {
+                  p0 = j > hi ? 0.f : p0;
+                  p1 = j + 1 > hi ? 0.f : p1;
+                  p2 = j + 2 > hi ? 0.f : p2;
+                  p3 = j + 3 > hi ? 0.f : p3;
+                }
+                w[j / 2] = pack_bf16x2(p0, p1);
+                w[j / 2 + 1] = pack_bf16x2(p2, p3);
+              }
+            } else {
+              // column j is |lane - j| tokens away; visible from / up to its own
+              const float step = a.reverse ? g2 : -g2, from = (a.reverse ? -lane : lane) * g2;
+              const int lo = a.reverse ? lane : 0, hi = a.reverse ? nv - 1 - c0 : lane;
+              tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < lo || j > hi) p[j] = 0.f;
+              for (int j = 0; j < 32; j += 2) {
+                float p0 = __uint_as_float(bits[j]) * exp2_ftz(fmaf(static_cast<float>(j), step, from));
+                float p1 = __uint_as_float(bits[j + 1]) * exp2_ftz(fmaf(static_cast<float>(j + 1), step, from));
+                p0 = j < lo || j > hi ? 0.f : p0;
+                p1 = j + 1 < lo || j + 1 > hi ? 0.f : p1;
+                w[j / 2] = pack_bf16x2(p0, p1);
+              }
             }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
           }
           __syncwarp();
           tmem_st16(tmem + lane_off + kG + c0, w);
         }
         if (nv < 128 && a.cu != nullptr) {   // rows of the next sequence: no part of any sum
-          const int st = t % NS;
-          if (!mbar_wait_warp(&z_full[st], (t / NS) & 1, abort_flag)) { failed = true; break; }
-          const uint32_t z = base + st * SM::kStage + 2 * SM::kXY;
-          for (int i = tid; i < (128 - nv) * (B / 8); i += 256) {
-            const int row = nv + i / (B / 8), u = i % (B / 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(z + (u >> 3) * kBox + row * 128 + (u & 7) * 16), "r"(0) : "memory");
-          }
+          if (!mbar_wait_warp(&z_full[t % NS], (t / NS) & 1, abort_flag)) { failed = true; break; }
+          linear_clear_rows<B>(z_of(t), nv, tid);
           fence_async_proxy();
         }
         tmem_st_wait();
@@ -361,31 +478,37 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         if (lane == 0) mbar_arrive(p_full);
 
         const int pos = a.reverse ? nv - 1 - r : r;
-        const float since = exp2f(g2 * static_cast<float>(max(pos, 0) + it.first_decay(a)));
+        const float since = a.scale * exp2f(g2 * static_cast<float>(max(pos, 0) + it.first_decay(a)));
+        const F32x2 ss = f32x2(since, since), sc = f32x2(a.scale, a.scale);
+        const int64_t o = ((it.s.entry * static_cast<int64_t>(a.L) + it.s.first + place + r) * a.heads + head) * B + half * (B / 2);
         if (!mbar_wait_warp(o_full, par, abort_flag)) { failed = true; break; }
         tc_fence_after();
-        const int64_t o = ((it.s.entry * static_cast<int64_t>(a.L) + it.s.first + place + r) * a.heads + head) * B + half * (B / 2);
 #pragma unroll
-        for (int c = 0; c < B / 2; c += 32) {
-          uint32_t bi[32], bx[32];
-          tmem_ld32(tmem + lane_off + kO + half * (B / 2) + c, bi);
-          tmem_ld32(tmem + lane_off + kOx + half * (B / 2) + c, bx);
+        for (int c = 0; c < B / 2; c += 16) {
+          uint32_t bi[16], bx[16];
+          tmem_ld16(tmem + lane_off + kO + half * (B / 2) + c, bi);
+          tmem_ld16(tmem + lane_off + kOx + half * (B / 2) + c, bx);
           tmem_ld_wait();
+          float v[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            bi[j] = __float_as_uint(a.scale * fmaf(since, __uint_as_float(bx[j]), __uint_as_float(bi[j])));
+          for (int j = 0; j < 16; j += 2) {
+            const F32x2 p = f32x2_fma(f32x2(__uint_as_float(bx[j]), __uint_as_float(bx[j + 1])), ss,
+                                      f32x2_mul(f32x2(__uint_as_float(bi[j]), __uint_as_float(bi[j + 1])), sc));
+            f32x2_split(p, v[j], v[j + 1]);
+          }
           if (r < nv) {
+            uint32_t w[8];
             if (a.out_f32) {
-              float* dst = static_cast<float*>(a.out) + o + c;
 #pragma unroll
-              for (int j = 0; j < 32; j += 8) st_global_32(dst + j, bi + j);
+              for (int h = 0; h < 16; h += 8) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[h + j]);
+                st_global_32(static_cast<float*>(a.out) + o + c + h, w);
+              }
             } else {
-              bf16* dst = static_cast<bf16*>(a.out) + o + c;
-              uint32_t w[16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(__uint_as_float(bi[2 * j]), __uint_as_float(bi[2 * j + 1]));
-              st_global_32(dst, w);
-              st_global_32(dst + 16, w + 8);
+              for (int j = 0; j < 8; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+              st_global_32(static_cast<bf16*>(a.out) + o + c, w);
             }
           }
           __syncwarp();
@@ -396,139 +519,125 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
       }
     }
   } else {
+    registers_grow<kLinearStateRegs>();
     // ---------------- state: lane = column of Z (B of them), two threads per lane, half of S's other side each
-    const int quarter = warp & 3, half = (warp - 2 - kLinearRowWarps) >> 2;
-    const int r = quarter * 32 + lane, tid = threadIdx.x - 64 - 32 * kLinearRowWarps;
+    const int quarter = warp & 3, half = (warp - 12) >> 2, r = quarter * 32 + lane, tid = threadIdx.x - 384;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const bool holds = quarter * 32 < B;    // (64 columns: the upper lanes of tensor memory are not part of S)
     constexpr int NC = A / 2;
     const int c0 = half * NC;
     int head = -1;
     float g2 = 0.f;
-    // where element (row of A: c0 + j, column r) of state number `n` of an array lies
-    auto element = [&](int64_t n, bool transposed, int j) {
-      return n * (A * B) + (transposed ? static_cast<int64_t>(r) * A + c0 + j : static_cast<int64_t>(c0 + j) * B + r);
+    float S[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) S[j] = 0.f;
+    // state number `n` of an array: element (row of A: c0 + j, column r), j up to NC
+    auto load_state = [&](const float* from, int64_t n, bool transposed, float mul) {
+      const float* p = from + n * (A * B) + (transposed ? static_cast<int64_t>(r) * A + c0 : static_cast<int64_t>(c0) * B + r);
+      const int step = transposed ? 1 : B;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) S[j] = p[j * step] * mul;
     };
-    for (int t = 0; t < count && !failed; ++t, it.next(a)) {
-      const uint32_t par = t & 1;
-      const int st = t % NS, place = it.place(a), nv = it.valid(place);
-      if (it.head != head) {
-        head = it.head;
-        g2 = decay_log2(a, head);
-      }
-      const int64_t state = static_cast<int64_t>(it.n) * a.heads + head;
-      const float decay = exp2f(g2 * static_cast<float>(nv - 1 + it.first_decay(a)));
-      if (t >= 1 && !mbar_wait_warp(s_full, par ^ 1, abort_flag)) { failed = true; break; }
-      tc_fence_after();
-      if (holds) {
-        const float* from = PIECE ? nullptr : it.c == 0 ? a.s_in : mid && t == 0 ? args.slots : nullptr;
-        const bool fresh = PIECE ? t == 0 : it.c == 0 || (mid && t == 0);
+    auto store_state = [&](float* to, int64_t n, bool transposed, float mul) {
+      float* p = to + n * (A * B) + (transposed ? static_cast<int64_t>(r) * A + c0 : static_cast<int64_t>(c0) * B + r);
+      const int step = transposed ? 1 : B;
 #pragma unroll
-        for (int c = 0; c < NC; c += 32) {
-          uint32_t v[32];
-          if (!fresh) {
-            tmem_ld32(tmem + lane_off + c0 + c, v);
-            tmem_ld_wait();
-          } else if (from == nullptr) {
+      for (int j = 0; j < NC; ++j) p[j * step] = S[j] * mul;
+    };
+    // S <- S * x + D * y
+    auto take = [&](uint32_t d, float x, float y) {
+      const F32x2 xx = f32x2(x, x), yy = f32x2(y, y);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0;
-          } else {
-            const bool own = it.c == 0;   // the caller's state, or what the CTA before this one has left
-            const float mul = own ? a.in_mul : 1.f;
-            const int64_t n = own ? state : blockIdx.x - 1;
-            const bool tr = own ? a.s_in_t : args.slots_t;
+      for (int c = 0; c < NC; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(tmem + lane_off + d + c0 + c, v);
+        tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(from[element(n, tr, c + j)] * mul);
-          }
-          if (!PIECE) {
-            // (K-major, 128-byte swizzle: row r of 128-byte rows of 64 columns)
-            const uint32_t row = base + SM::kS + ((c0 + c) >> 6) * kSBox + r * 128;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(__uint_as_float(v[g * 8 + 2 * e]), __uint_as_float(v[g * 8 + 2 * e + 1]));
-              const uint32_t unit = (((c0 + c) & 63) >> 3) + g;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((unit ^ (r & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                           "r"(w[3])
-                           : "memory");
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * decay);
-          tmem_st32(tmem + lane_off + c0 + c, v);
+        for (int j = 0; j < 16; j += 2) {
+          const F32x2 s = f32x2_fma(f32x2(S[c + j], S[c + j + 1]), xx, f32x2_mul(f32x2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), yy));
+          f32x2_split(s, S[c + j], S[c + j + 1]);
         }
-        tmem_st_wait();
       }
-      if (!PIECE) {
+    };
+    if constexpr (PIECE) {
+      int behind = 0;   // tokens of these tiles behind tile t
+      for (int t = 0; t < count && !failed; ++t, advance()) {
+        if (it.head != head) {
+          head = it.head;
+          g2 = decay_log2(a, head);
+        }
+        if (!mbar_wait_warp(&d_full[t & 1], (t >> 1) & 1, abort_flag)) { failed = true; break; }
+        tc_fence_after();
+        if (holds) take((t & 1) * kG, 1.f, exp2f(g2 * static_cast<float>(behind)));
+        behind += it.valid(it.place(a));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&d_read[t & 1]);
+      }
+      if (!failed && count > 0 && holds) store_state(args.slots, blockIdx.x, args.slots_t, 1.f);
+    } else {
+      float decay = 1.f;        // of the tile before
+      bool last = false;        // it was its sequence's last
+      int64_t state = 0;        // whose number
+      for (int t = 0;; ++t) {
+        const uint32_t par = t & 1;
+        if (t >= 1) {
+          if (!mbar_wait_warp(&d_full[0], par ^ 1, abort_flag)) { failed = true; break; }
+          tc_fence_after();
+          if (holds) {
+            take(0, decay, 1.f);
+            if (last && a.s_out != nullptr) store_state(a.s_out, state, a.s_out_t, a.out_mul * (a.reverse ? exp2f(g2) : 1.f));
+          }
+          advance();
+        }
+        if (t >= count || failed) break;
+        const int place = it.place(a), nv = it.valid(place);
+        if (it.head != head) {
+          head = it.head;
+          g2 = decay_log2(a, head);
+        }
+        state = static_cast<int64_t>(it.n) * a.heads + head;
+        last = it.c + 1 == it.tiles;
+        decay = exp2f(g2 * static_cast<float>(nv - 1 + it.first_decay(a)));
+        if (holds) {
+          if (it.c == 0) {
+            if (a.s_in != nullptr) {
+              load_state(a.s_in, state, a.s_in_t, a.in_mul);
+            } else {
+#pragma unroll
+              for (int j = 0; j < NC; ++j) S[j] = 0.f;
+            }
+          } else if (mid && t == 0) {   // what the CTA before this one has left
+            load_state(args.slots, blockIdx.x - 1, args.slots_t, 1.f);
+          }
+          // the copy (K-major, 128-byte swizzle: row r of 128-byte rows of 64 columns)
+          const uint32_t row = base + SM::kS + (c0 >> 6) * kSBox + r * 128;
+#pragma unroll
+          for (int g = 0; g < NC / 8; ++g) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(S[g * 8 + 2 * e], S[g * 8 + 2 * e + 1]);
+            const uint32_t unit = ((c0 & 63) >> 3) + g;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((unit ^ (r & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                         "r"(w[3])
+                         : "memory");
+          }
+        }
         tc_fence_before();
         fence_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_ready);
-      }
-      // Y -> pieces: row j of the tile decays until the tile's end (in the order of the walk); two threads a row
-      const int j = tid & 127, part = tid >> 7;
-      const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : nv - 1 - j));
-      if (!mbar_wait_warp(&xy_full[st], (t / NS) & 1, abort_flag) || (!PIECE && !mbar_wait_warp(x_done, par, abort_flag))) {
-        failed = true;
-        break;
-      }
-      const uint32_t x = base + st * SM::kStage, y = x + SM::kXY, s = base + SM::kS;
-#pragma unroll 4
-      for (int i = 0; i < A / 16; ++i) {
-        const int unit = part * (A / 16) + i;
-        const uint32_t off = (unit >> 3) * kBox + j * 128 + (((unit & 7) ^ (j & 7)) << 4);
-        uint4 u;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(y + off));
-        float v[8];
-        unpack_bf16x8(u, v);
-        uint32_t w[3][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float p0 = j < nv ? v[2 * e] * f : 0.f, p1 = j < nv ? v[2 * e + 1] * f : 0.f;
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            w[k][e] = pack_bf16x2(p0, p1);
-            p0 -= __uint_as_float(w[k][e] << 16);
-            p1 -= __uint_as_float(w[k][e] & 0xFFFF0000u);
-          }
+        // the pieces of Y, once G has used it (the third: once X S has used the copy)
+        const int j = tid & 127;
+        const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
+        if (!mbar_wait_warp(&xy_full[t % NS], (t / NS) & 1, abort_flag) || !mbar_wait_warp(three ? x_done : g_full, par, abort_flag)) {
+          failed = true;
+          break;
         }
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-          if (k < pieces)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((k == 0 ? y : k == 1 ? x : s) + off), "r"(w[k][0]), "r"(w[k][1]),
-                         "r"(w[k][2]), "r"(w[k][3])
-                         : "memory");
-      }
-      if (PIECE && nv < 128 && a.cu != nullptr) {
-        if (!mbar_wait_warp(&z_full[st], (t / NS) & 1, abort_flag)) { failed = true; break; }
-        for (int i = tid; i < (128 - nv) * (B / 8); i += 256) {
-          const int row = nv + i / (B / 8), u = i % (B / 8);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(y + SM::kXY + (u >> 3) * kBox + row * 128 + (u & 7) * 16), "r"(0) : "memory");
-        }
-      }
-      tc_fence_before();
-      fence_async_proxy();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(y_ready);
-      // the state behind the sequence, or behind this CTA's part of it
-      float* const to = PIECE ? (t + 1 == count ? args.slots : nullptr) : it.c + 1 == it.tiles ? a.s_out : nullptr;
-      if (to != nullptr) {
-        if (!mbar_wait_warp(s_full, par, abort_flag)) { failed = true; break; }
-        tc_fence_after();
-        if (holds) {
-          const float mul = PIECE ? 1.f : a.out_mul * (a.reverse ? exp2f(g2) : 1.f);
-          const int64_t n = PIECE ? blockIdx.x : state;
-          const bool tr = PIECE ? args.slots_t : a.s_out_t;
-#pragma unroll
-          for (int c = 0; c < NC; c += 32) {
-            uint32_t v[32];
-            tmem_ld32(tmem + lane_off + c0 + c, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) to[element(n, tr, c + e)] = __uint_as_float(v[e]) * mul;
-          }
-        }
+        linear_decay_rows<A>(y_of(t), base + SM::kLow, three ? base + SM::kS : 0, tid, f, j < nv);
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(y_ready);
       }
     }
   }
@@ -545,34 +654,44 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
-// What every CTA's first sequence begins with: slots[i] <- slots[i] + mult_i * (state before CTA i's part), in order of i.  One element
-// of the state per thread; 16 shares are fetched at a time.
+// What every CTA's first sequence begins with: along a sequence, slots[i] <- slots[i] + mult_i * (state before CTA i's part).  A block
+// takes 512 elements of the sequence whose first share is CTA blockIdx.y's; shares are fetched eight at a time.
 constexpr int kLinearMaxCtas = 256;
-__global__ void __launch_bounds__(128) linear_carry_kernel(const float* __restrict__ s_in, int32_t s_in_t, float in_mul, float* slots,
+__global__ void __launch_bounds__(128) linear_carry_kernel(const float* __restrict__ s_in, int32_t s_in_t, float in_mul, float* __restrict__ slots,
                                                            const LinearPiece* __restrict__ pieces, int32_t ctas, int32_t A, int32_t B) {
   __shared__ LinearPiece info[kLinearMaxCtas];
   griddep_launch_dependents();
   griddep_wait();
-  for (int i = threadIdx.x; i < ctas; i += 128) info[i] = pieces[i];
+  const int i0 = blockIdx.y;
+  if (!pieces[i0].goes_on || pieces[i0].inherits) return;
+  for (int i = i0 + threadIdx.x; i < ctas; i += 128) info[i] = pieces[i];
   __syncthreads();
-  const int e = blockIdx.x * 128 + threadIdx.x, size = A * B;    // element (e / B, e % B)
-  const int at = s_in_t ? (e % B) * A + e / B : e;
-  float carry = 0.f;
-  for (int i0 = 0; i0 + 1 < ctas; i0 += 16) {
-    float mine[16], before[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int i = i0 + k;
-      const bool on = i + 1 < ctas && info[i].goes_on;
-      mine[k] = on ? slots[static_cast<int64_t>(i) * size + e] : 0.f;
-      before[k] = on && !info[i].inherits && s_in != nullptr ? s_in[static_cast<int64_t>(info[i].state) * size + at] * in_mul : 0.f;
+  const int e = (blockIdx.x * 128 + threadIdx.x) * 4, size = A * B;    // elements (e / B, e % B) and on
+  float4 carry = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (s_in != nullptr) {
+    const float* from = s_in + static_cast<int64_t>(info[i0].state) * size;
+    if (!s_in_t) {
+      carry = *reinterpret_cast<const float4*>(from + e);
+    } else {
+      const float* p = from + (e % B) * A + e / B;
+      carry = make_float4(p[0], p[A], p[2 * A], p[3 * A]);
     }
+    carry.x *= in_mul; carry.y *= in_mul; carry.z *= in_mul; carry.w *= in_mul;
+  }
+  int last = i0;   // the sequence's last share
+  while (last + 1 < ctas && info[last + 1].goes_on && info[last + 1].inherits) ++last;
+  float4* const at = reinterpret_cast<float4*>(slots + e);
+  const int64_t step = size / 4;
+  for (int i = i0; i <= last; i += 8) {
+    float4 v[8];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int i = i0 + k;
-      if (i + 1 >= ctas || !info[i].goes_on) continue;
-      carry = fmaf(info[i].mult, info[i].inherits ? carry : before[k], mine[k]);
-      slots[static_cast<int64_t>(i) * size + e] = carry;
+    for (int k = 0; k < 8; ++k) v[k] = at[min(i + k, last) * step];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (i + k > last) break;
+      const float m = info[i + k].mult;
+      carry = make_float4(fmaf(m, carry.x, v[k].x), fmaf(m, carry.y, v[k].y), fmaf(m, carry.z, v[k].z), fmaf(m, carry.w, v[k].w));
+      at[(i + k) * step] = carry;
     }
   }
 }
