@@ -2054,7 +2054,9 @@ int linear_check(const lact_linear_config* c, const void* cu) {
   if (c->batch < 1 || c->tokens < 1 || c->heads < 1 || c->kv_heads < 1 || c->heads % c->kv_heads != 0) return LACT_ERR_SHAPE;
   if (c->batch > 65535 || c->heads > 65535 || c->tokens > (1ll << 30) || c->sequences < 0 || c->sequences > (1ll << 24)) return LACT_ERR_SHAPE;
   if ((c->sequences > 0) != (cu != nullptr) || (cu != nullptr && c->batch != 1)) return LACT_ERR_CONFIG;
-  if ((c->sequences > 0 ? c->sequences : c->batch) * c->heads > (1ll << 30)) return LACT_ERR_SHAPE;
+  // (sequence, head)s and their tiles of 128 tokens are counted in 31 bits
+  const int64_t n = c->sequences > 0 ? c->sequences : c->batch;
+  if (n * c->heads > (1ll << 30) || ((c->tokens + 127) / 128 * c->batch + n) * c->heads > (1ll << 30)) return LACT_ERR_SHAPE;
   if (!(c->scale > -INFINITY && c->scale < INFINITY) || c->scale == 0.f) return LACT_ERR_CONFIG;
   return LACT_OK;
 }
@@ -2110,6 +2112,9 @@ int launch_linear_chunks(const LinearChunkArgs& a, int ctas, cudaStream_t st) {
     std::lock_guard<std::mutex> lock(mu);
     if (dev >= 64 || !configured[dev]) {
       LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      cudaFuncAttributes f;   // the warpgroups share out what the launch has: fewer, and one of them would wait for good
+      LACT_CUDA(cudaFuncGetAttributes(&f, kernel));
+      if (f.numRegs != kLinearLaunchRegs) return LACT_ERR_CONFIG;
       if (dev < 64) configured[dev] = true;
     }
   }
@@ -2138,7 +2143,7 @@ int linear_run(const lact_linear_config* c, const LinearArgs& a, int64_t A, int6
   LACT_TRY(encode_map_heads(&k.x, a.x, c->batch, c->tokens, c->heads / a.x_share, A, a.x_ts, a.x_bs));
   LACT_TRY(encode_map_heads(&k.y, a.y, c->batch, c->tokens, c->heads / a.y_share, A, a.y_ts, a.y_bs));
   LACT_TRY(encode_map_heads(&k.z, a.z, c->batch, c->tokens, c->heads / a.z_share, B, a.z_ts, a.z_bs));
-  k.per = p.per;
+  k.per = static_cast<uint32_t>(p.per);
   k.slots = static_cast<float*>(slots);
   k.pieces = reinterpret_cast<LinearPiece*>(static_cast<uint8_t*>(slots) + static_cast<size_t>(p.ctas) * A * B * 4);
   k.slots_t = carried;

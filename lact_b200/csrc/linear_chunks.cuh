@@ -3,7 +3,7 @@
 //   S <- lambda^n S + D,  D = (diag(lambda^(n-1-j)) Y)^T Z                             (backwards in time: the mirror image).
 // A CTA takes a run of tiles of consecutive (sequence, head)s and reads every tile once:
 //   warp 0       loads the tiles of X, Y, Z through a ring of stages;
-//   warp 1       issues the products: G(t + 1) as soon as P(t) has been used and the tile is there;
+//   warp 1       issues the products: X S, P Z, D and the next tile's G (before D if D has to wait);
 //   warps 4-11   ("rows") G -> P (to tensor memory, the first operand of P Z from there), later both parts of the output -> memory;
 //   warps 12-19  ("state") keep S in registers: S <- lambda^n S + D, its copy in bf16 to shared memory for X S, then
 //                Y -> diag(lambda^(n-1-j)) Y in bf16 pieces, the first in place.
@@ -30,7 +30,7 @@ struct LinearPiece {
 struct LinearChunkArgs {
   LinearArgs a;
   CUtensorMap x, y, z;   // 4-D maps (feature, token, head, entry), box {64, 128, 1, 1}
-  int64_t per;           // tiles a CTA takes; packed sequences: 0, as many as make the CTAs even
+  uint32_t per;          // tiles a CTA takes; packed sequences: 0, as many as make the CTAs even
   float* slots;          // [CTA] states: what the next CTA's sequence begins with ([A][B], or [B][A] if slots_t)
   LinearPiece* pieces;   // [CTA]
   int32_t slots_t;
@@ -63,43 +63,43 @@ struct LinearTiles {
   LinearSpan s;
   static __device__ __forceinline__ int tiles_of(int len) { return (len + 127) >> 7; }
   // all tiles; every lane of a warp takes part
-  static __device__ __forceinline__ int64_t total(const LinearArgs& a) {
-    if (a.cu == nullptr) return static_cast<int64_t>(a.sequences) * a.heads * tiles_of(a.L);
-    int64_t sum = 0;
+  static __device__ __forceinline__ uint32_t total(const LinearArgs& a) {   // (the host has seen to it that 31 bits are enough)
+    if (a.cu == nullptr) return static_cast<uint32_t>(a.sequences) * a.heads * tiles_of(a.L);
+    uint32_t sum = 0;
     for (int n = threadIdx.x & 31; n < a.sequences; n += 32) sum += tiles_of(linear_span(a, n).len);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     return sum * a.heads;
   }
   // tile number f (< total); every lane of a warp takes part
-  __device__ __forceinline__ void seek(const LinearArgs& a, int64_t f) {
+  __device__ __forceinline__ void seek(const LinearArgs& a, uint32_t f) {
     if (a.cu == nullptr) {
       tiles = tiles_of(a.L);
-      c = static_cast<int>(f % tiles);
-      f /= tiles;
-      head = static_cast<int>(f % a.heads);
-      n = static_cast<int>(f / a.heads);
+      const uint32_t chain = f / static_cast<uint32_t>(tiles);
+      c = f - chain * tiles;
+      n = chain / static_cast<uint32_t>(a.heads);
+      head = chain - n * a.heads;
       s = linear_span(a, n);
       return;
     }
     const int lane = threadIdx.x & 31;
     for (int n0 = 0;; n0 += 32) {
       const int mine = n0 + lane < a.sequences ? tiles_of(linear_span(a, n0 + lane).len) : 0;
-      int upto = mine;   // tiles of one head (fewer than 2^24 + 2^24 in all)
+      uint32_t upto = mine;   // tiles of one head
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
         if (lane >= o) upto += v;
       }
-      const uint32_t past = __ballot_sync(0xFFFFFFFFu, static_cast<int64_t>(upto) * a.heads > f);
+      const uint32_t past = __ballot_sync(0xFFFFFFFFu, upto * a.heads > f);
       if (past != 0) {
         const int w = __ffs(past) - 1;
         n = n0 + w;
         tiles = __shfl_sync(0xFFFFFFFFu, mine, w);
-        f -= static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, upto, w) - tiles) * a.heads;
+        f -= (__shfl_sync(0xFFFFFFFFu, upto, w) - tiles) * a.heads;
         break;
       }
-      f -= static_cast<int64_t>(__shfl_sync(0xFFFFFFFFu, upto, 31)) * a.heads;
+      f -= __shfl_sync(0xFFFFFFFFu, upto, 31) * a.heads;
       if (n0 + 32 >= a.sequences) {   // (f is not below the total: cannot be)
         n = a.sequences - 1;
         tiles = 1;
@@ -107,8 +107,8 @@ struct LinearTiles {
         break;
       }
     }
-    head = static_cast<int>(f / tiles);
-    c = static_cast<int>(f % tiles);
+    head = f / static_cast<uint32_t>(tiles);
+    c = f - head * tiles;
     s = linear_span(a, n);
   }
   __device__ __forceinline__ void next(const LinearArgs& a) {
@@ -128,6 +128,11 @@ struct LinearTiles {
   __device__ __forceinline__ int first_decay(const LinearArgs& a) const { return a.reverse && c == 0 ? 0 : 1; }
 };
 
+struct LinearStart {
+  LinearTiles it;
+  int count, mid;
+};
+
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -140,39 +145,48 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Rows 32 * quarter + lane of a tile of Y times the decay until the tile's end, as bf16 pieces: the first in place, the second to `low`,
-// a third to `lowest` (0: none).  Two threads a row; rows past the sequence become zeros.
+// Rows of a tile of Y times their decay until the tile's end, as bf16 pieces: the first in place, the second to `low`, a third to
+// `lowest` (0: none).  Thread j of 256 works on row j % 128; rows past the sequence become zeros.  (Four loads before the first
+// store: one after the other, they took twice as long.)
 template <int A>
 __device__ __forceinline__ void linear_decay_rows(uint32_t y, uint32_t low, uint32_t lowest, int tid, float f, bool real) {
   constexpr uint32_t kBox = 128 * 128;
-  const int j = tid & 127, part = tid >> 7;
+  constexpr int kUnits = A / 16, kAtOnce = 4;   // 16-byte units a thread; loaded before the first is stored
+  const int j = tid & 127, first = (tid >> 7) * kUnits;
   const F32x2 ff = f32x2(f, f), minus = f32x2(-1.f, -1.f);
-#pragma unroll 4
-  for (int i = 0; i < A / 16; ++i) {
-    const int unit = part * (A / 16) + i;
-    const uint32_t off = (unit >> 3) * kBox + j * 128 + (((unit & 7) ^ (j & 7)) << 4);
-    uint32_t u[4], w[4], l[4], m[4];
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(y + off));
-    auto pair = [](uint32_t b) { return f32x2(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)); };
-    auto round = [](F32x2 p) {
-      float p0, p1;
-      f32x2_split(p, p0, p1);
-      return pack_bf16x2(p0, p1);
-    };
+  auto pair = [](uint32_t b) { return f32x2(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)); };
+  auto round = [](F32x2 p) {
+    float p0, p1;
+    f32x2_split(p, p0, p1);
+    return pack_bf16x2(p0, p1);
+  };
+#pragma unroll 1
+  for (int i = 0; i < kUnits; i += kAtOnce) {
+    uint32_t u[kAtOnce][4], off[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      F32x2 p = f32x2_mul(pair(real ? u[e] : 0u), ff);
-      w[e] = round(p);
-      p = f32x2_fma(pair(w[e]), minus, p);
-      l[e] = round(p);
-      if (lowest != 0) m[e] = round(f32x2_fma(pair(l[e]), minus, p));
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int unit = first + i + k;
+      off[k] = (unit >> 3) * kBox + j * 128 + (((unit & 7) ^ (j & 7)) << 4);
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[k][0]), "=r"(u[k][1]), "=r"(u[k][2]), "=r"(u[k][3]) : "r"(y + off[k]));
     }
-    auto put = [&](uint32_t to, const uint32_t (&v)[4]) {
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + off), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-    };
-    put(y, w);
-    put(low, l);
-    if (lowest != 0) put(lowest, m);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      uint32_t w[4], l[4], m[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        F32x2 p = f32x2_mul(pair(real ? u[k][e] : 0u), ff);
+        w[e] = round(p);
+        p = f32x2_fma(pair(w[e]), minus, p);
+        l[e] = round(p);
+        if (lowest != 0) m[e] = round(f32x2_fma(pair(l[e]), minus, p));
+      }
+      auto put = [&](uint32_t to, const uint32_t (&v)[4]) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + off[k]), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+      };
+      put(y, w);
+      put(low, l);
+      if (lowest != 0) put(lowest, m);
+    }
   }
 }
 // Rows `from` to 127 of a tile of Z become zeros (256 threads).
@@ -184,10 +198,18 @@ __device__ __forceinline__ void linear_clear_rows(uint32_t z, int from, int tid)
   }
 }
 
-constexpr int kLinearThreads = 640;   // a warpgroup for loads and products, two for the rows, two for the state
-// registers per thread of each: 128 x 64 + 256 x 80 + 256 x 128 = 640 x 96
+constexpr int kLinearThreads = 640;   // a warpgroup for loads and products, two for the rows, two for the state and the pieces of Y
+// registers per thread of each; together what the launch has.  (Nothing may spill: the little L1 beside 227 KB of shared memory misses,
+// and with 7 warpgroups of fewer registers a tile's bookkeeping alone waited 1700 clocks for it.)
 constexpr int kLinearIssueRegs = 64, kLinearRowRegs = 80, kLinearStateRegs = 128, kLinearLaunchRegs = 96;
 static_assert(kLinearIssueRegs + 2 * kLinearRowRegs + 2 * kLinearStateRegs <= 5 * kLinearLaunchRegs, "the shares of the registers");
+
+// A warpgroup's own number of registers: `dec` may not name more than the launch has, `inc` not less.
+template <int N>
+__device__ __forceinline__ void linear_registers() {
+  if constexpr (N > kLinearLaunchRegs) registers_grow<N>();
+  else registers_shrink<N>();
+}
 
 template <int A, int B, bool PIECE>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const __grid_constant__ LinearChunkArgs args) {
@@ -214,6 +236,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   uint64_t* d_read = bars + 21;         // [2] PIECE: an arrival per state warp
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  LinearStart* start = reinterpret_cast<LinearStart*>(tmem_slot + 2);
   const LinearArgs& a = args.a;
 
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
@@ -241,35 +264,37 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   griddep_launch_dependents();
   griddep_wait();
 
-  // this CTA's tiles
-  const int64_t total = LinearTiles::total(a);
-  const int64_t per = args.per > 0 ? args.per : (total + gridDim.x - 1) / gridDim.x;
-  const int64_t first = blockIdx.x * per, end = min(first + per, total);
-  int count = end > first ? static_cast<int>(end - first) : 0;
-  LinearTiles it;
-  bool mid = false;       // the first tile goes on with a sequence that the CTA before this one has begun
-  if (count > 0) {
-    if (PIECE) {   // the tiles of the last one's sequence, from the last to the first
-      it.seek(a, end - 1);
-      const bool goes_on = it.c + 1 < it.tiles;
-      const int back = min(it.c, count - 1);
-      mid = it.c - back > 0;
-      if (threadIdx.x == 0) {
-        LinearTiles at = it;
+  // This CTA's tiles: worked out by one warp (by every warp, its values lay on the stack for the rest of the kernel)
+  if (warp == 2) {
+    const uint32_t total = LinearTiles::total(a);
+    const uint32_t per = args.per > 0 ? args.per : (total + gridDim.x - 1) / gridDim.x;
+    const uint32_t first = blockIdx.x * per, end = min(first + per, total);
+    LinearStart w{};
+    w.count = end > first ? static_cast<int>(end - first) : 0;
+    if (w.count > 0) {
+      w.it.seek(a, PIECE ? end - 1 : first);
+      w.mid = w.it.c > 0;
+      if (PIECE) {   // the tiles of the last one's sequence, from the last to the first
+        const bool goes_on = w.it.c + 1 < w.it.tiles;
+        const int back = min(w.it.c, w.count - 1);
+        LinearTiles at = w.it;
         at.c -= back;
         // tokens of these tiles: all whole, but for the first of a walk backwards
-        const int tokens = (back + 1) * 128 - (a.reverse && !mid ? 128 - at.valid(at.place(a)) : 0);
-        args.pieces[blockIdx.x] = {goes_on, mid, it.n * a.heads + it.head,
-                                   exp2f(decay_log2(a, it.head) * static_cast<float>(tokens - 1 + at.first_decay(a)))};
+        const int tokens = (back + 1) * 128 - (a.reverse && at.c == 0 ? 128 - at.valid(at.place(a)) : 0);
+        if (lane == 0)
+          args.pieces[blockIdx.x] = {goes_on, at.c > 0, w.it.n * a.heads + w.it.head,
+                                     exp2f(decay_log2(a, w.it.head) * static_cast<float>(tokens - 1 + at.first_decay(a)))};
+        w.count = goes_on ? back + 1 : 0;
       }
-      count = goes_on ? back + 1 : 0;
-    } else {
-      it.seek(a, first);
-      mid = it.c > 0;
+    } else if (PIECE && lane == 0) {
+      args.pieces[blockIdx.x] = {0, 0, 0, 0.f};
     }
-  } else if (PIECE && threadIdx.x == 0) {
-    args.pieces[blockIdx.x] = {0, 0, 0, 0.f};
+    if (lane == 0) *start = w;
   }
+  __syncthreads();
+  const int count = start->count;
+  const bool mid = start->mid != 0;    // the first tile goes on with a sequence that the CTA before this one has begun
+  LinearTiles it = start->it;
   auto advance = [&]() {
     if (PIECE) --it.c;
     else it.next(a);
@@ -281,7 +306,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   auto z_of = [&](int t) { return PIECE ? y_of(t) + SM::kXY : base + SM::z(t); };
 
   if (warp < 4) {
-    registers_shrink<kLinearIssueRegs>();
+    linear_registers<kLinearIssueRegs>();
     if (warp == 0) {
       const uint32_t leader = elect_leader();
       for (int t = 0; t < count && !failed; ++t, advance()) {
@@ -340,7 +365,9 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
             umma_bf16_ta_if(leader, tmem + kO, tmem + kG + (k >> 1) * 32 + (k & 1) * 8, desc.at((z + k * 2048) >> 4), idesc_o, k != 0);
           umma_commit_if(leader, o_full);
           g_next = t + 1 < count;
-          if (g_next && __all_sync(0xFFFFFFFFu, mbar_test(&xy_full[(t + 1) % NS], ((t + 1) / NS) & 1))) {
+          // D before the next G, if its operands are there: what the next tile waits for comes behind D
+          if (g_next && !__all_sync(0xFFFFFFFFu, mbar_test(y_ready, par)) &&
+              __all_sync(0xFFFFFFFFu, mbar_test(&xy_full[(t + 1) % NS], ((t + 1) / NS) & 1))) {
             issue_g(t + 1);
             g_next = false;
           }
@@ -366,7 +393,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
       }
     }
   } else if (warp < 12) {
-    registers_shrink<kLinearRowRegs>();
+    linear_registers<kLinearRowRegs>();
     // ---------------- rows: two threads per row of the tile (tensor-memory lane), 64 columns of G and half of the output each
     const int quarter = warp & 3, half = (warp - 4) >> 2, r = quarter * 32 + lane, tid = threadIdx.x - 128;
     int head = -1;
@@ -489,26 +516,25 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           tmem_ld16(tmem + lane_off + kO + half * (B / 2) + c, bi);
           tmem_ld16(tmem + lane_off + kOx + half * (B / 2) + c, bx);
           tmem_ld_wait();
-          float v[16];
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             const F32x2 p = f32x2_fma(f32x2(__uint_as_float(bx[j]), __uint_as_float(bx[j + 1])), ss,
                                       f32x2_mul(f32x2(__uint_as_float(bi[j]), __uint_as_float(bi[j + 1])), sc));
-            f32x2_split(p, v[j], v[j + 1]);
+            float p0, p1;
+            f32x2_split(p, p0, p1);
+            if (a.out_f32) {
+              bi[j] = __float_as_uint(p0);
+              bi[j + 1] = __float_as_uint(p1);
+            } else {
+              bi[j / 2] = pack_bf16x2(p0, p1);
+            }
           }
           if (r < nv) {
-            uint32_t w[8];
             if (a.out_f32) {
-#pragma unroll
-              for (int h = 0; h < 16; h += 8) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[h + j]);
-                st_global_32(static_cast<float*>(a.out) + o + c + h, w);
-              }
+              st_global_32(static_cast<float*>(a.out) + o + c, bi);
+              st_global_32(static_cast<float*>(a.out) + o + c + 8, bi + 8);
             } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-              st_global_32(static_cast<bf16*>(a.out) + o + c, w);
+              st_global_32(static_cast<bf16*>(a.out) + o + c, bi);
             }
           }
           __syncwarp();
@@ -519,7 +545,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
       }
     }
   } else {
-    registers_grow<kLinearStateRegs>();
+    linear_registers<kLinearStateRegs>();
     // ---------------- state: lane = column of Z (B of them), two threads per lane, half of S's other side each
     const int quarter = warp & 3, half = (warp - 12) >> 2, r = quarter * 32 + lane, tid = threadIdx.x - 384;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
@@ -627,7 +653,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         fence_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_ready);
-        // the pieces of Y, once G has used it (the third: once X S has used the copy)
+        // the pieces of Y, once G has used it (a third takes the place of the copy of S: once X S has used that)
         const int j = tid & 127;
         const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
         if (!mbar_wait_warp(&xy_full[t % NS], (t / NS) & 1, abort_flag) || !mbar_wait_warp(three ? x_done : g_full, par, abort_flag)) {
