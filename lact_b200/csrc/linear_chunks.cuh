@@ -4,9 +4,11 @@
 // A CTA takes a run of tiles of consecutive (sequence, head)s and reads every tile once:
 //   warp 0       loads the tiles of X, Y, Z through a ring of stages;
 //   warp 1       issues the products: X S, P Z, D and the next tile's G (before D if D has to wait);
-//   warps 4-11   ("rows") G -> P (to tensor memory, the first operand of P Z from there), later both parts of the output -> memory;
-//   warps 12-19  ("state") keep S in registers: S <- lambda^n S + D, its copy in bf16 to shared memory for X S, then
-//                Y -> diag(lambda^(n-1-j)) Y in bf16 pieces, the first in place.
+//   warps 4-19   ("rows") G -> P (to tensor memory, the first operand of P Z from there), Y -> diag(lambda^(n-1-j)) Y in bf16 pieces,
+//                the first in place, then both parts of the output -> memory;
+//   warps 20-27  ("state") keep S in registers: S <- lambda^n S + D, its copy in bf16 to shared memory for X S.
+// A tile is 131 KB at 128 features and arrives in 5700 clocks; the chain from one D to the next through these passes has to be shorter,
+// and what a warp does one instruction after the other takes 7 clocks each: hence many warps with little work, four threads a row.
 // Roundings: P and the copy of S to bf16, as operands of products whose sum is rounded to bf16 in the end.  S itself is added up in
 // fp32 (D alone is summed by the tensor core, which truncates: over a long sequence that would show): the decayed rows of Y are two
 // bf16 pieces (16 bits of the product; what is lost, 2^-17, is far below the copy's rounding), three (24 bits) where the last state
@@ -19,6 +21,13 @@
 #include "umma_gemm.cuh"
 
 namespace lact {
+
+constexpr int kLinearThreads = 896;   // a warpgroup for loads and products, four for the rows, two for the state
+constexpr int kLinearRowThreads = 512, kLinearRowWarps = 16;
+// registers per thread of each; together what the launch has.  (Nothing may spill: the little L1 beside 227 KB of shared memory misses,
+// and a tile's bookkeeping alone then waited 1700 clocks for it.)
+constexpr int kLinearIssueRegs = 32, kLinearRowRegs = 64, kLinearStateRegs = 104, kLinearLaunchRegs = 72;
+static_assert(kLinearIssueRegs + 4 * kLinearRowRegs + 2 * kLinearStateRegs <= 7 * kLinearLaunchRegs, "the shares of the registers");
 
 struct LinearPiece {
   int32_t goes_on;    // the CTA's last sequence goes on in the next CTA
@@ -48,7 +57,7 @@ struct LinearSmem {
   static constexpr uint32_t kS = kLow + kXY;        // copy of S; third piece of Y
   static constexpr uint32_t kBars = kS + kXY;
   static constexpr uint32_t kFactors = kBars + 256; // a table of 32 decays per row warp
-  static constexpr uint32_t kBytes = kFactors + 8 * 128;
+  static constexpr uint32_t kBytes = kFactors + kLinearRowWarps * 128;
   static_assert(kPieceStages * (kXY + kZ) <= kTiles, "the stages of the shares fit");
   // where X, Y, Z of the CTA's tile t lie
   static __device__ __forceinline__ uint32_t x(int t) { return kRing5 ? 3 * t % 5 * kXY : t % kStages * (2 * kXY + kZ); }
@@ -146,12 +155,12 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 }
 
 // Rows of a tile of Y times their decay until the tile's end, as bf16 pieces: the first in place, the second to `low`, a third to
-// `lowest` (0: none).  Thread j of 256 works on row j % 128; rows past the sequence become zeros.  (Four loads before the first
-// store: one after the other, they took twice as long.)
+// `lowest` (0: none).  Thread j of 512 works on row j % 128; rows past the sequence become zeros.  (All loads before the
+// first store: one after the other, they took twice as long.)
 template <int A>
 __device__ __forceinline__ void linear_decay_rows(uint32_t y, uint32_t low, uint32_t lowest, int tid, float f, bool real) {
   constexpr uint32_t kBox = 128 * 128;
-  constexpr int kUnits = A / 16, kAtOnce = 4;   // 16-byte units a thread; loaded before the first is stored
+  constexpr int kUnits = A / 32;   // 16-byte units a thread
   const int j = tid & 127, first = (tid >> 7) * kUnits;
   const F32x2 ff = f32x2(f, f), minus = f32x2(-1.f, -1.f);
   auto pair = [](uint32_t b) { return f32x2(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)); };
@@ -160,17 +169,16 @@ __device__ __forceinline__ void linear_decay_rows(uint32_t y, uint32_t low, uint
     f32x2_split(p, p0, p1);
     return pack_bf16x2(p0, p1);
   };
-#pragma unroll 1
-  for (int i = 0; i < kUnits; i += kAtOnce) {
-    uint32_t u[kAtOnce][4], off[kAtOnce];
+  {
+    uint32_t u[kUnits][4], off[kUnits];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int unit = first + i + k;
+    for (int k = 0; k < kUnits; ++k) {
+      const int unit = first + k;
       off[k] = (unit >> 3) * kBox + j * 128 + (((unit & 7) ^ (j & 7)) << 4);
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[k][0]), "=r"(u[k][1]), "=r"(u[k][2]), "=r"(u[k][3]) : "r"(y + off[k]));
     }
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
+    for (int k = 0; k < kUnits; ++k) {
       uint32_t w[4], l[4], m[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -189,20 +197,14 @@ __device__ __forceinline__ void linear_decay_rows(uint32_t y, uint32_t low, uint
     }
   }
 }
-// Rows `from` to 127 of a tile of Z become zeros (256 threads).
+// Rows `from` to 127 of a tile of Z become zeros.
 template <int B>
 __device__ __forceinline__ void linear_clear_rows(uint32_t z, int from, int tid) {
-  for (int i = tid; i < (128 - from) * (B / 8); i += 256) {
+  for (int i = tid; i < (128 - from) * (B / 8); i += kLinearRowThreads) {
     const int row = from + i / (B / 8), u = i % (B / 8);
     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(z + (u >> 3) * (128 * 128) + row * 128 + (u & 7) * 16), "r"(0) : "memory");
   }
 }
-
-constexpr int kLinearThreads = 640;   // a warpgroup for loads and products, two for the rows, two for the state and the pieces of Y
-// registers per thread of each; together what the launch has.  (Nothing may spill: the little L1 beside 227 KB of shared memory misses,
-// and with 7 warpgroups of fewer registers a tile's bookkeeping alone waited 1700 clocks for it.)
-constexpr int kLinearIssueRegs = 64, kLinearRowRegs = 80, kLinearStateRegs = 128, kLinearLaunchRegs = 96;
-static_assert(kLinearIssueRegs + 2 * kLinearRowRegs + 2 * kLinearStateRegs <= 5 * kLinearLaunchRegs, "the shares of the registers");
 
 // A warpgroup's own number of registers: `dec` may not name more than the launch has, `inc` not less.
 template <int N>
@@ -243,12 +245,12 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) { mbar_init(&xy_full[s], 1); mbar_init(&z_full[s], 1); mbar_init(&stage_empty[s], 1); }
     mbar_init(g_full, 1);
-    mbar_init(p_full, 8);
+    mbar_init(p_full, kLinearRowWarps);
     mbar_init(s_ready, 8);
     mbar_init(x_done, 1);
     mbar_init(o_full, 1);
-    mbar_init(o_empty, 8);
-    mbar_init(y_ready, 8);
+    mbar_init(o_empty, kLinearRowWarps);
+    mbar_init(y_ready, kLinearRowWarps);
     for (int s = 0; s < 2; ++s) { mbar_init(&d_full[s], 1); mbar_init(&d_read[s], 8); }
     *abort_flag = 0;
     fence_mbar_init();
@@ -392,10 +394,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         }
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 4 + kLinearRowWarps) {
     linear_registers<kLinearRowRegs>();
-    // ---------------- rows: two threads per row of the tile (tensor-memory lane), 64 columns of G and half of the output each
-    const int quarter = warp & 3, half = (warp - 4) >> 2, r = quarter * 32 + lane, tid = threadIdx.x - 128;
+    // ---------------- rows: four threads per row of the tile (tensor-memory lane), 32 columns of G and a quarter of the output each
+    const int quarter = warp & 3, cb = (warp - 4) >> 2, r = quarter * 32 + lane, tid = threadIdx.x - 128;
     int head = -1;
     float g2 = 0.f;
     if constexpr (PIECE) {   // the pieces of Y; the tiles' own end is where their decays count from
@@ -420,12 +422,12 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
       }
     } else {
       const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-      linear_zero_rest<B>(a, static_cast<int64_t>(blockIdx.x) * 256 + tid, static_cast<int64_t>(gridDim.x) * 256);
+      linear_zero_rest<B>(a, static_cast<int64_t>(blockIdx.x) * kLinearRowThreads + tid, static_cast<int64_t>(gridDim.x) * kLinearRowThreads);
       if (a.cu != nullptr && a.s_out != nullptr) {   // empty sequences keep their states
         const int64_t size = static_cast<int64_t>(a.heads) * (A * B / 4);
         for (int n = 0; n < a.sequences; ++n) {
           if (linear_span(a, n).len != 0) continue;
-          for (int64_t i = blockIdx.x * 256ll + tid; i < size; i += gridDim.x * 256ll)
+          for (int64_t i = static_cast<int64_t>(blockIdx.x) * kLinearRowThreads + tid; i < size; i += static_cast<int64_t>(gridDim.x) * kLinearRowThreads)
             reinterpret_cast<float4*>(a.s_out)[n * size + i] =
                 a.s_in != nullptr ? reinterpret_cast<const float4*>(a.s_in)[n * size + i] : make_float4(0.f, 0.f, 0.f, 0.f);
         }
@@ -443,9 +445,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         }
         if (!mbar_wait_warp(g_full, par, abort_flag)) { failed = true; break; }
         tc_fence_after();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int cb = half * 2 + i, c0 = cb * 32;
+        {
+          const int c0 = cb * 32;
           uint32_t w[16];
           if (a.reverse ? cb < quarter : cb > quarter) {
 #pragma unroll
@@ -504,17 +505,33 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full);
 
+        // the pieces of Y: in the place of those of the tile before, once D has used them (a third takes the place of the copy of S:
+        // once X S has used that)
+        {
+          const int j = tid & 127;
+          const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
+          if (!mbar_wait_warp(&xy_full[t % NS], (t / NS) & 1, abort_flag) || (t >= 1 && !mbar_wait_warp(&d_full[0], par ^ 1, abort_flag)) ||
+              (three && !mbar_wait_warp(x_done, par, abort_flag))) {
+            failed = true;
+            break;
+          }
+          linear_decay_rows<A>(y_of(t), base + SM::kLow, three ? base + SM::kS : 0, tid, f, j < nv);
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(y_ready);
+        }
+
         const int pos = a.reverse ? nv - 1 - r : r;
         const float since = a.scale * exp2f(g2 * static_cast<float>(max(pos, 0) + it.first_decay(a)));
         const F32x2 ss = f32x2(since, since), sc = f32x2(a.scale, a.scale);
-        const int64_t o = ((it.s.entry * static_cast<int64_t>(a.L) + it.s.first + place + r) * a.heads + head) * B + half * (B / 2);
+        const int64_t o = ((it.s.entry * static_cast<int64_t>(a.L) + it.s.first + place + r) * a.heads + head) * B + cb * (B / 4);
         if (!mbar_wait_warp(o_full, par, abort_flag)) { failed = true; break; }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < B / 2; c += 16) {
+        for (int c = 0; c < B / 4; c += 16) {
           uint32_t bi[16], bx[16];
-          tmem_ld16(tmem + lane_off + kO + half * (B / 2) + c, bi);
-          tmem_ld16(tmem + lane_off + kOx + half * (B / 2) + c, bx);
+          tmem_ld16(tmem + lane_off + kO + cb * (B / 4) + c, bi);
+          tmem_ld16(tmem + lane_off + kOx + cb * (B / 4) + c, bx);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
@@ -547,7 +564,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   } else {
     linear_registers<kLinearStateRegs>();
     // ---------------- state: lane = column of Z (B of them), two threads per lane, half of S's other side each
-    const int quarter = warp & 3, half = (warp - 12) >> 2, r = quarter * 32 + lane, tid = threadIdx.x - 384;
+    const int quarter = warp & 3, half = (warp - 4 - kLinearRowWarps) >> 2, r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const bool holds = quarter * 32 < B;    // (64 columns: the upper lanes of tensor memory are not part of S)
     constexpr int NC = A / 2;
@@ -653,17 +670,6 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         fence_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_ready);
-        // the pieces of Y, once G has used it (a third takes the place of the copy of S: once X S has used that)
-        const int j = tid & 127;
-        const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
-        if (!mbar_wait_warp(&xy_full[t % NS], (t / NS) & 1, abort_flag) || !mbar_wait_warp(three ? x_done : g_full, par, abort_flag)) {
-          failed = true;
-          break;
-        }
-        linear_decay_rows<A>(y_of(t), base + SM::kLow, three ? base + SM::kS : 0, tid, f, j < nv);
-        fence_async_proxy();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(y_ready);
       }
     }
   }
