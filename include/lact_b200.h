@@ -357,14 +357,34 @@ int lact_linear_attention_fwd(const lact_linear_config *cfg, const void *q, cons
                               const int32_t *cu_seqlens, const float *state_in, float *state_out, void *o, void *workspace,
                               size_t workspace_bytes, int32_t *status_word, void *stream);
 /* Gradients dq [batch, tokens, heads, dk], dk and dv [batch, tokens, kv_heads, dk or dv] (bf16, contiguous, written; shared heads
- * added up) and dstate_in (NULL or fp32), from dout (bf16) and dstate_out (the gradient of state_out, NULL: zeros). */
+ * added up) and dstate_in (NULL or fp32), from dout (bf16) and dstate_out (the gradient of state_out, NULL: zeros).
+ * fwd_workspace: the forward's workspace as that call left it (NULL if it took none). */
 int lact_linear_attention_bwd(const lact_linear_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
-                              const int32_t *cu_seqlens, const float *state_in, const void *dout, const float *dstate_out, void *dq,
-                              void *dk, void *dv, float *dstate_in, void *workspace, size_t workspace_bytes,
-                              int32_t *status_word, void *stream);
+                              const int32_t *cu_seqlens, const float *state_in, const void *fwd_workspace,
+                              size_t fwd_workspace_bytes, const void *dout, const float *dstate_out, void *dq, void *dk, void *dv,
+                              float *dstate_in, void *workspace, size_t workspace_bytes, int32_t *status_word, void *stream);
 /* One token of every entry (tokens = 1): reads state_in, writes state_out, which may be the same array. */
 int lact_linear_attention_step(const lact_linear_config *cfg, const void *q, const void *k, const void *v, const float *log_decay,
                                const float *state_in, float *state_out, void *o, void *stream);
+
+/* Group norm with an activation, channels last: x [n, s, C] (fp32 or bf16, sample and spot strides in elements, channels adjacent,
+ * all multiples of the largest power of two up to 16 bytes that divides a spot) ->
+ * y [n, s, C] of x's type, contiguous; y = act((x - mean) / sqrt(var + eps) * weight + bias) with mean and var over a sample's s spots
+ * and the C / groups channels of a group; weight, bias fp32 [C] or NULL (ones, zeros); silu: the activation, or none.  stats (fp32
+ * [n, groups, 2]) receives means and 1 / sqrt(var + eps), what the backward reads.  Backward: dx of x's type, contiguous, and
+ * dweight, dbias ([2, C] fp32, one array), from dy.  workspace: 256-byte aligned, may be NULL if its size is 0.  No counterpart in the
+ * reference, whose norm behind the recurrence is the RMS norm of lact_out_epilogue. */
+typedef struct lact_group_norm_config {
+  int64_t n, s, channels, groups;
+  int64_t x_ns, x_ss, dy_ns, dy_ss;
+  int32_t dtype, silu;
+  float eps;
+} lact_group_norm_config;
+int lact_group_norm_workspace_bytes(const lact_group_norm_config *cfg, int32_t backward, size_t *bytes_out);
+int lact_group_norm_fwd(const lact_group_norm_config *cfg, const void *x, const float *weight, const float *bias, void *y, float *stats,
+                        void *workspace, size_t workspace_bytes, void *stream);
+int lact_group_norm_bwd(const lact_group_norm_config *cfg, const void *x, const float *weight, const float *bias, const float *stats,
+                        const void *dy, void *dx, float *dweight_dbias, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Backward of lact_qkv_prologue / lact_qkv_prologue_rope on the saved projections (same strides): dq, dk, dv are the
  * gradients of the head-major outputs ([(b n_heads), s, d] bf16, NULL = none), dxq, dxk, dxv the gradients of the

@@ -114,16 +114,31 @@ def _(q, k, v, o, lse, dout, window, softmax_scale, seq_start=None):
     return [q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)]
 
 
+class _LinearConfig(C.Structure):
+    """lact_linear_config of the C header."""
+    _fields_ = [(n, C.c_int64) for n in ("batch", "tokens", "heads", "kv_heads", "dk", "dv", "sequences", "q_ts", "q_bs", "k_ts", "k_bs",
+                                         "v_ts", "v_bs", "do_ts", "do_bs")] + [("scale", C.c_float)]
+
+
 @_fake("linear_attention_fwd")
-def _(q, k, v, log_decay, scale, state, cu_seqlens, want_state):
+def _(q, k, v, log_decay, scale, state, cu_seqlens, want_state, keep=False):
     b, l, h, dk = q.shape
     n = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
     outs = [q.new_empty((b, l, h, v.shape[3]))]
-    return outs + [q.new_empty((n, h, dk, v.shape[3]), dtype=F32)] if want_state else outs
+    if want_state:
+        outs.append(q.new_empty((n, h, dk, v.shape[3]), dtype=F32))
+    if keep:
+        c, need = _LinearConfig(), C.c_size_t(0)
+        c.batch, c.tokens, c.heads, c.kv_heads, c.dk, c.dv, c.scale = b, l, h, k.shape[2], dk, v.shape[3], 1.0
+        c.sequences = 0 if cu_seqlens is None else n
+        if b * l * n > 0:
+            L.check(L.lib().lact_linear_attention_workspace_bytes(C.byref(c), 0, C.byref(need)), "lact_linear_attention_workspace_bytes")
+        outs.append(q.new_empty((need.value,), dtype=torch.uint8))
+    return outs
 
 
 @_fake("linear_attention_bwd")
-def _(q, k, v, log_decay, scale, state, cu_seqlens, dout, dlast):
+def _(q, k, v, log_decay, scale, state, cu_seqlens, kept, dout, dlast):
     outs = [t.new_empty(t.shape) for t in (q, k, v)]
     return outs + [state.new_empty(state.shape)] if state is not None else outs
 
@@ -131,6 +146,16 @@ def _(q, k, v, log_decay, scale, state, cu_seqlens, dout, dlast):
 @_fake("linear_attention_step")
 def _(q, k, v, log_decay, scale, state, new_state):
     return q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
+
+
+@_fake("group_norm_fwd")
+def _(x, weight, bias, groups, eps, silu):
+    return [x.new_empty(x.shape), x.new_empty((x.shape[0], groups, 2), dtype=F32)]
+
+
+@_fake("group_norm_bwd")
+def _(x, weight, bias, stats, dy, groups, eps, silu):
+    return [x.new_empty(x.shape), x.new_empty((2, x.shape[2]), dtype=F32)]
 
 
 @_fake("seq_start")

@@ -24,6 +24,7 @@
 #include "swa_bwd.cuh"
 #include "swa_pairs.cuh"
 #include "linear_chunks.cuh"
+#include "group_norm.cuh"
 
 namespace lact {
 namespace {
@@ -2165,6 +2166,125 @@ LinearArgs linear_args(const lact_linear_config* c, const float* log_decay, cons
   return a;
 }
 
+// ------------------------------------------------------------------------------------------ group norm
+// How a call is computed: by rows (one spot a sample), or in chunks of spots.
+struct NormPlan {
+  bool rows;
+  int V;                  // channels of one access
+  int lpr, K;             // rows: threads a row, vectors a thread
+  int64_t blocks;         // rows: of the launch
+  int64_t chunks, per_chunk, cblocks;
+  size_t part, chan, coef;   // bytes, in this order in the workspace
+};
+// (by the sizes alone: the order of the sums, and with it a result's last bits, does not depend on where an array lies)
+int norm_width(const lact_group_norm_config* c, int64_t of) {
+  int v = c->dtype == LACT_F32 ? 4 : 8;
+  while (of % v != 0) v /= 2;
+  return v;
+}
+int norm_operand(const lact_group_norm_config* c, const void* p, int64_t ns, int64_t ss) {
+  const int v = norm_width(c, c->channels);
+  return ns % v != 0 || ss % v != 0 || reinterpret_cast<uintptr_t>(p) % (v * (c->dtype == LACT_F32 ? 4 : 2)) != 0 ? LACT_ERR_SHAPE : LACT_OK;
+}
+NormPlan norm_plan(const lact_group_norm_config* c, bool backward) {
+  NormPlan p;
+  std::memset(&p, 0, sizeof(p));
+  const int64_t cg = c->channels / c->groups;
+  p.V = norm_width(c, cg);
+  const int64_t nv = c->channels / p.V;
+  p.rows = c->s == 1 && nv <= 1024 && c->channels <= 4096;
+  if (p.rows) {
+    p.K = nv <= 256 ? 1 : nv <= 512 ? 2 : 4;
+    for (p.lpr = 1; p.lpr * p.K < nv;) p.lpr *= 2;
+    p.blocks = std::min<int64_t>((c->n + 256 / p.lpr - 1) / (256 / p.lpr), static_cast<int64_t>(sm_count()) * (backward ? 4 : 8));
+    if (backward) p.part = static_cast<size_t>(p.blocks) * 2 * c->channels * 4;
+    return p;
+  }
+  p.V = norm_width(c, c->channels);
+  const int64_t vecs = c->channels / p.V, at_once = 256 / std::min<int64_t>(vecs, 256);
+  p.cblocks = (vecs + 255) / 256;
+  // blocks for eight a SM, of four turns at least
+  const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(sm_count()) * 8 / (c->n * p.cblocks));
+  p.per_chunk = (c->s + want - 1) / want;
+  p.per_chunk = std::max<int64_t>((p.per_chunk + at_once - 1) / at_once, kNormAhead) * at_once;
+  p.per_chunk = std::min<int64_t>(p.per_chunk, c->s);
+  p.chunks = (c->s + p.per_chunk - 1) / p.per_chunk;
+  auto up = [](int64_t n) { return (static_cast<size_t>(n) + 255) / 256 * 256; };
+  p.part = up(c->n * p.chunks * c->channels * 8);
+  p.chan = up(c->n * c->channels * 8);
+  p.coef = backward ? up(c->n * c->groups * 8) : 0;
+  return p;
+}
+int norm_check(const lact_group_norm_config* c) {
+  if (c == nullptr) return LACT_ERR_NULL;
+  if (c->dtype != LACT_F32 && c->dtype != LACT_BF16) return LACT_ERR_DTYPE;
+  if (c->n < 1 || c->s < 1 || c->groups < 1 || c->channels < 1 || c->channels % c->groups != 0) return LACT_ERR_SHAPE;
+  if (c->channels > (1 << 20) || c->s > (1ll << 30) || c->n > (1ll << 30) || c->n * c->groups > (1ll << 30)) return LACT_ERR_SHAPE;
+  if (!(c->eps >= 0.f && c->eps < INFINITY)) return LACT_ERR_CONFIG;
+  return LACT_OK;
+}
+template <class T, int V, bool BACKWARD>
+int launch_norm(const GroupNormArgs& a, const NormPlan& p, cudaStream_t st) {
+  if (p.rows) {
+    const size_t smem = std::max<size_t>(8192, BACKWARD ? static_cast<size_t>(a.C) * 8 : 0);
+    const dim3 grid(static_cast<unsigned>(p.blocks));
+    {
+      KernelScope scope(kClsOther, st);
+      switch (p.K) {
+        case 1: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 1, BACKWARD>, grid, dim3(256), smem, st, a, p.lpr)); break;
+        case 2: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 2, BACKWARD>, grid, dim3(256), smem, st, a, p.lpr)); break;
+        default: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 4, BACKWARD>, grid, dim3(256), smem, st, a, p.lpr)); break;
+      }
+    }
+    return LACT_OK;
+  }
+  const int64_t blocks = a.n * p.chunks;
+  if (blocks > 0x7FFFFFFFll || p.cblocks > 65535) return LACT_ERR_SHAPE;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.cblocks));
+  { KernelScope scope(kClsOther, st); LACT_CUDA(launch_pdl(group_norm_sums_kernel<T, V, BACKWARD>, grid, dim3(256), 0, st, a)); }
+  { KernelScope scope(kClsOther, st); LACT_CUDA(launch_pdl(group_norm_groups_kernel<BACKWARD>, dim3(static_cast<unsigned>(a.n * a.G)), dim3(256), 0, st, a)); }
+  if (BACKWARD) {
+    KernelScope scope(kClsOther, st);
+    LACT_CUDA(launch_pdl(group_norm_weights_kernel, dim3(static_cast<unsigned>((a.C + 31) / 32)), dim3(256), 0, st, a));
+  }
+  KernelScope scope(kClsOther, st);
+  LACT_CUDA(launch_pdl(group_norm_apply_kernel<T, V, BACKWARD>, grid, dim3(256), 0, st, a));
+  return LACT_OK;
+}
+template <bool BACKWARD>
+int norm_run(const GroupNormArgs& a, const NormPlan& p, int dtype, cudaStream_t st) {
+  if (dtype == LACT_F32) {
+    switch (p.V) {
+      case 4: return launch_norm<float, 4, BACKWARD>(a, p, st);
+      case 2: return launch_norm<float, 2, BACKWARD>(a, p, st);
+      default: return launch_norm<float, 1, BACKWARD>(a, p, st);
+    }
+  }
+  switch (p.V) {
+    case 8: return launch_norm<bf16, 8, BACKWARD>(a, p, st);
+    case 4: return launch_norm<bf16, 4, BACKWARD>(a, p, st);
+    case 2: return launch_norm<bf16, 2, BACKWARD>(a, p, st);
+    default: return launch_norm<bf16, 1, BACKWARD>(a, p, st);
+  }
+}
+// The arguments both directions share; the workspace laid out.
+int norm_args(const lact_group_norm_config* c, const NormPlan& p, const void* x, const float* w, const float* b, void* workspace,
+              size_t workspace_bytes, GroupNormArgs* a) {
+  const size_t need = p.part + p.chan + p.coef;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return LACT_ERR_WORKSPACE;
+  std::memset(a, 0, sizeof(*a));
+  uint8_t* room = static_cast<uint8_t*>(workspace);
+  a->x = x; a->w = w; a->b = b;
+  a->part = reinterpret_cast<float*>(room);
+  a->chan = reinterpret_cast<float*>(room + p.part);
+  a->coef = reinterpret_cast<float*>(room + p.part + p.chan);
+  a->n = c->n; a->x_ns = c->x_ns; a->x_ss = c->x_ss; a->dy_ns = c->dy_ns; a->dy_ss = c->dy_ss;
+  a->s = static_cast<int32_t>(c->s); a->C = static_cast<int32_t>(c->channels); a->G = static_cast<int32_t>(c->groups);
+  a->silu = c->silu; a->eps = c->eps;
+  a->chunks = static_cast<int32_t>(p.chunks); a->per_chunk = static_cast<int32_t>(p.per_chunk);
+  return LACT_OK;
+}
+
 }  // namespace
 }  // namespace lact
 
@@ -3339,8 +3459,9 @@ int lact_linear_attention_step(const lact_linear_config* c, const void* q, const
 }
 
 int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const void* k, const void* v, const float* log_decay,
-                              const int32_t* cu, const float* state_in, const void* dout, const float* dstate_out, void* dq, void* dk,
-                              void* dv, float* dstate_in, void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream) {
+                              const int32_t* cu, const float* state_in, const void* fwd_workspace, size_t fwd_workspace_bytes,
+                              const void* dout, const float* dstate_out, void* dq, void* dk, void* dv, float* dstate_in, void* workspace,
+                              size_t workspace_bytes, int32_t* status_word, void* stream) {
   LACT_TRY(linear_check(c, cu));
   if (!log_decay || !dq || !dk || !dv || !status_word) return LACT_ERR_NULL;
   LACT_TRY(linear_operand(q, c->q_ts, c->q_bs, c->heads * c->dk));
@@ -3353,6 +3474,9 @@ int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const 
   size_t need = 0;
   LACT_TRY(lact_linear_attention_workspace_bytes(c, 1, &need));
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return LACT_ERR_WORKSPACE;
+  size_t fwd_need = 0;
+  LACT_TRY(lact_linear_attention_workspace_bytes(c, 0, &fwd_need));
+  if (fwd_need > 0 && (fwd_workspace == nullptr || fwd_workspace_bytes < fwd_need || (reinterpret_cast<uintptr_t>(fwd_workspace) & 255) != 0)) return LACT_ERR_WORKSPACE;
   float* const each_head = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (linear_slots(linear_plan(c), c->dk, c->dv) + 255) / 256 * 256);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int32_t share = static_cast<int32_t>(c->heads / c->kv_heads);
@@ -3387,7 +3511,8 @@ int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const 
   LinearArgs a = with(DO, V, K, dq, false);
   a.s_in = state_in;
   a.s_in_t = 1;
-  LACT_TRY(linear_run(c, a, c->dv, c->dk, workspace, false, status_word, st));
+  // (the CTAs begin with the forward's states, transposed; they are read alone)
+  LACT_TRY(linear_run(c, a, c->dv, c->dk, const_cast<void*>(fwd_workspace), true, status_word, st));
   a = with(K, Q, DO, dv, true);
   a.s_out = dstate_in;
   LACT_TRY(linear_run(c, a, c->dk, c->dv, workspace, false, status_word, st));
@@ -3396,6 +3521,50 @@ int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const 
   a.s_in_t = 1;
   LACT_TRY(linear_run(c, a, c->dv, c->dk, workspace, true, status_word, st));   // the CTAs begin with the states of dv, transposed
   return add_up(dk, c->dk);
+}
+
+// ------------------------------------------------------------------------------------------ group norm
+int lact_group_norm_workspace_bytes(const lact_group_norm_config* c, int32_t backward, size_t* bytes_out) {
+  if (bytes_out == nullptr) return LACT_ERR_NULL;
+  LACT_TRY(norm_check(c));
+  const NormPlan p = norm_plan(c, backward != 0);
+  *bytes_out = p.part + p.chan + p.coef;
+  return LACT_OK;
+}
+
+int lact_group_norm_fwd(const lact_group_norm_config* c, const void* x, const float* weight, const float* bias, void* y, float* stats,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  LACT_TRY(norm_check(c));
+  if (!x || !y || !stats) return LACT_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(y) & 15) != 0 || (reinterpret_cast<uintptr_t>(stats) & 7) != 0) return LACT_ERR_SHAPE;
+  LACT_TRY(check_device());
+  LACT_TRY(norm_operand(c, x, c->x_ns, c->x_ss));
+  const NormPlan p = norm_plan(c, false);
+  GroupNormArgs a;
+  LACT_TRY(norm_args(c, p, x, weight, bias, workspace, workspace_bytes, &a));
+  a.out = y;
+  a.stats = stats;
+  return norm_run<false>(a, p, c->dtype, static_cast<cudaStream_t>(stream));
+}
+
+int lact_group_norm_bwd(const lact_group_norm_config* c, const void* x, const float* weight, const float* bias, const float* stats,
+                        const void* dy, void* dx, float* dweight_dbias, void* workspace, size_t workspace_bytes, void* stream) {
+  LACT_TRY(norm_check(c));
+  if (!x || !stats || !dy || !dx || !dweight_dbias) return LACT_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(dx) & 15) != 0 || (reinterpret_cast<uintptr_t>(stats) & 7) != 0) return LACT_ERR_SHAPE;
+  LACT_TRY(check_device());
+  LACT_TRY(norm_operand(c, x, c->x_ns, c->x_ss));
+  LACT_TRY(norm_operand(c, dy, c->dy_ns, c->dy_ss));
+  const NormPlan p = norm_plan(c, true);
+  GroupNormArgs a;
+  LACT_TRY(norm_args(c, p, x, weight, bias, workspace, workspace_bytes, &a));
+  a.dy = dy;
+  a.out = dx;
+  a.stats = const_cast<float*>(stats);
+  a.dw = dweight_dbias;
+  a.db = dweight_dbias + c->channels;
+  LACT_TRY(norm_run<true>(a, p, c->dtype, static_cast<cudaStream_t>(stream)));
+  return p.rows ? lact_column_sums(a.part, dweight_dbias, p.blocks, 2 * c->channels, stream) : LACT_OK;
 }
 
 int lact_l2_norm_add(const void* x, int32_t x_dtype, const void* x_add, int32_t add_dtype, const void* scale, void* y,

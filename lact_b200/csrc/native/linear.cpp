@@ -35,13 +35,14 @@ lact_linear_config config(const Tensor& q, const Tensor& k, const Tensor& v, dou
 }
 int64_t states_of(const Tensor& q, const OptTensor& cu) { return given(cu) ? cu->numel() - 1 : q.size(0); }
 
-// o, and the last state with `want_state`
+// o, the last state with `want_state`, and with `keep` what the backward takes over of this call's workspace (the states that its
+// pieces of sequences begin with)
 std::vector<Tensor> fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, double scale, const OptTensor& state_,
-                        const OptTensor& cu, bool want_state) {
+                        const OptTensor& cu, bool want_state, bool keep) {
   const c10::cuda::CUDAGuard guard(q_.device());
   const int64_t b = q_.size(0), l = q_.size(1), h = q_.size(2), dk = q_.size(3), dv = v_.size(3), n = states_of(q_, cu);
   const Tensor g = g_.contiguous(), state = whole(state_);
-  Tensor o = empty({b, l, h, dv}, at::kBFloat16, q_), last;
+  Tensor o = empty({b, l, h, dv}, at::kBFloat16, q_), last, room;
   if (want_state) last = empty({n, h, dk, dv}, at::kFloat, q_);
   if (b * l == 0 || n == 0) {   // no tokens: the state stays what it was
     o.zero_();
@@ -51,7 +52,6 @@ std::vector<Tensor> fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, co
     const lact_linear_config c = config(q, k, v, scale, cu);
     size_t need = 0;
     check(lact_linear_attention_workspace_bytes(&c, 0, &need), "lact_linear_attention_workspace_bytes");
-    Tensor room;
     if (need > 0) room = bytes(need, q);
     check(lact_linear_attention_fwd(&c, ptr(q), ptr(k), ptr(v), f32(g), static_cast<const int32_t*>(ptr(cu)), f32(state),
                                     want_state ? last.data_ptr<float>() : nullptr, ptr(o), need > 0 ? ptr(room) : nullptr, need,
@@ -60,12 +60,13 @@ std::vector<Tensor> fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, co
   }
   std::vector<Tensor> r{o};
   if (want_state) r.push_back(last);
+  if (keep) r.push_back(room.defined() ? room : empty({0}, at::kByte, q_));
   return r;
 }
 
 // dq, dk, dv, and the first state's gradient where there is a first state
 std::vector<Tensor> bwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, double scale, const OptTensor& state_,
-                        const OptTensor& cu, const OptTensor& dout_, const OptTensor& dlast_) {
+                        const OptTensor& cu, const Tensor& kept, const OptTensor& dout_, const OptTensor& dlast_) {
   const c10::cuda::CUDAGuard guard(q_.device());
   const int64_t b = q_.size(0), l = q_.size(1), h = q_.size(2), n = states_of(q_, cu);
   const Tensor g = g_.contiguous(), state = whole(state_);
@@ -87,8 +88,8 @@ std::vector<Tensor> bwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, co
   check(lact_linear_attention_workspace_bytes(&c, 1, &need), "lact_linear_attention_workspace_bytes");
   Tensor room;
   if (need > 0) room = bytes(need, q);
-  check(lact_linear_attention_bwd(&c, ptr(q), ptr(k), ptr(v), f32(g), static_cast<const int32_t*>(ptr(cu)), f32(state), ptr(dout),
-                                  f32(dlast), ptr(dq), ptr(dk), ptr(dv), state.defined() ? r[3].data_ptr<float>() : nullptr,
+  check(lact_linear_attention_bwd(&c, ptr(q), ptr(k), ptr(v), f32(g), static_cast<const int32_t*>(ptr(cu)), f32(state),
+                                  kept.numel() > 0 ? ptr(kept) : nullptr, static_cast<size_t>(kept.numel()), ptr(dout), f32(dlast), ptr(dq), ptr(dk), ptr(dv), state.defined() ? r[3].data_ptr<float>() : nullptr,
                                   need > 0 ? ptr(room) : nullptr, need, status_word(q), stream_of(q)),
         "lact_linear_attention_bwd");
   settle(q);
@@ -114,9 +115,10 @@ Tensor step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& 
   return o;
 }
 
-using FwdSig = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double, const OptTensor&, const OptTensor&, bool);
+using FwdSig = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double, const OptTensor&, const OptTensor&, bool,
+                                   bool);
 using BwdSig = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double, const OptTensor&, const OptTensor&,
-                                   const OptTensor&, const OptTensor&);
+                                   const Tensor&, const OptTensor&, const OptTensor&);
 const auto& fwd_op() {
   static const auto o = c10::Dispatcher::singleton().findSchemaOrThrow("lact_b200::linear_attention_fwd", "").typed<FwdSig>();
   return o;
@@ -131,37 +133,39 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale,
                                const OptTensor& state, const OptTensor& cu, bool want_state) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    ctx->save_for_backward({q, k, v, g, value(state), value(cu)});
+    variable_list r = fwd_op().call(q, k, v, g, scale, state, cu, want_state, true);
+    ctx->save_for_backward({q, k, v, g, value(state), value(cu), r.back()});
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
-    return fwd_op().call(q, k, v, g, scale, state, cu, want_state);
+    r.pop_back();
+    return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto t = ctx->get_saved_variables();
     g.resize(2);
     if (!g[0].defined() && !g[1].defined()) return variable_list(8);
-    const variable_list r = bwd_op().call(t[0], t[1], t[2], t[3], ctx->saved_data["scale"].toDouble(), opt(t[4]), opt(t[5]), opt(g[0]), opt(g[1]));
+    const variable_list r = bwd_op().call(t[0], t[1], t[2], t[3], ctx->saved_data["scale"].toDouble(), opt(t[4]), opt(t[5]), t[6], opt(g[0]), opt(g[1]));
     return {r[0], r[1], r[2], Tensor(), Tensor(), r.size() > 3 ? r[3] : Tensor(), Tensor(), Tensor()};
   }
 };
 std::vector<Tensor> linear_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale, const OptTensor& state,
-                                    const OptTensor& cu, bool want_state) {
+                                    const OptTensor& cu, bool want_state, bool keep) {
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK_NOT_IMPLEMENTED(!g.requires_grad(), "linear_attention has no gradient for log_decay");
     if (q.requires_grad() || k.requires_grad() || v.requires_grad() || value(state).requires_grad())
       return LinearFunction::apply(q, k, v, g, scale, state, cu, want_state);
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return fwd_op().call(q, k, v, g, scale, state, cu, want_state);
+  return fwd_op().call(q, k, v, g, scale, state, cu, want_state, keep);
 }
 
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(lact_b200, m) {
   m.def("linear_attention_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, float scale, Tensor? state, Tensor? cu_seqlens, "
-        "bool want_state) -> Tensor[]");
+        "bool want_state, bool keep=False) -> Tensor[]");
   m.def("linear_attention_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, float scale, Tensor? state, Tensor? cu_seqlens, "
-        "Tensor? dout, Tensor? dlast) -> Tensor[]");
+        "Tensor kept, Tensor? dout, Tensor? dlast) -> Tensor[]");
   m.def("linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, float scale, Tensor state, Tensor(a!) new_state) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(lact_b200, CUDA, m) {

@@ -101,6 +101,38 @@ def out_epilogue(fw_x: torch.Tensor, norm_weight: torch.Tensor, num_heads: int, 
     return L.call(_op("out_epilogue"), fw_x, norm_weight, scale_proj, o, num_heads, float(eps))
 
 
+# ------------------------------------------------------------------------------------------ group norm
+def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, activation: Optional[str] = None) -> torch.Tensor:
+    """Group norm with an activation, channels last: `act((x - mean) / sqrt(var + eps) * weight + bias)`, x [n, ..., C] bf16 or
+    float32, mean and var over all spots of a sample and the C / num_groups adjacent channels of a group, activation None or
+    "silu"; weight, bias [C] float32 or bf16, or None.  Behind a token mixer, x [tokens, heads * d] with num_groups = heads is
+    the norm of every head of every token (one spot a sample); maps and frames are [n, h, w, C] or [n, frames, h, w, C].
+    Result: x's shape and type, contiguous.  Differentiable with respect to x, weight and bias."""
+    if x.dim() < 2:
+        raise ValueError("x: [n, ..., channels]")
+    if x.dtype not in (BF16, torch.float32):
+        raise TypeError("x: bf16 or float32")
+    C = x.shape[-1]
+    if num_groups < 1 or C == 0 or C % num_groups:
+        raise ValueError("num_groups must divide the channels")
+    if activation not in (None, "silu"):
+        raise ValueError("activation: None or 'silu'")
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError("eps must be finite and not negative")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.shape != (C,) or t.device != x.device:
+            raise ValueError(f"{name}: [channels] on the device of x")
+        if t.dtype not in (BF16, torch.float32):
+            raise TypeError(f"{name}: bf16 or float32")
+    if not x.is_cuda:
+        raise ValueError("group_norm needs CUDA tensors (there is no CPU implementation)")
+    flat = x if x.dim() == 3 else x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
+    return L.call(_op("group_norm_fwd"), flat, weight, bias, int(num_groups), float(eps), activation == "silu")[0].reshape(x.shape)
+
+
 # ------------------------------------------------------------------------------------------ linear attention
 def _linear_heads(what, q, k, v, log_decay, dims):
     """Checks shared by the prompt and the token form (`dims` axes, heads and features last); returns heads, dk, dv."""

@@ -872,3 +872,14 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, cu=None):
         last.append(S)
     outs.append(q.new_zeros(b, l - cu_[-1], h, v.shape[3]))
     return torch.cat(outs, 1), torch.cat(last)
+
+
+# --------------------------------------------------------------------------- group norm with an activation
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, silu=False):
+    """64 bits, channels last: x [n, ..., C]."""
+    n, C = x.shape[0], x.shape[-1]
+    v = x.double().reshape(n, -1, groups, C // groups)
+    var, mean = torch.var_mean(v, dim=(1, 3), keepdim=True, correction=0)
+    z = ((v - mean) / torch.sqrt(var + eps)).reshape(x.shape)
+    z = z * (1.0 if weight is None else weight.double()) + (0.0 if bias is None else bias.double())
+    return z * torch.sigmoid(z) if silu else z

@@ -40,7 +40,8 @@ def test_bad_configurations_are_refused(lib, over, code):
     p = C.c_void_p(4096)   # (never looked at)
     one = C.c_void_p(4096)
     assert lib.lact_linear_attention_fwd(C.byref(c), p, p, p, p, None, None, None, p, None, C.c_size_t(0), one, None) == code
-    assert lib.lact_linear_attention_bwd(C.byref(c), p, p, p, p, None, None, p, None, p, p, p, None, None, C.c_size_t(0), one, None) == code
+    assert lib.lact_linear_attention_bwd(C.byref(c), p, p, p, p, None, None, None, C.c_size_t(0), p, None, p, p, p, None, None, C.c_size_t(0),
+                                         one, None) == code
 
 
 @pytest.mark.parametrize("over", [dict(q_ts=255), dict(q_ts=248), dict(k_bs=9), dict(v_ts=128)])
