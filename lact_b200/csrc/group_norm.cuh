@@ -23,7 +23,7 @@ struct GroupNormArgs {
   const float *w, *b;         // [C] or nullptr: ones, zeros
   void* out;                  // y, or dx: contiguous
   float* stats;               // [n][G][2]: mean, 1 / sqrt(var + eps)
-  float* part;                // [n][chunks][C][2]; one spot, backward: [blocks][2][C]
+  float* part;                // [n][C][chunks][2]; one spot, backward: [blocks][2][C]
   float* chan;                // [n][C][2]
   float* coef;                // backward: [n][G][2]: c1, c2
   float *dw, *db;             // [C]
@@ -34,8 +34,6 @@ struct GroupNormArgs {
 };
 
 // V values of type T, as one access
-template <class T, int V>
-struct Vec;
 template <int BYTES>
 struct Raw;
 template <> struct Raw<16> { using type = uint4; };
@@ -43,52 +41,134 @@ template <> struct Raw<8> { using type = uint2; };
 template <> struct Raw<4> { using type = uint32_t; };
 template <> struct Raw<2> { using type = uint16_t; };
 template <class T, int V>
-__device__ __forceinline__ void load_values(const T* p, float (&f)[V]) {
-  using R = typename Raw<V * sizeof(T)>::type;
-  const R r = *reinterpret_cast<const R*>(p);
+using RawOf = typename Raw<V * sizeof(T)>::type;
+template <class T, int V>
+__device__ __forceinline__ RawOf<T, V> load_raw(const T* p) {
+  return *reinterpret_cast<const RawOf<T, V>*>(p);
+}
+template <class T, int V>
+__device__ __forceinline__ void values_of(const RawOf<T, V>& r, float (&f)[V]) {
   const T* t = reinterpret_cast<const T*>(&r);
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = static_cast<float>(t[i]);
 }
 template <class T, int V>
 __device__ __forceinline__ void store_values(T* p, const float (&f)[V]) {
-  using R = typename Raw<V * sizeof(T)>::type;
-  R r;
+  RawOf<T, V> r;
   T* t = reinterpret_cast<T*>(&r);
 #pragma unroll
   for (int i = 0; i < V; ++i) t[i] = static_cast<T>(f[i]);
-  *reinterpret_cast<R*>(p) = r;
+  *reinterpret_cast<RawOf<T, V>*>(p) = r;
 }
-__device__ __forceinline__ float silu_of(float z) { return z * sigmoidf_fast(z); }
-__device__ __forceinline__ float silu_slope(float z) {
-  const float g = sigmoidf_fast(z);
-  return g * fmaf(z, 1.f - g, 1.f);
+// Arithmetic on V values, two at a time (a large call has a budget of 20 instructions an element while its memory arrives)
+template <int V>
+__device__ __forceinline__ void v_fma(float (&d)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V == 1) d[0] = fmaf(a[0], b[0], c[0]);
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) f32x2_split(f32x2_fma(f32x2(a[i], a[i + 1]), f32x2(b[i], b[i + 1]), f32x2(c[i], c[i + 1])), d[i], d[i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void v_mul(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) d[0] = a[0] * b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) f32x2_split(f32x2_mul(f32x2(a[i], a[i + 1]), f32x2(b[i], b[i + 1])), d[i], d[i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void v_add(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) d[0] = a[0] + b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) f32x2_split(f32x2_add(f32x2(a[i], a[i + 1]), f32x2(b[i], b[i + 1])), d[i], d[i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void v_set(float (&d)[V], float x) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) d[i] = x;
+}
+template <int V>
+__device__ __forceinline__ float v_sum(const float (&a)[V]) {
+  float t[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = a[i];
+#pragma unroll
+  for (int n = V / 2; n > 0; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) t[i] += t[i + n];
+  return t[0];
+}
+// sum of products
+template <int V>
+__device__ __forceinline__ float v_dot(const float (&a)[V], const float (&b)[V]) {
+  float t[V];
+  v_mul(t, a, b);
+  return v_sum(t);
+}
+
+// sigmoid(z) of V values.  Two special-function results an element (16 a clock and SM) take as long as the memory of a large call
+// (77 million elements: 34 us; two frames of 480 x 832 x 96 come and go in 47): two neighbours share one reciprocal, 1 / a = b (1 / ab).
+// Below z = -41 the sigmoid stays at 2^-60, so that the product stays finite.
+template <int V>
+__device__ __forceinline__ void sigmoids(const float (&z)[V], float (&g)[V]) {
+  if constexpr (V == 1) {
+    g[0] = sigmoidf_fast(z[0]);
+  } else {
+    const F32x2 k = f32x2(-1.4426950408889634f, -1.4426950408889634f), one = f32x2(1.f, 1.f);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      float x0, x1, a, b;
+      f32x2_split(f32x2_mul(f32x2(z[i], z[i + 1]), k), x0, x1);
+      x0 = x0 > 60.f ? 60.f : x0;   // (not a minimum: NaN stays)
+      x1 = x1 > 60.f ? 60.f : x1;
+      f32x2_split(f32x2_add(f32x2(exp2_ftz(x0), exp2_ftz(x1)), one), a, b);
+      const float r = rcp_ftz(a * b);
+      f32x2_split(f32x2_mul(f32x2(r, r), f32x2(b, a)), g[i], g[i + 1]);
+    }
+  }
+}
+// z -> z sigmoid(z), and its slope
+template <int V>
+__device__ __forceinline__ void silu_of(float (&z)[V]) {
+  float g[V];
+  sigmoids(z, g);
+  v_mul(z, z, g);
+}
+template <int V>
+__device__ __forceinline__ void silu_slope(float (&z)[V]) {   // g (1 + z (1 - g)) = g + z (g - g g)
+  float g[V], h[V], n[V];
+  sigmoids(z, g);
+#pragma unroll
+  for (int i = 0; i < V; ++i) n[i] = -g[i];
+  v_fma(h, n, g, g);
+  v_fma(z, z, h, g);
 }
 
 // ---------------------------------------------------------------- one spot a sample
-// LPR threads a row (a power of two), K vectors of V channels each (a group holds whole vectors); 256 / LPR rows a block at a time.
-// Sums of a group: among neighbouring lanes where it has 1, 2, .. 32 vectors, through shared memory otherwise.
-template <int K>
+// A row is a thread per vector of V channels (a group holds whole vectors) and as many rows a block as make 256 threads, or, past 256
+// vectors, K of them a thread.  Sums of a group: among neighbouring lanes where it has 1, 2, .. 32 vectors, through shared memory
+// otherwise.
 struct GroupSums {
   float* vec;     // [rows][vectors]
   float* sum;     // [rows][G]
-  int gv, G, nv, lpr, rows;
-  bool lanes;     // gv a power of two, at most 32 and lpr
-  // p[i]: this thread's sum of vector l + i * lpr -> the sum over the vector's group
-  __device__ __forceinline__ void operator()(float (&p)[K], int row, int l) const {
-    if (lanes) {
+  int gv, G, nv, rows;
+  bool lanes;     // gv a power of two, at most 32
+  // p[i]: this thread's sum of vector l + 256 i of its row -> the sum over the vector's group
+  template <int K>
+  __device__ __forceinline__ void among_lanes(float (&p)[K]) const {
+    for (int o = 1; o < gv; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < K; ++i)
-        for (int o = 1; o < gv; o <<= 1) p[i] += __shfl_xor_sync(0xFFFFFFFFu, p[i], o);
-      return;
-    }
+      for (int i = 0; i < K; ++i) p[i] += __shfl_xor_sync(0xFFFFFFFFu, p[i], o);
+  }
+  template <int K>
+  __device__ __forceinline__ void in_memory(float* p, int row, int l, bool here) const {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < K; ++i)
-      if (l + i * lpr < nv) vec[row * nv + l + i * lpr] = p[i];
+      if (here && l + i * 256 < nv) vec[row * nv + l + i * 256] = p[i];
     __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int it = warp; it < rows * G; it += 8) {
+    for (int it = warp; it < rows * G; it += blockDim.x >> 5) {
       const float* from = vec + it / G * nv + it % G * gv;
       float t = 0.f;
       for (int j = lane; j < gv; j += 32) t += from[j];
@@ -99,134 +179,169 @@ struct GroupSums {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < K; ++i)
-      if (l + i * lpr < nv) p[i] = sum[row * G + (l + i * lpr) / gv];
+      if (here && l + i * 256 < nv) p[i] = sum[row * G + (l + i * 256) / gv];
+  }
+  // M = K vectors of each of several rows
+  template <int K, int M>
+  __device__ __forceinline__ void operator()(float (&p)[M], int row, int l, bool here) const {
+    if (lanes) among_lanes(p);
+    else
+#pragma unroll
+      for (int r = 0; r < M; r += K) in_memory<K>(p + r, row, l, here);
   }
 };
 
-template <class T, int V, int K, bool BACKWARD>
-__global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_constant__ GroupNormArgs a, int32_t lpr) {
+// R rows of a thread at a time, fetched together and worked on side by side.
+template <class T, int V, int K, int R, bool BACKWARD>
+__global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_constant__ GroupNormArgs a, int32_t rows) {
+  constexpr int M = K * R;
   extern __shared__ float norm_smem[];
   griddep_launch_dependents();
   griddep_wait();
-  const int l = threadIdx.x & (lpr - 1), row = threadIdx.x / lpr, rows = 256 / lpr;
   const int nv = a.C / V, gv = nv / a.G;
-  const GroupSums<K> sums{norm_smem, norm_smem + rows * nv, gv, a.G, nv, lpr, rows, (gv & (gv - 1)) == 0 && gv <= 32 && gv <= lpr};
+  const int row = K > 1 ? 0 : threadIdx.x / nv, l = K > 1 ? threadIdx.x : threadIdx.x - row * nv;
+  const bool here = row < rows;
+  const GroupSums sums{norm_smem, norm_smem + rows * nv, gv, a.G, nv, rows, (gv & (gv - 1)) == 0 && gv <= 32};
   const float inv = 1.f / (gv * V);
   float w[K][V], b[K][V];
 #pragma unroll
   for (int i = 0; i < K; ++i)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int v = l + i * lpr, c = v * V + e;
-      w[i][e] = v < nv && a.w != nullptr ? a.w[c] : 1.f;
-      b[i][e] = v < nv && a.b != nullptr ? a.b[c] : 0.f;
+      const int v = l + i * 256, c = v * V + e;
+      w[i][e] = here && v < nv && a.w != nullptr ? a.w[c] : 1.f;
+      b[i][e] = here && v < nv && a.b != nullptr ? a.b[c] : 0.f;
     }
   [[maybe_unused]] float dw[BACKWARD ? K : 1][V], db[BACKWARD ? K : 1][V];
   if (BACKWARD) {
 #pragma unroll
-    for (int i = 0; i < K; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) dw[i][e] = db[i][e] = 0.f;
-  }
-  for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * rows; n0 < a.n; n0 += static_cast<int64_t>(gridDim.x) * rows) {
-    const int64_t n = n0 + row;
-    const bool on = n < a.n;    // (all threads take part in the sums)
-    float x[K][V], p[K];
-#pragma unroll
     for (int i = 0; i < K; ++i) {
-      const int v = l + i * lpr;
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[i][e] = 0.f;
-      if (on && v < nv) load_values<T, V>(static_cast<const T*>(a.x) + n * a.x_ns + v * V, x[i]);
+      v_set(dw[i], 0.f);
+      v_set(db[i], 0.f);
     }
+  }
+  const int64_t step = static_cast<int64_t>(gridDim.x) * rows * R;
+  for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * rows * R; n0 < a.n; n0 += step) {
+    // (entry j: vector l + 256 (j % K) of row n0 + row + rows (j / K))
+    auto sample = [&](int j) { return n0 + row + static_cast<int64_t>(rows) * (j / K); };
+    auto vector = [&](int j) { return l + 256 * (j % K); };
+    auto on = [&](int j) { return here && vector(j) < nv && sample(j) < a.n; };
+    RawOf<T, V> raw[M];
+    [[maybe_unused]] RawOf<T, V> raw_dy[BACKWARD ? M : 1];
+    [[maybe_unused]] float2 st[BACKWARD ? M : 1];
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      raw[j] = RawOf<T, V>{};
+      if constexpr (BACKWARD) {
+        raw_dy[j] = RawOf<T, V>{};
+        st[j] = make_float2(0.f, 0.f);
+      }
+      if (!on(j)) continue;
+      raw[j] = load_raw<T, V>(static_cast<const T*>(a.x) + sample(j) * a.x_ns + vector(j) * V);
+      if constexpr (BACKWARD) {
+        raw_dy[j] = load_raw<T, V>(static_cast<const T*>(a.dy) + sample(j) * a.dy_ns + vector(j) * V);
+        st[j] = *reinterpret_cast<const float2*>(a.stats + (sample(j) * a.G + vector(j) / gv) * 2);
+      }
+    }
+    float x[M][V], p[M];
     if constexpr (!BACKWARD) {
+      float mean[M];
 #pragma unroll
-      for (int i = 0; i < K; ++i) {
-        p[i] = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) p[i] += x[i][e];
+      for (int j = 0; j < M; ++j) {
+        values_of<T, V>(raw[j], x[j]);
+        p[j] = v_sum(x[j]);
       }
-      sums(p, row, l);
+      sums.template operator()<K>(p, row, l, here);
 #pragma unroll
-      for (int i = 0; i < K; ++i) {
-        const float mean = p[i] * inv;
-        if (on && l + i * lpr < nv && (l + i * lpr) % gv == 0) a.stats[(n * a.G + (l + i * lpr) / gv) * 2] = mean;
-        p[i] = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          x[i][e] -= mean;
-          p[i] = fmaf(x[i][e], x[i][e], p[i]);
-        }
-        if (l + i * lpr >= nv) p[i] = 0.f;
+      for (int j = 0; j < M; ++j) {
+        mean[j] = p[j] * inv;
+        float m[V];
+        v_set(m, -mean[j]);
+        v_add(x[j], x[j], m);
+        p[j] = v_dot(x[j], x[j]);
       }
-      sums(p, row, l);
+      sums.template operator()<K>(p, row, l, here);
 #pragma unroll
-      for (int i = 0; i < K; ++i) {
-        const int v = l + i * lpr;
-        const float rstd = rsqrtf(fmaf(p[i], inv, a.eps));
-        if (!on || v >= nv) continue;
-        if (v % gv == 0) a.stats[(n * a.G + v / gv) * 2 + 1] = rstd;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float z = fmaf(x[i][e] * rstd, w[i][e], b[i][e]);
-          x[i][e] = a.silu ? silu_of(z) : z;
-        }
-        store_values<T, V>(static_cast<T*>(a.out) + n * a.C + v * V, x[i]);
+      for (int j = 0; j < M; ++j) {
+        const float rstd = rsqrtf(fmaf(p[j], inv, a.eps));
+        if (!on(j)) continue;
+        if (vector(j) % gv == 0) *reinterpret_cast<float2*>(a.stats + (sample(j) * a.G + vector(j) / gv) * 2) = make_float2(mean[j], rstd);
+        float k[V];
+        v_set(k, rstd);
+        v_mul(k, k, w[j % K]);
+        v_fma(x[j], x[j], k, b[j % K]);
+        if (a.silu) silu_of(x[j]);
+        store_values<T, V>(static_cast<T*>(a.out) + sample(j) * a.C + vector(j) * V, x[j]);
       }
     } else {
-      float t[K][V], q[K], rstd[K];
+      float t[M][V], q[M];
 #pragma unroll
-      for (int i = 0; i < K; ++i) {
-        const int v = l + i * lpr;
-        p[i] = q[i] = rstd[i] = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) t[i][e] = 0.f;
-        if (!on || v >= nv) continue;
-        load_values<T, V>(static_cast<const T*>(a.dy) + n * a.dy_ns + v * V, t[i]);
-        const float2 st = *reinterpret_cast<const float2*>(a.stats + (n * a.G + v / gv) * 2);
-        rstd[i] = st.y;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          x[i][e] = (x[i][e] - st.x) * st.y;
-          if (a.silu) t[i][e] *= silu_slope(fmaf(x[i][e], w[i][e], b[i][e]));
-          db[i][e] += t[i][e];
-          dw[i][e] = fmaf(t[i][e], x[i][e], dw[i][e]);
-          t[i][e] *= w[i][e];
-          p[i] += t[i][e];
-          q[i] = fmaf(t[i][e], x[i][e], q[i]);
+      for (int j = 0; j < M; ++j) {   // (entries that are not there: zeros all through)
+        values_of<T, V>(raw[j], x[j]);
+        values_of<T, V>(raw_dy[j], t[j]);
+        float k[V], z[V];
+        v_set(k, -st[j].x);
+        v_add(x[j], x[j], k);
+        v_set(k, st[j].y);
+        v_mul(x[j], x[j], k);
+        if (a.silu) {
+          v_fma(z, x[j], w[j % K], b[j % K]);
+          silu_slope(z);
+          v_mul(t[j], t[j], z);
         }
+        v_add(db[j % K], db[j % K], t[j]);
+        v_fma(dw[j % K], t[j], x[j], dw[j % K]);
+        v_mul(t[j], t[j], w[j % K]);
+        p[j] = v_sum(t[j]);
+        q[j] = v_dot(t[j], x[j]);
       }
-      sums(p, row, l);
-      sums(q, row, l);
+      sums.template operator()<K>(p, row, l, here);
+      sums.template operator()<K>(q, row, l, here);
 #pragma unroll
-      for (int i = 0; i < K; ++i) {
-        const int v = l + i * lpr;
-        if (!on || v >= nv) continue;
-        const float c1 = p[i] * inv, c2 = q[i] * inv;
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[i][e] = rstd[i] * (t[i][e] - c1 - x[i][e] * c2);
-        store_values<T, V>(static_cast<T*>(a.out) + n * a.C + v * V, x[i]);
+      for (int j = 0; j < M; ++j) {
+        if (!on(j)) continue;
+        float c1[V], c2[V], k[V];   // (dz w - c1 first: where a group is one value, nothing is left of it)
+        v_set(c1, -p[j] * inv);
+        v_set(c2, -q[j] * inv);
+        v_set(k, st[j].y);
+        v_add(t[j], t[j], c1);
+        v_fma(x[j], x[j], c2, t[j]);
+        v_mul(x[j], x[j], k);
+        store_values<T, V>(static_cast<T*>(a.out) + sample(j) * a.C + vector(j) * V, x[j]);
       }
     }
   }
   if constexpr (BACKWARD) {
-    // the block's sums over its rows: [2][C], rows of threads added in their order
-    float* const acc = norm_smem;
-    for (int turn = 0; turn < rows; ++turn) {
-      __syncthreads();
-      if (row != turn) continue;
+    // the block's sums over its rows, [2][C]: a column's rows of threads are added in their order
+    float* const part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.C;
+    if (K > 1) {
 #pragma unroll
       for (int i = 0; i < K; ++i)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const int v = l + i * lpr, c = v * V + e;
-          if (v >= nv) continue;
-          acc[c] = turn == 0 ? dw[i][e] : acc[c] + dw[i][e];
-          acc[a.C + c] = turn == 0 ? db[i][e] : acc[a.C + c] + db[i][e];
+          const int c = (l + i * 256) * V + e;
+          if (l + i * 256 >= nv) continue;
+          part[c] = dw[i][e];
+          part[a.C + c] = db[i][e];
         }
+      return;
+    }
+    float* const acc = norm_smem;   // [2][rows][C]
+    __syncthreads();
+    if (here) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        acc[row * a.C + l * V + e] = dw[0][e];
+        acc[(rows + row) * a.C + l * V + e] = db[0][e];
+      }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < 2 * a.C; c += 256) a.part[static_cast<int64_t>(blockIdx.x) * 2 * a.C + c] = acc[c];
+    for (int c = threadIdx.x; c < 2 * a.C; c += blockDim.x) {
+      const float* from = acc + (c < a.C ? c : rows * a.C + c - a.C);
+      float t = 0.f;
+      for (int r = 0; r < rows; ++r) t += from[r * a.C];
+      part[c] = t;
+    }
   }
 }
 
@@ -248,11 +363,31 @@ __device__ __forceinline__ NormSpots norm_spots(const GroupNormArgs& a, int chun
   p.last = min(p.first + a.per_chunk, a.s);
   return p;
 }
-constexpr int kNormAhead = 4;   // spots fetched before the first is worked on
+// A thread's spots, N of them fetched together.
+constexpr int kNormAhead = 4;
+template <class T, int V, bool BOTH, class Work>
+__device__ __forceinline__ void norm_walk(const T* x, const T* dy, const GroupNormArgs& a, const NormSpots& p, const Work& work) {
+  constexpr int N = kNormAhead;
+  int i = p.first + p.row;
+  for (; i + (N - 1) * p.rows < p.last; i += N * p.rows) {
+    RawOf<T, V> rx[N], rdy[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      rx[k] = load_raw<T, V>(x + (i + k * p.rows) * a.x_ss);
+      if (BOTH) rdy[k] = load_raw<T, V>(dy + (i + k * p.rows) * a.dy_ss);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) work(i + k * p.rows, rx[k], BOTH ? rdy[k] : rx[k]);
+  }
+  for (; i < p.last; i += p.rows) {
+    const RawOf<T, V> rx = load_raw<T, V>(x + i * a.x_ss);
+    work(i, rx, BOTH ? load_raw<T, V>(dy + i * a.dy_ss) : rx);
+  }
+}
 
-// Per channel of a chunk -> part[n][chunk][c]: forward the mean and the sum of squares around it, backward the sums of dz and dz xhat.
+// Per channel of a chunk -> part[n][c][chunk]: forward the mean and the sum of squares around it, backward the sums of dz and dz xhat.
 template <class T, int V, bool BACKWARD>
-__global__ void __launch_bounds__(256) group_norm_sums_kernel(const __grid_constant__ GroupNormArgs a) {
+__global__ void __launch_bounds__(256, BACKWARD ? 2 : 4) group_norm_sums_kernel(const __grid_constant__ GroupNormArgs a) {
   __shared__ float acc[256 * V * 2];
   griddep_launch_dependents();
   griddep_wait();
@@ -261,57 +396,47 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(const __grid_const
   const NormSpots p = norm_spots<V>(a, chunk, blockIdx.y);
   const T* const x = static_cast<const T*>(a.x) + n * a.x_ns + p.v * V;
   const T* const dy = BACKWARD ? static_cast<const T*>(a.dy) + n * a.dy_ns + p.v * V : nullptr;
-  float s0[V], s1[V], ref[V];   // ref: the first value (forward), the mean (backward)
+  float s0[V], s1[V], ref[V];   // ref: minus the first value (forward) or the mean (backward)
   [[maybe_unused]] float rs[V], w[V], b[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) s0[e] = s1[e] = 0.f;
   const auto spots_of = [&](int row) { return max(0, (p.last - p.first - row + p.rows - 1) / p.rows); };
   if (p.on && spots_of(p.row) > 0) {
     if (!BACKWARD) {
-      load_values<T, V>(x + (p.first + p.row) * a.x_ss, ref);
+      values_of<T, V>(load_raw<T, V>(x + (p.first + p.row) * a.x_ss), ref);
+#pragma unroll
+      for (int e = 0; e < V; ++e) ref[e] = -ref[e];
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int c = p.v * V + e;
         const float2 st = *reinterpret_cast<const float2*>(a.stats + (n * a.G + c / (a.C / a.G)) * 2);
-        ref[e] = st.x;
+        ref[e] = -st.x;
         rs[e] = st.y;
         w[e] = a.w != nullptr ? a.w[c] : 1.f;
         b[e] = a.b != nullptr ? a.b[c] : 0.f;
       }
     }
-    auto take = [&](const float (&f)[V], const float (&g)[V]) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (!BACKWARD) {
-          const float d = f[e] - ref[e];
-          s0[e] += d;
-          s1[e] = fmaf(d, d, s1[e]);
-        } else {
-          const float h = (f[e] - ref[e]) * rs[e];
-          const float dz = a.silu ? g[e] * silu_slope(fmaf(h, w[e], b[e])) : g[e];
-          s0[e] += dz;
-          s1[e] = fmaf(dz, h, s1[e]);
+    auto take = [&](const RawOf<T, V>& rx, const RawOf<T, V>& rdy) {
+      float f[V], g[V], z[V];
+      values_of<T, V>(rx, f);
+      v_add(f, f, ref);
+      if (!BACKWARD) {
+        v_add(s0, s0, f);
+        v_fma(s1, f, f, s1);
+      } else {
+        values_of<T, V>(rdy, g);
+        v_mul(f, f, rs);
+        if (a.silu) {
+          v_fma(z, f, w, b);
+          silu_slope(z);
+          v_mul(g, g, z);
         }
+        v_add(s0, s0, g);
+        v_fma(s1, g, f, s1);
       }
     };
-    int i = p.first + p.row;
-    for (; i + (kNormAhead - 1) * p.rows < p.last; i += kNormAhead * p.rows) {
-      float f[kNormAhead][V], g[kNormAhead][V];
-#pragma unroll
-      for (int k = 0; k < kNormAhead; ++k) {
-        load_values<T, V>(x + (i + k * p.rows) * a.x_ss, f[k]);
-        if (BACKWARD) load_values<T, V>(dy + (i + k * p.rows) * a.dy_ss, g[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < kNormAhead; ++k) take(f[k], g[k]);
-    }
-    for (; i < p.last; i += p.rows) {
-      float f[V], g[V];
-      load_values<T, V>(x + i * a.x_ss, f);
-      if (BACKWARD) load_values<T, V>(dy + i * a.dy_ss, g);
-      take(f, g);
-    }
+    norm_walk<T, V, BACKWARD>(x, dy, a, p, [&](int, const RawOf<T, V>& rx, const RawOf<T, V>& rdy) { take(rx, rdy); });
   }
   const int here = min(a.C / V, 256);
 #pragma unroll
@@ -319,7 +444,7 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(const __grid_const
     if (!BACKWARD && p.on && spots_of(p.row) > 0) {
       const float d = s0[e] / static_cast<float>(spots_of(p.row));
       s1[e] = fmaf(-d, s0[e], s1[e]);
-      s0[e] = ref[e] + d;
+      s0[e] = d - ref[e];
     }
     acc[(threadIdx.x * V + e) * 2] = s0[e];
     acc[(threadIdx.x * V + e) * 2 + 1] = s1[e];
@@ -341,7 +466,7 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(const __grid_const
         n0 += n1;
       }
     }
-    *reinterpret_cast<float2*>(a.part + ((n * a.chunks + chunk) * a.C + at) * 2) = make_float2(t0, t1);
+    reinterpret_cast<float2*>(a.part)[(n * a.C + at) * a.chunks + chunk] = make_float2(t0, t1);
   }
 }
 
@@ -373,11 +498,12 @@ __global__ void __launch_bounds__(256) group_norm_groups_kernel(const __grid_con
   float u0 = 0.f, u1 = 0.f;
   for (int j = warp; j < cg; j += 8) {
     const int c = g * cg + j;
-    const float2* const part = reinterpret_cast<const float2*>(a.part) + n * a.chunks * a.C + c;
+    const float2* const part = reinterpret_cast<const float2*>(a.part) + (n * a.C + c) * a.chunks;
     auto weight = [&](int k) { return static_cast<float>(min(a.per_chunk, a.s - k * a.per_chunk)); };
     float t0 = 0.f, t1 = 0.f;
+#pragma unroll 4
     for (int k = lane; k < a.chunks; k += 32) {
-      const float2 v = part[static_cast<int64_t>(k) * a.C];
+      const float2 v = part[k];
       t0 += BACKWARD ? v.x : v.x * weight(k);
       if (BACKWARD) t1 += v.y;
     }
@@ -388,8 +514,9 @@ __global__ void __launch_bounds__(256) group_norm_groups_kernel(const __grid_con
     }
     if (!BACKWARD) {   // the channel's mean, and its squares around it
       t0 /= spots;
+#pragma unroll 4
       for (int k = lane; k < a.chunks; k += 32) {
-        const float2 v = part[static_cast<int64_t>(k) * a.C];
+        const float2 v = part[k];
         const float d = v.x - t0;
         t1 += fmaf(d * d, weight(k), v.y);
       }
@@ -443,7 +570,7 @@ __global__ void __launch_bounds__(256) group_norm_weights_kernel(const __grid_co
 
 // y, or dx.  The blocks go through samples and chunks from the last to the first: what the sums have read last is still in L2.
 template <class T, int V, bool BACKWARD>
-__global__ void __launch_bounds__(256) group_norm_apply_kernel(const __grid_constant__ GroupNormArgs a) {
+__global__ void __launch_bounds__(256, BACKWARD ? 2 : 4) group_norm_apply_kernel(const __grid_constant__ GroupNormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
   const int turn = gridDim.x - 1 - blockIdx.x;
@@ -453,7 +580,7 @@ __global__ void __launch_bounds__(256) group_norm_apply_kernel(const __grid_cons
   const T* const x = static_cast<const T*>(a.x) + n * a.x_ns + p.v * V;
   const T* const dy = BACKWARD ? static_cast<const T*>(a.dy) + n * a.dy_ns + p.v * V : nullptr;
   T* const out = static_cast<T*>(a.out) + n * a.s * a.C + p.v * V;
-  // forward: z = (x - m) k + b;  backward: xhat = (x - m) k, z = xhat w + b, dx = dz w k - (c1 + xhat c2) k
+  // forward: z = (x + m) k + b, m minus the mean;  backward: xhat = (x + m) k, z = xhat w + b, dx = (dz w - c1 - xhat c2) k
   float k[V], m[V], b[V];
   [[maybe_unused]] float w[V], c1[V], c2[V];
 #pragma unroll
@@ -461,7 +588,7 @@ __global__ void __launch_bounds__(256) group_norm_apply_kernel(const __grid_cons
     const int c = p.v * V + e, g = c / (a.C / a.G);
     const float2 st = *reinterpret_cast<const float2*>(a.stats + (n * a.G + g) * 2);
     const float wc = a.w != nullptr ? a.w[c] : 1.f;
-    m[e] = st.x;
+    m[e] = -st.x;
     b[e] = a.b != nullptr ? a.b[c] : 0.f;
     if (!BACKWARD) {
       k[e] = st.y * wc;
@@ -469,44 +596,32 @@ __global__ void __launch_bounds__(256) group_norm_apply_kernel(const __grid_cons
       const float2 cc = *reinterpret_cast<const float2*>(a.coef + (n * a.G + g) * 2);
       k[e] = st.y;
       w[e] = wc;
-      c1[e] = cc.x * st.y;
-      c2[e] = cc.y * st.y;
+      c1[e] = -cc.x;
+      c2[e] = -cc.y;
     }
   }
-  auto work = [&](float (&f)[V], const float (&g)[V]) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      if (!BACKWARD) {
-        const float z = fmaf(f[e] - m[e], k[e], b[e]);
-        f[e] = a.silu ? silu_of(z) : z;
-      } else {
-        const float h = (f[e] - m[e]) * k[e];
-        const float dz = a.silu ? g[e] * silu_slope(fmaf(h, w[e], b[e])) : g[e];
-        f[e] = fmaf(dz, w[e] * k[e], -fmaf(h, c2[e], c1[e]));
+  norm_walk<T, V, BACKWARD>(x, dy, a, p, [&](int i, const RawOf<T, V>& rx, const RawOf<T, V>& rdy) {
+    float f[V], g[V], z[V];
+    values_of<T, V>(rx, f);
+    v_add(f, f, m);
+    if (!BACKWARD) {
+      v_fma(f, f, k, b);
+      if (a.silu) silu_of(f);
+    } else {
+      values_of<T, V>(rdy, g);
+      v_mul(f, f, k);
+      if (a.silu) {
+        v_fma(z, f, w, b);
+        silu_slope(z);
+        v_mul(g, g, z);
       }
+      v_mul(g, g, w);
+      v_add(g, g, c1);
+      v_fma(f, f, c2, g);
+      v_mul(f, f, k);
     }
-  };
-  int i = p.first + p.row;
-  for (; i + (kNormAhead - 1) * p.rows < p.last; i += kNormAhead * p.rows) {
-    float f[kNormAhead][V], g[kNormAhead][V];
-#pragma unroll
-    for (int j = 0; j < kNormAhead; ++j) {
-      load_values<T, V>(x + (i + j * p.rows) * a.x_ss, f[j]);
-      if (BACKWARD) load_values<T, V>(dy + (i + j * p.rows) * a.dy_ss, g[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < kNormAhead; ++j) {
-      work(f[j], g[j]);
-      store_values<T, V>(out + static_cast<int64_t>(i + j * p.rows) * a.C, f[j]);
-    }
-  }
-  for (; i < p.last; i += p.rows) {
-    float f[V], g[V];
-    load_values<T, V>(x + i * a.x_ss, f);
-    if (BACKWARD) load_values<T, V>(dy + i * a.dy_ss, g);
-    work(f, g);
     store_values<T, V>(out + static_cast<int64_t>(i) * a.C, f);
-  }
+  });
 }
 
 }  // namespace lact

@@ -2171,7 +2171,8 @@ LinearArgs linear_args(const lact_linear_config* c, const float* log_decay, cons
 struct NormPlan {
   bool rows;
   int V;                  // channels of one access
-  int lpr, K;             // rows: threads a row, vectors a thread
+  int block_rows, K;      // rows: of a block, vectors a thread
+  bool many;              // rows: several of a thread at a time
   int64_t blocks;         // rows: of the launch
   int64_t chunks, per_chunk, cblocks;
   size_t part, chan, coef;   // bytes, in this order in the workspace
@@ -2195,16 +2196,20 @@ NormPlan norm_plan(const lact_group_norm_config* c, bool backward) {
   p.rows = c->s == 1 && nv <= 1024 && c->channels <= 4096;
   if (p.rows) {
     p.K = nv <= 256 ? 1 : nv <= 512 ? 2 : 4;
-    for (p.lpr = 1; p.lpr * p.K < nv;) p.lpr *= 2;
-    p.blocks = std::min<int64_t>((c->n + 256 / p.lpr - 1) / (256 / p.lpr), static_cast<int64_t>(sm_count()) * (backward ? 4 : 8));
+    p.block_rows = p.K > 1 ? 1 : static_cast<int>(256 / nv);
+    // several rows of a thread at a time once every block of the launch has as many
+    const int64_t turns = (c->n + p.block_rows - 1) / p.block_rows, most = static_cast<int64_t>(sm_count()) * (backward ? 4 : 6);
+    const int at_once = backward ? 2 : 4;
+    p.many = p.K == 1 && turns >= at_once * most;
+    p.blocks = std::min<int64_t>(turns, p.many ? most : 2 * most);
     if (backward) p.part = static_cast<size_t>(p.blocks) * 2 * c->channels * 4;
     return p;
   }
   p.V = norm_width(c, c->channels);
   const int64_t vecs = c->channels / p.V, at_once = 256 / std::min<int64_t>(vecs, 256);
   p.cblocks = (vecs + 255) / 256;
-  // blocks for eight a SM, of four turns at least
-  const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(sm_count()) * 8 / (c->n * p.cblocks));
+  // blocks for four a SM, of eight turns at least
+  const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(sm_count()) * 4 / (c->n * p.cblocks));
   p.per_chunk = (c->s + want - 1) / want;
   p.per_chunk = std::max<int64_t>((p.per_chunk + at_once - 1) / at_once, kNormAhead) * at_once;
   p.per_chunk = std::min<int64_t>(p.per_chunk, c->s);
@@ -2226,14 +2231,19 @@ int norm_check(const lact_group_norm_config* c) {
 template <class T, int V, bool BACKWARD>
 int launch_norm(const GroupNormArgs& a, const NormPlan& p, cudaStream_t st) {
   if (p.rows) {
-    const size_t smem = std::max<size_t>(8192, BACKWARD ? static_cast<size_t>(a.C) * 8 : 0);
+    const size_t smem = std::max<size_t>(8192, BACKWARD && p.K == 1 ? static_cast<size_t>(p.block_rows) * a.C * 8 : 0);   // (at most 256 vectors of 64 bytes)
     const dim3 grid(static_cast<unsigned>(p.blocks));
     {
       KernelScope scope(kClsOther, st);
+      constexpr int kMany = BACKWARD ? 2 : 4;
+      const dim3 threads(p.K > 1 ? 256 : (p.block_rows * (a.C / V) + 31) / 32 * 32);
       switch (p.K) {
-        case 1: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 1, BACKWARD>, grid, dim3(256), smem, st, a, p.lpr)); break;
-        case 2: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 2, BACKWARD>, grid, dim3(256), smem, st, a, p.lpr)); break;
-        default: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 4, BACKWARD>, grid, dim3(256), smem, st, a, p.lpr)); break;
+        case 1:
+          if (p.many) LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 1, kMany, BACKWARD>, grid, threads, smem, st, a, p.block_rows));
+          else LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 1, 1, BACKWARD>, grid, threads, smem, st, a, p.block_rows));
+          break;
+        case 2: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 2, 1, BACKWARD>, grid, threads, smem, st, a, p.block_rows)); break;
+        default: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 4, 1, BACKWARD>, grid, threads, smem, st, a, p.block_rows)); break;
       }
     }
     return LACT_OK;
