@@ -89,21 +89,28 @@ __device__ __forceinline__ void v_set(float (&d)[V], float x) {
 }
 template <int V>
 __device__ __forceinline__ float v_sum(const float (&a)[V]) {
-  float t[V];
+  if constexpr (V == 1) return a[0];
+  else {
+    F32x2 t = f32x2(a[0], a[1]);
 #pragma unroll
-  for (int i = 0; i < V; ++i) t[i] = a[i];
-#pragma unroll
-  for (int n = V / 2; n > 0; n /= 2)
-#pragma unroll
-    for (int i = 0; i < n; ++i) t[i] += t[i + n];
-  return t[0];
+    for (int i = 2; i < V; i += 2) t = f32x2_add(t, f32x2(a[i], a[i + 1]));
+    float x, y;
+    f32x2_split(t, x, y);
+    return x + y;
+  }
 }
 // sum of products
 template <int V>
 __device__ __forceinline__ float v_dot(const float (&a)[V], const float (&b)[V]) {
-  float t[V];
-  v_mul(t, a, b);
-  return v_sum(t);
+  if constexpr (V == 1) return a[0] * b[0];
+  else {
+    F32x2 t = f32x2_mul(f32x2(a[0], a[1]), f32x2(b[0], b[1]));
+#pragma unroll
+    for (int i = 2; i < V; i += 2) t = f32x2_fma(f32x2(a[i], a[i + 1]), f32x2(b[i], b[i + 1]), t);
+    float x, y;
+    f32x2_split(t, x, y);
+    return x + y;
+  }
 }
 
 // sigmoid(z) of V values.  Two special-function results an element (16 a clock and SM) take as long as the memory of a large call
@@ -119,11 +126,11 @@ __device__ __forceinline__ void sigmoids(const float (&z)[V], float (&g)[V]) {
     for (int i = 0; i < V; i += 2) {
       float x0, x1, a, b;
       f32x2_split(f32x2_mul(f32x2(z[i], z[i + 1]), k), x0, x1);
-      x0 = x0 > 60.f ? 60.f : x0;   // (not a minimum: NaN stays)
-      x1 = x1 > 60.f ? 60.f : x1;
-      f32x2_split(f32x2_add(f32x2(exp2_ftz(x0), exp2_ftz(x1)), one), a, b);
+      // (of NaN the minimum is 60: the callers multiply by z)
+      f32x2_split(f32x2_add(f32x2(exp2_ftz(fminf(x0, 60.f)), exp2_ftz(fminf(x1, 60.f))), one), a, b);
       const float r = rcp_ftz(a * b);
-      f32x2_split(f32x2_mul(f32x2(r, r), f32x2(b, a)), g[i], g[i + 1]);
+      g[i] = r * b;
+      g[i + 1] = r * a;
     }
   }
 }
@@ -191,9 +198,10 @@ struct GroupSums {
   }
 };
 
-// R rows of a thread at a time, fetched together and worked on side by side.
+// R rows of a thread at a time, fetched together while those before are worked on side by side.
+constexpr int kNormRowsAtOnce = 2;
 template <class T, int V, int K, int R, bool BACKWARD>
-__global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_constant__ GroupNormArgs a, int32_t rows) {
+__global__ void __launch_bounds__(256, 3) group_norm_rows_kernel(const __grid_constant__ GroupNormArgs a, int32_t rows) {
   constexpr int M = K * R;
   extern __shared__ float norm_smem[];
   griddep_launch_dependents();
@@ -221,14 +229,15 @@ __global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_const
     }
   }
   const int64_t step = static_cast<int64_t>(gridDim.x) * rows * R;
-  for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * rows * R; n0 < a.n; n0 += step) {
-    // (entry j: vector l + 256 (j % K) of row n0 + row + rows (j / K))
-    auto sample = [&](int j) { return n0 + row + static_cast<int64_t>(rows) * (j / K); };
-    auto vector = [&](int j) { return l + 256 * (j % K); };
-    auto on = [&](int j) { return here && vector(j) < nv && sample(j) < a.n; };
-    RawOf<T, V> raw[M];
-    [[maybe_unused]] RawOf<T, V> raw_dy[BACKWARD ? M : 1];
-    [[maybe_unused]] float2 st[BACKWARD ? M : 1];
+  int64_t n0 = static_cast<int64_t>(blockIdx.x) * rows * R;
+  // (entry j: vector l + 256 (j % K) of row n0 + row + rows (j / K))
+  auto sample = [&](int j) { return n0 + row + static_cast<int64_t>(rows) * (j / K); };
+  auto vector = [&](int j) { return l + 256 * (j % K); };
+  auto on = [&](int j) { return here && vector(j) < nv && sample(j) < a.n; };
+  RawOf<T, V> raw[M];
+  [[maybe_unused]] RawOf<T, V> raw_dy[BACKWARD ? M : 1];
+  [[maybe_unused]] float2 st[BACKWARD ? M : 1];
+  auto fetch = [&]() {   // entries that are not there: zeros all through
 #pragma unroll
     for (int j = 0; j < M; ++j) {
       raw[j] = RawOf<T, V>{};
@@ -243,6 +252,14 @@ __global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_const
         st[j] = *reinterpret_cast<const float2*>(a.stats + (sample(j) * a.G + vector(j) / gv) * 2);
       }
     }
+  };
+  fetch();
+  for (; n0 < a.n; n0 += step) {
+    auto fetch_next = [&]() {   // (on their way while the values of these are worked on)
+      n0 += step;
+      fetch();
+      n0 -= step;
+    };
     float x[M][V], p[M];
     if constexpr (!BACKWARD) {
       float mean[M];
@@ -251,6 +268,7 @@ __global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_const
         values_of<T, V>(raw[j], x[j]);
         p[j] = v_sum(x[j]);
       }
+      fetch_next();
       sums.template operator()<K>(p, row, l, here);
 #pragma unroll
       for (int j = 0; j < M; ++j) {
@@ -274,9 +292,10 @@ __global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_const
         store_values<T, V>(static_cast<T*>(a.out) + sample(j) * a.C + vector(j) * V, x[j]);
       }
     } else {
-      float t[M][V], q[M];
+      float t[M][V], q[M], rstd[M];
 #pragma unroll
-      for (int j = 0; j < M; ++j) {   // (entries that are not there: zeros all through)
+      for (int j = 0; j < M; ++j) {
+        rstd[j] = st[j].y;
         values_of<T, V>(raw[j], x[j]);
         values_of<T, V>(raw_dy[j], t[j]);
         float k[V], z[V];
@@ -295,6 +314,7 @@ __global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_const
         p[j] = v_sum(t[j]);
         q[j] = v_dot(t[j], x[j]);
       }
+      fetch_next();
       sums.template operator()<K>(p, row, l, here);
       sums.template operator()<K>(q, row, l, here);
 #pragma unroll
@@ -303,7 +323,7 @@ __global__ void __launch_bounds__(256) group_norm_rows_kernel(const __grid_const
         float c1[V], c2[V], k[V];   // (dz w - c1 first: where a group is one value, nothing is left of it)
         v_set(c1, -p[j] * inv);
         v_set(c2, -q[j] * inv);
-        v_set(k, st[j].y);
+        v_set(k, rstd[j]);
         v_add(t[j], t[j], c1);
         v_fma(x[j], x[j], c2, t[j]);
         v_mul(x[j], x[j], k);

@@ -2197,11 +2197,12 @@ NormPlan norm_plan(const lact_group_norm_config* c, bool backward) {
   if (p.rows) {
     p.K = nv <= 256 ? 1 : nv <= 512 ? 2 : 4;
     p.block_rows = p.K > 1 ? 1 : static_cast<int>(256 / nv);
-    // several rows of a thread at a time once every block of the launch has as many
-    const int64_t turns = (c->n + p.block_rows - 1) / p.block_rows, most = static_cast<int64_t>(sm_count()) * (backward ? 4 : 6);
-    const int at_once = backward ? 2 : 4;
-    p.many = p.K == 1 && turns >= at_once * most;
-    p.blocks = std::min<int64_t>(turns, p.many ? most : 2 * most);
+    // blocks of 768 threads a SM are there at once: as many as that in the launch, and (forward) several rows of a thread at a time once
+    // every block has them
+    const int64_t threads = p.K > 1 ? 256 : (p.block_rows * nv + 31) / 32 * 32;
+    const int64_t turns = (c->n + p.block_rows - 1) / p.block_rows, most = sm_count() * (768 / threads);
+    p.many = !backward && p.K == 1 && turns >= 2 * kNormRowsAtOnce * most;
+    p.blocks = std::min<int64_t>(turns, most);
     if (backward) p.part = static_cast<size_t>(p.blocks) * 2 * c->channels * 4;
     return p;
   }
@@ -2235,12 +2236,16 @@ int launch_norm(const GroupNormArgs& a, const NormPlan& p, cudaStream_t st) {
     const dim3 grid(static_cast<unsigned>(p.blocks));
     {
       KernelScope scope(kClsOther, st);
-      constexpr int kMany = BACKWARD ? 2 : 4;
       const dim3 threads(p.K > 1 ? 256 : (p.block_rows * (a.C / V) + 31) / 32 * 32);
       switch (p.K) {
         case 1:
-          if (p.many) LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 1, kMany, BACKWARD>, grid, threads, smem, st, a, p.block_rows));
-          else LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 1, 1, BACKWARD>, grid, threads, smem, st, a, p.block_rows));
+          if constexpr (!BACKWARD) {
+            if (p.many) {
+              LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 1, kNormRowsAtOnce, false>, grid, threads, smem, st, a, p.block_rows));
+              break;
+            }
+          }
+          LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 1, 1, BACKWARD>, grid, threads, smem, st, a, p.block_rows));
           break;
         case 2: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 2, 1, BACKWARD>, grid, threads, smem, st, a, p.block_rows)); break;
         default: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 4, 1, BACKWARD>, grid, threads, smem, st, a, p.block_rows)); break;
