@@ -372,7 +372,7 @@ int lact_linear_attention_step(const lact_linear_config *cfg, const void *q, con
  * y [n, s, C] of x's type, contiguous; y = act((x - mean) / sqrt(var + eps) * weight + bias) with mean and var over a sample's s spots
  * and the C / groups channels of a group; weight, bias fp32 [C] or NULL (ones, zeros); silu: the activation, or none.  stats (fp32
  * [n, groups, 2]) receives means and 1 / sqrt(var + eps), what the backward reads.  Backward: dx of x's type, contiguous, and
- * dweight, dbias ([2, C] fp32, one array), from dy.  workspace: 256-byte aligned, may be NULL if its size is 0.  No counterpart in the
+ * dweight, dbias (fp32 [C]), from dy.  workspace: 256-byte aligned, may be NULL if its size is 0.  No counterpart in the
  * reference, whose norm behind the recurrence is the RMS norm of lact_out_epilogue. */
 typedef struct lact_group_norm_config {
   int64_t n, s, channels, groups;
@@ -384,7 +384,8 @@ int lact_group_norm_workspace_bytes(const lact_group_norm_config *cfg, int32_t b
 int lact_group_norm_fwd(const lact_group_norm_config *cfg, const void *x, const float *weight, const float *bias, void *y, float *stats,
                         void *workspace, size_t workspace_bytes, void *stream);
 int lact_group_norm_bwd(const lact_group_norm_config *cfg, const void *x, const float *weight, const float *bias, const float *stats,
-                        const void *dy, void *dx, float *dweight_dbias, void *workspace, size_t workspace_bytes, void *stream);
+                        const void *dy, void *dx, float *dweight, float *dbias, void *workspace,
+                        size_t workspace_bytes, void *stream);
 
 /* Backward of lact_qkv_prologue / lact_qkv_prologue_rope on the saved projections (same strides): dq, dk, dv are the
  * gradients of the head-major outputs ([(b n_heads), s, d] bf16, NULL = none), dxq, dxk, dxv the gradients of the

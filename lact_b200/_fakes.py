@@ -155,7 +155,7 @@ def _(x, weight, bias, groups, eps, silu):
 
 @_fake("group_norm_bwd")
 def _(x, weight, bias, stats, dy, groups, eps, silu):
-    return [x.new_empty(x.shape), x.new_empty((2, x.shape[2]), dtype=F32)]
+    return [x.new_empty(x.shape)] + [x.new_empty((x.shape[-1],), dtype=F32) for _ in range(2)]
 
 
 @_fake("seq_start")

@@ -567,25 +567,32 @@ __global__ void __launch_bounds__(256) group_norm_groups_kernel(const __grid_con
   }
 }
 
-// Backward: dw, db = sums of `chan` over the samples: 32 channels a block, 8 samples at a time.
-__global__ void __launch_bounds__(256) group_norm_weights_kernel(const __grid_constant__ GroupNormArgs a) {
+// Backward: dw, db: 32 channels, from sums of `n` rows, eight at a time.
+__device__ __forceinline__ void norm_weights(const GroupNormArgs& a, int c, int64_t n, const float* first, const float* second, int64_t step,
+                                             int64_t next) {
   __shared__ float2 acc[8][32];
-  griddep_launch_dependents();
-  griddep_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float2 t = make_float2(0.f, 0.f);
-  if (c < a.C)
-    for (int64_t n = warp; n < a.n; n += 8) {
-      const float2 v = reinterpret_cast<const float2*>(a.chan)[n * a.C + c];
-      t = make_float2(t.x + v.x, t.y + v.y);
+  if (c < a.C) {
+#pragma unroll 4
+    for (int64_t i = warp; i < n; i += 8) {
+      t.x += first[c * step + i * next];
+      t.y += second[c * step + i * next];
     }
+  }
   acc[warp][lane] = t;
   __syncthreads();
   if (warp == 0 && c < a.C) {
     for (int i = 1; i < 8; ++i) t = make_float2(t.x + acc[i][lane].x, t.y + acc[i][lane].y);
-    a.db[c] = t.x;
-    a.dw[c] = t.y;
+    a.dw[c] = t.x;
+    a.db[c] = t.y;
   }
+}
+// ... of the blocks of group_norm_rows_kernel
+__global__ void __launch_bounds__(256) group_norm_weights_kernel(const __grid_constant__ GroupNormArgs a, int32_t blocks) {
+  griddep_launch_dependents();
+  griddep_wait();
+  norm_weights(a, blockIdx.x * 32 + (threadIdx.x & 31), blocks, a.part, a.part + a.C, 1, 2ll * a.C);
 }
 
 // y, or dx.  The blocks go through samples and chunks from the last to the first: what the sums have read last is still in L2.
@@ -593,7 +600,13 @@ template <class T, int V, bool BACKWARD>
 __global__ void __launch_bounds__(256, BACKWARD ? 2 : 4) group_norm_apply_kernel(const __grid_constant__ GroupNormArgs a) {
   griddep_launch_dependents();
   griddep_wait();
-  const int turn = gridDim.x - 1 - blockIdx.x;
+  const int64_t most = a.n * a.chunks;
+  if (BACKWARD && blockIdx.x >= most) {   // (sums of dz and of dz xhat per sample and channel)
+    const int64_t c = ((blockIdx.x - most) * gridDim.y + blockIdx.y) * 32 + (threadIdx.x & 31);
+    norm_weights(a, static_cast<int>(min(c, static_cast<int64_t>(a.C))), a.n, a.chan + 1, a.chan, 2, 2ll * a.C);
+    return;
+  }
+  const int turn = static_cast<int>(most - 1 - blockIdx.x);
   const int64_t n = turn / a.chunks;
   const NormSpots p = norm_spots<V>(a, turn % a.chunks, blockIdx.y);
   if (!p.on) return;

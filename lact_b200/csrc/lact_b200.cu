@@ -2134,16 +2134,32 @@ int linear_chunks(const LinearChunkArgs& a, const LinearPlan& p, bool carried, c
   }
   return launch_linear_chunks<A, B, false>(a, p.ctas, st);
 }
-int linear_run(const lact_linear_config* c, const LinearArgs& a, int64_t A, int64_t B, void* slots, bool carried, int32_t* status,
-               cudaStream_t st) {
+// An operand of a call: its array, and the map of its tiles (encoded once where several launches read it).
+struct LinearOperand {
+  const void* p;
+  int64_t ts, bs, heads, d;
+  CUtensorMap map;
+};
+int linear_map(const lact_linear_config* c, LinearOperand* o) {
+  return linear_plan(c).steps ? LACT_OK : encode_map_heads(&o->map, o->p, c->batch, c->tokens, o->heads, o->d, o->ts, o->bs);
+}
+void linear_operands(LinearArgs* a, const LinearOperand& x, const LinearOperand& y, const LinearOperand& z) {
+  a->x = static_cast<const bf16*>(x.p); a->x_ts = x.ts; a->x_bs = x.bs; a->x_share = a->heads / static_cast<int32_t>(x.heads);
+  a->y = static_cast<const bf16*>(y.p); a->y_ts = y.ts; a->y_bs = y.bs; a->y_share = a->heads / static_cast<int32_t>(y.heads);
+  a->z = static_cast<const bf16*>(z.p); a->z_ts = z.ts; a->z_bs = z.bs; a->z_share = a->heads / static_cast<int32_t>(z.heads);
+}
+int linear_run(const lact_linear_config* c, LinearArgs& a, const LinearOperand& x, const LinearOperand& y, const LinearOperand& z, void* slots,
+               bool carried, int32_t* status, cudaStream_t st) {
   const LinearPlan p = linear_plan(c);
+  const int64_t A = x.d, B = z.d;
+  linear_operands(&a, x, y, z);
   if (p.steps) return linear_steps(a, A, B, st);
   LinearChunkArgs k;
   std::memset(&k, 0, sizeof(k));
   k.a = a;
-  LACT_TRY(encode_map_heads(&k.x, a.x, c->batch, c->tokens, c->heads / a.x_share, A, a.x_ts, a.x_bs));
-  LACT_TRY(encode_map_heads(&k.y, a.y, c->batch, c->tokens, c->heads / a.y_share, A, a.y_ts, a.y_bs));
-  LACT_TRY(encode_map_heads(&k.z, a.z, c->batch, c->tokens, c->heads / a.z_share, B, a.z_ts, a.z_bs));
+  k.x = x.map;
+  k.y = y.map;
+  k.z = z.map;
   k.per = static_cast<uint32_t>(p.per);
   k.slots = static_cast<float*>(slots);
   k.pieces = reinterpret_cast<LinearPiece*>(static_cast<uint8_t*>(slots) + static_cast<size_t>(p.ctas) * A * B * 4);
@@ -2251,19 +2267,21 @@ int launch_norm(const GroupNormArgs& a, const NormPlan& p, cudaStream_t st) {
         default: LACT_CUDA(launch_pdl(group_norm_rows_kernel<T, V, 4, 1, BACKWARD>, grid, threads, smem, st, a, p.block_rows)); break;
       }
     }
+    if (BACKWARD) {
+      KernelScope scope(kClsOther, st);
+      LACT_CUDA(launch_pdl(group_norm_weights_kernel, dim3(static_cast<unsigned>((a.C + 31) / 32)), dim3(256), 0, st, a, static_cast<int32_t>(p.blocks)));
+    }
     return LACT_OK;
   }
   const int64_t blocks = a.n * p.chunks;
-  if (blocks > 0x7FFFFFFFll || p.cblocks > 65535) return LACT_ERR_SHAPE;
+  if (blocks + a.C > 0x7FFFFFFFll || p.cblocks > 65535) return LACT_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.cblocks));
   { KernelScope scope(kClsOther, st); LACT_CUDA(launch_pdl(group_norm_sums_kernel<T, V, BACKWARD>, grid, dim3(256), 0, st, a)); }
   { KernelScope scope(kClsOther, st); LACT_CUDA(launch_pdl(group_norm_groups_kernel<BACKWARD>, dim3(static_cast<unsigned>(a.n * a.G)), dim3(256), 0, st, a)); }
-  if (BACKWARD) {
-    KernelScope scope(kClsOther, st);
-    LACT_CUDA(launch_pdl(group_norm_weights_kernel, dim3(static_cast<unsigned>((a.C + 31) / 32)), dim3(256), 0, st, a));
-  }
+  // (backward: behind the blocks that write dx, one for every 32 channels of the weights' gradients)
+  const dim3 all(static_cast<unsigned>(blocks + (BACKWARD ? ceil_div(a.C, 32 * p.cblocks) : 0)), grid.y);
   KernelScope scope(kClsOther, st);
-  LACT_CUDA(launch_pdl(group_norm_apply_kernel<T, V, BACKWARD>, grid, dim3(256), 0, st, a));
+  LACT_CUDA(launch_pdl(group_norm_apply_kernel<T, V, BACKWARD>, all, dim3(256), 0, st, a));
   return LACT_OK;
 }
 template <bool BACKWARD>
@@ -3442,15 +3460,13 @@ int lact_linear_attention_fwd(const lact_linear_config* c, const void* q, const 
   size_t need = 0;
   LACT_TRY(lact_linear_attention_workspace_bytes(c, 0, &need));
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return LACT_ERR_WORKSPACE;
+  LinearOperand Q{q, c->q_ts, c->q_bs, c->heads, c->dk}, K{k, c->k_ts, c->k_bs, c->kv_heads, c->dk}, V{v, c->v_ts, c->v_bs, c->kv_heads, c->dv};
+  for (LinearOperand* t : {&Q, &K, &V}) LACT_TRY(linear_map(c, t));
   LinearArgs a = linear_args(c, log_decay, cu);
-  a.x = static_cast<const bf16*>(q); a.x_ts = c->q_ts; a.x_bs = c->q_bs;
-  a.y = static_cast<const bf16*>(k); a.y_ts = c->k_ts; a.y_bs = c->k_bs;
-  a.z = static_cast<const bf16*>(v); a.z_ts = c->v_ts; a.z_bs = c->v_bs;
-  a.y_share = a.z_share = static_cast<int32_t>(c->heads / c->kv_heads);
   a.out = o;
   a.s_in = state_in;
   a.s_out = state_out;
-  return linear_run(c, a, c->dk, c->dv, workspace, false, status_word, static_cast<cudaStream_t>(stream));
+  return linear_run(c, a, Q, K, V, workspace, false, status_word, static_cast<cudaStream_t>(stream));
 }
 
 int lact_linear_attention_step(const lact_linear_config* c, const void* q, const void* k, const void* v, const float* log_decay,
@@ -3463,10 +3479,8 @@ int lact_linear_attention_step(const lact_linear_config* c, const void* q, const
   LACT_TRY(linear_operand(v, c->v_ts, c->v_bs, c->kv_heads * c->dv));
   LACT_TRY(check_device());
   LinearArgs a = linear_args(c, log_decay, nullptr);
-  a.x = static_cast<const bf16*>(q); a.x_ts = c->q_ts; a.x_bs = c->q_bs;
-  a.y = static_cast<const bf16*>(k); a.y_ts = c->k_ts; a.y_bs = c->k_bs;
-  a.z = static_cast<const bf16*>(v); a.z_ts = c->v_ts; a.z_bs = c->v_bs;
-  a.y_share = a.z_share = static_cast<int32_t>(c->heads / c->kv_heads);
+  linear_operands(&a, {q, c->q_ts, c->q_bs, c->heads, c->dk, {}}, {k, c->k_ts, c->k_bs, c->kv_heads, c->dk, {}},
+                  {v, c->v_ts, c->v_bs, c->kv_heads, c->dv, {}});
   a.out = o;
   a.s_in = state_in;
   a.s_out = state_out;
@@ -3495,24 +3509,17 @@ int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const 
   float* const each_head = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (linear_slots(linear_plan(c), c->dk, c->dv) + 255) / 256 * 256);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int32_t share = static_cast<int32_t>(c->heads / c->kv_heads);
-  struct Operand { const void* p; int64_t ts, bs; int32_t share; };
-  const Operand Q{q, c->q_ts, c->q_bs, 1}, K{k, c->k_ts, c->k_bs, share}, V{v, c->v_ts, c->v_bs, share}, DO{dout, c->do_ts, c->do_bs, 1};
-  auto with = [&](const Operand& x, const Operand& y, const Operand& z, void* out, bool reverse) {
+  LinearOperand Q{q, c->q_ts, c->q_bs, c->heads, c->dk}, K{k, c->k_ts, c->k_bs, c->kv_heads, c->dk}, V{v, c->v_ts, c->v_bs, c->kv_heads, c->dv},
+      DO{dout, c->do_ts, c->do_bs, c->heads, c->dv};
+  for (LinearOperand* t : {&Q, &K, &V, &DO}) LACT_TRY(linear_map(c, t));
+  auto backwards = [&](void* out) {
     LinearArgs a = linear_args(c, log_decay, cu);
-    a.x = static_cast<const bf16*>(x.p); a.x_ts = x.ts; a.x_bs = x.bs; a.x_share = x.share;
-    a.y = static_cast<const bf16*>(y.p); a.y_ts = y.ts; a.y_bs = y.bs; a.y_share = y.share;
-    a.z = static_cast<const bf16*>(z.p); a.z_ts = z.ts; a.z_bs = z.bs; a.z_share = z.share;
-    a.out = out;
-    a.reverse = reverse;
-    if (reverse) {
-      a.in_mul = 1.f / c->scale;
-      a.out_mul = c->scale;
-      a.s_in = dstate_out;
-      if (share > 1) {
-        a.out = each_head;
-        a.out_f32 = 1;
-      }
-    }
+    a.out = share > 1 ? each_head : out;
+    a.out_f32 = share > 1;
+    a.reverse = 1;
+    a.in_mul = 1.f / c->scale;
+    a.out_mul = c->scale;
+    a.s_in = dstate_out;
     return a;
   };
   auto add_up = [&](void* out, int64_t d) -> int {
@@ -3523,18 +3530,19 @@ int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const 
                          static_cast<const float*>(each_head), static_cast<bf16*>(out), n4, share, static_cast<int32_t>(d / 4)));
     return LACT_OK;
   };
-  LinearArgs a = with(DO, V, K, dq, false);
+  LinearArgs a = linear_args(c, log_decay, cu);
+  a.out = dq;
   a.s_in = state_in;
   a.s_in_t = 1;
   // (the CTAs begin with the forward's states, transposed; they are read alone)
-  LACT_TRY(linear_run(c, a, c->dv, c->dk, const_cast<void*>(fwd_workspace), true, status_word, st));
-  a = with(K, Q, DO, dv, true);
+  LACT_TRY(linear_run(c, a, DO, V, K, const_cast<void*>(fwd_workspace), true, status_word, st));
+  a = backwards(dv);
   a.s_out = dstate_in;
-  LACT_TRY(linear_run(c, a, c->dk, c->dv, workspace, false, status_word, st));
+  LACT_TRY(linear_run(c, a, K, Q, DO, workspace, false, status_word, st));
   LACT_TRY(add_up(dv, c->dv));
-  a = with(V, DO, Q, dk, true);
+  a = backwards(dk);
   a.s_in_t = 1;
-  LACT_TRY(linear_run(c, a, c->dv, c->dk, workspace, true, status_word, st));   // the CTAs begin with the states of dv, transposed
+  LACT_TRY(linear_run(c, a, V, DO, Q, workspace, true, status_word, st));   // the CTAs begin with the states of dv, transposed
   return add_up(dk, c->dk);
 }
 
@@ -3563,9 +3571,9 @@ int lact_group_norm_fwd(const lact_group_norm_config* c, const void* x, const fl
 }
 
 int lact_group_norm_bwd(const lact_group_norm_config* c, const void* x, const float* weight, const float* bias, const float* stats,
-                        const void* dy, void* dx, float* dweight_dbias, void* workspace, size_t workspace_bytes, void* stream) {
+                        const void* dy, void* dx, float* dweight, float* dbias, void* workspace, size_t workspace_bytes, void* stream) {
   LACT_TRY(norm_check(c));
-  if (!x || !stats || !dy || !dx || !dweight_dbias) return LACT_ERR_NULL;
+  if (!x || !stats || !dy || !dx || !dweight || !dbias) return LACT_ERR_NULL;
   if ((reinterpret_cast<uintptr_t>(dx) & 15) != 0 || (reinterpret_cast<uintptr_t>(stats) & 7) != 0) return LACT_ERR_SHAPE;
   LACT_TRY(check_device());
   LACT_TRY(norm_operand(c, x, c->x_ns, c->x_ss));
@@ -3576,10 +3584,9 @@ int lact_group_norm_bwd(const lact_group_norm_config* c, const void* x, const fl
   a.dy = dy;
   a.out = dx;
   a.stats = const_cast<float*>(stats);
-  a.dw = dweight_dbias;
-  a.db = dweight_dbias + c->channels;
-  LACT_TRY(norm_run<true>(a, p, c->dtype, static_cast<cudaStream_t>(stream)));
-  return p.rows ? lact_column_sums(a.part, dweight_dbias, p.blocks, 2 * c->channels, stream) : LACT_OK;
+  a.dw = dweight;
+  a.db = dbias;
+  return norm_run<true>(a, p, c->dtype, static_cast<cudaStream_t>(stream));
 }
 
 int lact_l2_norm_add(const void* x, int32_t x_dtype, const void* x_add, int32_t add_dtype, const void* scale, void* y,

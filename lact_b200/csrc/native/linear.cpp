@@ -15,6 +15,15 @@ Tensor head_view(const Tensor& t) {
   return t;
 }
 
+// [b, h, d] likewise
+Tensor token_view(const Tensor& t) {
+  if (t.stride(2) != 1 || t.stride(1) != t.size(2) || t.stride(0) % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) {
+    Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+  }
+  return t;
+}
+
 const float* f32(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 Tensor whole(const OptTensor& t) {
   if (!given(t)) return Tensor();
@@ -106,8 +115,13 @@ Tensor step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& 
   TORCH_CHECK_VALUE(from == to || from + size <= to || to + size <= from, "new_state overlaps state without being the same array");
   Tensor o = empty({q_.size(0), q_.size(1), v_.size(2)}, at::kBFloat16, q_);
   if (q_.size(0) == 0) return o;
-  const Tensor q = head_view(q_.unsqueeze(1)), k = head_view(k_.unsqueeze(1)), v = head_view(v_.unsqueeze(1)), g = g_.contiguous();
-  const lact_linear_config c = config(q, k, v, scale, {});
+  const Tensor q = token_view(q_), k = token_view(k_), v = token_view(v_), g = g_.contiguous();
+  lact_linear_config c{};
+  c.batch = q.size(0); c.tokens = 1; c.heads = q.size(1); c.kv_heads = k.size(1); c.dk = q.size(2); c.dv = v.size(2);
+  c.q_bs = q.stride(0); c.q_ts = c.heads * c.dk;
+  c.k_bs = k.stride(0); c.k_ts = c.kv_heads * c.dk;
+  c.v_bs = v.stride(0); c.v_ts = c.kv_heads * c.dv;
+  c.scale = static_cast<float>(scale);
   poll_status(q);
   check(lact_linear_attention_step(&c, ptr(q), ptr(k), ptr(v), f32(g), state.data_ptr<float>(), new_state.data_ptr<float>(), ptr(o),
                                    stream_of(q)),

@@ -29,12 +29,15 @@ lact_group_norm_config config(const Tensor& x, int64_t groups, double eps, bool 
   return c;
 }
 
+// [n, ..., C] as [n, s, C]
+Tensor three(const Tensor& t) { return t.dim() == 3 ? t : t.dim() == 2 ? t.unsqueeze(1) : t.flatten(1, -2); }
+
 // y and the statistics
 std::vector<Tensor> fwd(const Tensor& x_, const OptTensor& w_, const OptTensor& b_, int64_t groups, double eps, bool silu) {
   const c10::cuda::CUDAGuard guard(x_.device());
   Tensor y = empty(x_.sizes(), x_.scalar_type(), x_), stats = empty({x_.size(0), groups, 2}, at::kFloat, x_);
   if (x_.numel() == 0) return {y, stats.zero_()};
-  const Tensor x = rows_of(x_), w = weights_of(w_), b = weights_of(b_);
+  const Tensor x = rows_of(three(x_)), w = weights_of(w_), b = weights_of(b_);
   const lact_group_norm_config c = config(x, groups, eps, silu);
   size_t need = 0;
   check(lact_group_norm_workspace_bytes(&c, 0, &need), "lact_group_norm_workspace_bytes");
@@ -46,13 +49,13 @@ std::vector<Tensor> fwd(const Tensor& x_, const OptTensor& w_, const OptTensor& 
   return {y, stats};
 }
 
-// dx, and dw, db ([2, C] fp32)
+// dx, dw, db
 std::vector<Tensor> bwd(const Tensor& x_, const OptTensor& w_, const OptTensor& b_, const Tensor& stats_, const Tensor& dy_, int64_t groups,
                         double eps, bool silu) {
   const c10::cuda::CUDAGuard guard(x_.device());
-  Tensor dx = empty(x_.sizes(), x_.scalar_type(), x_), dwb = empty({2, x_.size(2)}, at::kFloat, x_);
-  if (x_.numel() == 0) return {dx, dwb.zero_()};
-  const Tensor x = rows_of(x_), dy = rows_of(dy_.to(x_.scalar_type())), w = weights_of(w_), b = weights_of(b_), stats = stats_.contiguous();
+  Tensor dx = empty(x_.sizes(), x_.scalar_type(), x_), dw = empty({x_.size(-1)}, at::kFloat, x_), db = at::empty_like(dw);
+  if (x_.numel() == 0) return {dx, dw.zero_(), db.zero_()};
+  const Tensor x = rows_of(three(x_)), dy = rows_of(three(dy_.to(x_.scalar_type()))), w = weights_of(w_), b = weights_of(b_), stats = stats_.contiguous();
   lact_group_norm_config c = config(x, groups, eps, silu);
   c.dy_ns = c.n > 1 ? dy.stride(0) : 0;
   c.dy_ss = c.s > 1 ? dy.stride(1) : 0;
@@ -61,11 +64,11 @@ std::vector<Tensor> bwd(const Tensor& x_, const OptTensor& w_, const OptTensor& 
   Tensor room;
   if (need > 0) room = bytes(need, x);
   poll_status(x);
-  check(lact_group_norm_bwd(&c, ptr(x), f32(w), f32(b), stats.data_ptr<float>(), ptr(dy), ptr(dx), dwb.data_ptr<float>(),
-                            need > 0 ? ptr(room) : nullptr, need, stream_of(x)),
+  check(lact_group_norm_bwd(&c, ptr(x), f32(w), f32(b), stats.data_ptr<float>(), ptr(dy), ptr(dx), dw.data_ptr<float>(),
+                            db.data_ptr<float>(), need > 0 ? ptr(room) : nullptr, need, stream_of(x)),
         "lact_group_norm_bwd");
   settle(x);
-  return {dx, dwb};
+  return {dx, dw, db};
 }
 
 using FwdSig = std::vector<Tensor>(const Tensor&, const OptTensor&, const OptTensor&, int64_t, double, bool);
@@ -98,8 +101,8 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
     if (!g[0].defined()) return variable_list(6);
     const auto r = bwd_op().call(t[0], opt(t[1]), opt(t[2]), t[3], g[0], ctx->saved_data["groups"].toInt(),
                                  ctx->saved_data["eps"].toDouble(), ctx->saved_data["silu"].toBool());
-    auto row = [&](const Tensor& like, int i) { return like.defined() ? r[1].select(0, i).to(like.scalar_type()) : Tensor(); };
-    return {r[0], row(t[1], 0), row(t[2], 1), Tensor(), Tensor(), Tensor()};
+    auto as = [&](const Tensor& like, const Tensor& g) { return like.defined() ? g.to(like.scalar_type()) : Tensor(); };
+    return {r[0], as(t[1], r[1]), as(t[2], r[2]), Tensor(), Tensor(), Tensor()};
   }
 };
 std::vector<Tensor> norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t groups, double eps, bool silu) {

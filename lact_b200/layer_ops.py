@@ -109,6 +109,8 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     "silu"; weight, bias [C] float32 or bf16, or None.  Behind a token mixer, x [tokens, heads * d] with num_groups = heads is
     the norm of every head of every token (one spot a sample); maps and frames are [n, h, w, C] or [n, frames, h, w, C].
     Result: x's shape and type, contiguous.  Differentiable with respect to x, weight and bias."""
+    if activation not in (None, "silu"):
+        raise ValueError("activation: None or 'silu'")
     if x.dim() < 2:
         raise ValueError("x: [n, ..., channels]")
     if x.dtype not in (BF16, torch.float32):
@@ -116,41 +118,39 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     C = x.shape[-1]
     if num_groups < 1 or C == 0 or C % num_groups:
         raise ValueError("num_groups must divide the channels")
-    if activation not in (None, "silu"):
-        raise ValueError("activation: None or 'silu'")
-    if not (eps >= 0.0 and math.isfinite(eps)):
+    if not 0.0 <= eps < math.inf:
         raise ValueError("eps must be finite and not negative")
-    for name, t in (("weight", weight), ("bias", bias)):
+    for t in (weight, bias):
         if t is None:
             continue
-        if t.shape != (C,) or t.device != x.device:
-            raise ValueError(f"{name}: [channels] on the device of x")
+        if t.dim() != 1 or t.shape[0] != C or t.get_device() != x.get_device():
+            raise ValueError("weight, bias: [channels] on the device of x")
         if t.dtype not in (BF16, torch.float32):
-            raise TypeError(f"{name}: bf16 or float32")
+            raise TypeError("weight, bias: bf16 or float32")
     if not x.is_cuda:
         raise ValueError("group_norm needs CUDA tensors (there is no CPU implementation)")
-    flat = x if x.dim() == 3 else x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
-    return L.call(_op("group_norm_fwd"), flat, weight, bias, int(num_groups), float(eps), activation == "silu")[0].reshape(x.shape)
+    return L.call(_op("group_norm_fwd"), x, weight, bias, num_groups, eps, activation == "silu")[0]
 
 
 # ------------------------------------------------------------------------------------------ linear attention
 def _linear_heads(what, q, k, v, log_decay, dims):
     """Checks shared by the prompt and the token form (`dims` axes, heads and features last); returns heads, dk, dv."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != dims:
-            raise ValueError(f"{name} must have {dims} axes")
-        if t.dtype != BF16:
-            raise TypeError(f"{name}: bf16 activations")
-    h, hk, dk, dv = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
-    if q.shape[:-2] != k.shape[:-2] or k.shape[:-1] != v.shape[:-1] or k.shape[-1] != dk:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != dims or len(ks) != dims or len(vs) != dims:
+        raise ValueError(f"q, k, v must have {dims} axes")
+    if q.dtype != BF16 or k.dtype != BF16 or v.dtype != BF16:
+        raise TypeError("q, k, v: bf16 activations")
+    h, dk, dv = qs[-2], qs[-1], vs[-1]
+    if qs[:-2] != ks[:-2] or ks[:-1] != vs[:-1] or ks[-1] != dk:
         raise ValueError("q [..., h, dk], k [..., h_kv, dk], v [..., h_kv, dv] of the same batch and tokens")
     if dk not in (64, 128) or dv not in (64, 128):
         raise ValueError("dk and dv must be 64 or 128")
-    if h == 0 or hk == 0 or h % hk:
+    if h == 0 or ks[-2] == 0 or h % ks[-2]:
         raise ValueError("the heads of k and v must divide those of q")
-    if log_decay.shape != (h,) or log_decay.dtype != torch.float32:
+    if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or log_decay.shape[0] != h:
         raise ValueError("log_decay: [heads] in float32")
-    if any(t.device != q.device for t in (k, v, log_decay)):
+    at = q.get_device()
+    if k.get_device() != at or v.get_device() != at or log_decay.get_device() != at:
         raise ValueError("all tensors must be on the same device")
     if not q.is_cuda:
         raise ValueError(f"{what} needs CUDA tensors (there is no CPU implementation)")
@@ -158,14 +158,16 @@ def _linear_heads(what, q, k, v, log_decay, dims):
 
 
 def _linear_scale(scale, dk):
-    scale = float(scale) if scale is not None else dk ** -0.5
+    if scale is None:
+        return dk ** -0.5
+    scale = float(scale)
     if not math.isfinite(scale) or abs(scale) < 1e-30 or abs(scale) > 1e30:
         raise ValueError("scale must be finite and not zero")
     return scale
 
 
 def _linear_state(name, state, shape, device):
-    if tuple(state.shape) != shape or state.dtype != torch.float32 or state.device != device:
+    if state.shape != shape or state.dtype != torch.float32 or state.get_device() != device:
         raise ValueError(f"{name}: a float32 {list(shape)} tensor on the device of q")
 
 
@@ -194,7 +196,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         cu_seqlens = cu_seqlens.to(device=q.device, dtype=torch.int32).contiguous()
         n = cu_seqlens.numel() - 1
     if initial_state is not None:
-        _linear_state("initial_state", initial_state, (n, h, dk, dv), q.device)
+        _linear_state("initial_state", initial_state, (n, h, dk, dv), q.get_device())
     r = L.call(_op("linear_attention_fwd"), q, k, v, log_decay, _linear_scale(scale, dk), initial_state, cu_seqlens,
                bool(output_final_state))
     return r[0], r[1] if output_final_state else None
@@ -206,14 +208,17 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     v [b, h_kv, dv] bf16, state [b, h, dk, dv] float32, contiguous: read, and written in place, or to `new_state` (an array apart
     from it).  Returns o [b, h, dv] bf16.  No backward: a call with gradients raises."""
     h, dk, dv = _linear_heads("linear_attention_step", q, k, v, log_decay, 3)
-    for name, t in (("state", state), ("new_state", state if new_state is None else new_state)):
-        _linear_state(name, t, (q.shape[0], h, dk, dv), q.device)
+    shape, at = (q.shape[0], h, dk, dv), q.get_device()
+    if new_state is None:
+        new_state = state
+    for t in (state,) if new_state is state else (state, new_state):
+        _linear_state("state, new_state", t, shape, at)
         if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous: it is written where it lies")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, state, new_state)):
+            raise ValueError("state and new_state must be contiguous: they are read and written where they lie")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad or state.requires_grad or
+                                    new_state.requires_grad):
         raise NotImplementedError("linear_attention_step has no backward: use linear_attention")
-    return L.call(_op("linear_attention_step"), q, k, v, log_decay, _linear_scale(scale, dk), state,
-                  state if new_state is None else new_state)
+    return L.call(_op("linear_attention_step"), q, k, v, log_decay, _linear_scale(scale, dk), state, new_state)
 
 
 # ------------------------------------------------------------------------------------------ sliding-window attention

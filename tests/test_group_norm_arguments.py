@@ -35,7 +35,7 @@ def test_bad_configurations_are_refused(lib, over, code):
     n, c, p = C.c_size_t(0), _config(**over), C.c_void_p(4096)
     assert lib.lact_group_norm_workspace_bytes(C.byref(c), 0, C.byref(n)) == code
     assert lib.lact_group_norm_fwd(C.byref(c), p, p, p, p, p, None, C.c_size_t(0), None) == code
-    assert lib.lact_group_norm_bwd(C.byref(c), p, p, p, p, p, p, p, None, C.c_size_t(0), None) == code
+    assert lib.lact_group_norm_bwd(C.byref(c), p, p, p, p, p, p, p, p, None, C.c_size_t(0), None) == code
 
 
 def test_missing_and_crooked_pointers_are_refused(lib):
@@ -43,7 +43,7 @@ def test_missing_and_crooked_pointers_are_refused(lib):
     assert lib.lact_group_norm_fwd(C.byref(c), None, p, p, p, p, None, z, None) == -1
     assert lib.lact_group_norm_fwd(C.byref(c), p, None, None, None, p, None, z, None) == -1
     assert lib.lact_group_norm_fwd(C.byref(c), p, p, p, C.c_void_p(4098), p, None, z, None) == -2
-    assert lib.lact_group_norm_bwd(C.byref(c), p, p, p, p, None, p, p, None, z, None) == -1
+    assert lib.lact_group_norm_bwd(C.byref(c), p, p, p, p, None, p, p, p, None, z, None) == -1
     assert lib.lact_group_norm_workspace_bytes(None, 0, C.byref(z)) == -1
 
 
@@ -51,7 +51,7 @@ def test_missing_and_crooked_pointers_are_refused(lib):
 def test_strides_that_break_an_access_are_refused(lib, over, back):
     c, p, z = _config(**over), C.c_void_p(4096), C.c_size_t(0)
     if back:
-        assert lib.lact_group_norm_bwd(C.byref(c), p, p, p, p, p, p, p, None, z, None) in (-2, -7, -8)
+        assert lib.lact_group_norm_bwd(C.byref(c), p, p, p, p, p, p, p, p, None, z, None) in (-2, -7, -8)
     else:
         assert lib.lact_group_norm_fwd(C.byref(c), p, p, p, p, p, None, z, None) in (-2, -7, -8)   # (-7, -8: no device here)
 
