@@ -574,7 +574,7 @@ __device__ __forceinline__ void norm_weights(const GroupNormArgs& a, int c, int6
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float2 t = make_float2(0.f, 0.f);
   if (c < a.C) {
-#pragma unroll 4
+#pragma unroll 16
     for (int64_t i = warp; i < n; i += 8) {
       t.x += first[c * step + i * next];
       t.y += second[c * step + i * next];

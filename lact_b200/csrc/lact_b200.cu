@@ -2057,7 +2057,7 @@ int linear_check(const lact_linear_config* c, const void* cu) {
   if ((c->sequences > 0) != (cu != nullptr) || (cu != nullptr && c->batch != 1)) return LACT_ERR_CONFIG;
   // (sequence, head)s and their tiles of 128 tokens are counted in 31 bits
   const int64_t n = c->sequences > 0 ? c->sequences : c->batch;
-  if (n * c->heads > (1ll << 30) || ((c->tokens + 127) / 128 * c->batch + n) * c->heads > (1ll << 30)) return LACT_ERR_SHAPE;
+  if (n * c->heads > (1ll << 28) || ((c->tokens + 127) / 128 * c->batch + n) * c->heads > (1ll << 30)) return LACT_ERR_SHAPE;
   if (!(c->scale > -INFINITY && c->scale < INFINITY) || c->scale == 0.f) return LACT_ERR_CONFIG;
   return LACT_OK;
 }
@@ -2069,12 +2069,23 @@ int linear_operand(const void* p, int64_t ts, int64_t bs, int64_t row) {
 template <int A, int B>
 int launch_linear_steps(const LinearArgs& a, cudaStream_t st) {
   KernelScope scope(kClsOther, st);
-  LACT_CUDA(launch_pdl(linear_steps_kernel<A, B>, dim3(static_cast<unsigned>(a.sequences) * a.heads, B / 32), dim3(256), 0, st, a));
+  LACT_CUDA(launch_pdl(linear_steps_kernel<A, B>, dim3(static_cast<unsigned>(a.sequences) * a.heads * (B / 32)), dim3(256), 0, st, a));
   return LACT_OK;
 }
 int linear_steps(const LinearArgs& a, int64_t A, int64_t B, cudaStream_t st) {
   if (A == 64) return B == 64 ? launch_linear_steps<64, 64>(a, st) : launch_linear_steps<64, 128>(a, st);
   return B == 64 ? launch_linear_steps<128, 64>(a, st) : launch_linear_steps<128, 128>(a, st);
+}
+
+template <int A, int B>
+int launch_linear_token(const LinearArgs& a, cudaStream_t st) {
+  KernelScope scope(kClsOther, st);
+  LACT_CUDA(launch_pdl(linear_token_kernel<A, B>, dim3(static_cast<unsigned>(a.sequences) * a.heads * (B / 32)), dim3(256), 0, st, a));
+  return LACT_OK;
+}
+int linear_token(const LinearArgs& a, int64_t A, int64_t B, cudaStream_t st) {
+  if (A == 64) return B == 64 ? launch_linear_token<64, 64>(a, st) : launch_linear_token<64, 128>(a, st);
+  return B == 64 ? launch_linear_token<128, 64>(a, st) : launch_linear_token<128, 128>(a, st);
 }
 
 // How a call's tiles are dealt to CTAs.
@@ -3484,7 +3495,7 @@ int lact_linear_attention_step(const lact_linear_config* c, const void* q, const
   a.out = o;
   a.s_in = state_in;
   a.s_out = state_out;
-  return linear_steps(a, c->dk, c->dv, static_cast<cudaStream_t>(stream));
+  return linear_token(a, c->dk, c->dv, static_cast<cudaStream_t>(stream));
 }
 
 int lact_linear_attention_bwd(const lact_linear_config* c, const void* q, const void* k, const void* v, const float* log_decay,

@@ -15,7 +15,7 @@
 // is an output.
 // Long sequences of few heads: `per` tiles a CTA may begin within a sequence.  linear_chunks_kernel<..., PIECE> first leaves every CTA's
 // share of the state of the sequence that goes on behind it, linear_carry_kernel adds the shares up in order.  The shares are taken
-// from the last tile to the first, so that the tiles the CTA begins with afterwards have been read last and are still in L2.
+// from the last tile to the first, so that the tiles the CTA begins with afterwards have been read last and are still in L2, and only as far as fp32 has room for their decay.
 #pragma once
 #include "linear_steps.cuh"
 #include "umma_gemm.cuh"
@@ -50,7 +50,7 @@ template <int A, int B>
 struct LinearSmem {
   static constexpr bool kRing5 = A == 128 && B == 128;   // no room for two whole stages beside the rest: five tiles of 32 KB in a ring
   static constexpr int kStages = kRing5 || A == 128 ? 2 : B == 128 ? 3 : 4;
-  static constexpr int kPieceStages = kRing5 ? 2 : A == 128 ? 3 : 4;                     // of Y and Z alone
+  static constexpr int kPieceStages = kRing5 || A == 128 ? 3 : 4;   // of Y and Z alone (the ring of five holds two and a half)
   static constexpr uint32_t kXY = 128 * A * 2, kZ = 128 * B * 2;
   static constexpr uint32_t kTiles = kRing5 ? 5 * kXY : kStages * (2 * kXY + kZ);
   static constexpr uint32_t kLow = kTiles;          // second piece of Y
@@ -58,12 +58,13 @@ struct LinearSmem {
   static constexpr uint32_t kBars = kS + kXY;
   static constexpr uint32_t kFactors = kBars + 256; // a table of 32 decays per row warp
   static constexpr uint32_t kBytes = kFactors + kLinearRowWarps * 128;
-  static_assert(kPieceStages * (kXY + kZ) <= kTiles, "the stages of the shares fit");
+  static_assert(kRing5 || kPieceStages * (kXY + kZ) <= kTiles, "the stages of the shares fit");
   // where X, Y, Z of the CTA's tile t lie
   static __device__ __forceinline__ uint32_t x(int t) { return kRing5 ? 3 * t % 5 * kXY : t % kStages * (2 * kXY + kZ); }
   static __device__ __forceinline__ uint32_t y(int t) { return kRing5 ? (3 * t + 1) % 5 * kXY : x(t) + kXY; }
   static __device__ __forceinline__ uint32_t z(int t) { return kRing5 ? (3 * t + 2) % 5 * kXY : x(t) + 2 * kXY; }
-  static __device__ __forceinline__ uint32_t piece_y(int t) { return t % kPieceStages * (kXY + kZ); }
+  static __device__ __forceinline__ uint32_t piece_y(int t) { return kRing5 ? 2 * t % 5 * kXY : t % kPieceStages * (kXY + kZ); }
+  static __device__ __forceinline__ uint32_t piece_z(int t) { return kRing5 ? (2 * t + 1) % 5 * kXY : piece_y(t) + kXY; }
 };
 
 // The tiles of a launch in order: sequence, head, tile (backwards in time: from the last).
@@ -217,16 +218,16 @@ template <int A, int B, bool PIECE>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const __grid_constant__ LinearChunkArgs args) {
   static_assert((A == 64 || A == 128) && (B == 64 || B == 128), "64 or 128 features");
   using SM = LinearSmem<A, B>;
-  constexpr int NS = PIECE ? SM::kPieceStages : SM::kStages;
+  constexpr int NS = PIECE ? SM::kPieceStages : SM::kStages;   // tiles on their way or in use, at most
   constexpr uint32_t kBox = 128 * 128;       // [128 rows][64 features] box of a tile
   constexpr uint32_t kSBox = B * 128;        // [B rows][64 columns] box of the copy of S
   constexpr uint32_t kTmemCols = 512, kG = 128, kO = 256, kOx = 384;   // D at 0, G and P (PIECE: a second D), P Z, X S
   extern __shared__ __align__(1024) uint8_t linear_smem[];
   const uint32_t base = smem_u32(linear_smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(linear_smem + SM::kBars);
-  uint64_t* xy_full = bars;             // [NS]
-  uint64_t* z_full = bars + 4;          // [NS]
-  uint64_t* stage_empty = bars + 8;     // [NS] Y and Z (and, the ring of five aside, X) have been used
+  uint64_t* xy_full = bars;             // [stages, at most 4]
+  uint64_t* z_full = bars + 4;          // [..]
+  uint64_t* stage_empty = bars + 8;     // [..] Y and Z (and, the ring of five aside, X) have been used
   uint64_t* g_full = bars + 12;         // G is in tensor memory
   uint64_t* p_full = bars + 13;         // an arrival per row warp: P is there (and Z is clean)
   uint64_t* s_ready = bars + 14;        // an arrival per state warp: D has been read, the copy of S is there
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
 
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NS; ++s) { mbar_init(&xy_full[s], 1); mbar_init(&z_full[s], 1); mbar_init(&stage_empty[s], 1); }
+    for (int s = 0; s < 4; ++s) { mbar_init(&xy_full[s], 1); mbar_init(&z_full[s], 1); mbar_init(&stage_empty[s], 1); }
     mbar_init(g_full, 1);
     mbar_init(p_full, kLinearRowWarps);
     mbar_init(s_ready, 8);
@@ -287,6 +288,9 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           args.pieces[blockIdx.x] = {goes_on, at.c > 0, w.it.n * a.heads + w.it.head,
                                      exp2f(decay_log2(a, w.it.head) * static_cast<float>(tokens - 1 + at.first_decay(a)))};
         w.count = goes_on ? back + 1 : 0;
+        // tiles whose decay is below the smallest fp32 would be added as zeros
+        const float g2 = decay_log2(a, w.it.head);
+        if (g2 * 128.f * static_cast<float>(w.count) < -160.f) w.count = min(w.count, static_cast<int>(160.f / (-128.f * g2)) + 2);
       }
     } else if (PIECE && lane == 0) {
       args.pieces[blockIdx.x] = {0, 0, 0, 0.f};
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   bool failed = uniform(static_cast<uint32_t>(*reinterpret_cast<volatile int32_t*>(args.status))) != kStatusOk || (base & 1023u) != 0;
   const bool three = a.s_out != nullptr;
   auto y_of = [&](int t) { return base + (PIECE ? SM::piece_y(t) : SM::y(t)); };
-  auto z_of = [&](int t) { return PIECE ? y_of(t) + SM::kXY : base + SM::z(t); };
+  auto z_of = [&](int t) { return base + (PIECE ? SM::piece_z(t) : SM::z(t)); };
 
   if (warp < 4) {
     linear_registers<kLinearIssueRegs>();
@@ -319,8 +323,9 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           if (!PIECE) tma_load_4d_if(leader, base + SM::x(t) + j * kBox, &args.x, &xy_full[st], 64 * j, row, it.head / a.x_share, it.s.entry);
           tma_load_4d_if(leader, y_of(t) + j * kBox, &args.y, &xy_full[st], 64 * j, row, it.head / a.y_share, it.s.entry);
         }
-        // (ring of five: Z comes to where X of the tile before was)
-        if (!PIECE && SM::kRing5 && t >= 1 && !mbar_wait_warp(x_done, (t - 1) & 1, abort_flag)) { failed = true; break; }
+        // (ring of five: Z comes to where X of the tile before was; for the shares, where Y of the tile two before was)
+        if (SM::kRing5 && (PIECE ? t >= 2 && !mbar_wait_warp(&stage_empty[(t - 2) % NS], ((t - 2) / NS) & 1, abort_flag)
+                                 : t >= 1 && !mbar_wait_warp(x_done, (t - 1) & 1, abort_flag))) { failed = true; break; }
         mbar_expect_tx_if(leader, &z_full[st], SM::kZ);
         for (int j = 0; j < B / 64; ++j)
           tma_load_4d_if(leader, z_of(t) + j * kBox, &args.z, &z_full[st], 64 * j, row, it.head / a.z_share, it.s.entry);
