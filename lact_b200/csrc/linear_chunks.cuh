@@ -49,22 +49,28 @@ struct LinearChunkArgs {
 template <int A, int B>
 struct LinearSmem {
   static constexpr bool kRing5 = A == 128 && B == 128;   // no room for two whole stages beside the rest: five tiles of 32 KB in a ring
-  static constexpr int kStages = kRing5 || A == 128 ? 2 : B == 128 ? 3 : 4;
-  static constexpr int kPieceStages = kRing5 || A == 128 ? 3 : 4;   // of Y and Z alone (the ring of five holds two and a half)
+  static constexpr bool kTwice = A == 64;                // room for two sets of the second and third pieces of Y
+  static constexpr int kStages = A == 128 || B == 128 ? 2 : 3;
+  static constexpr int kPieceStages = B == 128 || A == 128 ? 3 : 4;   // of Y and Z alone (the ring of five holds two and a half)
   static constexpr uint32_t kXY = 128 * A * 2, kZ = 128 * B * 2;
   static constexpr uint32_t kTiles = kRing5 ? 5 * kXY : kStages * (2 * kXY + kZ);
-  static constexpr uint32_t kLow = kTiles;          // second piece of Y
-  static constexpr uint32_t kS = kLow + kXY;        // copy of S; third piece of Y
-  static constexpr uint32_t kBars = kS + kXY;
-  static constexpr uint32_t kFactors = kBars + 256; // a table of 32 decays per row warp
+  static constexpr uint32_t kS = kTiles;            // copy of S; one set of pieces: the third of Y
+  static constexpr uint32_t kLow = kS + kXY;        // second piece of Y (two sets: two of them, two of the third)
+  static constexpr uint32_t kBars = kLow + (kTwice ? 4 : 1) * kXY;
+  static constexpr uint32_t kFactors = kBars + 320; // a table of 32 decays per row warp
   static constexpr uint32_t kBytes = kFactors + kLinearRowWarps * 128;
-  static_assert(kRing5 || kPieceStages * (kXY + kZ) <= kTiles, "the stages of the shares fit");
+  static_assert(kRing5 || kPieceStages * (kXY + kZ) <= kTiles + (kTwice ? kXY : 0), "the stages of the shares fit");
   // where X, Y, Z of the CTA's tile t lie
   static __device__ __forceinline__ uint32_t x(int t) { return kRing5 ? 3 * t % 5 * kXY : t % kStages * (2 * kXY + kZ); }
   static __device__ __forceinline__ uint32_t y(int t) { return kRing5 ? (3 * t + 1) % 5 * kXY : x(t) + kXY; }
   static __device__ __forceinline__ uint32_t z(int t) { return kRing5 ? (3 * t + 2) % 5 * kXY : x(t) + 2 * kXY; }
   static __device__ __forceinline__ uint32_t piece_y(int t) { return kRing5 ? 2 * t % 5 * kXY : t % kPieceStages * (kXY + kZ); }
   static __device__ __forceinline__ uint32_t piece_z(int t) { return kRing5 ? (2 * t + 1) % 5 * kXY : piece_y(t) + kXY; }
+  // the second and third pieces of Y; `spare`: the place of the copy of S is free for every other second one
+  static __device__ __forceinline__ uint32_t low(int t, bool spare) {
+    return kTwice ? kLow + (t & 1) * kXY : spare && (t & 1) ? kS : kLow;
+  }
+  static __device__ __forceinline__ uint32_t lowest(int t) { return kTwice ? kLow + (2 + (t & 1)) * kXY : kS; }
 };
 
 // The tiles of a launch in order: sequence, head, tile (backwards in time: from the last).
@@ -155,49 +161,51 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Rows of a tile of Y times their decay until the tile's end, as bf16 pieces: the first in place, the second to `low`, a third to
-// `lowest` (0: none).  Thread j of 512 works on row j % 128; rows past the sequence become zeros.  (All loads before the
-// first store: one after the other, they took twice as long.)
+// Rows of a tile of Y times their decay until the tile's end, as bf16 pieces: the first in place, the second to `low`, a third (with
+// `three`) into `rest`, which put_rest stores.  Thread j of 512 works on row j % 128; rows past the sequence become
+// zeros.  (All loads before the first store: one after the other, they took twice as long.)
 template <int A>
-__device__ __forceinline__ void linear_decay_rows(uint32_t y, uint32_t low, uint32_t lowest, int tid, float f, bool real) {
-  constexpr uint32_t kBox = 128 * 128;
-  constexpr int kUnits = A / 32;   // 16-byte units a thread
-  const int j = tid & 127, first = (tid >> 7) * kUnits;
-  const F32x2 ff = f32x2(f, f), minus = f32x2(-1.f, -1.f);
-  auto pair = [](uint32_t b) { return f32x2(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)); };
-  auto round = [](F32x2 p) {
-    float p0, p1;
-    f32x2_split(p, p0, p1);
-    return pack_bf16x2(p0, p1);
-  };
-  {
-    uint32_t u[kUnits][4], off[kUnits];
+struct LinearRows {
+  static constexpr int kUnits = A / 32;   // 16-byte units a thread
+  static __device__ __forceinline__ uint32_t place(int tid, int k) {
+    const int j = tid & 127, unit = (tid >> 7) * kUnits + k;
+    return (unit >> 3) * (128 * 128) + j * 128 + (((unit & 7) ^ (j & 7)) << 4);
+  }
+  static __device__ __forceinline__ void put(uint32_t to, const uint32_t* v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+  }
+  uint32_t rest[kUnits][4];
+  __device__ __forceinline__ void decay(uint32_t y, uint32_t low, bool three, int tid, float f, bool real) {
+    const F32x2 ff = f32x2(f, f), minus = f32x2(-1.f, -1.f);
+    auto pair = [](uint32_t b) { return f32x2(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)); };
+    auto round = [](F32x2 p) {
+      float p0, p1;
+      f32x2_split(p, p0, p1);
+      return pack_bf16x2(p0, p1);
+    };
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(rest[k][0]), "=r"(rest[k][1]), "=r"(rest[k][2]), "=r"(rest[k][3]) : "r"(y + place(tid, k)));
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
-      const int unit = first + k;
-      off[k] = (unit >> 3) * kBox + j * 128 + (((unit & 7) ^ (j & 7)) << 4);
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[k][0]), "=r"(u[k][1]), "=r"(u[k][2]), "=r"(u[k][3]) : "r"(y + off[k]));
-    }
-#pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      uint32_t w[4], l[4], m[4];
+      uint32_t w[4], l[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        F32x2 p = f32x2_mul(pair(real ? u[k][e] : 0u), ff);
+        F32x2 p = f32x2_mul(pair(real ? rest[k][e] : 0u), ff);
         w[e] = round(p);
         p = f32x2_fma(pair(w[e]), minus, p);
         l[e] = round(p);
-        if (lowest != 0) m[e] = round(f32x2_fma(pair(l[e]), minus, p));
+        if (three) rest[k][e] = round(f32x2_fma(pair(l[e]), minus, p));
       }
-      auto put = [&](uint32_t to, const uint32_t (&v)[4]) {
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + off[k]), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-      };
-      put(y, w);
-      put(low, l);
-      if (lowest != 0) put(lowest, m);
+      put(y + place(tid, k), w);
+      put(low + place(tid, k), l);
     }
   }
-}
+  __device__ __forceinline__ void put_rest(uint32_t lowest, int tid) const {
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) put(lowest + place(tid, k), rest[k]);
+  }
+};
 // Rows `from` to 127 of a tile of Z become zeros.
 template <int B>
 __device__ __forceinline__ void linear_clear_rows(uint32_t z, int from, int tid) {
@@ -231,13 +239,16 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   uint64_t* g_full = bars + 12;         // G is in tensor memory
   uint64_t* p_full = bars + 13;         // an arrival per row warp: P is there (and Z is clean)
   uint64_t* s_ready = bars + 14;        // an arrival per state warp: D has been read, the copy of S is there
-  uint64_t* x_done = bars + 15;         // X and the copy of S have been used
   uint64_t* o_full = bars + 16;         // both parts of the output are there
   uint64_t* o_empty = bars + 17;        // an arrival per row warp: they have been read
-  uint64_t* y_ready = bars + 18;        // an arrival per warp that makes them: the pieces of Y are there
-  uint64_t* d_full = bars + 19;         // [2] D is there (PIECE: two of them in turn)
-  uint64_t* d_read = bars + 21;         // [2] PIECE: an arrival per state warp
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  // Two of each of these, for every other tile: one role may be a tile ahead of another that waits (the rows of the products, with two
+  // sets of pieces; X S of the loads, in the ring of five), and a wait by parity on one barrier would then miss a phase.
+  uint64_t* x_done = bars + 18;         // [2] X and the copy of S have been used
+  uint64_t* y_ready = bars + 20;        // [2] an arrival per warp that makes them: the first two pieces of Y are there
+  uint64_t* rest_ready = bars + 22;     // [2] likewise the third
+  uint64_t* d_full = bars + 24;         // [2] D is there
+  uint64_t* d_read = bars + 26;         // [2] PIECE: an arrival per state warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   LinearStart* start = reinterpret_cast<LinearStart*>(tmem_slot + 2);
   const LinearArgs& a = args.a;
@@ -248,11 +259,15 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
     mbar_init(g_full, 1);
     mbar_init(p_full, kLinearRowWarps);
     mbar_init(s_ready, 8);
-    mbar_init(x_done, 1);
     mbar_init(o_full, 1);
     mbar_init(o_empty, kLinearRowWarps);
-    mbar_init(y_ready, kLinearRowWarps);
-    for (int s = 0; s < 2; ++s) { mbar_init(&d_full[s], 1); mbar_init(&d_read[s], 8); }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&x_done[s], 1);
+      mbar_init(&y_ready[s], kLinearRowWarps);
+      mbar_init(&rest_ready[s], kLinearRowWarps);
+      mbar_init(&d_full[s], 1);
+      mbar_init(&d_read[s], 8);
+    }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -325,7 +340,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         }
         // (ring of five: Z comes to where X of the tile before was; for the shares, where Y of the tile two before was)
         if (SM::kRing5 && (PIECE ? t >= 2 && !mbar_wait_warp(&stage_empty[(t - 2) % NS], ((t - 2) / NS) & 1, abort_flag)
-                                 : t >= 1 && !mbar_wait_warp(x_done, (t - 1) & 1, abort_flag))) { failed = true; break; }
+                                 : t >= 1 && !mbar_wait_warp(&x_done[(t - 1) & 1], ((t - 1) >> 1) & 1, abort_flag))) { failed = true; break; }
         mbar_expect_tx_if(leader, &z_full[st], SM::kZ);
         for (int j = 0; j < B / 64; ++j)
           tma_load_4d_if(leader, z_of(t) + j * kBox, &args.z, &z_full[st], 64 * j, row, it.head / a.z_share, it.s.entry);
@@ -364,7 +379,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
             for (int k4 = 0; k4 < 4; ++k4)
               umma_bf16_if(leader, tmem + kOx, desc.at((x + kk * kBox + k4 * 32) >> 4),
                            desc.at((base + SM::kS + kk * kSBox + k4 * 32) >> 4), idesc_ox, (kk | k4) != 0);
-          umma_commit_if(leader, x_done);
+          umma_commit_if(leader, &x_done[par]);
           if (!mbar_wait_warp(p_full, par, abort_flag) || !mbar_wait_warp(&z_full[t % NS], (t / NS) & 1, abort_flag)) { failed = true; break; }
           tc_fence_after();
 #pragma unroll
@@ -373,25 +388,30 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           umma_commit_if(leader, o_full);
           g_next = t + 1 < count;
           // D before the next G, if its operands are there: what the next tile waits for comes behind D
-          if (g_next && !__all_sync(0xFFFFFFFFu, mbar_test(y_ready, par)) &&
+          if (g_next && !__all_sync(0xFFFFFFFFu, mbar_test(&y_ready[par], (t >> 1) & 1)) &&
               __all_sync(0xFFFFFFFFu, mbar_test(&xy_full[(t + 1) % NS], ((t + 1) / NS) & 1))) {
             issue_g(t + 1);
             g_next = false;
           }
         }
-        if (!mbar_wait_warp(y_ready, par, abort_flag)) { failed = true; break; }
+        if (!mbar_wait_warp(&y_ready[par], (t >> 1) & 1, abort_flag)) { failed = true; break; }
         if (PIECE && (!mbar_wait_warp(&z_full[t % NS], (t / NS) & 1, abort_flag) ||
                       (t >= 2 && !mbar_wait_warp(&d_read[t & 1], ((t >> 1) - 1) & 1, abort_flag)))) { failed = true; break; }
         tc_fence_after();
         const uint32_t d = tmem + (PIECE ? par * kG : 0);
-        const uint32_t low = base + (PIECE && !three && par ? SM::kS : SM::kLow);
-        for (int p = 0; p < (three ? 3 : 2); ++p) {
-          const uint32_t yp = p == 0 ? y : p == 1 ? low : base + SM::kS;
+        auto add = [&](uint32_t piece, bool fresh) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_bf16_if(leader, d, desc.at((z + k * 2048) >> 4), desc.at((yp + k * 2048) >> 4), idesc_d, (p | k) != 0);
+            umma_bf16_if(leader, d, desc.at((z + k * 2048) >> 4), desc.at((piece + k * 2048) >> 4), idesc_d, !fresh || k != 0);
+        };
+        add(y, true);
+        add(base + SM::low(t, PIECE && !three), false);
+        if (three) {
+          if (!mbar_wait_warp(&rest_ready[par], (t >> 1) & 1, abort_flag)) { failed = true; break; }
+          tc_fence_after();
+          add(base + SM::lowest(t), false);
         }
-        umma_commit_if(leader, &d_full[PIECE ? par : 0]);
+        umma_commit_if(leader, &d_full[par]);
         umma_commit_if(leader, &stage_empty[t % NS]);
         if (g_next) {
           if (!mbar_wait_warp(&xy_full[(t + 1) % NS], ((t + 1) / NS) & 1, abort_flag)) { failed = true; break; }
@@ -407,7 +427,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
     float g2 = 0.f;
     if constexpr (PIECE) {   // the pieces of Y; the tiles' own end is where their decays count from
       for (int t = 0; t < count && !failed; ++t, advance()) {
-        const int st = t % NS, nv = it.valid(it.place(a)), used = three ? t - 1 : t - 2;   // (the tile that used this place last)
+        const int st = t % NS, nv = it.valid(it.place(a)), used = three && !SM::kTwice ? t - 1 : t - 2;   // (the tile whose places these are)
         if (it.head != head) {
           head = it.head;
           g2 = decay_log2(a, head);
@@ -416,14 +436,19 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
         if (!mbar_wait_warp(&xy_full[st], (t / NS) & 1, abort_flag) ||
             (used >= 0 && !mbar_wait_warp(&d_full[used & 1], (used >> 1) & 1, abort_flag))) { failed = true; break; }
-        linear_decay_rows<A>(y_of(t), base + (!three && (t & 1) ? SM::kS : SM::kLow), three ? base + SM::kS : 0, tid, f, j < nv);
+        LinearRows<A> rows;
+        rows.decay(y_of(t), base + SM::low(t, !three), three, tid, f, j < nv);
+        if (three) rows.put_rest(base + SM::lowest(t), tid);
         if (nv < 128 && a.cu != nullptr) {
           if (!mbar_wait_warp(&z_full[st], (t / NS) & 1, abort_flag)) { failed = true; break; }
           linear_clear_rows<B>(z_of(t), nv, tid);
         }
         fence_async_proxy();
         __syncwarp();
-        if (lane == 0) mbar_arrive(y_ready);
+        if (lane == 0) {
+          mbar_arrive(&y_ready[t & 1]);
+          if (three) mbar_arrive(&rest_ready[t & 1]);
+        }
       }
     } else {
       const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
@@ -510,20 +535,25 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full);
 
-        // the pieces of Y: in the place of those of the tile before, once D has used them (a third takes the place of the copy of S:
-        // once X S has used that)
+        // the pieces of Y, where those of the tile before (two sets: before that one) were, once D has used them.  A third, where there is
+        // one set, takes the place of the copy of S once X S has used that.
         {
-          const int j = tid & 127;
+          const int j = tid & 127, used = t - (SM::kTwice ? 2 : 1);
           const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
-          if (!mbar_wait_warp(&xy_full[t % NS], (t / NS) & 1, abort_flag) || (t >= 1 && !mbar_wait_warp(&d_full[0], par ^ 1, abort_flag)) ||
-              (three && !mbar_wait_warp(x_done, par, abort_flag))) {
-            failed = true;
-            break;
-          }
-          linear_decay_rows<A>(y_of(t), base + SM::kLow, three ? base + SM::kS : 0, tid, f, j < nv);
+          if (!mbar_wait_warp(&xy_full[t % NS], (t / NS) & 1, abort_flag) ||
+              (used >= 0 && !mbar_wait_warp(&d_full[used & 1], (used >> 1) & 1, abort_flag))) { failed = true; break; }
+          LinearRows<A> rows;
+          rows.decay(y_of(t), base + SM::low(t, false), three, tid, f, j < nv);
           fence_async_proxy();
           __syncwarp();
-          if (lane == 0) mbar_arrive(y_ready);
+          if (lane == 0) mbar_arrive(&y_ready[par]);
+          if (three) {
+            if (!SM::kTwice && !mbar_wait_warp(&x_done[par], (t >> 1) & 1, abort_flag)) { failed = true; break; }
+            rows.put_rest(base + SM::lowest(t), tid);
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&rest_ready[par]);
+          }
         }
 
         const int pos = a.reverse ? nv - 1 - r : r;
@@ -630,7 +660,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
       for (int t = 0;; ++t) {
         const uint32_t par = t & 1;
         if (t >= 1) {
-          if (!mbar_wait_warp(&d_full[0], par ^ 1, abort_flag)) { failed = true; break; }
+          if (!mbar_wait_warp(&d_full[par ^ 1], ((t - 1) >> 1) & 1, abort_flag)) { failed = true; break; }
           tc_fence_after();
           if (holds) {
             take(0, decay, 1.f);
