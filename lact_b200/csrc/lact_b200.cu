@@ -2111,9 +2111,9 @@ LinearPlan linear_plan(const lact_linear_config* c) {
 }
 size_t linear_slots(const LinearPlan& p, int64_t dk, int64_t dv) { return p.cut ? static_cast<size_t>(p.ctas) * (dk * dv * 4 + sizeof(LinearPiece)) : 0; }
 
-template <int A, int B, bool PIECE>
+template <int A, int B, bool PIECE, bool THREE>
 int launch_linear_chunks(const LinearChunkArgs& a, int ctas, cudaStream_t st) {
-  auto kernel = linear_chunks_kernel<A, B, PIECE>;
+  auto kernel = linear_chunks_kernel<A, B, PIECE, THREE>;
   constexpr uint32_t smem = LinearSmem<A, B>::kBytes;
   static_assert(smem <= 232448, "shared memory budget exceeded");
   static std::mutex mu;
@@ -2134,16 +2134,16 @@ int launch_linear_chunks(const LinearChunkArgs& a, int ctas, cudaStream_t st) {
   LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kLinearThreads), smem, st, a));
   return LACT_OK;
 }
-// `carried`: the slots hold what the CTAs begin with already
-template <int A, int B>
+// `carried`: the slots hold what the CTAs begin with already.  THREE: the last states are an output
+template <int A, int B, bool THREE>
 int linear_chunks(const LinearChunkArgs& a, const LinearPlan& p, bool carried, cudaStream_t st) {
   if (p.cut && !carried) {
-    LACT_TRY((launch_linear_chunks<A, B, true>(a, p.ctas, st)));
+    LACT_TRY((launch_linear_chunks<A, B, true, THREE>(a, p.ctas, st)));
     KernelScope scope(kClsOther, st);
     LACT_CUDA(launch_pdl(linear_carry_kernel, dim3(A * B / 512, p.ctas), dim3(128), 0, st, a.a.s_in, a.a.s_in_t, a.a.in_mul, a.slots, a.pieces,
                          p.ctas, A, B));
   }
-  return launch_linear_chunks<A, B, false>(a, p.ctas, st);
+  return launch_linear_chunks<A, B, false, THREE>(a, p.ctas, st);
 }
 // An operand of a call: its array, and the map of its tiles (encoded once where several launches read it).
 struct LinearOperand {
@@ -2176,8 +2176,14 @@ int linear_run(const lact_linear_config* c, LinearArgs& a, const LinearOperand& 
   k.pieces = reinterpret_cast<LinearPiece*>(static_cast<uint8_t*>(slots) + static_cast<size_t>(p.ctas) * A * B * 4);
   k.slots_t = carried;
   k.status = status;
-  if (A == 64) return B == 64 ? linear_chunks<64, 64>(k, p, carried, st) : linear_chunks<64, 128>(k, p, carried, st);
-  return B == 64 ? linear_chunks<128, 64>(k, p, carried, st) : linear_chunks<128, 128>(k, p, carried, st);
+  auto run = [&](auto a_, auto b_) {
+    constexpr int kA = decltype(a_)::value, kB = decltype(b_)::value;
+    return a.s_out != nullptr ? linear_chunks<kA, kB, true>(k, p, carried, st) : linear_chunks<kA, kB, false>(k, p, carried, st);
+  };
+  using Narrow = std::integral_constant<int, 64>;
+  using Wide = std::integral_constant<int, 128>;
+  if (A == 64) return B == 64 ? run(Narrow{}, Narrow{}) : run(Narrow{}, Wide{});
+  return B == 64 ? run(Wide{}, Narrow{}) : run(Wide{}, Wide{});
 }
 LinearArgs linear_args(const lact_linear_config* c, const float* log_decay, const int32_t* cu) {
   LinearArgs a;

@@ -13,7 +13,7 @@
 // fp32 (D alone is summed by the tensor core, which truncates: over a long sequence that would show): the decayed rows of Y are two
 // bf16 pieces (16 bits of the product; what is lost, 2^-17, is far below the copy's rounding), three (24 bits) where the last state
 // is an output.
-// Long sequences of few heads: `per` tiles a CTA may begin within a sequence.  linear_chunks_kernel<..., PIECE> first leaves every CTA's
+// Long sequences of few heads: `per` tiles a CTA may begin within a sequence.  linear_chunks_kernel<.., PIECE, ..> first leaves every CTA's
 // share of the state of the sequence that goes on behind it, linear_carry_kernel adds the shares up in order.  The shares are taken
 // from the last tile to the first, so that the tiles the CTA begins with afterwards have been read last and are still in L2, and only as far as fp32 has room for their decay.
 #pragma once
@@ -26,7 +26,7 @@ constexpr int kLinearThreads = 896;   // a warpgroup for loads and products, fou
 constexpr int kLinearRowThreads = 512, kLinearRowWarps = 16;
 // registers per thread of each; together what the launch has.  (Nothing may spill: the little L1 beside 227 KB of shared memory misses,
 // and a tile's bookkeeping alone then waited 1700 clocks for it.)
-constexpr int kLinearIssueRegs = 32, kLinearRowRegs = 64, kLinearStateRegs = 104, kLinearLaunchRegs = 72;
+constexpr int kLinearIssueRegs = 40, kLinearRowRegs = 56, kLinearStateRegs = 120, kLinearLaunchRegs = 72;
 static_assert(kLinearIssueRegs + 4 * kLinearRowRegs + 2 * kLinearStateRegs <= 7 * kLinearLaunchRegs, "the shares of the registers");
 
 struct LinearPiece {
@@ -57,8 +57,7 @@ struct LinearSmem {
   static constexpr uint32_t kS = kTiles;            // copy of S; one set of pieces: the third of Y
   static constexpr uint32_t kLow = kS + kXY;        // second piece of Y (two sets: two of them, two of the third)
   static constexpr uint32_t kBars = kLow + (kTwice ? 4 : 1) * kXY;
-  static constexpr uint32_t kFactors = kBars + 320; // a table of 32 decays per row warp
-  static constexpr uint32_t kBytes = kFactors + kLinearRowWarps * 128;
+  static constexpr uint32_t kBytes = kBars + 320;
   static_assert(kRing5 || kPieceStages * (kXY + kZ) <= kTiles + (kTwice ? kXY : 0), "the stages of the shares fit");
   // where X, Y, Z of the CTA's tile t lie
   static __device__ __forceinline__ uint32_t x(int t) { return kRing5 ? 3 * t % 5 * kXY : t % kStages * (2 * kXY + kZ); }
@@ -222,7 +221,8 @@ __device__ __forceinline__ void linear_registers() {
   else registers_shrink<N>();
 }
 
-template <int A, int B, bool PIECE>
+// THREE: pieces of Y (a parameter of the template: as a run-time choice in the rows' loop it cost the calls with two 12 %, 150 -> 170 us)
+template <int A, int B, bool PIECE, bool THREE>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const __grid_constant__ LinearChunkArgs args) {
   static_assert((A == 64 || A == 128) && (B == 64 || B == 128), "64 or 128 features");
   using SM = LinearSmem<A, B>;
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   };
   // (swizzled tiles need the alignment asked for above)
   bool failed = uniform(static_cast<uint32_t>(*reinterpret_cast<volatile int32_t*>(args.status))) != kStatusOk || (base & 1023u) != 0;
-  const bool three = a.s_out != nullptr;
+  constexpr bool three = THREE;
   auto y_of = [&](int t) { return base + (PIECE ? SM::piece_y(t) : SM::y(t)); };
   auto z_of = [&](int t) { return base + (PIECE ? SM::piece_z(t) : SM::z(t)); };
 
@@ -462,16 +462,14 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
                 a.s_in != nullptr ? reinterpret_cast<const float4*>(a.s_in)[n * size + i] : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
-      float* const factors = reinterpret_cast<float*>(linear_smem + SM::kFactors) + (warp - 4) * 32;
+      float lambda = 0.f;
       for (int t = 0; t < count && !failed; ++t, advance()) {
         const uint32_t par = t & 1;
         const int place = it.place(a), nv = it.valid(place);
-        if (it.head != head) {   // the decays of 32 columns among themselves
+        if (it.head != head) {
           head = it.head;
           g2 = decay_log2(a, head);
-          __syncwarp();
-          factors[lane] = exp2f(g2 * static_cast<float>(a.reverse ? lane : 31 - lane));
-          __syncwarp();
+          lambda = exp2f(g2);
         }
         if (!mbar_wait_warp(g_full, par, abort_flag)) { failed = true; break; }
         tc_fence_after();
@@ -485,27 +483,29 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
             uint32_t bits[32];
             tmem_ld32(tmem + lane_off + kG + c0, bits);
             if (cb != quarter) {
-              // lambda^(distance to the column nearest to the diagonal) * lambda^(from there)
-              const float f = exp2_ftz(g2 * static_cast<float>(a.reverse ? c0 - r : r - c0 - 31));
-              const F32x2 ff = f32x2(f, f);
+              // from the column nearest to the diagonal on, a factor of lambda each (two columns at a time; no table of them: shared memory is
+              // what the products wait for)
+              const float f = exp2_ftz(g2 * static_cast<float>(a.reverse ? c0 - r : r - c0 - 31)), f1 = f * lambda;
+              const F32x2 two = f32x2(lambda * lambda, lambda * lambda);
               const int hi = a.reverse ? nv - 1 - c0 : 31;
+              F32x2 d = a.reverse ? f32x2(f, f1) : f32x2(f1, f);
               tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 c = *reinterpret_cast<const float4*>(factors + j);
-                const F32x2 p01 = f32x2_mul(f32x2(__uint_as_float(bits[j]), __uint_as_float(bits[j + 1])), f32x2_mul(f32x2(c.x, c.y), ff));
-                const F32x2 p23 = f32x2_mul(f32x2(__uint_as_float(bits[j + 2]), __uint_as_float(bits[j + 3])), f32x2_mul(f32x2(c.z, c.w), ff));
-                float p0, p1, p2, p3;
-                f32x2_split(p01, p0, p1);
-                f32x2_split(p23, p2, p3);
+              auto column = [&](int j) {
+                float p0, p1;
+                f32x2_split(f32x2_mul(f32x2(__uint_as_float(bits[j]), __uint_as_float(bits[j + 1])), d), p0, p1);
                 if (hi < 31) {
                   p0 = j > hi ? 0.f : p0;
                   p1 = j + 1 > hi ? 0.f : p1;
-                  p2 = j + 2 > hi ? 0.f : p2;
-                  p3 = j + 3 > hi ? 0.f : p3;
                 }
                 w[j / 2] = pack_bf16x2(p0, p1);
-                w[j / 2 + 1] = pack_bf16x2(p2, p3);
+                d = f32x2_mul(d, two);
+              };
+              if (a.reverse) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) column(j);
+              } else {
+#pragma unroll
+                for (int j = 30; j >= 0; j -= 2) column(j);
               }
             } else {
               // column j is |lane - j| tokens away; visible from / up to its own
@@ -611,16 +611,24 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
     for (int j = 0; j < NC; ++j) S[j] = 0.f;
     // state number `n` of an array: element (row of A: c0 + j, column r), j up to NC
     auto load_state = [&](const float* from, int64_t n, bool transposed, float mul) {
-      const float* p = from + n * (A * B) + (transposed ? static_cast<int64_t>(r) * A + c0 : static_cast<int64_t>(c0) * B + r);
-      const int step = transposed ? 1 : B;
+      from += n * (A * B) + (transposed ? r * A + c0 : c0 * B + r);
+      if (transposed) {
 #pragma unroll
-      for (int j = 0; j < NC; ++j) S[j] = p[j * step] * mul;
+        for (int j = 0; j < NC; ++j) S[j] = from[j] * mul;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) S[j] = from[j * B] * mul;
+      }
     };
     auto store_state = [&](float* to, int64_t n, bool transposed, float mul) {
-      float* p = to + n * (A * B) + (transposed ? static_cast<int64_t>(r) * A + c0 : static_cast<int64_t>(c0) * B + r);
-      const int step = transposed ? 1 : B;
+      to += n * (A * B) + (transposed ? r * A + c0 : c0 * B + r);
+      if (transposed) {
 #pragma unroll
-      for (int j = 0; j < NC; ++j) p[j * step] = S[j] * mul;
+        for (int j = 0; j < NC; ++j) to[j] = S[j] * mul;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) to[j * B] = S[j] * mul;
+      }
     };
     // S <- S * x + D * y
     auto take = [&](uint32_t d, float x, float y) {
@@ -656,7 +664,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
     } else {
       float decay = 1.f;        // of the tile before
       bool last = false;        // it was its sequence's last
-      int64_t state = 0;        // whose number
+      int state = 0;            // whose number
       for (int t = 0;; ++t) {
         const uint32_t par = t & 1;
         if (t >= 1) {
@@ -674,7 +682,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           head = it.head;
           g2 = decay_log2(a, head);
         }
-        state = static_cast<int64_t>(it.n) * a.heads + head;
+        state = it.n * a.heads + head;
         last = it.c + 1 == it.tiles;
         decay = exp2f(g2 * static_cast<float>(nv - 1 + it.first_decay(a)));
         if (holds) {
