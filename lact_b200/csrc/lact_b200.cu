@@ -2111,9 +2111,9 @@ LinearPlan linear_plan(const lact_linear_config* c) {
 }
 size_t linear_slots(const LinearPlan& p, int64_t dk, int64_t dv) { return p.cut ? static_cast<size_t>(p.ctas) * (dk * dv * 4 + sizeof(LinearPiece)) : 0; }
 
-template <int A, int B, bool PIECE, bool THREE>
+template <int A, int B, bool PIECE, bool THREE, bool BACK>
 int launch_linear_chunks(const LinearChunkArgs& a, int ctas, cudaStream_t st) {
-  auto kernel = linear_chunks_kernel<A, B, PIECE, THREE>;
+  auto kernel = linear_chunks_kernel<A, B, PIECE, THREE, BACK>;
   constexpr uint32_t smem = LinearSmem<A, B>::kBytes;
   static_assert(smem <= 232448, "shared memory budget exceeded");
   static std::mutex mu;
@@ -2138,12 +2138,12 @@ int launch_linear_chunks(const LinearChunkArgs& a, int ctas, cudaStream_t st) {
 template <int A, int B, bool THREE>
 int linear_chunks(const LinearChunkArgs& a, const LinearPlan& p, bool carried, cudaStream_t st) {
   if (p.cut && !carried) {
-    LACT_TRY((launch_linear_chunks<A, B, true, THREE>(a, p.ctas, st)));
+    LACT_TRY((launch_linear_chunks<A, B, true, THREE, false>(a, p.ctas, st)));
     KernelScope scope(kClsOther, st);
     LACT_CUDA(launch_pdl(linear_carry_kernel, dim3(A * B / 512, p.ctas), dim3(128), 0, st, a.a.s_in, a.a.s_in_t, a.a.in_mul, a.slots, a.pieces,
                          p.ctas, A, B));
   }
-  return launch_linear_chunks<A, B, false, THREE>(a, p.ctas, st);
+  return a.a.reverse ? launch_linear_chunks<A, B, false, THREE, true>(a, p.ctas, st) : launch_linear_chunks<A, B, false, THREE, false>(a, p.ctas, st);
 }
 // An operand of a call: its array, and the map of its tiles (encoded once where several launches read it).
 struct LinearOperand {

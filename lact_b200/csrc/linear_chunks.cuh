@@ -137,10 +137,10 @@ struct LinearTiles {
     } while (s.len == 0);
     tiles = tiles_of(s.len);
   }
-  __device__ __forceinline__ int place(const LinearArgs& a) const { return (a.reverse ? tiles - 1 - c : c) * 128; }  // first token
+  __device__ __forceinline__ int place(bool reverse) const { return (reverse ? tiles - 1 - c : c) * 128; }  // first token
   __device__ __forceinline__ int valid(int place) const { return min(128, s.len - place); }
   // backwards in time the state before the first token (the gradient of the last state) is not decayed by it
-  __device__ __forceinline__ int first_decay(const LinearArgs& a) const { return a.reverse && c == 0 ? 0 : 1; }
+  __device__ __forceinline__ int first_decay(bool reverse) const { return reverse && c == 0 ? 0 : 1; }
 };
 
 struct LinearStart {
@@ -221,8 +221,9 @@ __device__ __forceinline__ void linear_registers() {
   else registers_shrink<N>();
 }
 
-// THREE: pieces of Y (a parameter of the template: as a run-time choice in the rows' loop it cost the calls with two 12 %, 150 -> 170 us)
-template <int A, int B, bool PIECE, bool THREE>
+// THREE: pieces of Y; BACK: backwards in time (the shares' pass takes both).  Parameters of the template: as run-time choices in the rows'
+// loop the one cost 12 %, the other 5 % (170 and 153 us of calls that take 151 and 145).
+template <int A, int B, bool PIECE, bool THREE, bool BACK>
 __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const __grid_constant__ LinearChunkArgs args) {
   static_assert((A == 64 || A == 128) && (B == 64 || B == 128), "64 or 128 features");
   using SM = LinearSmem<A, B>;
@@ -252,6 +253,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
   volatile uint32_t* abort_flag = tmem_slot + 1;
   LinearStart* start = reinterpret_cast<LinearStart*>(tmem_slot + 2);
   const LinearArgs& a = args.a;
+  const bool reverse = PIECE ? a.reverse != 0 : BACK;
 
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -298,10 +300,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         LinearTiles at = w.it;
         at.c -= back;
         // tokens of these tiles: all whole, but for the first of a walk backwards
-        const int tokens = (back + 1) * 128 - (a.reverse && at.c == 0 ? 128 - at.valid(at.place(a)) : 0);
+        const int tokens = (back + 1) * 128 - (reverse && at.c == 0 ? 128 - at.valid(at.place(reverse)) : 0);
         if (lane == 0)
           args.pieces[blockIdx.x] = {goes_on, at.c > 0, w.it.n * a.heads + w.it.head,
-                                     exp2f(decay_log2(a, w.it.head) * static_cast<float>(tokens - 1 + at.first_decay(a)))};
+                                     exp2f(decay_log2(a, w.it.head) * static_cast<float>(tokens - 1 + at.first_decay(reverse)))};
         w.count = goes_on ? back + 1 : 0;
         // tiles whose decay is below the smallest fp32 would be added as zeros
         const float g2 = decay_log2(a, w.it.head);
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
     if (warp == 0) {
       const uint32_t leader = elect_leader();
       for (int t = 0; t < count && !failed; ++t, advance()) {
-        const int st = t % NS, row = it.s.first + it.place(a);
+        const int st = t % NS, row = it.s.first + it.place(reverse);
         if (t >= NS && !mbar_wait_warp(&stage_empty[st], (t / NS - 1) & 1, abort_flag)) { failed = true; break; }
         mbar_expect_tx_if(leader, &xy_full[st], PIECE ? SM::kXY : 2 * SM::kXY);
         for (int j = 0; j < A / 64; ++j) {
@@ -427,13 +429,13 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
     float g2 = 0.f;
     if constexpr (PIECE) {   // the pieces of Y; the tiles' own end is where their decays count from
       for (int t = 0; t < count && !failed; ++t, advance()) {
-        const int st = t % NS, nv = it.valid(it.place(a)), used = three && !SM::kTwice ? t - 1 : t - 2;   // (the tile whose places these are)
+        const int st = t % NS, nv = it.valid(it.place(reverse)), used = three && !SM::kTwice ? t - 1 : t - 2;   // (the tile whose places these are)
         if (it.head != head) {
           head = it.head;
           g2 = decay_log2(a, head);
         }
         const int j = tid & 127;
-        const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
+        const float f = exp2f(g2 * static_cast<float>(reverse ? j : max(nv - 1 - j, 0)));
         if (!mbar_wait_warp(&xy_full[st], (t / NS) & 1, abort_flag) ||
             (used >= 0 && !mbar_wait_warp(&d_full[used & 1], (used >> 1) & 1, abort_flag))) { failed = true; break; }
         LinearRows<A> rows;
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
       float lambda = 0.f;
       for (int t = 0; t < count && !failed; ++t, advance()) {
         const uint32_t par = t & 1;
-        const int place = it.place(a), nv = it.valid(place);
+        const int place = it.place(reverse), nv = it.valid(place);
         if (it.head != head) {
           head = it.head;
           g2 = decay_log2(a, head);
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         {
           const int c0 = cb * 32;
           uint32_t w[16];
-          if (a.reverse ? cb < quarter : cb > quarter) {
+          if (reverse ? cb < quarter : cb > quarter) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = 0;
           } else {
@@ -485,10 +487,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
             if (cb != quarter) {
               // from the column nearest to the diagonal on, a factor of lambda each (two columns at a time; no table of them: shared memory is
               // what the products wait for)
-              const float f = exp2_ftz(g2 * static_cast<float>(a.reverse ? c0 - r : r - c0 - 31)), f1 = f * lambda;
+              const float f = exp2_ftz(g2 * static_cast<float>(reverse ? c0 - r : r - c0 - 31)), f1 = f * lambda;
               const F32x2 two = f32x2(lambda * lambda, lambda * lambda);
-              const int hi = a.reverse ? nv - 1 - c0 : 31;
-              F32x2 d = a.reverse ? f32x2(f, f1) : f32x2(f1, f);
+              const int hi = reverse ? nv - 1 - c0 : 31;
+              F32x2 d = reverse ? f32x2(f, f1) : f32x2(f1, f);
               tmem_ld_wait();
               auto column = [&](int j) {
                 float p0, p1;
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
                 w[j / 2] = pack_bf16x2(p0, p1);
                 d = f32x2_mul(d, two);
               };
-              if (a.reverse) {
+              if (reverse) {
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) column(j);
               } else {
@@ -509,8 +511,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
               }
             } else {
               // column j is |lane - j| tokens away; visible from / up to its own
-              const float step = a.reverse ? g2 : -g2, from = (a.reverse ? -lane : lane) * g2;
-              const int lo = a.reverse ? lane : 0, hi = a.reverse ? nv - 1 - c0 : lane;
+              const float step = reverse ? g2 : -g2, from = (reverse ? -lane : lane) * g2;
+              const int lo = reverse ? lane : 0, hi = reverse ? nv - 1 - c0 : lane;
               tmem_ld_wait();
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
@@ -539,7 +541,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         // one set, takes the place of the copy of S once X S has used that.
         {
           const int j = tid & 127, used = t - (SM::kTwice ? 2 : 1);
-          const float f = exp2f(g2 * static_cast<float>(a.reverse ? j : max(nv - 1 - j, 0)));
+          const float f = exp2f(g2 * static_cast<float>(reverse ? j : max(nv - 1 - j, 0)));
           if (!mbar_wait_warp(&xy_full[t % NS], (t / NS) & 1, abort_flag) ||
               (used >= 0 && !mbar_wait_warp(&d_full[used & 1], (used >> 1) & 1, abort_flag))) { failed = true; break; }
           LinearRows<A> rows;
@@ -556,8 +558,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           }
         }
 
-        const int pos = a.reverse ? nv - 1 - r : r;
-        const float since = a.scale * exp2f(g2 * static_cast<float>(max(pos, 0) + it.first_decay(a)));
+        const int pos = reverse ? nv - 1 - r : r;
+        const float since = a.scale * exp2f(g2 * static_cast<float>(max(pos, 0) + it.first_decay(reverse)));
         const F32x2 ss = f32x2(since, since), sc = f32x2(a.scale, a.scale);
         const int64_t o = ((it.s.entry * static_cast<int64_t>(a.L) + it.s.first + place + r) * a.heads + head) * B + cb * (B / 4);
         if (!mbar_wait_warp(o_full, par, abort_flag)) { failed = true; break; }
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         if (!mbar_wait_warp(&d_full[t & 1], (t >> 1) & 1, abort_flag)) { failed = true; break; }
         tc_fence_after();
         if (holds) take((t & 1) * kG, 1.f, exp2f(g2 * static_cast<float>(behind)));
-        behind += it.valid(it.place(a));
+        behind += it.valid(it.place(reverse));
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&d_read[t & 1]);
@@ -672,19 +674,19 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           tc_fence_after();
           if (holds) {
             take(0, decay, 1.f);
-            if (last && a.s_out != nullptr) store_state(a.s_out, state, a.s_out_t, a.out_mul * (a.reverse ? exp2f(g2) : 1.f));
+            if (last && a.s_out != nullptr) store_state(a.s_out, state, a.s_out_t, a.out_mul * (reverse ? exp2f(g2) : 1.f));
           }
           advance();
         }
         if (t >= count || failed) break;
-        const int place = it.place(a), nv = it.valid(place);
+        const int place = it.place(reverse), nv = it.valid(place);
         if (it.head != head) {
           head = it.head;
           g2 = decay_log2(a, head);
         }
         state = it.n * a.heads + head;
         last = it.c + 1 == it.tiles;
-        decay = exp2f(g2 * static_cast<float>(nv - 1 + it.first_decay(a)));
+        decay = exp2f(g2 * static_cast<float>(nv - 1 + it.first_decay(reverse)));
         if (holds) {
           if (it.c == 0) {
             if (a.s_in != nullptr) {
