@@ -346,7 +346,7 @@ typedef struct lact_linear_config {
   int64_t sequences; /* with cu_seqlens: packed sequences within the one batch entry; else 0 */
   int64_t q_ts, q_bs, k_ts, k_bs, v_ts, v_bs;
   int64_t do_ts, do_bs; /* of dout (lact_linear_attention_bwd) */
-  float scale;          /* finite, not zero */
+  float scale;          /* of a size between 1e-18 and 1e18 */
 } lact_linear_config;
 /* Scratch of one forward (backward = 0) or backward call, 256-byte aligned. */
 int lact_linear_attention_workspace_bytes(const lact_linear_config *cfg, int32_t backward, size_t *bytes_out);

@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -2058,7 +2059,7 @@ int linear_check(const lact_linear_config* c, const void* cu) {
   // (sequence, head)s and their tiles of 128 tokens are counted in 31 bits
   const int64_t n = c->sequences > 0 ? c->sequences : c->batch;
   if (n * c->heads > (1ll << 28) || ((c->tokens + 127) / 128 * c->batch + n) * c->heads > (1ll << 30)) return LACT_ERR_SHAPE;
-  if (!(c->scale > -INFINITY && c->scale < INFINITY) || c->scale == 0.f) return LACT_ERR_CONFIG;
+  if (!(std::fabs(c->scale) >= 1e-18f && std::fabs(c->scale) <= 1e18f)) return LACT_ERR_CONFIG;   // (states of the backward are kept divided by it)
   return LACT_OK;
 }
 int linear_operand(const void* p, int64_t ts, int64_t bs, int64_t row) {

@@ -456,12 +456,12 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
       const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
       linear_zero_rest<B>(a, static_cast<int64_t>(blockIdx.x) * kLinearRowThreads + tid, static_cast<int64_t>(gridDim.x) * kLinearRowThreads);
       if (a.cu != nullptr && a.s_out != nullptr) {   // empty sequences keep their states
-        const int64_t size = static_cast<int64_t>(a.heads) * (A * B / 4);
-        for (int n = 0; n < a.sequences; ++n) {
-          if (linear_span(a, n).len != 0) continue;
-          for (int64_t i = static_cast<int64_t>(blockIdx.x) * kLinearRowThreads + tid; i < size; i += static_cast<int64_t>(gridDim.x) * kLinearRowThreads)
-            reinterpret_cast<float4*>(a.s_out)[n * size + i] =
-                a.s_in != nullptr ? reinterpret_cast<const float4*>(a.s_in)[n * size + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = blockIdx.x; i < a.sequences * a.heads; i += gridDim.x) {
+          if (linear_span(a, i / a.heads).len != 0) continue;
+          const int64_t at = static_cast<int64_t>(i) * (A * B / 4);
+          for (int e = tid; e < A * B / 4; e += kLinearRowThreads)
+            reinterpret_cast<float4*>(a.s_out)[at + e] =
+                a.s_in != nullptr ? reinterpret_cast<const float4*>(a.s_in)[at + e] : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
       float lambda = 0.f;

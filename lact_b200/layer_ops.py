@@ -9,7 +9,11 @@ Attention half of the hybrid layers (tcgen05 kernels, forward and backward, head
 `sliding_window_attention` (causal band; packed sequences by `cu_seqlens`, padded batches by `attention_mask`),
 `block_attention` (not causal, own key count) and, under the reference's names, the autoregressive-video layer's
 `batched_sliding_window_attention`, `batched_sliding_window_attention_with_repeated_chunks` and
-`sliding_window_attention_inference`."""
+`sliding_window_attention_inference`.
+
+Linear attention with a decay per head (`linear_attention` for prompts and training, `linear_attention_step` for single tokens): the
+recurrence with a linear memory, beside the fast weights.  `group_norm`: channels last, with an activation; with one spot a sample
+the norm of every head of every token behind such a mixer.  Neither has a counterpart in the reference."""
 from __future__ import annotations
 
 import math
@@ -161,8 +165,8 @@ def _linear_scale(scale, dk):
     if scale is None:
         return dk ** -0.5
     scale = float(scale)
-    if not math.isfinite(scale) or abs(scale) < 1e-30 or abs(scale) > 1e30:
-        raise ValueError("scale must be finite and not zero")
+    if not 1e-18 <= abs(scale) <= 1e18:
+        raise ValueError("scale must be of a size between 1e-18 and 1e18")
     return scale
 
 
@@ -181,11 +185,12 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     key and value head; views of a fused projection are read where they lie), log_decay [h] float32, not above 0 (-inf: a head
     without memory); it gets no gradient.  `scale`: dk ** -0.5 by default.  initial_state [b, h, dk, dv] float32 or None (zeros).
     `cu_seqlens` (int32 [n + 1] on the device, b must be 1): n sequences packed back to back, empty ones allowed, each with its
-    own state ([n, h, dk, dv]); tokens outside of them have zero outputs.  Returns o [b, l, h, dv] bf16 and the state behind the
+    own state ([n, h, dk, dv]); tokens outside of them have zero outputs (bounds that fall or pass the end stay inside the arrays, with
+    numbers that mean nothing).  Returns o [b, l, h, dv] bf16 and the state behind the
     last token (None without `output_final_state`).  Differentiable with respect to q, k, v and initial_state, through both.
     Products take q, k, v as they are and round the weights of a tile's tokens and its incoming state to bf16; sums and the state
     itself are kept in float32.  A NaN or an infinity in k, v reaches the outputs of its whole tile of 128 tokens (counted from
-    the start of its sequence) and, as the formula has it, all later ones."""
+    the start of its sequence) and later ones, for as long at least as its weight has not decayed below the smallest float32."""
     h, dk, dv = _linear_heads("linear_attention", q, k, v, log_decay, 4)
     n = q.shape[0]
     if cu_seqlens is not None:
