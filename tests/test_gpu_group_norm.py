@@ -234,6 +234,6 @@ def test_a_layer_of_both(lo):
     ry = orc.group_norm(ro.reshape(b * l, h * d), h, ref[3], silu=True)
     want = torch.autograd.grad(ry, ref, dy.reshape(b * l, h * d).double())
     # three roundings of half a step one after the other (weights, o, y), four for the gradients (dy's way back through o)
-    assert float((y.double() - ry).norm()) <= 3 * 2.0 ** -8 * float(ry.norm())
+    assert float((y.detach().double() - ry.detach()).norm()) <= 3 * 2.0 ** -8 * float(ry.detach().norm())
     for a, r in zip(got, want):
         assert float((a.double() - r).norm()) <= 4 * 2.0 ** -8 * float(r.norm())

@@ -114,6 +114,43 @@ def test_a_long_sequence_of_few_heads(lo):
     _check(lo, _inputs(1, 5000, 2, 2, 64, 64), grads=False)
 
 
+def _tiles(q, k, v, decay, S, size=100):
+    """The same in 64 bits by tiles of `size` tokens (differentiable; the oracle goes token by token)."""
+    b, l, h, dk = q.shape
+    share = h // k.shape[2]
+    q, k, v = (t.double().transpose(1, 2) for t in (q * dk ** -0.5, k.repeat_interleave(share, 2), v.repeat_interleave(share, 2)))
+    g, outs = decay.double(), []
+    for a in range(0, l, size):
+        qc, kc, vc = q[:, :, a:a + size], k[:, :, a:a + size], v[:, :, a:a + size]
+        i = torch.arange(qc.shape[2], device=q.device, dtype=torch.float64)
+        gap = i[:, None] - i
+        W = torch.exp(g[:, None, None] * gap.clamp(min=0)) * (gap >= 0)
+        outs.append((qc @ kc.transpose(2, 3) * W) @ vc + torch.exp(g[:, None] * (i + 1))[..., None] * (qc @ S))
+        S = torch.exp(g * len(i))[:, None, None] * S + (kc * torch.exp(g[:, None] * (len(i) - 1 - i))[..., None]).transpose(2, 3) @ vc
+    return torch.cat(outs, 2).transpose(1, 2), S
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 128), (128, 64)])
+@pytest.mark.parametrize("b,l,h,hk", [(10, 1411, 16, 8), (2, 9001, 10, 10)])
+def test_many_tiles_a_block(lo, b, l, h, hk, dk, dv):
+    """Runs of ten tiles a block, over whole sequences and over cut ones (20 sequences and heads of 71 tiles)."""
+    from lact_b200 import synchronize_and_check
+    x = _inputs(b, l, h, hk, dk, dv)
+    leaves = [x[n].clone().requires_grad_() for n in ("q", "k", "v", "S")]
+    o, last = lo.linear_attention(*leaves[:3], x["g"], None, leaves[3], True)
+    got = torch.autograd.grad([o, last], leaves, [x["do"], x["dS"]])
+    short = lo.linear_attention(*leaves[:3], x["g"], None, leaves[3])[0]     # (without the last state: two pieces of the keys)
+    ref = [x[n].double().requires_grad_() for n in ("q", "k", "v", "S")]
+    ro, rlast = _tiles(*ref[:3], x["g"], ref[3])
+    want = torch.autograd.grad([ro, rlast], ref, [x["do"].double(), x["dS"].double()])
+    synchronize_and_check()
+    for name, a, w in zip(("o", "o2", "dq", "dk", "dv"), (o, short, *got[:3]), (ro, ro, *want[:3])):
+        a, w = a.detach(), w.detach()
+        assert float((a.double() - w).norm()) <= OUT["norm"] * float(w.norm()), name
+    for name, a, w in (("last", last.detach(), rlast.detach()), ("dS", got[3], want[3])):
+        assert float((a.double() - w).norm()) <= STATE["norm"] * float(w.norm()), name
+
+
 def test_decays_at_the_ends(lo):
     """No decay, no memory (-inf), and decays that underflow within a tile."""
     x = _inputs(1, 400, 6, 6, 64, 64)
@@ -316,3 +353,10 @@ def test_compiled_caller(lo):
     got = torch.compile(f, fullgraph=True, backend="aot_eager")(other, x["k"], x["v"], x["g"], x["S"])
     got.backward()
     assert torch.equal(got, want) and torch.equal(other.grad, leaf.grad)
+    step = lambda q, k, v, g, S, new: lo.linear_attention_step(q * 1.0, k, v, g, S, new_state=new)
+    token = tuple(x[n][:, 0] for n in "qkv")
+    news = [torch.zeros_like(x["S"]) for _ in range(2)]
+    with torch.no_grad():
+        plain = step(*token, x["g"], x["S"], news[0])
+        traced = torch.compile(step, fullgraph=True, backend="aot_eager")(*token, x["g"], x["S"], news[1])
+    assert torch.equal(plain, traced) and torch.equal(news[0], news[1])
