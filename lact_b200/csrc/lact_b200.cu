@@ -2098,15 +2098,22 @@ struct LinearPlan {
 };
 LinearPlan linear_plan(const lact_linear_config* c) {
   const int64_t sms = std::min(sm_count(), kLinearMaxCtas);
-  if (c->sequences > 0) {
+  if (c->sequences > 0) {   // (their lengths are on the device: cut, into runs that the kernel works out to be even)
     const int64_t most = c->heads * (c->tokens / 128 + std::min(c->sequences, c->tokens));
     const int ctas = static_cast<int>(std::min(sms, most));
     return {false, ctas > 1, ctas, 0};
   }
+  // Token by token (us against tiles, forward, heads of 128): 12 heads, 8 tokens 4.7 / 7.8, 16 6.5 / 8.0, 32 10.0 / 7.9; 64 x 12 heads, 4
+  // tokens 19.6 / 22.7, 8 28.7 / 22.8.  8 heads of 64, 16 tokens 5.8 / 6.8, 32 9.0 / 6.8.
   const int64_t tiles = ceil_div(c->tokens, 128), chains = c->batch * c->heads, total = tiles * chains;
-  if (c->tokens <= 8) return {true, false, 0, 0};
-  const int64_t whole = tiles * ((chains + sms - 1) / sms), even = (total + sms - 1) / sms;
-  const bool cut = 3 * whole > 4 * even + 10;
+  if (c->tokens <= (chains <= sms ? 16 : 4)) return {true, false, 0, 0};
+  // Whole sequences, or cut ones with a pass over their shares before.  Measured with heads of 128, us of whole / cut: 12 heads, 512
+  // tokens 16.6 / 18.2, 1024 28.2 / 21.1, 4096 97.6 / 33.5; 48 heads, 2048 54 / 44; 96 heads, 2048 56 / 69; 156 heads, 1024 55 / 59, 4096
+  // 196 / 169; 288 heads, 4096 228 / 271; 300 heads 307 / 281.  That is 5 + 3.2 a tile of the longest run of whole ones, 16 + 4.5 a tile of the even runs.  Heads of 64:
+  // 8 heads, 512 tokens 13.2 / 14.6, 1024 21.6 / 15.6; 128 heads, 1024 24 / 37; 160 heads, 8192 267 / 208: 4.6 + 2.1 and 13 + 3.1.
+  const int64_t whole = tiles * ((chains + sms - 1) / sms), even = (total + sms - 1) / sms, wide = c->dk + c->dv;
+  const double once = wide == 256 ? 3.2 : wide == 192 ? 2.7 : 2.1, twice = wide == 256 ? 4.5 : wide == 192 ? 3.8 : 3.1;
+  const bool cut = once * whole > twice * even + (wide == 256 ? 11.0 : wide == 192 ? 9.7 : 8.4);
   const int64_t per = cut ? even : whole;
   return {false, cut, static_cast<int>((total + per - 1) / per), per};
 }
