@@ -13,6 +13,8 @@
 // fp32 (D alone is summed by the tensor core, which truncates: over a long sequence that would show): the decayed rows of Y are two
 // bf16 pieces (16 bits of the product; what is lost, 2^-17, is far below the copy's rounding), three (24 bits) where the last state
 // is an output.
+// Measured (2 x 32768 tokens, 12 heads of 128, 42 tiles a CTA): 141 us forwards, 805 MB at 5.7 TB/s, 3.4 us a tile where its 131 KB take 3.0;
+// with three pieces 4.0 (48 products of 68 clocks).  What is left is the chain from D through the state's copy, X S and P Z to the next G.
 // Long sequences of few heads: `per` tiles a CTA may begin within a sequence.  linear_chunks_kernel<.., PIECE, ..> first leaves every CTA's
 // share of the state of the sequence that goes on behind it, linear_carry_kernel adds the shares up in order.  The shares are taken
 // from the last tile to the first, so that the tiles the CTA begins with afterwards have been read last and are still in L2, and only as far as fp32 has room for their decay.

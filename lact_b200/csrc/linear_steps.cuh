@@ -68,7 +68,7 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* f) {
 
 // One CTA per (sequence, head, 32 columns of the state); 8 threads hold a row's columns, 4 each, 32 rows at a time.
 // Bound by the state's bytes (8 A B a head and token of generation): 32 columns a CTA keep 148 SMs busy from about 40 heads on and
-// have 16 KB in flight per CTA, 8 CTAs an SM.
+// have 16 KB in flight per CTA.  (8 tokens of 12 heads of 128: 4.7 us; linear_plan has the rule between this and the tiles.)
 constexpr int kStepTokens = 8;   // tokens staged at a time
 template <int A, int B>
 __global__ void __launch_bounds__(256) linear_steps_kernel(const __grid_constant__ LinearArgs a) {
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256) linear_steps_kernel(const __grid_constant
 }
 
 // One token of every sequence, forward, states as they are stored: the same split without the staging and the loops, so that more CTAs
-// are resident (192 sequences of 12 heads of 128 x 128, 304 MB: 66 us with the kernel above).
+// are resident (192 sequences of 12 heads of 128 x 128, 304 MB: 46.4 us, 6.5 TB/s; 66 with the kernel above).
 template <int A, int B>
 __global__ void __launch_bounds__(256, 6) linear_token_kernel(const __grid_constant__ LinearArgs a) {
   constexpr int R = A / 32;
