@@ -78,9 +78,6 @@ __global__ void __launch_bounds__(256) linear_steps_kernel(const __grid_constant
   griddep_wait();
   const int tid = threadIdx.x, cl = tid & 7, rg = tid >> 3, warp = tid >> 5, lane = tid & 31;
   const int unit = blockIdx.x / (B / 32), n = unit / a.heads, head = unit % a.heads, c0 = blockIdx.x % (B / 32) * 32;
-  linear_zero_rest<B>(a, static_cast<int64_t>(blockIdx.x) * 256 + tid, static_cast<int64_t>(gridDim.x) * 256);
-  const LinearSpan s = linear_span(a, n);
-  if (s.len == 0 && a.s_out == nullptr) return;
   float S[R][4];
   const int64_t at = (static_cast<int64_t>(n) * a.heads + head) * (A * B);
 #pragma unroll
@@ -98,12 +95,12 @@ __global__ void __launch_bounds__(256) linear_steps_kernel(const __grid_constant
     }
   }
   const float lambda = exp2f(decay_log2(a, head));
-  const bf16* const x = a.x + s.entry * a.x_bs + (head / a.x_share) * A;
-  const bf16* const y = a.y + s.entry * a.y_bs + (head / a.y_share) * A;
-  const bf16* const z = a.z + s.entry * a.z_bs + (head / a.z_share) * B + c0;
-  for (int p0 = 0; p0 < s.len; p0 += kStepTokens) {
-    const int count = min(kStepTokens, s.len - p0);
-    auto token = [&](int tt) { return static_cast<int64_t>(s.first + (a.reverse ? s.len - 1 - p0 - tt : p0 + tt)); };
+  const bf16* const x = a.x + n * a.x_bs + (head / a.x_share) * A;
+  const bf16* const y = a.y + n * a.y_bs + (head / a.y_share) * A;
+  const bf16* const z = a.z + n * a.z_bs + (head / a.z_share) * B + c0;
+  for (int p0 = 0; p0 < a.L; p0 += kStepTokens) {
+    const int count = min(kStepTokens, a.L - p0);
+    auto token = [&](int tt) { return static_cast<int64_t>(a.reverse ? a.L - 1 - p0 - tt : p0 + tt); };
     for (int u = tid; u < count * (A / 8); u += 256) {
       const int tt = u / (A / 8), c = u % (A / 8) * 8;
       unpack_bf16x8(*reinterpret_cast<const uint4*>(x + token(tt) * a.x_ts + c), &sx[tt][c]);
@@ -138,14 +135,14 @@ __global__ void __launch_bounds__(256) linear_steps_kernel(const __grid_constant
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) sum += part[tt][w][c];
-      const int64_t o = ((s.entry * static_cast<int64_t>(a.L) + token(tt)) * a.heads + head) * B + c0 + c;
+      const int64_t o = ((n * static_cast<int64_t>(a.L) + token(tt)) * a.heads + head) * B + c0 + c;
       if (a.out_f32) static_cast<float*>(a.out)[o] = sum * a.scale;
       else static_cast<bf16*>(a.out)[o] = __float2bfloat16_rn(sum * a.scale);
     }
     __syncthreads();
   }
   if (a.s_out == nullptr) return;
-  const float mul = a.out_mul * (a.reverse && s.len > 0 ? lambda : 1.f);
+  const float mul = a.out_mul * (a.reverse ? lambda : 1.f);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int row = rg + 32 * i;
