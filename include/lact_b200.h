@@ -339,7 +339,8 @@ int lact_swa_bwd(const void *q, const void *k, const void *v, const void *o, con
  *   S_t = exp(log_decay[head]) S_(t-1) + k_t v_t^T,   o_t = scale q_t^T S_t .
  * q [batch, tokens, heads, dk], k and v [batch, tokens, kv_heads, dk or dv] bf16, heads adjacent within a token, token / batch
  * strides in elements (multiples of 8), bases 16-byte aligned; dk, dv 64 or 128 each; kv_heads divides heads (consecutive heads
- * share).  log_decay: fp32 [heads], meant to be <= 0 (-inf: no memory).  states fp32, contiguous [sequences, heads, dk, dv].  No counterpart in the
+ * share).  log_decay: fp32 [heads], meant to be <= 0 (-inf: no memory).  states fp32, contiguous [sequences, heads, dk, dv], bases
+ * 16-byte aligned; o, dq, dk and dv 32-byte aligned.  No counterpart in the
  * reference, whose recurrences have nonlinear memories. */
 typedef struct lact_linear_config {
   int64_t batch, tokens, heads, kv_heads, dk, dv;

@@ -133,7 +133,7 @@ __device__ __forceinline__ float v_dot(const float (&a)[V], const float (&b)[V])
 
 // sigmoid(z) of V values.  Two special-function results an element (16 a clock and SM) take as long as the memory of a large call
 // (77 million elements: 34 us; two frames of 480 x 832 x 96 come and go in 47): two neighbours share one reciprocal, 1 / a = b (1 / ab).
-// Below z = -41 the sigmoid stays at 2^-60, so that the product stays finite.
+// Below z = -41 the sigmoid stays at 2^-60, so that the product stays finite (silu is off by |z| 2^-60: less than 2^-40 at z = -10^6).
 template <int V>
 __device__ __forceinline__ void sigmoids(const float (&z)[V], float (&g)[V]) {
   if constexpr (V == 1) {

@@ -60,6 +60,17 @@ def test_missing_and_crooked_pointers_are_refused(lib):
     assert lib.lact_linear_attention_step(C.byref(c), p, p, p, p, None, p, p, None) == -1
 
 
+def test_crooked_states_are_refused(lib):
+    c, p, bad, z = _config(), C.c_void_p(4096), C.c_void_p(4104), C.c_size_t(0)
+    for s_in, s_out in ((bad, None), (None, bad)):
+        assert lib.lact_linear_attention_fwd(C.byref(c), p, p, p, p, None, s_in, s_out, p, None, z, p, None) == -2
+    for s_in, d_out, d_in in ((bad, None, None), (None, bad, None), (None, None, bad)):
+        assert lib.lact_linear_attention_bwd(C.byref(c), p, p, p, p, None, s_in, None, z, p, d_out, p, p, p, d_in, None, z, p, None) == -2
+    c = _config(tokens=1)
+    for s_in, s_out in ((bad, p), (p, bad)):
+        assert lib.lact_linear_attention_step(C.byref(c), p, p, p, p, s_in, s_out, p, None) == -2
+
+
 def _args(h=4, hk=2, dk=64, dv=128, l=5, b=2):
     return (torch.zeros(b, l, h, dk, dtype=BF16), torch.zeros(b, l, hk, dk, dtype=BF16), torch.zeros(b, l, hk, dv, dtype=BF16),
             torch.zeros(h))
