@@ -190,7 +190,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     last token (None without `output_final_state`).  Differentiable with respect to q, k, v and initial_state, through both.
     Products take q, k, v as they are and round the weights of a tile's tokens and its incoming state to bf16; sums and the state
     itself are kept in float32.  A NaN or an infinity in k, v reaches the outputs of its whole tile of 128 tokens (counted from
-    the start of its sequence) and later ones, for as long at least as its weight has not decayed below the smallest float32."""
+    the start of its sequence) and later ones, for as long at least as its weight has not decayed below the smallest float32: the rows
+    that pad a batch hold finite numbers, or its sequences are packed (what lies behind those is not looked at)."""
     h, dk, dv = _linear_heads("linear_attention", q, k, v, log_decay, 4)
     n = q.shape[0]
     if cu_seqlens is not None:
