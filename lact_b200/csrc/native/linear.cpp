@@ -129,6 +129,33 @@ Tensor step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& 
   return o;
 }
 
+// The step as autograd sees it.  `new_state` gets a new version, so that a backward that has saved it (linear_attention saves its first
+// state) raises in place of reading what is there now.  (PyTorch's own fallback for operators without a backward goes past the key that
+// does this.  Tensors of inference mode have no version, and no backward can have saved them.)
+using StepSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double, const Tensor&, const Tensor&);
+const auto& step_op() {
+  static const auto o = c10::Dispatcher::singleton().findSchemaOrThrow("lact_b200::linear_attention_step", "").typed<StepSig>();
+  return o;
+}
+Tensor step_versioned(c10::DispatchKeySet keys, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale,
+                      const Tensor& state, const Tensor& new_state) {
+  Tensor o;
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    o = step_op().redispatch(keys & c10::after_ADInplaceOrView_keyset, q, k, v, g, scale, state, new_state);
+  }
+  if (!new_state.is_inference()) torch::autograd::impl::bump_version(new_state);
+  return o;
+}
+Tensor step_autograd(c10::DispatchKeySet keys, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale,
+                     const Tensor& state, const Tensor& new_state) {
+  for (const Tensor* t : {&q, &k, &v, &g, &state, &new_state})
+    TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t->requires_grad()) && !t->_fw_grad(0).defined(),
+                                "linear_attention_step has no derivatives: use linear_attention");
+  at::AutoDispatchBelowAutograd guard;
+  return step_op().redispatch(keys & c10::after_autograd_keyset, q, k, v, g, scale, state, new_state);
+}
+
 using FwdSig = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double, const OptTensor&, const OptTensor&, bool,
                                    bool);
 using BwdSig = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, double, const OptTensor&, const OptTensor&,
@@ -187,9 +214,10 @@ TORCH_LIBRARY_IMPL(lact_b200, CUDA, m) {
   m.impl("linear_attention_bwd", &bwd);
   m.impl("linear_attention_step", &step);
 }
+TORCH_LIBRARY_IMPL(lact_b200, ADInplaceOrView, m) { m.impl("linear_attention_step", &step_versioned); }
 TORCH_LIBRARY_IMPL(lact_b200, Autograd, m) {
   m.impl("linear_attention_bwd", torch::autograd::autogradNotImplementedFallback());
-  m.impl("linear_attention_step", torch::autograd::autogradNotImplementedFallback());
+  m.impl("linear_attention_step", &step_autograd);
   m.impl("linear_attention_fwd", &linear_autograd);
 }
 
