@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <optional>
 #include <vector>
 
@@ -46,6 +47,12 @@ inline void* ptr(const OptTensor& t) { return t.has_value() && t->defined() ? t-
 inline bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 inline Tensor value(const OptTensor& t) { return given(t) ? *t : Tensor(); }
 inline OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+// None of the operators has a formula for forward-mode derivatives, and below autograd a tangent would be dropped without a word.
+inline void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!(t->defined() && t->_fw_grad(/*level=*/0).defined()), what, " has no forward-mode derivatives");
+}
 
 inline void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 

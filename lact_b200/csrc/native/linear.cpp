@@ -149,9 +149,9 @@ Tensor step_versioned(c10::DispatchKeySet keys, const Tensor& q, const Tensor& k
 }
 Tensor step_autograd(c10::DispatchKeySet keys, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale,
                      const Tensor& state, const Tensor& new_state) {
+  no_tangents("linear_attention_step", {&q, &k, &v, &g, &state, &new_state});
   for (const Tensor* t : {&q, &k, &v, &g, &state, &new_state})
-    TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t->requires_grad()) && !t->_fw_grad(0).defined(),
-                                "linear_attention_step has no derivatives: use linear_attention");
+    TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t->requires_grad()), "linear_attention_step has no backward: use linear_attention");
   at::AutoDispatchBelowAutograd guard;
   return step_op().redispatch(keys & c10::after_autograd_keyset, q, k, v, g, scale, state, new_state);
 }
@@ -191,9 +191,11 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
 };
 std::vector<Tensor> linear_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale, const OptTensor& state,
                                     const OptTensor& cu, bool want_state, bool keep) {
+  const Tensor first = value(state);
+  no_tangents("linear_attention", {&q, &k, &v, &g, &first});
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK_NOT_IMPLEMENTED(!g.requires_grad(), "linear_attention has no gradient for log_decay");
-    if (q.requires_grad() || k.requires_grad() || v.requires_grad() || value(state).requires_grad())
+    if (q.requires_grad() || k.requires_grad() || v.requires_grad() || first.requires_grad())
       return LinearFunction::apply(q, k, v, g, scale, state, cu, want_state);
   }
   at::AutoDispatchBelowADInplaceOrView guard;

@@ -106,7 +106,9 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
   }
 };
 std::vector<Tensor> norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t groups, double eps, bool silu) {
-  if (at::GradMode::is_enabled() && (x.requires_grad() || value(w).requires_grad() || value(b).requires_grad()))
+  const Tensor weight = value(w), bias = value(b);
+  no_tangents("group_norm", {&x, &weight, &bias});
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || bias.requires_grad()))
     return NormFunction::apply(x, w, b, groups, eps, silu);
   at::AutoDispatchBelowADInplaceOrView guard;
   return fwd_op().call(x, w, b, groups, eps, silu);
