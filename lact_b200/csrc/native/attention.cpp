@@ -116,6 +116,7 @@ class SwaFunction : public torch::autograd::Function<SwaFunction> {
 };
 std::vector<Tensor> swa_autograd(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, double scale,
                                  const OptTensor& seq) {
+  no_tangents("attention", {&q, &k, &v});
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return SwaFunction::apply(q, k, v, window, scale, seq);
   at::AutoDispatchBelowADInplaceOrView guard;
@@ -126,6 +127,7 @@ using CacheSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const Tenso
 // (with gradients the keys and values are put together first: the backward reads them as one array)
 Tensor swa_cache_autograd(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& k, const Tensor& v, double scale) {
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("lact_b200::swa_fwd_cache", "").typed<CacheSig>();
+  no_tangents("attention", {&q, &kc, &vc, &k, &v});
   bool grad = false;
   for (const Tensor* t : {&q, &kc, &vc, &k, &v}) grad = grad || t->requires_grad();
   if (at::GradMode::is_enabled() && grad) return fwd_op().call(q, at::cat({kc, k}, 1), at::cat({vc, v}, 1), -1, scale, {})[0];

@@ -92,6 +92,7 @@ class QkvFunction : public torch::autograd::Function<QkvFunction> {
 };
 std::vector<Tensor> qkv_autograd(const Tensor& xq, const Tensor& xk, const Tensor& xv, int64_t n_h, bool silu, bool v_silu,
                                  const OptTensor& cos, const OptTensor& sin, int64_t hd, int64_t offset, const OptTensor& seq) {
+  no_tangents("qkv_prologue", {&xq, &xk, &xv});
   if (at::GradMode::is_enabled() && (wants_grad(xq) || wants_grad(xk) || wants_grad(xv)))
     return QkvFunction::apply(xq, xk, xv, n_h, silu, v_silu, cos, sin, hd, offset, seq);
   at::AutoDispatchBelowADInplaceOrView guard;
@@ -164,7 +165,9 @@ class LrFunction : public torch::autograd::Function<LrFunction> {
   }
 };
 std::vector<Tensor> lr_autograd(const Tensor& proj, const OptTensor& logits, int64_t n_h, double base_inv) {
-  if (at::GradMode::is_enabled() && (wants_grad(proj) || (given(logits) && wants_grad(*logits))))
+  const Tensor log = value(logits);
+  no_tangents("lr_prologue", {&proj, &log});
+  if (at::GradMode::is_enabled() && (wants_grad(proj) || wants_grad(log)))
     return LrFunction::apply(proj, logits, n_h, base_inv);
   at::AutoDispatchBelowADInplaceOrView guard;
   return lr_op().call(proj, logits, n_h, base_inv);
@@ -233,7 +236,9 @@ class OutFunction : public torch::autograd::Function<OutFunction> {
   }
 };
 Tensor out_autograd(const Tensor& x, const Tensor& w, const OptTensor& gate, const OptTensor& res, int64_t n_h, double eps) {
-  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(value(gate)) || wants_grad(value(res))))
+  const Tensor g = value(gate), r = value(res);
+  no_tangents("out_epilogue", {&x, &w, &g, &r});
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(g) || wants_grad(r)))
     return OutFunction::apply(x, w, gate, res, n_h, eps);
   at::AutoDispatchBelowADInplaceOrView guard;
   return out_op().call(x, w, gate, res, n_h, eps);

@@ -182,6 +182,8 @@ std::vector<Tensor> scan_autograd(const Tensor& w0, const Tensor& w1, const Tens
                                   const Tensor& v, const Tensor& lr0, const Tensor& lr1, const Tensor& lr2,
                                   const OptTensor& momentum, const OptTensor& m0, const OptTensor& m1, const OptTensor& m2,
                                   at::IntArrayRef steps, at::IntArrayRef cfg, double w_scale) {
+  const Tensor mom = value(momentum), s0 = value(m0), s1 = value(m1), s2 = value(m2);
+  no_tangents("the recurrence", {&w0, &w1, &w2, &q, &k, &v, &lr0, &lr1, &lr2, &mom, &s0, &s1, &s2});
   bool grad = false;
   if (at::GradMode::is_enabled()) {
     for (const Tensor* t : {&w0, &w1, &w2, &q, &k, &v, &lr0, &lr1, &lr2}) grad = grad || t->requires_grad();

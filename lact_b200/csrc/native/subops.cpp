@@ -62,6 +62,7 @@ class FfnFunction : public torch::autograd::Function<FfnFunction> {
   }
 };
 Tensor ffn_autograd(const Tensor& w02, const Tensor& w1, const Tensor& x) {
+  no_tangents("swiglu_ffn", {&w02, &w1, &x});
   if (wants_grad({&w02, &w1, &x})) return FfnFunction::apply(w02, w1, x);
   at::AutoDispatchBelowADInplaceOrView guard;
   return ffn_op().call(w02, w1, x);
@@ -128,6 +129,7 @@ class GradsFunction : public torch::autograd::Function<GradsFunction> {
 };
 std::vector<Tensor> grads_autograd(const Tensor& w02, const Tensor& w1, const Tensor& k, const Tensor& v, const Tensor& lr0,
                                    const Tensor& lr1, const Tensor& lr2) {
+  no_tangents("fw_grads", {&w02, &w1, &k, &v, &lr0, &lr1, &lr2});
   if (wants_grad({&w02, &w1, &k, &v, &lr0, &lr1, &lr2})) return GradsFunction::apply(w02, w1, k, v, lr0, lr1, lr2);
   at::AutoDispatchBelowADInplaceOrView guard;
   return grads_op().call(w02, w1, k, v, lr0, lr1, lr2);
@@ -186,6 +188,7 @@ class L2Function : public torch::autograd::Function<L2Function> {
   }
 };
 Tensor l2_autograd(const Tensor& x, const Tensor& xa, const Tensor& scale, double eps, bool out_bf16) {
+  no_tangents("l2_norm_add", {&x, &xa, &scale});
   if (wants_grad({&x, &xa, &scale})) return L2Function::apply(x, xa, scale, eps, out_bf16);
   at::AutoDispatchBelowADInplaceOrView guard;
   return l2_op().call(x, xa, scale, eps, out_bf16);

@@ -31,7 +31,48 @@ def _norm():
     return [_t(3, 8, 64), _t(64, dtype=F32), _t(64, dtype=F32), 4, 1e-5, True]
 
 
-CASES = [("linear_attention_fwd", _linear), ("linear_attention_step", _step), ("group_norm_fwd", _norm)]
+def _swa():
+    return [_t(1, 8, 4, 64), _t(1, 8, 4, 64), _t(1, 8, 4, 64), 0, 0.1]
+
+
+def _swa_cache():
+    return [_t(1, 8, 4, 64), _t(1, 9, 4, 64), _t(1, 9, 4, 64), _t(1, 8, 4, 64), _t(1, 8, 4, 64), 0.1]
+
+
+def _qkv():
+    return [_t(1, 8, 64), _t(1, 8, 64), _t(1, 8, 64), 1, True, True, None, None, 64, 0, None]
+
+
+def _lr():
+    return [_t(1, 8, 3, dtype=F32), _t(1, 8, 1), 1, 0.1]
+
+
+def _out():
+    return [_t(2, 8, 64), _t(64, dtype=F32), _t(1, 8, 128), _t(1, 8, 128), 2, 1e-5]
+
+
+def _ffn():
+    return [_t(1, 128, 64), _t(1, 64, 64), _t(1, 8, 64)]
+
+
+def _fw_grads():
+    return _ffn() + [_t(1, 8, 64)] + [_t(1, 8, 1, dtype=F32) for _ in range(3)]
+
+
+def _l2():
+    return [_t(1, 8, 64, dtype=F32), _t(1, 8, 64), _t(1, 8, 1, dtype=F32), 1e-5, True]
+
+
+def _scan():
+    from lact_b200 import program as P
+    w = [_t(1, 64, 64, dtype=F32) for _ in range(3)]
+    steps, cfg = [P.UPDATE, 0, 8, 0, P.APPLY, 0, 8, 0], [0] * 10 + [-1, 0, 0, 0]
+    return w + [_t(1, 8, 64) for _ in range(3)] + [_t(1, 8, 1, dtype=F32) for _ in range(4)] + [None, None, None, steps, cfg, 0.0]
+
+
+CASES = [("swa_fwd", _swa), ("swa_fwd_cache", _swa_cache), ("qkv_prologue", _qkv), ("lr_prologue", _lr), ("out_epilogue", _out),
+         ("swiglu_ffn_fwd", _ffn), ("fw_grads_fwd", _fw_grads), ("l2_norm_add_fwd", _l2), ("scan_fwd", _scan),
+         ("linear_attention_fwd", _linear), ("linear_attention_step", _step), ("group_norm_fwd", _norm)]
 
 
 @pytest.mark.parametrize("name,make", CASES)
