@@ -78,6 +78,14 @@ void poll_status(const Tensor& like);
 // are waited for in Python).
 void settle(const Tensor& like);
 
+// `t` contiguous, on a 16-byte boundary, and with the strides that its sizes give.  (PyTorch calls a tensor contiguous whatever stands as
+// the stride of an axis of one entry, and wherever it begins: `contiguous` by itself returns such a tensor as it is.)
+inline Tensor plain(const Tensor& t) {
+  Tensor c = t.contiguous();
+  if (reinterpret_cast<uintptr_t>(c.data_ptr()) % 16) c = c.clone();
+  return c.as_strided(c.sizes(), c10::contiguous_strides(c.sizes()));
+}
+
 // A [batch, rows, cols] bf16 activation whose last axis is contiguous and whose strides and base keep 16-byte alignment
 // (views of fused projections pass through); anything else is copied.
 inline Tensor aligned(const Tensor& t, int64_t elems = 8) {

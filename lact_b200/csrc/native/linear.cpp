@@ -8,19 +8,14 @@ namespace {
 Tensor head_view(const Tensor& t) {
   const int64_t h = t.size(2), d = t.size(3);
   if (t.stride(3) != 1 || t.stride(2) != d || t.stride(1) % 8 || t.stride(0) % 8 || t.stride(1) < h * d ||
-      (t.stride(0) == 0 && t.size(0) > 1) || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) {
-    Tensor c = t.contiguous();   // (a contiguous view off a 16-byte boundary is returned as it is)
-    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
-  }
+      (t.stride(0) == 0 && t.size(0) > 1) || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16)
+    return plain(t);
   return t;
 }
 
 // [b, h, d] likewise
 Tensor token_view(const Tensor& t) {
-  if (t.stride(2) != 1 || t.stride(1) != t.size(2) || t.stride(0) % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) {
-    Tensor c = t.contiguous();
-    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
-  }
+  if (t.stride(2) != 1 || t.stride(1) != t.size(2) || t.stride(0) % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return plain(t);
   return t;
 }
 
