@@ -10,7 +10,7 @@ Tensor head_view(const Tensor& t) {
   const int64_t h = t.size(2), d = t.size(3);
   if (t.stride(3) != 1 || t.stride(2) != d || t.stride(1) % 8 || t.stride(0) % 8 || t.stride(1) < h * d ||
       reinterpret_cast<uintptr_t>(t.data_ptr()) % 16)
-    return t.contiguous();
+    return plain(t);
   return t;
 }
 
