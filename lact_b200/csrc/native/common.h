@@ -91,7 +91,7 @@ inline Tensor plain(const Tensor& t) {
 inline Tensor aligned(const Tensor& t, int64_t elems = 8) {
   if (t.stride(-1) != 1 || t.stride(1) % elems || t.stride(0) % elems || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ||
       t.stride(1) < t.size(-1))
-    return t.contiguous();
+    return plain(t);
   return t;
 }
 

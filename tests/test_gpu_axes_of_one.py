@@ -53,3 +53,27 @@ def test_attention_over_a_cache(lo):
     q, kc, vc, k, v = (next(_heads(1, n, 4, 64, i)) for i, n in enumerate((1, 40, 40, 1, 1)))
     op = torch.ops.lact_b200.swa_fwd_cache
     assert torch.equal(op(q, kc, vc, k, v, 0.125), op(*(_copy(t) for t in (q, kc, vc, k, v)), 0.125))
+
+
+def _rows(b, s, n, seed):
+    x = _rn(b, s, n, seed=seed)
+    yield torch.empty(x.numel() + 1, dtype=BF16, device="cuda")[1:].view(x.shape).copy_(x)
+    if b == 1:
+        yield x.as_strided((b, s, n), (s * n + 3, n, 1))
+    if s == 1:
+        yield x.as_strided((b, s, n), (n, 3, 1))
+        yield x.transpose(1, 2).contiguous().transpose(1, 2)
+
+
+@pytest.mark.parametrize("b,s", [(1, 1), (3, 1), (1, 7)])
+def test_layer_passes(lo, b, s):
+    w = torch.ones(64, device="cuda")
+    x = _rn(b * 2, s, 64, seed=9)
+    for a, c, d in zip(*(_rows(b, s, 128, i) for i in range(3))):
+        for call in (lambda p, q, r: lo.qkv_prologue(p, q, r, 2), lambda p, q, r: (lo.out_epilogue(x, w, 2, p, q),)):
+            got, want = [], []
+            for out, ts in ((got, (a, c, d)), (want, [_copy(t) for t in (a, c, d)])):
+                leaves = [t.detach().requires_grad_() for t in ts]
+                o = call(*leaves)
+                out += [*o, *torch.autograd.grad(sum(t.float().square().sum() for t in o), leaves, allow_unused=True)]
+            assert all(torch.equal(g, w_) for g, w_ in zip(got, want) if w_ is not None)
