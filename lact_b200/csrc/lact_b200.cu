@@ -2144,14 +2144,14 @@ int launch_linear_chunks(const LinearChunkArgs& a, int ctas, cudaStream_t st) {
   LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kLinearThreads), smem, st, a));
   return LACT_OK;
 }
-// `carried`: the slots hold what the CTAs begin with already.  THREE: the last states are an output
+// `carried`: the slots hold what the CTAs begin with already.  THREE: the last states are an output.  (A first state that is stored
+// transposed comes with carried slots: the shares' passes and the carry read it as it is.)
 template <int A, int B, bool THREE>
 int linear_chunks(const LinearChunkArgs& a, const LinearPlan& p, bool carried, cudaStream_t st) {
   if (p.cut && !carried) {
     LACT_TRY((launch_linear_chunks<A, B, true, THREE, false>(a, p.ctas, st)));
     KernelScope scope(kClsOther, st);
-    LACT_CUDA(launch_pdl(linear_carry_kernel, dim3(A * B / 512, p.ctas), dim3(128), 0, st, a.a.s_in, a.a.s_in_t, a.a.in_mul, a.slots, a.pieces,
-                         p.ctas, A, B));
+    LACT_CUDA(launch_pdl(linear_carry_kernel, dim3(A * B / 512, p.ctas), dim3(128), 0, st, a.a.s_in, a.a.in_mul, a.slots, a.pieces, p.ctas, A * B));
   }
   return a.a.reverse ? launch_linear_chunks<A, B, false, THREE, true>(a, p.ctas, st) : launch_linear_chunks<A, B, false, THREE, false>(a, p.ctas, st);
 }

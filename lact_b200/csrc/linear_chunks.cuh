@@ -42,7 +42,7 @@ struct LinearChunkArgs {
   LinearArgs a;
   CUtensorMap x, y, z;   // 4-D maps (feature, token, head, entry), box {64, 128, 1, 1}
   uint32_t per;          // tiles a CTA takes; packed sequences: 0, as many as make the CTAs even
-  float* slots;          // [CTA] states: what the next CTA's sequence begins with ([A][B], or [B][A] if slots_t)
+  float* slots;          // [CTA] states: what the next CTA's sequence begins with ([A][B]; those of another pass may be read as [B][A]: slots_t)
   LinearPiece* pieces;   // [CTA]
   int32_t slots_t;
   int32_t* status;
@@ -624,15 +624,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         for (int j = 0; j < NC; ++j) S[j] = from[j * B] * mul;
       }
     };
-    auto store_state = [&](float* to, int64_t n, bool transposed, float mul) {
-      to += n * (A * B) + (transposed ? r * A + c0 : c0 * B + r);
-      if (transposed) {
+    auto store_state = [&](float* to, int64_t n, float mul) {
+      to += n * (A * B) + c0 * B + r;
 #pragma unroll
-        for (int j = 0; j < NC; ++j) to[j] = S[j] * mul;
-      } else {
-#pragma unroll
-        for (int j = 0; j < NC; ++j) to[j * B] = S[j] * mul;
-      }
+      for (int j = 0; j < NC; ++j) to[j * B] = S[j] * mul;
     };
     // S <- S * x + D * y
     auto take = [&](uint32_t d, float x, float y) {
@@ -664,7 +659,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
         __syncwarp();
         if (lane == 0) mbar_arrive(&d_read[t & 1]);
       }
-      if (!failed && count > 0 && holds) store_state(args.slots, blockIdx.x, args.slots_t, 1.f);
+      if (!failed && count > 0 && holds) store_state(args.slots, blockIdx.x, 1.f);
     } else {
       float decay = 1.f;        // of the tile before
       bool last = false;        // it was its sequence's last
@@ -676,7 +671,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
           tc_fence_after();
           if (holds) {
             take(0, decay, 1.f);
-            if (last && a.s_out != nullptr) store_state(a.s_out, state, a.s_out_t, a.out_mul * (reverse ? exp2f(g2) : 1.f));
+            if (last && a.s_out != nullptr) store_state(a.s_out, state, a.out_mul * (reverse ? exp2f(g2) : 1.f));
           }
           advance();
         }
@@ -736,8 +731,8 @@ __global__ void __launch_bounds__(kLinearThreads, 1) linear_chunks_kernel(const 
 // What every CTA's first sequence begins with: along a sequence, slots[i] <- slots[i] + mult_i * (state before CTA i's part).  A block
 // takes 512 elements of the sequence whose first share is CTA blockIdx.y's; shares are fetched eight at a time.
 constexpr int kLinearMaxCtas = 256;
-__global__ void __launch_bounds__(128) linear_carry_kernel(const float* __restrict__ s_in, int32_t s_in_t, float in_mul, float* __restrict__ slots,
-                                                           const LinearPiece* __restrict__ pieces, int32_t ctas, int32_t A, int32_t B) {
+__global__ void __launch_bounds__(128) linear_carry_kernel(const float* __restrict__ s_in, float in_mul, float* __restrict__ slots,
+                                                           const LinearPiece* __restrict__ pieces, int32_t ctas, int32_t size) {
   __shared__ LinearPiece info[kLinearMaxCtas];
   griddep_launch_dependents();
   griddep_wait();
@@ -745,16 +740,10 @@ __global__ void __launch_bounds__(128) linear_carry_kernel(const float* __restri
   if (!pieces[i0].goes_on || pieces[i0].inherits) return;
   for (int i = i0 + threadIdx.x; i < ctas; i += 128) info[i] = pieces[i];
   __syncthreads();
-  const int e = (blockIdx.x * 128 + threadIdx.x) * 4, size = A * B;    // elements (e / B, e % B) and on
+  const int e = (blockIdx.x * 128 + threadIdx.x) * 4;    // of a state's `size` elements
   float4 carry = make_float4(0.f, 0.f, 0.f, 0.f);
   if (s_in != nullptr) {
-    const float* from = s_in + static_cast<int64_t>(info[i0].state) * size;
-    if (!s_in_t) {
-      carry = *reinterpret_cast<const float4*>(from + e);
-    } else {
-      const float* p = from + (e % B) * A + e / B;
-      carry = make_float4(p[0], p[A], p[2 * A], p[3 * A]);
-    }
+    carry = *reinterpret_cast<const float4*>(s_in + static_cast<int64_t>(info[i0].state) * size + e);
     carry.x *= in_mul; carry.y *= in_mul; carry.z *= in_mul; carry.w *= in_mul;
   }
   int last = i0;   // the sequence's last share

@@ -24,7 +24,7 @@ struct LinearArgs {
   int32_t sequences, L, heads;         // L: tokens of an entry
   const float* s_in;                   // [sequences][heads] states, or nullptr: zeros
   float* s_out;                        // or nullptr
-  int32_t s_in_t, s_out_t;             // stored [B][A] instead of [A][B]
+  int32_t s_in_t;                      // stored [B][A] instead of [A][B]
   float scale, in_mul, out_mul;        // of the outputs; of a state that is read / written
   int32_t reverse;
 };
@@ -146,13 +146,7 @@ __global__ void __launch_bounds__(256) linear_steps_kernel(const __grid_constant
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int row = rg + 32 * i;
-    if (!a.s_out_t) {
-      *reinterpret_cast<float4*>(a.s_out + at + row * B + c0 + cl * 4) =
-          make_float4(S[i][0] * mul, S[i][1] * mul, S[i][2] * mul, S[i][3] * mul);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) a.s_out[at + (c0 + cl * 4 + e) * A + row] = S[i][e] * mul;
-    }
+    *reinterpret_cast<float4*>(a.s_out + at + row * B + c0 + cl * 4) = make_float4(S[i][0] * mul, S[i][1] * mul, S[i][2] * mul, S[i][3] * mul);
   }
 }
 
