@@ -17,7 +17,8 @@
 // with three pieces 4.0 (48 products of 68 clocks).  What is left is the chain from D through the state's copy, X S and P Z to the next G.
 // Long sequences of few heads: `per` tiles a CTA may begin within a sequence.  linear_chunks_kernel<.., PIECE, ..> first leaves every CTA's
 // share of the state of the sequence that goes on behind it, linear_carry_kernel adds the shares up in order.  The shares are taken
-// from the last tile to the first, so that the tiles the CTA begins with afterwards have been read last and are still in L2, and only as far as fp32 has room for their decay.
+// from the last tile to the first, and only as far as fp32 has room for their decay.  (So the tiles that a CTA begins with afterwards have
+// been read last; what that leaves in L2 has not been measured by itself.)
 #pragma once
 #include "linear_steps.cuh"
 #include "umma_gemm.cuh"
@@ -26,8 +27,8 @@ namespace lact {
 
 constexpr int kLinearThreads = 896;   // a warpgroup for loads and products, four for the rows, two for the state
 constexpr int kLinearRowThreads = 512, kLinearRowWarps = 16;
-// registers per thread of each; together what the launch has.  (Nothing may spill: the little L1 beside 227 KB of shared memory misses,
-// and a tile's bookkeeping alone then waited 1700 clocks for it.)
+// registers per thread of each; together what the launch has.  (The little L1 beside 227 KB of shared memory misses: with a tile's
+// bookkeeping on the stack it alone waited 1700 clocks.  Two of 128 features spill 10 bytes a thread, their shares' pass 68; the others none.)
 constexpr int kLinearIssueRegs = 40, kLinearRowRegs = 56, kLinearStateRegs = 120, kLinearLaunchRegs = 72;
 static_assert(kLinearIssueRegs + 4 * kLinearRowRegs + 2 * kLinearStateRegs <= 7 * kLinearLaunchRegs, "the shares of the registers");
 

@@ -182,7 +182,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     `S_t = exp(log_decay[h]) S_(t-1) + k_t v_t^T`, `o_t = scale q_t^T S_t` with S [dk, dv] in float32.
 
     q [b, l, h, dk], k [b, l, h_kv, dk], v [b, l, h_kv, dv] bf16 (dk, dv 64 or 128; h a multiple of h_kv: consecutive heads share a
-    key and value head; views of a fused projection are read where they lie), log_decay [h] float32, not above 0 (-inf: a head
+    key and value head; views of a fused projection are read where they lie, whatever strides axes of one entry have), log_decay [h] float32, not above 0 (-inf: a head
     without memory); it gets no gradient.  `scale`: dk ** -0.5 by default.  initial_state [b, h, dk, dv] float32 or None (zeros).
     `cu_seqlens` (int32 [n + 1] on the device, b must be 1): n sequences packed back to back, empty ones allowed, each with its
     own state ([n, h, dk, dv]); tokens outside of them have zero outputs (bounds that fall or pass the end stay inside the arrays, with
@@ -212,7 +212,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
                           scale: Optional[float] = None, new_state: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One new token of every sequence (generation): `linear_attention` in its recurrent form.  q [b, h, dk], k [b, h_kv, dk],
     v [b, h_kv, dv] bf16, state [b, h, dk, dv] float32, contiguous: read, and written in place, or to `new_state` (an array apart
-    from it).  Returns o [b, h, dv] bf16.  No backward: a call with gradients raises."""
+    from it).  Returns o [b, h, dv] bf16.  No backward: a call with gradients raises.  To autograd the array that is written has
+    changed in place: a backward that has saved it (as `linear_attention` saves its `initial_state`) raises."""
     h, dk, dv = _linear_heads("linear_attention_step", q, k, v, log_decay, 3)
     shape, at = (q.shape[0], h, dk, dv), q.get_device()
     if new_state is None:
