@@ -101,7 +101,8 @@ typedef struct lact_scan_io {
  * lact_swiglu_ffn_hidden_bytes, lact_swa_fwd_cache_bytes and lact_swa_fwd_cache; larger workspaces (asked for as before):
  * programs of many short steps by up to 128 MB for weights and 58 MB for hidden activations, fp32 programs by their
  * operands in bf16 pieces (6 bytes a value: an update and apply of D = H take 30 H bytes per token, 12 H before).  1003: new
- * entries lact_linear_attention_* and lact_group_norm_*.  No counterpart in the reference. */
+ * entries lact_linear_attention_* and lact_group_norm_*.  1004: new entries lact_rotary_axes, lact_paged_cache_* and
+ * lact_paged_attention_*, device status 102.  No counterpart in the reference. */
 int lact_version(void);
 
 /* Human-readable text for a return code.  No counterpart in the reference. */
@@ -387,6 +388,62 @@ int lact_group_norm_fwd(const lact_group_norm_config *cfg, const void *x, const 
 int lact_group_norm_bwd(const lact_group_norm_config *cfg, const void *x, const float *weight, const float *bias, const float *stats,
                         const void *dy, void *dx, float *dweight, float *dbias, void *workspace,
                         size_t workspace_bytes, void *stream);
+
+/* Rotary positions with several axes: q [batch, tokens, q_heads, head_dim], k likewise with k_heads (0: none) -> q_out, k_out of
+ * the same shape, contiguous.  Pair j (of sections[0] + sections[1] + .. = P pairs, at most head_dim / 2) belongs to the axis whose
+ * section holds it and turns by t = position[axis] * frequencies[j]: (x, y) -> (x cos t - y sin t, y cos t + x sin t); pairs are
+ * (j, j + P), or neighbours (2j, 2j + 1) with `interleaved`; features from 2P on are copied.  `backwards` turns by -t (the
+ * gradient).  frequencies: fp64 [P] on the device; positions: whole numbers of position_bytes (4 or 8) [batch, tokens, axes], a
+ * batch stride of 0 for shared ones.  Strides in elements, features adjacent; head_dim even, at most 512; accesses are as wide
+ * as bases and strides allow, up to 16 bytes.  q_out, k_out may not overlap q, k.  Replaces the rotation of the attention's q and k
+ * (layer_lact_swiglu.py:324-343; the video layer's three axes, ar_lact_swa_repeat.py). */
+#define LACT_ROTARY_AXES 8
+typedef struct lact_rotary_config {
+  int64_t batch, tokens, q_heads, k_heads, head_dim;
+  int64_t q_bs, q_ts, q_hs, k_bs, k_ts, k_hs; /* batch, token, head strides */
+  int64_t position_bs, position_ts, position_as;
+  int64_t sections[LACT_ROTARY_AXES];
+  int32_t axes, position_bytes, dtype, interleaved, backwards;
+} lact_rotary_config;
+int lact_rotary_axes(const lact_rotary_config *cfg, const void *q, const void *k, const void *positions, const double *frequencies,
+                     void *q_out, void *k_out, void *stream);
+
+/* A paged cache of keys and values: k, v [pages, kv_heads, page_size, head_dim], 32-byte aligned, pages contiguous in themselves, page
+ * strides in elements (multiples of 32 bytes).  bf16 without exponents; with k_exponent, v_exponent ([pages, kv_heads, page_size]
+ * bytes) e4m3 values that stand for themselves times 2^(byte - 127), 255: NaN.  head_dim 64 or 128; page_size 16, 32, 64, 128 or 256.
+ * Position p of sequence i lies in page page_table[i * table_stride + p / page_size], row p % page_size, for p below lengths[i];
+ * table_cols * page_size at most 2^30.  Entries of the table past a sequence's length are not looked at; a page or a position that
+ * the cache does not have is left out, and device status 102 goes to the host's word (lact_status_host_word).  No counterpart in the
+ * reference, whose cache is left to the attention library's caller (layer_lact_swiglu.py:328-343). */
+typedef struct lact_paged_cache {
+  void *k, *v;
+  void *k_exponent, *v_exponent;
+  int64_t pages, kv_heads, page_size, head_dim;
+  int64_t k_page_stride, v_page_stride, ke_page_stride, ve_page_stride;
+  const int32_t *page_table;
+  int64_t table_cols, table_stride;
+  const int32_t *lengths;
+  int64_t sequences;
+} lact_paged_cache;
+/* Writes k, v [batch, tokens, kv_heads, head_dim] bf16 (16-byte aligned, features adjacent, strides in elements, multiples of 8) as the
+ * last rows of their sequences: row j of n has position lengths[i] - n + j and is not written where that is negative.
+ * cu_seqlens: NULL (batch = sequences), or int32 [sequences + 1] on the device for a batch of one: sequences back to back; rows
+ * outside of them are not written.  Two rows of a call must not have the same place. */
+int lact_paged_cache_write(const lact_paged_cache *cache, const void *k, int64_t k_ts, int64_t k_bs, int64_t k_hs, const void *v,
+                           int64_t v_ts, int64_t v_bs, int64_t v_hs, int64_t batch, int64_t tokens, const int32_t *cu_seqlens,
+                           void *stream);
+/* The same rows back: out [2, batch, tokens, kv_heads, head_dim] bf16 (keys, then values), 16-byte aligned; rows without a position
+ * are zeros. */
+int lact_paged_cache_read(const lact_paged_cache *cache, void *out, int64_t batch, int64_t tokens, const int32_t *cu_seqlens,
+                          void *stream);
+/* Attention of one token of every sequence: q [sequences, heads, head_dim] bf16 (16-byte aligned, strides multiples of 8), kv_heads divides
+ * heads (consecutive heads share) -> o [sequences, heads, head_dim] bf16, contiguous: softmax(softmax_scale q K^T) V over positions
+ * max(0, length - window) .. length - 1 (window 0: all); zeros where the length is not above 0.  counters, workspace: sizes from
+ * lact_paged_attention_step_bytes (uint32 words, zero before the first call and zero again after every one; bytes, 16-byte
+ * aligned; both may be 0); calls that share them must follow one another. */
+int lact_paged_attention_step_bytes(const lact_paged_cache *cache, int64_t heads, int64_t window, size_t *bytes, int64_t *counters);
+int lact_paged_attention_step(const lact_paged_cache *cache, const void *q, int64_t q_bs, int64_t q_hs, int64_t heads, int64_t window,
+                              float softmax_scale, void *o, void *counters, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Backward of lact_qkv_prologue / lact_qkv_prologue_rope on the saved projections (same strides): dq, dk, dv are the
  * gradients of the head-major outputs ([(b n_heads), s, d] bf16, NULL = none), dxq, dxk, dxv the gradients of the

@@ -158,6 +158,27 @@ def _(x, weight, bias, stats, dy, groups, eps, silu):
     return [x.new_empty(x.shape)] + [x.new_empty((x.shape[-1],), dtype=F32) for _ in range(2)]
 
 
+@_fake("rotary_axes")
+def _(q, k, positions, frequencies, sections, interleaved, backwards=False):
+    return [t.new_empty(t.shape) for t in (q, k) if t is not None]
+
+
+@_fake("paged_cache_write")
+def _(k_cache, v_cache, k_exponent, v_exponent, k, v, page_table, lengths, cu_seqlens):
+    return None
+
+
+@_fake("paged_cache_read")
+def _(k_cache, v_cache, k_exponent, v_exponent, page_table, lengths, tokens, cu_seqlens):
+    batch = 1 if cu_seqlens is not None else lengths.shape[0]
+    return k_cache.new_empty((2 * batch, tokens, k_cache.shape[1], k_cache.shape[3]), dtype=BF16)
+
+
+@_fake("paged_attention_step")
+def _(q, k_cache, v_cache, k_exponent, v_exponent, page_table, lengths, window, softmax_scale):
+    return q.new_empty(q.shape)
+
+
 @_fake("seq_start")
 def _(cu_seqlens, n_tokens):
     return cu_seqlens.new_empty((n_tokens,), dtype=torch.int32)

@@ -26,6 +26,8 @@
 #include "swa_pairs.cuh"
 #include "linear_chunks.cuh"
 #include "group_norm.cuh"
+#include "rotary.cuh"
+#include "paged_attention.cuh"
 
 namespace lact {
 namespace {
@@ -2347,6 +2349,130 @@ int norm_args(const lact_group_norm_config* c, const NormPlan& p, const void* x,
   return LACT_OK;
 }
 
+// ------------------------------------------------------------------------------------------ rotary positions
+template <class T, int V>
+int launch_rotary(RotaryArgs a, bool halves, cudaStream_t st) {
+  // as many thread groups a token as give four blocks a SM, for each of which it has a head; the angles of a token are worked out once
+  const int64_t groups = kRotaryThreads / (a.d / (2 * V)), heads = a.heads[0] + a.heads[1];
+  int64_t share = 1;
+  while (2 * share <= std::min(groups, heads) && a.tokens * share < groups * 4 * sm_count()) share *= 2;
+  a.share = static_cast<int32_t>(share);
+  a.per_block = static_cast<int32_t>(groups / share);
+  const int64_t grid = (a.tokens + a.per_block - 1) / a.per_block;
+  if (grid > 0x7FFFFFFF) return LACT_ERR_SHAPE;
+  const size_t smem = static_cast<size_t>(a.per_block) * a.P * sizeof(float2);
+  KernelScope scope(kClsOther, st);
+  if (halves) LACT_CUDA(launch_pdl(rotary_kernel<T, V, true>, dim3(static_cast<unsigned>(grid)), dim3(kRotaryThreads), smem, st, a));
+  else LACT_CUDA(launch_pdl(rotary_kernel<T, V, false>, dim3(static_cast<unsigned>(grid)), dim3(kRotaryThreads), smem, st, a));
+  return LACT_OK;
+}
+int rotary_check(const lact_rotary_config* c) {
+  if (c == nullptr) return LACT_ERR_NULL;
+  if (c->dtype != LACT_F32 && c->dtype != LACT_BF16) return LACT_ERR_DTYPE;
+  if (c->batch < 1 || c->tokens < 1 || c->q_heads < 1 || c->k_heads < 0 || c->head_dim < 2 || c->head_dim % 2 != 0 || c->head_dim > 512) return LACT_ERR_SHAPE;
+  if (c->q_heads > 65535 || c->k_heads > 65535 || c->tokens > (1ll << 30) || c->batch > (1ll << 30) || c->batch * c->tokens > (1ll << 36)) return LACT_ERR_SHAPE;
+  if (c->axes < 1 || c->axes > LACT_ROTARY_AXES) return LACT_ERR_SHAPE;
+  int64_t pairs = 0;
+  for (int i = 0; i < c->axes; ++i) {
+    if (c->sections[i] < 0 || c->sections[i] > c->head_dim) return LACT_ERR_SHAPE;
+    pairs += c->sections[i];
+  }
+  if (pairs < 1 || 2 * pairs > c->head_dim) return LACT_ERR_SHAPE;
+  if (c->position_bytes != 4 && c->position_bytes != 8) return LACT_ERR_DTYPE;
+  return LACT_OK;
+}
+
+// ------------------------------------------------------------------------------------------ paged cache
+int paged_check(const lact_paged_cache* c) {
+  if (c == nullptr) return LACT_ERR_NULL;
+  if (c->k == nullptr || c->v == nullptr || c->page_table == nullptr || c->lengths == nullptr) return LACT_ERR_NULL;
+  if ((c->k_exponent == nullptr) != (c->v_exponent == nullptr)) return LACT_ERR_CONFIG;
+  if (c->head_dim != 64 && c->head_dim != 128) return LACT_ERR_SHAPE;
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) != 0) return LACT_ERR_SHAPE;
+  if (c->pages < 1 || c->pages > 0x7FFFFFFF || c->kv_heads < 1 || c->kv_heads > 65535 || c->sequences < 1 || c->sequences > (1 << 24)) return LACT_ERR_SHAPE;
+  if (c->table_cols < 1 || c->table_cols * c->page_size > (1ll << 30)) return LACT_ERR_SHAPE;   // positions are counted in 31 bits
+  const int64_t size = c->k_exponent == nullptr ? 2 : 1, page = c->kv_heads * c->page_size * c->head_dim;
+  for (const void* p : {c->k, c->v})
+    if ((reinterpret_cast<uintptr_t>(p) & 31) != 0) return LACT_ERR_SHAPE;
+  for (int64_t ps : {c->k_page_stride, c->v_page_stride})
+    if (c->pages > 1 && (ps < page || ps * size % 32 != 0)) return LACT_ERR_SHAPE;
+  if (c->k_exponent != nullptr)
+    for (int64_t ps : {c->ke_page_stride, c->ve_page_stride})
+      if (c->pages > 1 && ps < c->kv_heads * c->page_size) return LACT_ERR_SHAPE;
+  return LACT_OK;
+}
+PagedCache paged_args(const lact_paged_cache* c) {
+  PagedCache a;
+  const int64_t size = c->k_exponent == nullptr ? 2 : 1;
+  a.k = static_cast<uint8_t*>(c->k); a.v = static_cast<uint8_t*>(c->v);
+  a.ke = static_cast<uint8_t*>(c->k_exponent); a.ve = static_cast<uint8_t*>(c->v_exponent);
+  a.k_ps = c->k_page_stride * size; a.v_ps = c->v_page_stride * size;
+  a.ke_ps = c->ke_page_stride; a.ve_ps = c->ve_page_stride;
+  a.pages = static_cast<int32_t>(c->pages); a.heads = static_cast<int32_t>(c->kv_heads);
+  a.shift = 0;
+  while ((1 << a.shift) < c->page_size) ++a.shift;
+  a.table = c->page_table; a.table_rs = c->table_stride; a.cols = static_cast<int32_t>(c->table_cols);
+  a.lengths = c->lengths; a.sequences = static_cast<int32_t>(c->sequences);
+  return a;
+}
+template <int D, bool E4>
+int launch_paged_rows(const PagedRows& a, bool write, int64_t grid, cudaStream_t st) {
+  KernelScope scope(kClsOther, st);
+  const dim3 blocks(static_cast<unsigned>(grid), 2);
+  if (write) LACT_CUDA(launch_pdl(paged_rows_kernel<D, E4, true>, blocks, dim3(kPagedThreads), 0, st, a));
+  else LACT_CUDA(launch_pdl(paged_rows_kernel<D, E4, false>, blocks, dim3(kPagedThreads), 0, st, a));
+  return LACT_OK;
+}
+int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t tokens, const int32_t* cu, bool write, cudaStream_t st) {
+  if (entries < 1 || tokens < 1 || tokens > (1ll << 30) || entries * tokens > (1ll << 36)) return LACT_ERR_SHAPE;
+  if (cu == nullptr ? entries != c->sequences : entries != 1) return LACT_ERR_CONFIG;
+  a.c = paged_args(c);
+  a.cu = cu;
+  a.tokens = entries * tokens;
+  a.L = static_cast<int32_t>(tokens);
+  // tokens of a block: four blocks a SM, and at most four turns of four rows a thread
+  const int64_t rows_at_once = kPagedThreads / (c->head_dim / 8) * kPagedAhead;
+  int64_t n = 1;
+  while (2 * n <= kPagedTokens && 2 * n * c->kv_heads <= 4 * rows_at_once && a.tokens >= 2 * n * 2 * sm_count()) n *= 2;
+  a.per_block = static_cast<int32_t>(n);
+  const int64_t grid = (a.tokens + n - 1) / n;
+  if (grid > 0x7FFFFFFF) return LACT_ERR_SHAPE;
+  const bool e4 = c->k_exponent != nullptr;
+  if (c->head_dim == 64) return e4 ? launch_paged_rows<64, true>(a, write, grid, st) : launch_paged_rows<64, false>(a, write, grid, st);
+  return e4 ? launch_paged_rows<128, true>(a, write, grid, st) : launch_paged_rows<128, false>(a, write, grid, st);
+}
+
+// How a call's tiles are dealt out.
+struct PagedStepPlan {
+  int nq, blocks, runs;
+  size_t bytes;
+};
+constexpr int kPagedWarps = 6, kPagedPerSm = 2;
+constexpr int kPagedLeast = 2;   // tiles of a run at least
+constexpr int kPagedWhole = 4;   // tiles of a unit up to which a CTA takes a unit
+int paged_step_plan(const lact_paged_cache* c, int64_t heads, int64_t window, PagedStepPlan* p) {
+  if (heads < 1 || heads > 65535 || heads % c->kv_heads != 0 || window < 0) return LACT_ERR_SHAPE;
+  const int64_t share = heads / c->kv_heads, tile = 16 * kPagedWarps;
+  p->nq = share > 8 ? 2 : 1;
+  p->blocks = ceil_div(share, 8 * p->nq);
+  const int64_t units = c->sequences * c->kv_heads * p->blocks, room = c->table_cols * c->page_size;
+  const int64_t most = (std::min(window > 0 ? window + 15 : room, room) + tile - 1) / tile;   // of a unit
+  if (units > 0x7FFFFFFF) return LACT_ERR_SHAPE;
+  p->runs = most <= kPagedWhole ? 0 : static_cast<int>(std::min<int64_t>(sm_count() * kPagedPerSm, (units * most + kPagedLeast - 1) / kPagedLeast));
+  p->bytes = static_cast<size_t>(p->runs) * 2 * 8 * p->nq * kPagedPieceRow(static_cast<int>(c->head_dim)) * 4;
+  return LACT_OK;
+}
+template <int D, bool E4, int NQ>
+int launch_paged_step(const PagedStepArgs& a, cudaStream_t st) {
+  auto kernel = paged_step_kernel<D, E4, NQ, kPagedWarps, kPagedPerSm>;
+  constexpr size_t smem = static_cast<size_t>(kPagedWarps) * 8 * NQ * kPagedPieceRow(D) * 4;
+  if (smem > 48 * 1024) LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  const int64_t grid = a.runs > 0 ? a.runs : static_cast<int64_t>(a.c.sequences) * a.c.heads * a.blocks;
+  KernelScope scope(kClsOther, st);
+  LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kPagedWarps * 32), smem, st, a));
+  return LACT_OK;
+}
+
 }  // namespace
 }  // namespace lact
 
@@ -2357,7 +2483,7 @@ using namespace lact;
 
 extern "C" {
 
-int lact_version(void) { return 1003; }
+int lact_version(void) { return 1004; }
 
 const char* lact_error_string(int code) {
   switch (code) {
@@ -2374,6 +2500,7 @@ const char* lact_error_string(int code) {
       return "problem needs more scratch than the library's built-in static buffer holds (16 MiB): "
              "use the workspace variant or a smaller B * N * H";
     case kStatusWaitTimeout: return "device: a bounded barrier wait timed out";
+    case kStatusBadPage: return "device: a page number or a length outside of the paged cache (left out)";
     default: return "unknown code";
   }
 }
@@ -3464,6 +3591,122 @@ int lact_swa_bwd(const void* q, const void* k, const void* v, const void* o, con
   a.o_bs = l * n_heads * d;
   const int64_t ctas = b * n_heads * q_tiles;
   return d == 64 ? launch_swa_bwd<64, 1>(a, ctas, st) : launch_swa_bwd<128, 1>(a, ctas, st);
+}
+
+int lact_rotary_axes(const lact_rotary_config* c, const void* q, const void* k, const void* positions, const double* frequencies, void* q_out,
+                     void* k_out, void* stream) {
+  LACT_TRY(rotary_check(c));
+  if (q == nullptr || q_out == nullptr || positions == nullptr || frequencies == nullptr || (c->k_heads > 0 && (k == nullptr || k_out == nullptr))) return LACT_ERR_NULL;
+  RotaryArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.x[0] = q; a.y[0] = q_out; a.heads[0] = static_cast<int32_t>(c->q_heads); a.bs[0] = c->q_bs; a.ts[0] = c->q_ts; a.hs[0] = c->q_hs;
+  a.x[1] = k; a.y[1] = k_out; a.heads[1] = static_cast<int32_t>(c->k_heads); a.bs[1] = c->k_bs; a.ts[1] = c->k_ts; a.hs[1] = c->k_hs;
+  a.pos = positions; a.pos_bs = c->position_bs; a.pos_ts = c->position_ts; a.pos_as = c->position_as;
+  a.pos_wide = c->position_bytes == 8; a.axes = c->axes;
+  for (int i = 0, end = 0; i < c->axes; ++i) a.ends[i] = end += static_cast<int>(c->sections[i]);
+  a.freq = frequencies;
+  a.tokens = c->batch * c->tokens; a.L = static_cast<int32_t>(c->tokens); a.d = static_cast<int32_t>(c->head_dim); a.P = a.ends[c->axes - 1];
+  a.sign = c->backwards ? -1.f : 1.f;
+  // whole accesses of up to 16 bytes: as many features as divide the pairs, half a head, the strides and the bases
+  const int size = c->dtype == LACT_F32 ? 4 : 2;
+  int v = 16 / size;
+  auto fits = [&](int n) {
+    if (a.P % n != 0 || a.d % (2 * n) != 0 || 256 / (a.d / (2 * n)) < 1) return false;
+    for (int i = 0; i < (c->k_heads > 0 ? 2 : 1); ++i) {
+      for (int64_t s : {c->batch > 1 ? a.bs[i] : 0, c->tokens > 1 ? a.ts[i] : 0, a.heads[i] > 1 ? a.hs[i] : 0})
+        if (s % n != 0) return false;
+      if (reinterpret_cast<uintptr_t>(a.x[i]) % (n * size) != 0 || reinterpret_cast<uintptr_t>(a.y[i]) % (n * size) != 0) return false;
+    }
+    return true;
+  };
+  while (v > 1 && !fits(v)) v /= 2;
+  if (!fits(v)) return LACT_ERR_SHAPE;
+  LACT_TRY(check_device());
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool halves = c->interleaved == 0;
+  if (c->dtype == LACT_F32) {
+    switch (v) {
+      case 4: return launch_rotary<float, 4>(a, halves, st);
+      case 2: return launch_rotary<float, 2>(a, halves, st);
+      default: return launch_rotary<float, 1>(a, halves, st);
+    }
+  }
+  switch (v) {
+    case 8: return launch_rotary<bf16, 8>(a, halves, st);
+    case 4: return launch_rotary<bf16, 4>(a, halves, st);
+    case 2: return launch_rotary<bf16, 2>(a, halves, st);
+    default: return launch_rotary<bf16, 1>(a, halves, st);
+  }
+}
+
+int lact_paged_cache_write(const lact_paged_cache* c, const void* k, int64_t k_ts, int64_t k_bs, int64_t k_hs, const void* v, int64_t v_ts,
+                           int64_t v_bs, int64_t v_hs, int64_t batch, int64_t tokens, const int32_t* cu_seqlens, void* stream) {
+  LACT_TRY(paged_check(c));
+  if (k == nullptr || v == nullptr) return LACT_ERR_NULL;
+  for (const void* p : {k, v})
+    if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return LACT_ERR_SHAPE;
+  for (int64_t s : {k_ts, k_bs, k_hs, v_ts, v_bs, v_hs})
+    if (s % 8 != 0) return LACT_ERR_SHAPE;
+  PagedRows a;
+  std::memset(&a, 0, sizeof(a));
+  a.xk = static_cast<const bf16*>(k); a.k_ts = k_ts; a.k_bs = k_bs; a.k_hs = k_hs;
+  a.xv = static_cast<const bf16*>(v); a.v_ts = v_ts; a.v_bs = v_bs; a.v_hs = v_hs;
+  return paged_rows(c, a, batch, tokens, cu_seqlens, true, static_cast<cudaStream_t>(stream));
+}
+
+int lact_paged_cache_read(const lact_paged_cache* c, void* out, int64_t batch, int64_t tokens, const int32_t* cu_seqlens, void* stream) {
+  LACT_TRY(paged_check(c));
+  if (out == nullptr) return LACT_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0) return LACT_ERR_SHAPE;
+  PagedRows a;
+  std::memset(&a, 0, sizeof(a));
+  a.out = static_cast<bf16*>(out);
+  return paged_rows(c, a, batch, tokens, cu_seqlens, false, static_cast<cudaStream_t>(stream));
+}
+
+int lact_paged_attention_step_bytes(const lact_paged_cache* c, int64_t heads, int64_t window, size_t* bytes_out, int64_t* counters_out) {
+  if (bytes_out == nullptr || counters_out == nullptr) return LACT_ERR_NULL;
+  LACT_TRY(paged_check(c));
+  PagedStepPlan p;
+  LACT_TRY(paged_step_plan(c, heads, window, &p));
+  *bytes_out = p.bytes;
+  *counters_out = p.runs;
+  return LACT_OK;
+}
+
+int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t q_bs, int64_t q_hs, int64_t heads, int64_t window,
+                              float softmax_scale, void* o, void* counters, void* workspace, size_t workspace_bytes, void* stream) {
+  LACT_TRY(paged_check(c));
+  if (q == nullptr || o == nullptr) return LACT_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || (reinterpret_cast<uintptr_t>(o) & 1) != 0 || q_bs % 8 != 0 || q_hs % 8 != 0) return LACT_ERR_SHAPE;
+  if (!(std::fabs(softmax_scale) <= 1e18f)) return LACT_ERR_CONFIG;
+  PagedStepPlan p;
+  LACT_TRY(paged_step_plan(c, heads, window, &p));
+  if (p.runs > 0 && (counters == nullptr || workspace == nullptr || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) return LACT_ERR_WORKSPACE;
+  LACT_TRY(check_device());
+  PagedStepArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.c = paged_args(c);
+  a.q = static_cast<const bf16*>(q); a.q_bs = q_bs; a.q_hs = q_hs;
+  a.o = static_cast<bf16*>(o);
+  a.heads = static_cast<int32_t>(heads); a.share = static_cast<int32_t>(heads / c->kv_heads); a.blocks = p.blocks;
+  a.window = static_cast<int32_t>(std::min<int64_t>(window, 0x7FFFFFFF));
+  a.scale = softmax_scale * 1.4426950408889634f;
+  a.runs = p.runs; a.least = kPagedLeast;
+  a.counters = static_cast<uint32_t*>(counters);
+  a.pieces = static_cast<float*>(workspace);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int form = (c->head_dim == 128 ? 4 : 0) + (c->k_exponent != nullptr ? 2 : 0) + p.nq - 1;
+  switch (form) {
+    case 0: return launch_paged_step<64, false, 1>(a, st);
+    case 1: return launch_paged_step<64, false, 2>(a, st);
+    case 2: return launch_paged_step<64, true, 1>(a, st);
+    case 3: return launch_paged_step<64, true, 2>(a, st);
+    case 4: return launch_paged_step<128, false, 1>(a, st);
+    case 5: return launch_paged_step<128, false, 2>(a, st);
+    case 6: return launch_paged_step<128, true, 1>(a, st);
+    default: return launch_paged_step<128, true, 2>(a, st);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ linear attention

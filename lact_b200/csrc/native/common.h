@@ -8,8 +8,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <initializer_list>
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "../../../include/lact_b200.h"
@@ -74,6 +76,9 @@ struct StatusWord {
 };
 StatusWord status_word(const Tensor& like);
 void poll_status(const Tensor& like);
+// `words` 32-bit counters that are zero, and that the call leaves at zero: shared by the calls on (device of `like`, current stream), of a
+// call that is being captured its own, which the graph clears at every replay.
+Tensor zeroed_counters(const Tensor& like, int64_t words);
 // End of a backward: with LACT_B200_SYNC_CHECK=1 (and no capture) waits for the stream and reports what it has left (forwards
 // are waited for in Python).
 void settle(const Tensor& like);

@@ -1,0 +1,205 @@
+// A paged cache of keys and values: pages [page][kv head][row][d] of bf16, or of e4m3 with one byte a row of a head for a power of two.
+// Sequence i has lengths[i] tokens; token p lies in page table[i][p / page_size], row p % page_size.  The calls below deal with the
+// last n_i tokens of every sequence (the rows of a batch entry, or of a packed sequence): row j has position lengths[i] - n_i + j, and
+// none where that is negative (rows that pad a batch in front).
+//
+// 8 bits: x = e4m3 * 2^(byte - 127), the smallest power of two with max |x| over the row at most 448 times it (between 2^-126
+// and 2^119: values above 1.75 x 2^127 would come back as infinities, and are cut to that).
+// Powers of two make scaling exact, so that e4m3 alone rounds (2^-4 of a value at most, 2^-10 of the power for the smallest); a scale
+// of max / 448 would gain at most one bit of the range below 2^-15 of the row's largest value, and round twice.  Byte 255 is NaN: a
+// row with a NaN or an infinity is NaN throughout.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "group_norm.cuh"
+
+namespace lact {
+
+struct PagedCache {
+  uint8_t *k, *v;                  // pages
+  uint8_t *ke, *ve;                // exponents [page][kv head][row], or nullptr: bf16
+  int64_t k_ps, v_ps;              // bytes from page to page
+  int64_t ke_ps, ve_ps;
+  int32_t pages, heads, shift;     // page_size = 1 << shift
+  const int32_t* table;            // [sequences][cols]
+  int64_t table_rs;
+  int32_t cols;
+  const int32_t* lengths;
+  int32_t sequences;
+};
+
+// A page number or a length that the cache does not have is left out, and told to the host (which raises on its next call).
+__device__ __forceinline__ void report_bad_page() {
+  if (g_host_status != nullptr) {
+    *reinterpret_cast<volatile int32_t*>(g_host_status) = kStatusBadPage;
+    __threadfence_system();
+  }
+}
+
+// 2^(byte - 127)
+__device__ __forceinline__ float exponent_value(uint32_t byte) {
+  return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
+}
+// The byte of a row whose largest |bf16| has these 15 bits
+__device__ __forceinline__ uint32_t exponent_byte(uint32_t top) {
+  const int e = static_cast<int>(top >> 7);
+  if (e == 255) return 255;
+  return static_cast<uint32_t>(min(max(e - 8 + ((top & 0x7F) > 0x60 ? 1 : 0), 1), 246));
+}
+// Two e4m3 values (low byte first) as two halves, exactly
+__device__ __forceinline__ uint32_t halves_of_e4m3(uint32_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two)));
+  return r;
+}
+// Two values in e4m3 (low byte: the first)
+__device__ __forceinline__ uint32_t e4m3_of(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+struct PagedRows {
+  PagedCache c;
+  const bf16 *xk, *xv;             // written: [entry][token][head][D], features adjacent, other strides in elements
+  int64_t k_bs, k_ts, k_hs, v_bs, v_ts, v_hs;
+  bf16* out;                       // read: [2][entries][tokens][heads][D]
+  const int32_t* cu;               // packed: [sequences + 1] bounds within the one entry
+  int64_t tokens;                  // of all entries
+  int32_t L, per_block;            // of an entry; of a block
+};
+
+// Where row `t` of the batch lies: its page (-1: nowhere) and row.
+__device__ __forceinline__ int2 paged_place(const PagedRows& a, int64_t t) {
+  int64_t seq, pos;
+  if (a.cu == nullptr) {
+    seq = t / a.L;
+    pos = static_cast<int64_t>(a.c.lengths[seq]) - a.L + (t - seq * a.L);
+  } else {
+    int lo = 0, hi = a.c.sequences;   // the last sequence that begins at or before t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    seq = lo;
+    if (a.cu[seq] > t || t >= a.cu[seq + 1]) return make_int2(-1, 0);   // outside of the sequences
+    pos = static_cast<int64_t>(a.c.lengths[seq]) - (a.cu[seq + 1] - t);
+  }
+  if (pos < 0) return make_int2(-1, 0);
+  if (pos >> a.c.shift >= a.c.cols) {
+    report_bad_page();
+    return make_int2(-1, 0);
+  }
+  const int page = a.c.table[seq * a.c.table_rs + (pos >> a.c.shift)];
+  if (page < 0 || page >= a.c.pages) {
+    report_bad_page();
+    return make_int2(-1, 0);
+  }
+  return make_int2(page, static_cast<int>(pos & ((1 << a.c.shift) - 1)));
+}
+
+// Both directions are bound by memory.  A block finds the places of its tokens once; D / 8 threads hold a row of a head, 8 values each;
+// blockIdx.y says keys or values.  Four rows of a thread are fetched together.
+constexpr int kPagedThreads = 256, kPagedTokens = 64, kPagedAhead = 4;
+template <int D, bool E4, bool WRITE>
+__global__ void __launch_bounds__(kPagedThreads) paged_rows_kernel(const __grid_constant__ PagedRows a) {
+  constexpr int LANES = D / 8, ROWS = kPagedThreads / LANES, N = kPagedAhead;
+  __shared__ int2 place[kPagedTokens];
+  griddep_launch_dependents();
+  griddep_wait();
+  const bool values = blockIdx.y != 0;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
+  const int here = static_cast<int>(min(static_cast<int64_t>(a.per_block), a.tokens - t0));
+  for (int i = threadIdx.x; i < here; i += kPagedThreads) place[i] = paged_place(a, t0 + i);
+  __syncthreads();
+  const int lane = threadIdx.x % LANES, rows = here * a.c.heads;
+  uint8_t* const pages = values ? a.c.v : a.c.k;
+  uint8_t* const exps = values ? a.c.ve : a.c.ke;
+  const int64_t ps = values ? a.c.v_ps : a.c.k_ps, eps = values ? a.c.ve_ps : a.c.ke_ps;
+  const bf16* const x = values ? a.xv : a.xk;
+  const int64_t bs = values ? a.v_bs : a.k_bs, ts = values ? a.v_ts : a.k_ts, hs = values ? a.v_hs : a.k_hs;
+  bf16* const out = a.out + (values ? a.tokens * a.c.heads * D : 0);
+  constexpr int BYTES = E4 ? 8 : 16;   // of the cache, a thread
+  // (every thread of a warp takes part in every turn: rows that are not there have no page)
+  for (int r0 = threadIdx.x / LANES; r0 - static_cast<int>(threadIdx.x / LANES) < rows; r0 += N * ROWS) {
+    uint4 raw[N];
+    [[maybe_unused]] uint32_t byte[N];
+    int2 at[N];
+    int64_t to[N];
+    int head[N], tok[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = r0 + i * ROWS;
+      tok[i] = r / a.c.heads;
+      head[i] = r - tok[i] * a.c.heads;
+      at[i] = r < rows ? place[tok[i]] : make_int2(-1, 0);
+      to[i] = (static_cast<int64_t>(head[i]) << a.c.shift) + at[i].y;   // row within the page
+      raw[i] = make_uint4(0, 0, 0, 0);
+      byte[i] = 127;
+      if (at[i].x < 0) continue;
+      if constexpr (WRITE) {
+        const int64_t t = t0 + tok[i], b = t / a.L;
+        raw[i] = *reinterpret_cast<const uint4*>(x + b * bs + (t - b * a.L) * ts + head[i] * hs + lane * 8);
+      } else {
+        const uint8_t* from = pages + at[i].x * ps + (to[i] * LANES + lane) * BYTES;
+        if constexpr (E4) {
+          const uint2 two = *reinterpret_cast<const uint2*>(from);
+          raw[i].x = two.x;
+          raw[i].y = two.y;
+          byte[i] = exps[at[i].x * eps + to[i]];
+        } else {
+          raw[i] = *reinterpret_cast<const uint4*>(from);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (WRITE) {
+        if constexpr (E4) {
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = __vmaxu2(top, w[e] & 0x7FFF7FFFu);
+          top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+          if (at[i].x < 0) continue;
+          const uint32_t b = exponent_byte(top);
+          const float by = __uint_as_float((254u - min(b, 253u)) << 23);   // 2^(127 - byte)
+          uint32_t q[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
+          if (b != 255) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t lo = w[2 * e], hi = w[2 * e + 1];
+              q[e] = e4m3_of(__uint_as_float(lo << 16) * by, __uint_as_float(lo & 0xFFFF0000u) * by) |
+                     e4m3_of(__uint_as_float(hi << 16) * by, __uint_as_float(hi & 0xFFFF0000u) * by) << 16;
+            }
+          }
+          *reinterpret_cast<uint2*>(pages + at[i].x * ps + (to[i] * LANES + lane) * BYTES) = make_uint2(q[0], q[1]);
+          if (lane == 0) exps[at[i].x * eps + to[i]] = static_cast<uint8_t>(b);
+        } else {
+          if (at[i].x < 0) continue;
+          *reinterpret_cast<uint4*>(pages + at[i].x * ps + (to[i] * LANES + lane) * BYTES) = raw[i];
+        }
+      } else {
+        if (r0 + i * ROWS >= rows) continue;
+        if constexpr (E4) {
+          const float by = exponent_value(byte[i]);
+          const uint32_t w[2] = {raw[i].x, raw[i].y};
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t two = halves_of_e4m3(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+            o[e] = pack_bf16x2(f.x * by, f.y * by);
+          }
+          raw[i] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        *reinterpret_cast<uint4*>(out + ((t0 + tok[i]) * a.c.heads + head[i]) * D + lane * 8) = raw[i];
+      }
+    }
+  }
+}
+
+}  // namespace lact

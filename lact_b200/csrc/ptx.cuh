@@ -12,6 +12,7 @@ namespace lact {
 enum : int32_t {
   kStatusOk = 0,
   kStatusWaitTimeout = 101,  // a bounded mbarrier wait ran out
+  kStatusBadPage = 102,      // a paged cache does not have a page or a position that a call named (left out)
 };
 
 // A failure is recorded twice: in the call's device status word (later kernels of the call look at it and stand aside)

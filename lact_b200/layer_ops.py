@@ -13,11 +13,15 @@ Attention half of the hybrid layers (tcgen05 kernels, forward and backward, head
 
 Linear attention with a decay per head (`linear_attention` for prompts and training, `linear_attention_step` for single tokens): the
 recurrence with a linear memory, beside the fast weights.  `group_norm`: channels last, with an activation; with one spot a sample
-the norm of every head of every token behind such a mixer.  Neither has a counterpart in the reference."""
+the norm of every head of every token behind such a mixer.  Neither has a counterpart in the reference.
+
+Generation: `rotary_axes` (rotary positions of the attention's q and k, one axis or several; also for training), `PagedCache` with
+`paged_cache_write` / `paged_cache_read` (keys and values in pages, bf16 or 8 bits) and `paged_attention_step` (one new token of every
+sequence over its pages, with the layer's window)."""
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -226,6 +230,86 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
                                     new_state.requires_grad):
         raise NotImplementedError("linear_attention_step has no backward: use linear_attention")
     return L.call(_op("linear_attention_step"), q, k, v, log_decay, _linear_scale(scale, dk), state, new_state)
+
+
+# ------------------------------------------------------------------------------------------ rotary positions
+def rotary_frequencies(sections: Sequence[int], base: float = 10000.0, shared: bool = False, device=None) -> torch.Tensor:
+    """Frequencies of `rotary_axes`, float64 [sum(sections)]: every axis its own `base ** (-j / n)`, j < n pairs of its section (the video
+    layer's three axes; with one axis of half a head the usual table), or with `shared` one table over all pairs."""
+    sections = [sum(sections)] if shared else sections
+    return torch.cat([base ** (-torch.arange(n, dtype=torch.float64, device=device) / max(n, 1)) for n in sections])
+
+
+def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor, sections: Sequence[int],
+                interleaved: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotary positions with several axes (text: one; images: rows and columns; video: time, height, width) of the attention's q
+    [b, l, h, d] and k [b, l, h_kv, d] (or None), or of new tokens [n, h, d]; bf16 or float32, d even, 512 at most, any strides.
+    positions (int32 or int64) [l, axes], or [b, l, axes].  The first 2 P features of a head are P = sum(sections) pairs, (j, j + P) or, with
+    `interleaved`, (2j, 2j + 1); pairs go to the axes in sections (at most 8), and pair j turns by `positions[axis] * frequencies[j]`
+    (float64 [P], `rotary_frequencies`): (x, y) -> (x cos - y sin, y cos + x sin).  Features from 2 P on are copied.  Returns the turned q
+    and k, contiguous.  Differentiable with respect to q and k, any number of times.  Angles are taken in float64 and reduced before
+    they become float32, so that far positions are as exact as near ones; the results are rounded once."""
+    r = L.call(_op("rotary_axes"), q, k, positions, frequencies, sections, interleaved)
+    return r[0], r[1] if k is not None else None
+
+
+# ------------------------------------------------------------------------------------------ paged cache
+class PagedCache(NamedTuple):
+    """Keys and values in pages.  k, v [pages, kv_heads, page_size, head_dim]: bf16, or float8_e4m3fn with k_exponent, v_exponent (uint8
+    [pages, kv_heads, page_size]): a row of a head stands for its values times 2 ** (byte - 127) (byte 255: NaN).  Pages are contiguous in
+    themselves; page_size 16, 32, 64, 128 or 256, head_dim 64 or 128.  Which pages a sequence has says its row of a page table (int32
+    [sequences, pages of the longest]): position p lies in page `page_table[i, p // page_size]`, row `p % page_size`; entries past its
+    length are not looked at.  An entry that the cache does not have, or a length past the table's end, is left out, and a later call
+    raises LactError.  Page tables and lengths are read on the device: a captured call follows what they hold at its replay."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exponent: Optional[torch.Tensor] = None
+    v_exponent: Optional[torch.Tensor] = None
+
+
+def paged_cache(num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = BF16, device=None) -> PagedCache:
+    """An empty (zero) cache of bf16, or of 8 bits with `dtype=torch.float8_e4m3fn`."""
+    if dtype not in (BF16, torch.float8_e4m3fn):
+        raise TypeError("dtype: bf16 or float8_e4m3fn")
+    shape = (num_pages, kv_heads, page_size, head_dim)
+    zeros = lambda s, dt: torch.zeros(s, dtype=dt, device=device)
+    if dtype == BF16:
+        return PagedCache(zeros(shape, BF16), zeros(shape, BF16))
+    return PagedCache(*(zeros(shape, torch.uint8).view(dtype) for _ in range(2)), *(zeros(shape[:3], torch.uint8) for _ in range(2)))
+
+
+def paged_cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                      cu_seqlens: Optional[torch.Tensor] = None) -> None:
+    """New keys and values into the cache, in place: k, v [sequences, l, kv_heads, head_dim] bf16 (views of a fused projection are read where
+    they lie) become the last l tokens of sequences that then have lengths[i] (int32) tokens: row j goes to position `lengths[i] - l + j`,
+    and nowhere where that is negative (rows that pad a batch in front; a sequence of length 0 is not touched).  `cu_seqlens` (int32
+    [sequences + 1] on the device, b = 1): the rows of all sequences packed back to back, empty ones allowed; rows outside of them are not
+    written.  A cache of 8 bits gets e4m3 values of the row divided by a power of two, the smallest (from 2^-126 to 2^119) that leaves none
+    above 448; a row of a head with a NaN or an infinity is NaN when it is read.  Two rows of one call must not have the same place: what is
+    there then is not defined.  To autograd the cache has changed in place.  No backward: a call with gradients raises."""
+    L.call(_op("paged_cache_write"), *cache, k, v, page_table, lengths, cu_seqlens)
+
+
+def paged_cache_read(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, num_tokens: int,
+                     cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The last `num_tokens` tokens of every sequence out of the cache: bf16 [2 sequences, num_tokens, kv_heads, head_dim], the keys of all
+    sequences and then their values (what `sliding_window_attention_inference` takes as `kv_cache`).  Row j is position
+    `lengths[i] - num_tokens + j`, zeros where that is negative.  `cu_seqlens` (int32 [sequences + 1]): [2, num_tokens, kv_heads, head_dim], of
+    sequence i the last cu_seqlens[i + 1] - cu_seqlens[i] tokens; rows outside of them are zeros.  8 bits become the bf16 values that
+    they stand for, exactly.  No backward."""
+    return L.call(_op("paged_cache_read"), *cache, page_table, lengths, num_tokens, cu_seqlens)
+
+
+def paged_attention_step(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, window_size: Optional[int] = None,
+                         softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of one new token of every sequence over its cache (generation): q [sequences, heads, head_dim] bf16, keys and values those
+    of positions `max(0, lengths[i] - window_size)` to `lengths[i] - 1` (`window_size` None: all; the new token's own are written before,
+    and lengths count them).  The heads of the cache divide those of q (consecutive heads share).  softmax_scale: head_dim ** -0.5 by
+    default.  Returns o [sequences, heads, head_dim] bf16; a sequence without tokens has zeros.  Scores, maxima and sums are float32; weights
+    are rounded to two bf16 pieces (bf16 cache) or to fp16 (8 bits) for their product with the values.  Rows outside of the window are not
+    read; a NaN within it makes its heads' outputs NaN.  No backward: a call with gradients raises."""
+    return L.call(_op("paged_attention_step"), q, *cache, page_table, lengths, int(window_size) if window_size else 0,
+                  float(softmax_scale) if softmax_scale is not None else cache[0].shape[-1] ** -0.5)
 
 
 # ------------------------------------------------------------------------------------------ sliding-window attention

@@ -883,3 +883,71 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, silu=False):
     z = ((v - mean) / torch.sqrt(var + eps)).reshape(x.shape)
     z = z * (1.0 if weight is None else weight.double()) + (0.0 if bias is None else bias.double())
     return z * torch.sigmoid(z) if silu else z
+
+
+# --------------------------------------------------------------------------- rotary positions with several axes
+def rotary_axes(x, positions, frequencies, sections, interleaved=False):
+    """64 bits: x [.., tokens, heads, d], positions [(batch,) tokens, axes]; complex products of the pairs."""
+    v, P = x.double(), int(sum(sections))
+    axis = torch.repeat_interleave(torch.arange(len(sections), device=x.device), torch.tensor(sections, device=x.device))
+    t = (positions.double()[..., axis] * frequencies.double())[..., None, :]
+    a, b = (v[..., 0:2 * P:2], v[..., 1:2 * P:2]) if interleaved else (v[..., :P], v[..., P:2 * P])
+    z = torch.complex(a, b) * torch.polar(torch.ones_like(t), t)
+    turned = torch.stack([z.real, z.imag], -1).flatten(-2) if interleaved else torch.cat([z.real, z.imag], -1)
+    return torch.cat([turned, v[..., 2 * P:]], -1)
+
+
+# --------------------------------------------------------------------------- paged cache
+def rows_in_8_bits(x):
+    """(values that rows (last axis) of bf16 stand for in 64 bits, bytes of their powers of two), by search over the values of e4m3."""
+    grid = torch.tensor([m * 2.0 ** (max(e, 1) - 10) if e == 0 else (8 + m) * 2.0 ** (e - 10) for e in range(16) for m in range(8)][:127],
+                        dtype=torch.float64, device=x.device)
+    v = x.double()
+    top = v.abs().amax(-1, keepdim=True)
+    byte = torch.ones_like(top)
+    for e in range(1, 247):   # the smallest that leaves none above 448; at 246 what is above is cut
+        byte = torch.where(top > 448 * 2.0 ** (e - 127), torch.full_like(byte, min(e + 1, 246)), byte)
+    u = (v.abs() * torch.exp2(127 - byte)).clamp(max=448.0)
+    hi = torch.searchsorted(grid, u.nan_to_num()).clamp(max=126)
+    lo = (hi - 1).clamp(min=0)
+    up, down = grid[hi] - u, u - grid[lo]
+    near = torch.where((up < down) | ((up == down) & (hi % 2 == 0)), grid[hi], grid[lo])
+    out = torch.copysign(near, v) * torch.exp2(byte - 127)
+    bad = ~torch.isfinite(top)
+    return torch.where(bad, torch.nan, out), torch.where(bad, 255.0, byte)[..., 0].to(torch.uint8)
+
+
+def paged_places(lengths, rows, page_table, page_size):
+    """For sequence after sequence (rows[i] rows each): (row of the batch, page, row of the page) of the rows that have a place."""
+    out, at = [], 0
+    for i, n in enumerate(rows):
+        for j in range(n):
+            p = int(lengths[i]) - n + j
+            if p >= 0:
+                out.append((at + j, int(page_table[i][p // page_size]), p % page_size))
+        at += n
+    return out
+
+
+def paged_attention_step(q, k, v, page_table, lengths, window=None, scale=None):
+    """64 bits: q [n, h, d], k, v [pages, kv_heads, page_size, d] (the values that they stand for).  Returns o and, per output, what
+    tolerances are made of: sums of w |v|, the largest scale sum |q k|, and the largest w 2^e of a row's power of two (8 bits)."""
+    n, h, d = q.shape
+    hk, ps = k.shape[1], k.shape[2]
+    scale = d ** -0.5 if scale is None else scale
+    o = torch.zeros(n, h, d, dtype=torch.float64, device=q.device)
+    size, score = torch.zeros_like(o), torch.zeros(n, h, 1, dtype=torch.float64, device=q.device)
+    for i in range(n):
+        length = int(lengths[i])
+        if length <= 0:
+            continue
+        p = torch.arange(max(0, length - window) if window else 0, length, device=q.device)
+        page = page_table[i].long()[p // ps]
+        kk, vv = k[page, :, p % ps].double(), v[page, :, p % ps].double()   # [l, hk, d]
+        qq = q[i].double().reshape(hk, h // hk, d)
+        x = torch.einsum("jgd,ljd->jgl", qq, kk) * scale
+        w = torch.softmax(x, -1)
+        o[i] = torch.einsum("jgl,ljd->jgd", w, vv).reshape(h, d)
+        size[i] = torch.einsum("jgl,ljd->jgd", w, vv.abs()).reshape(h, d)
+        score[i] = (torch.einsum("jgd,ljd->jgl", qq.abs(), kk.abs()).amax(-1) * abs(scale)).reshape(h, 1)
+    return o, size, score
