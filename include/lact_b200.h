@@ -410,7 +410,7 @@ int lact_rotary_axes(const lact_rotary_config *cfg, const void *q, const void *k
 
 /* A paged cache of keys and values: k, v [pages, kv_heads, page_size, head_dim], 32-byte aligned, pages contiguous in themselves, page
  * strides in elements (multiples of 32 bytes).  bf16 without exponents; with k_exponent, v_exponent ([pages, kv_heads, page_size]
- * bytes) e4m3 values that stand for themselves times 2^(byte - 127), 255: NaN.  head_dim 64 or 128; page_size 16, 32, 64, 128 or 256.
+ * bytes, 16-byte aligned, page strides multiples of 16) e4m3 values that stand for themselves times 2^(byte - 127), 255: NaN.  head_dim 64 or 128; page_size 16, 32, 64, 128 or 256.
  * Position p of sequence i lies in page page_table[i * table_stride + p / page_size], row p % page_size, for p below lengths[i];
  * table_cols * page_size at most 2^30.  Entries of the table past a sequence's length are not looked at; a page or a position that
  * the cache does not have is left out, and device status 102 goes to the host's word (lact_status_host_word).  No counterpart in the
@@ -440,10 +440,11 @@ int lact_paged_cache_read(const lact_paged_cache *cache, void *out, int64_t batc
  * heads (consecutive heads share) -> o [sequences, heads, head_dim] bf16, contiguous: softmax(softmax_scale q K^T) V over positions
  * max(0, length - window) .. length - 1 (window 0: all); zeros where the length is not above 0.  counters, workspace: sizes from
  * lact_paged_attention_step_bytes (uint32 words, zero before the first call and zero again after every one; bytes, 16-byte
- * aligned; both may be 0); calls that share them must follow one another. */
+ * aligned; both may be 0); calls that share them must follow one another.  o: 16-byte aligned. */
 int lact_paged_attention_step_bytes(const lact_paged_cache *cache, int64_t heads, int64_t window, size_t *bytes, int64_t *counters);
 int lact_paged_attention_step(const lact_paged_cache *cache, const void *q, int64_t q_bs, int64_t q_hs, int64_t heads, int64_t window,
-                              float softmax_scale, void *o, void *counters, void *workspace, size_t workspace_bytes, void *stream);
+                              float softmax_scale, void *o, void *counters, void *workspace, size_t workspace_bytes,
+                              int32_t *status_word, void *stream);
 
 /* Backward of lact_qkv_prologue / lact_qkv_prologue_rope on the saved projections (same strides): dq, dk, dv are the
  * gradients of the head-major outputs ([(b n_heads), s, d] bf16, NULL = none), dxq, dxk, dxv the gradients of the

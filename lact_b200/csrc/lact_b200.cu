@@ -2396,9 +2396,10 @@ int paged_check(const lact_paged_cache* c) {
     if ((reinterpret_cast<uintptr_t>(p) & 31) != 0) return LACT_ERR_SHAPE;
   for (int64_t ps : {c->k_page_stride, c->v_page_stride})
     if (c->pages > 1 && (ps < page || ps * size % 32 != 0)) return LACT_ERR_SHAPE;
+  if (((reinterpret_cast<uintptr_t>(c->k_exponent) | reinterpret_cast<uintptr_t>(c->v_exponent)) & 15) != 0) return LACT_ERR_SHAPE;
   if (c->k_exponent != nullptr)
     for (int64_t ps : {c->ke_page_stride, c->ve_page_stride})
-      if (c->pages > 1 && ps < c->kv_heads * c->page_size) return LACT_ERR_SHAPE;
+      if (c->pages > 1 && (ps < c->kv_heads * c->page_size || ps % 16 != 0)) return LACT_ERR_SHAPE;
   return LACT_OK;
 }
 PagedCache paged_args(const lact_paged_cache* c) {
@@ -2444,10 +2445,10 @@ int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t
 
 // How a call's tiles are dealt out.
 struct PagedStepPlan {
-  int nq, blocks, runs;
-  size_t bytes;
+  int nq, blocks, runs, stages;
+  size_t bytes, smem;
 };
-constexpr int kPagedWarps = 6, kPagedPerSm = 2;
+constexpr int kPagedWarps = 4, kPagedPerSm = 2;
 constexpr int kPagedLeast = 2;   // tiles of a run at least
 constexpr int kPagedWhole = 4;   // tiles of a unit up to which a CTA takes a unit
 int paged_step_plan(const lact_paged_cache* c, int64_t heads, int64_t window, PagedStepPlan* p) {
@@ -2458,18 +2459,28 @@ int paged_step_plan(const lact_paged_cache* c, int64_t heads, int64_t window, Pa
   const int64_t units = c->sequences * c->kv_heads * p->blocks, room = c->table_cols * c->page_size;
   const int64_t most = (std::min(window > 0 ? window + 15 : room, room) + tile - 1) / tile;   // of a unit
   if (units > 0x7FFFFFFF) return LACT_ERR_SHAPE;
+  const int64_t rows = std::min<int64_t>(share, 8 * p->nq), sums = rows * kPagedPieceRow(static_cast<int>(c->head_dim)) * 4;
   p->runs = most <= kPagedWhole ? 0 : static_cast<int>(std::min<int64_t>(sm_count() * kPagedPerSm, (units * most + kPagedLeast - 1) / kPagedLeast));
-  p->bytes = static_cast<size_t>(p->runs) * 2 * 8 * p->nq * kPagedPieceRow(static_cast<int>(c->head_dim)) * 4;
+  p->bytes = static_cast<size_t>(p->runs) * 2 * sums;
+  const int64_t stage = 32 * c->head_dim * (c->k_exponent != nullptr ? 1 : 2) + (c->k_exponent != nullptr ? 32 : 0);
+  // (the sums of a row hold the factors of all of a unit's pieces later on; 3 KB: alignment, and what the kernel has beside)
+  const int64_t room_cta = 227 * 1024 / kPagedPerSm - 3072, at_end = std::max<int64_t>(kPagedWarps * sums, rows * p->runs * 4);
+  p->stages = static_cast<int>(std::min<int64_t>(kPagedStages, (room_cta - at_end) / (kPagedWarps * stage)));
+  p->smem = static_cast<size_t>(kPagedWarps * p->stages * stage + at_end) + 1024;
   return LACT_OK;
 }
 template <int D, bool E4, int NQ>
-int launch_paged_step(const PagedStepArgs& a, cudaStream_t st) {
-  auto kernel = paged_step_kernel<D, E4, NQ, kPagedWarps, kPagedPerSm>;
-  constexpr size_t smem = static_cast<size_t>(kPagedWarps) * 8 * NQ * kPagedPieceRow(D) * 4;
-  if (smem > 48 * 1024) LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+int launch_paged_step(const lact_paged_cache* c, const PagedStepArgs& a, size_t smem, cudaStream_t st) {
+  auto kernel = paged_step_kernel<D, E4, NQ, kPagedWarps>;
+  CUtensorMap k_map, v_map;
+  constexpr int64_t cols = E4 ? D / 2 : D;   // of 16 bits
+  const int64_t rows = c->kv_heads * c->page_size;
+  LACT_TRY(encode_map(&k_map, {c->k, rows, cols, cols, c->pages, a.c.k_ps / 2}, 16, cols < 64 ? 32 : 64));
+  LACT_TRY(encode_map(&v_map, {c->v, rows, cols, cols, c->pages, a.c.v_ps / 2}, 16, cols < 64 ? 32 : 64));
+  LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   const int64_t grid = a.runs > 0 ? a.runs : static_cast<int64_t>(a.c.sequences) * a.c.heads * a.blocks;
   KernelScope scope(kClsOther, st);
-  LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kPagedWarps * 32), smem, st, a));
+  LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kPagedWarps * 32), smem, st, a, k_map, v_map));
   return LACT_OK;
 }
 
@@ -3675,10 +3686,10 @@ int lact_paged_attention_step_bytes(const lact_paged_cache* c, int64_t heads, in
 }
 
 int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t q_bs, int64_t q_hs, int64_t heads, int64_t window,
-                              float softmax_scale, void* o, void* counters, void* workspace, size_t workspace_bytes, void* stream) {
+                              float softmax_scale, void* o, void* counters, void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream) {
   LACT_TRY(paged_check(c));
-  if (q == nullptr || o == nullptr) return LACT_ERR_NULL;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || (reinterpret_cast<uintptr_t>(o) & 1) != 0 || q_bs % 8 != 0 || q_hs % 8 != 0) return LACT_ERR_SHAPE;
+  if (q == nullptr || o == nullptr || status_word == nullptr) return LACT_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || (reinterpret_cast<uintptr_t>(o) & 15) != 0 || q_bs % 8 != 0 || q_hs % 8 != 0) return LACT_ERR_SHAPE;
   if (!(std::fabs(softmax_scale) <= 1e18f)) return LACT_ERR_CONFIG;
   PagedStepPlan p;
   LACT_TRY(paged_step_plan(c, heads, window, &p));
@@ -3695,17 +3706,19 @@ int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t 
   a.runs = p.runs; a.least = kPagedLeast;
   a.counters = static_cast<uint32_t*>(counters);
   a.pieces = static_cast<float*>(workspace);
+  a.status = status_word;
+  a.stages = p.stages;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int form = (c->head_dim == 128 ? 4 : 0) + (c->k_exponent != nullptr ? 2 : 0) + p.nq - 1;
   switch (form) {
-    case 0: return launch_paged_step<64, false, 1>(a, st);
-    case 1: return launch_paged_step<64, false, 2>(a, st);
-    case 2: return launch_paged_step<64, true, 1>(a, st);
-    case 3: return launch_paged_step<64, true, 2>(a, st);
-    case 4: return launch_paged_step<128, false, 1>(a, st);
-    case 5: return launch_paged_step<128, false, 2>(a, st);
-    case 6: return launch_paged_step<128, true, 1>(a, st);
-    default: return launch_paged_step<128, true, 2>(a, st);
+    case 0: return launch_paged_step<64, false, 1>(c, a, p.smem, st);
+    case 1: return launch_paged_step<64, false, 2>(c, a, p.smem, st);
+    case 2: return launch_paged_step<64, true, 1>(c, a, p.smem, st);
+    case 3: return launch_paged_step<64, true, 2>(c, a, p.smem, st);
+    case 4: return launch_paged_step<128, false, 1>(c, a, p.smem, st);
+    case 5: return launch_paged_step<128, false, 2>(c, a, p.smem, st);
+    case 6: return launch_paged_step<128, true, 1>(c, a, p.smem, st);
+    default: return launch_paged_step<128, true, 2>(c, a, p.smem, st);
   }
 }
 

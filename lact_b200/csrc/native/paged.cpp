@@ -160,9 +160,8 @@ Tensor step(const Tensor& q_, const Tensor& kc, const Tensor& vc, const OptTenso
     room = bytes(need, q);
     counters = zeroed_counters(q, words);
   }
-  poll_status(q);
   check(lact_paged_attention_step(&r.c, ptr(q), stride_of(q, 0), stride_of(q, 1), q.size(1), window, static_cast<float>(scale), ptr(o),
-                                  need > 0 ? ptr(counters) : nullptr, need > 0 ? ptr(room) : nullptr, need, stream_of(q)),
+                                  need > 0 ? ptr(counters) : nullptr, need > 0 ? ptr(room) : nullptr, need, status_word(q), stream_of(q)),
         "lact_paged_attention_step");
   return o;
 }

@@ -20,6 +20,7 @@
 
 namespace lact {
 
+constexpr int kPagedStages = 8;   // at most
 struct PagedStepArgs {
   PagedCache c;
   const bf16* q;                   // [sequences][heads][D], features adjacent, other strides in elements
@@ -30,7 +31,9 @@ struct PagedStepArgs {
   float scale;                     // softmax scale * log2(e)
   int32_t runs, least;             // CTAs that share the tiles; tiles of a run at least
   uint32_t* counters;              // [runs], zero before and after
-  float* pieces;                   // [runs][2][rows of a block][D + 4]
+  float* pieces;                   // [runs][2][min(share, rows of a block)][D + 4]
+  int32_t* status;
+  int32_t stages;                  // steps of 16 tokens that a warp has on their way or in work
 };
 
 __device__ __forceinline__ void mma_16x8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool halves) {
@@ -49,23 +52,6 @@ __device__ __forceinline__ uint32_t transposed_8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// N words of a row of the cache, read once; zeros where `there` is false
-template <int N>
-__device__ __forceinline__ void load_cache(uint32_t (&w)[N], const uint8_t* p, bool there) {
-  static_assert(N == 2 || N == 4 || N == 8);
-#pragma unroll
-  for (int i = 0; i < N; ++i) w[i] = 0;
-  if (!there) return;
-  if constexpr (N == 8)
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                 : "l"(p));
-  else if constexpr (N == 4)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
-  else
-    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-}
-
 // Tiles of a sequence (one at least: an empty sequence's zeros are a unit's result, too)
 struct PagedSpan {
   int first, last;   // positions [first, last)
@@ -86,32 +72,73 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedStepArgs& a, int seq)
 constexpr float kLowest = -3.402823466e38f;
 __host__ __device__ constexpr int kPagedPieceRow(int D) { return D + 4; }   // sums, then m, l, M
 
-template <int D, bool E4, int NQ, int W, int PER_SM>
-__global__ void __launch_bounds__(W * 32, PER_SM) paged_step_kernel(const __grid_constant__ PagedStepArgs a) {
+// 2^4 bytes of exponents: an untiled copy (both addresses on 16 bytes)
+__device__ __forceinline__ void bulk_load_16_if(uint32_t leader, uint32_t smem_dst, const void* from, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\t"
+      "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];\n\t}" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(from)), "r"(bar), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_shared_8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+
+// Where a walk over a run's tiles is.
+struct PagedWalk {
+  int seq, unit, t, t1, left;      // left: tiles of the run from this unit's first on
+  int head, first, last, base, tiles;
+  const int32_t* table;
+};
+
+template <int D, bool E4, int NQ, int W>
+__global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constant__ PagedStepArgs a, const __grid_constant__ CUtensorMap k_map,
+                                                            const __grid_constant__ CUtensorMap v_map) {
   constexpr int ROWS = 8 * NQ, TILE = 16 * W, ROW = kPagedPieceRow(D), THREADS = W * 32;
   constexpr int BYTES = E4 ? D : 2 * D;                  // of a row
-  constexpr int KL = BYTES >= 128 ? 32 : 16;             // bytes of a K row that a lane loads at a time
-  constexpr int KN = BYTES / (4 * KL);                   // times
-  constexpr int KW = KL / 4;                             // words of one
-  constexpr int VW = BYTES / 32;                         // words of a V row that a lane holds
+  constexpr int BOX = BYTES >= 128 ? 128 : 64;           // bytes of a row in a box of 16 rows; swizzled over as many
+  constexpr int BOXES = BYTES / BOX;
+  constexpr int KB = 16 * BYTES, STAGE = 2 * KB;
+  constexpr int KW = BOX / 16;                           // words of a box's K row that a lane has
+  constexpr int VW = BOX / 32;                           // words of a box's V row that a lane has
   constexpr int MT = D / 16;                             // products of 16 features
   constexpr int QW = D / 8;                              // words of a lane's queries: two a step of 16 features
-  extern __shared__ __align__(16) float paged_smem[];    // [W][ROWS][ROW]
+  extern __shared__ uint8_t smem_raw[];   // [W][stages] of K and V, [W][stages][32] exponents, sums [W][rows][ROW]
+  __shared__ uint64_t full[W * kPagedStages];
   __shared__ int plan[4];
   __shared__ int64_t warp_sum[W];
-  __shared__ uint32_t arrived;
+  __shared__ uint32_t arrived, gave_up;
+  __shared__ float scales[ROWS];
+  const int warp = uniform_warp_index(), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int stages = a.stages;
+  const uint32_t leader = elect_leader();
+  uint8_t* const paged_smem = smem_raw + ((smem_u32(smem_raw) + 1023u & ~1023u) - smem_u32(smem_raw));
+  const uint32_t ring = smem_u32(paged_smem) + warp * stages * STAGE, exp_ring = smem_u32(paged_smem) + W * stages * STAGE + warp * stages * 32;
+  float* const sums = reinterpret_cast<float*>(paged_smem + W * stages * (STAGE + (E4 ? 32 : 0)));
+  if (lane == 0)
+    for (int i = 0; i < stages; ++i) mbar_init(&full[warp * kPagedStages + i], 1);
+  if (threadIdx.x == 0) gave_up = 0;
+  fence_mbar_init();
   griddep_launch_dependents();
   griddep_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int units = a.c.heads * a.blocks;                // of a sequence
+  const int sum_rows = min(a.share, ROWS);
   // -------- this CTA's run
-  int seq, unit, t0, left;                               // first unit, its first tile of the run, tiles of the run
+  PagedWalk make;                                        // (the copies run ahead of the products)
   int64_t run0 = 0, per = 0;
   if (a.runs == 0) {
-    seq = blockIdx.x / units;
-    unit = blockIdx.x - seq * units;
-    t0 = 0;
-    left = paged_span<TILE>(a, seq).tiles;
+    make.seq = blockIdx.x / units;
+    make.unit = blockIdx.x - make.seq * units;
+    make.t = 0;
+    make.left = paged_span<TILE>(a, make.seq).tiles;
+    __syncthreads();
   } else {
     const int chunk = (a.c.sequences + THREADS - 1) / THREADS, s0 = min(static_cast<int>(threadIdx.x) * chunk, a.c.sequences), s1 = min(s0 + chunk, a.c.sequences);
     int64_t mine = 0;
@@ -134,7 +161,7 @@ __global__ void __launch_bounds__(W * 32, PER_SM) paged_step_kernel(const __grid
     per = max((all + a.runs - 1) / a.runs, static_cast<int64_t>(a.least));
     run0 = blockIdx.x * per;
     if (run0 >= all) return;
-    left = static_cast<int>(min(per, all - run0));
+    make.left = static_cast<int>(min(per, all - run0));
     int64_t at = (upto - mine) * units;
     if (run0 >= at && run0 < upto * units) {
       for (int s = s0; s < s1; ++s) {
@@ -149,20 +176,71 @@ __global__ void __launch_bounds__(W * 32, PER_SM) paged_step_kernel(const __grid
       }
     }
     __syncthreads();
-    seq = plan[0];
-    unit = plan[1];
-    t0 = plan[2];
+    make.seq = plan[0];
+    make.unit = plan[1];
+    make.t = plan[2];
   }
-  // -------- its units
-  for (int64_t done = 0; left > 0; ++unit) {
-    if (unit == units) {
-      unit = 0;
-      ++seq;
+  auto enter = [&](PagedWalk& w) {                       // seq, unit, t and left are set
+    const PagedSpan span = paged_span<TILE>(a, w.seq);
+    w.first = span.first; w.last = span.last; w.tiles = span.tiles;
+    w.base = span.first & ~15;
+    w.t1 = min(span.tiles, w.t + w.left);
+    w.head = w.unit / a.blocks;
+    w.table = a.c.table + w.seq * a.c.table_rs;
+  };
+  auto leave = [&](PagedWalk& w, int from) {             // to the next unit; `from`: the tile that this one began with
+    w.left -= w.t1 - from;
+    w.t = 0;
+    if (++w.unit == units) {
+      w.unit = 0;
+      ++w.seq;
     }
-    const PagedSpan span = paged_span<TILE>(a, seq);
-    const int head = unit / a.blocks, row0 = (unit - head * a.blocks) * ROWS, rows = min(a.share - row0, ROWS);
-    const int t1 = min(span.tiles, t0 + left), base = span.first & ~15;
-    if (threadIdx.x == 0 && a.c.lengths[seq] > span.last && t1 == span.tiles) report_bad_page();
+  };
+  auto position = [&](const PagedWalk& w) { return w.base + (w.t * W + warp) * 16; };
+  // (a step of 16 tokens lies in one page; past the end none is looked up)
+  auto page_of = [&](const PagedWalk& w) { return position(w) < w.last ? w.table[position(w) >> a.c.shift] : -1; };
+  enter(make);
+  PagedWalk use = make;
+  int make_from = make.t, page = page_of(make), make_slot = 0, use_slot = 0;
+  uint32_t has = 0, phase = 0;                           // slots that hold a step; parities of their next waits
+  // the copies of this warp's 16 tokens of the next tile
+  auto issue = [&]() {
+    if (make.left <= 0) return;
+    const int p = position(make);
+    bool real = p < make.last;
+    if (real && static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.c.pages)) {
+      if (lane == 0) report_bad_page();
+      real = false;
+    }
+    has = real ? has | 1u << make_slot : has & ~(1u << make_slot);
+    if (real) {
+      const int row = (make.head << a.c.shift) + (p & ((1 << a.c.shift) - 1));
+      const uint32_t bar = smem_u32(&full[warp * kPagedStages + make_slot]), to = ring + make_slot * STAGE;
+      mbar_expect_tx_if(leader, bar, STAGE + (E4 ? 32 : 0));
+#pragma unroll
+      for (int i = 0; i < BOXES; ++i) tma_load_3d_if(leader, to + i * 16 * BOX, &k_map, bar, i * 64, row, page);
+#pragma unroll
+      for (int i = 0; i < BOXES; ++i) tma_load_3d_if(leader, to + KB + i * 16 * BOX, &v_map, bar, i * 64, row, page);
+      if constexpr (E4) {
+        bulk_load_16_if(leader, exp_ring + make_slot * 32, a.c.ke + page * a.c.ke_ps + row, bar);
+        bulk_load_16_if(leader, exp_ring + make_slot * 32 + 16, a.c.ve + page * a.c.ve_ps + row, bar);
+      }
+    }
+    if (++make_slot == stages) make_slot = 0;
+    if (++make.t == make.t1) {
+      leave(make, make_from);
+      make_from = 0;
+      if (make.left > 0) enter(make);
+    }
+    if (make.left > 0) page = page_of(make);
+  };
+  for (int i = 0; i < stages; ++i) issue();
+  bool failed = false;
+  // -------- its units
+  for (int64_t done = 0; use.left > 0;) {
+    if (done > 0) enter(use);
+    const int t0 = use.t, seq = use.seq, head = use.head, row0 = (use.unit - head * a.blocks) * ROWS, rows = min(a.share - row0, ROWS);
+    if (threadIdx.x == 0 && a.c.lengths[seq] > use.last && use.t1 == use.tiles) report_bad_page();
     // queries: column r of a product is query head row0 + r (+ 8)
     uint32_t q[NQ][QW];
     float qm[NQ][2];                                     // what scores of columns 2 c, 2 c + 1 are multiplied by
@@ -172,25 +250,22 @@ __global__ void __launch_bounds__(W * 32, PER_SM) paged_step_kernel(const __grid
       const bf16* from = a.q + seq * a.q_bs + (static_cast<int64_t>(head) * a.share + row0 + n * 8 + r) * a.q_hs;
       if constexpr (!E4) {
 #pragma unroll
-        for (int i = 0; i < KN; ++i)
+        for (int i = 0; i < BOXES; ++i)
 #pragma unroll
           for (int e = 0; e < KW; e += 4) {
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (on) w = *reinterpret_cast<const uint4*>(from + (i * 4 + c) * (KL / 2) + e * 2);
+            if (on) w = *reinterpret_cast<const uint4*>(from + i * 64 + c * 16 + e * 2);
             q[n][i * KW + e] = w.x; q[n][i * KW + e + 1] = w.y; q[n][i * KW + e + 2] = w.z; q[n][i * KW + e + 3] = w.w;
           }
         qm[n][0] = qm[n][1] = a.scale;
       } else {
         uint32_t raw[QW], top = 0;
 #pragma unroll
-        for (int i = 0; i < KN; ++i)
-#pragma unroll
-          for (int e = 0; e < 2 * KW; e += 4) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (on) w = *reinterpret_cast<const uint4*>(from + (i * 4 + c) * KL + e * 2);
-            uint32_t* const to = raw + i * 2 * KW + e;
-            to[0] = w.x; to[1] = w.y; to[2] = w.z; to[3] = w.w;
-          }
+        for (int e = 0; e < QW; e += 4) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (on) w = *reinterpret_cast<const uint4*>(from + c * (2 * QW) + e * 2);
+          raw[e] = w.x; raw[e + 1] = w.y; raw[e + 2] = w.z; raw[e + 3] = w.w;
+        }
 #pragma unroll
         for (int i = 0; i < QW; ++i) top = __vmaxu2(top, raw[i] & 0x7FFF7FFFu);
         top = max(top & 0xFFFFu, top >> 16);
@@ -220,78 +295,96 @@ __global__ void __launch_bounds__(W * 32, PER_SM) paged_step_kernel(const __grid
       m[n][0] = m[n][1] = M[n][0] = M[n][1] = kLowest;
       l[n][0] = l[n][1] = 0.f;
     }
-    const int32_t* const table = a.c.table + seq * a.c.table_rs;
-    const uint8_t* const kh = a.c.k + (static_cast<int64_t>(head) << a.c.shift) * BYTES;
-    const uint8_t* const vh = a.c.v + (static_cast<int64_t>(head) << a.c.shift) * BYTES;
-    auto position = [&](int t) { return base + (t * W + warp) * 16; };
-    // (a step of 16 tokens lies in one page; past the end none is looked up)
-    auto page_of = [&](int t) { return t < t1 && position(t) < span.last ? table[position(t) >> a.c.shift] : -2; };
-    uint32_t kr[2][KN][KW], vr[4][VW];
-    [[maybe_unused]] uint32_t ke[2], ve[2];
-    auto load_k = [&](int t, int page) {
-      const int p = position(t), row = p & ((1 << a.c.shift) - 1);
-      const bool there = page >= 0 && page < a.c.pages;
-      if (!there && page != -2 && lane == 0) report_bad_page();
-      const uint8_t* const from = kh + page * a.c.k_ps + static_cast<int64_t>(row) * BYTES;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool on = there && p + r + 8 * h >= span.first && p + r + 8 * h < span.last;
-#pragma unroll
-        for (int i = 0; i < KN; ++i) load_cache<KW>(kr[h][i], from + (r + 8 * h) * BYTES + (i * 4 + c) * KL, on);
-        if constexpr (E4) {
-          const int64_t at = (static_cast<int64_t>(head) << a.c.shift) + row + r + 8 * h;
-          ke[h] = on ? a.c.ke[page * a.c.ke_ps + at] : 127u;
-          ve[h] = on ? a.c.ve[page * a.c.ve_ps + at] : 127u;
+    for (; use.t < use.t1; ++use.t) {
+      const int slot = use_slot, p = position(use);
+      if (++use_slot == stages) use_slot = 0;
+      if ((has >> slot & 1) && !failed) {
+        if (!mbar_wait_warp(&full[warp * kPagedStages + slot], phase >> slot & 1, &gave_up)) {
+          // out of time: nothing more is copied or computed; what is on its way gets as long again to arrive
+          failed = true;
+          gave_up = 1;
+          if (lane == 0) report_timeout(a.status);
+          make.left = 0;
+          for (int s = 0; s < stages; ++s)
+            if (has >> s & 1) mbar_wait(&full[warp * kPagedStages + s], phase >> s & 1);
         }
+        phase ^= 1u << slot;
       }
-    };
-    auto load_v = [&](int t, int page) {
-      const int p = position(t), row = p & ((1 << a.c.shift) - 1);
-      const bool there = page >= 0 && page < a.c.pages;
-      const uint8_t* const from = vh + page * a.c.v_ps + static_cast<int64_t>(row) * BYTES;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = 2 * c + (i & 1) + 8 * (i >> 1);
-        load_cache<VW>(vr[i], from + tok * BYTES + r * (VW * 4), there && p + tok >= span.first && p + tok < span.last);
+      if (!(has >> slot & 1) || failed) {
+        issue();
+        continue;
       }
-    };
-    int page = page_of(t0), next = page_of(t0 + 1);
-    load_k(t0, page);
-    load_v(t0, page);
-    for (int t = t0; t < t1; ++t) {
+      const uint32_t ks = ring + slot * STAGE, vs = ks + KB;
       float x[NQ][4];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < KN; ++i)
+      for (int i = 0; i < BOXES; ++i) {
+        uint32_t kr[2][KW];                              // rows r, r + 8: a lane's BOX / 4 bytes
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < KW / 4; ++e) {
+            const int row = r + 8 * h;
+            const uint4 w = ld_shared_16(ks + i * 16 * BOX + row * BOX + ((c * (KW / 4) + e) ^ (BOX == 128 ? r : r >> 1 & 3)) * 16);
+            kr[h][4 * e] = w.x; kr[h][4 * e + 1] = w.y; kr[h][4 * e + 2] = w.z; kr[h][4 * e + 3] = w.w;
+          }
 #pragma unroll
         for (int e = 0; e < KW; e += E4 ? 1 : 2) {
           uint32_t a0, a1, a2, a3;
           if constexpr (E4) {
-            a0 = halves_of_e4m3(kr[0][i][e] & 0xFFFFu); a1 = halves_of_e4m3(kr[1][i][e] & 0xFFFFu);
-            a2 = halves_of_e4m3(kr[0][i][e] >> 16); a3 = halves_of_e4m3(kr[1][i][e] >> 16);
+            a0 = halves_of_e4m3(kr[0][e] & 0xFFFFu); a1 = halves_of_e4m3(kr[1][e] & 0xFFFFu);
+            a2 = halves_of_e4m3(kr[0][e] >> 16); a3 = halves_of_e4m3(kr[1][e] >> 16);
           } else {
-            a0 = kr[0][i][e]; a1 = kr[1][i][e]; a2 = kr[0][i][e + 1]; a3 = kr[1][i][e + 1];
+            a0 = kr[0][e]; a1 = kr[1][e]; a2 = kr[0][e + 1]; a3 = kr[1][e + 1];
           }
-          const int s = E4 ? 2 * (i * KW + e) : i * KW + e;
+          const int s = E4 ? 2 * e : i * KW + e;
 #pragma unroll
           for (int n = 0; n < NQ; ++n) mma_16x8(x[n], a0, a1, a2, a3, q[n][s], q[n][s + 1], E4);
         }
+      }
       [[maybe_unused]] float kx[2], vx[2];
-      if constexpr (E4)
+      if constexpr (E4) {
+        const uint8_t* const exps = paged_smem + (exp_ring - smem_u32(paged_smem)) + slot * 32;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          kx[h] = exponent_value(ke[h]);
-          vx[h] = ve[h] == 255 ? __uint_as_float(0x7FC00000u) : static_cast<float>(static_cast<int>(ve[h]) - 127);
+          const uint32_t kb = exps[r + 8 * h], vb = exps[16 + r + 8 * h];
+          kx[h] = exponent_value(kb);
+          vx[h] = vb == 255 ? __uint_as_float(0x7FC00000u) : static_cast<float>(static_cast<int>(vb) - 127);
         }
-      const int p = position(t);
-      const bool there = page >= 0 && page < a.c.pages;
-      const bool on[2] = {there && p + r >= span.first && p + r < span.last, there && p + r + 8 >= span.first && p + r + 8 < span.last};
-      page = next;
-      if (t + 1 < t1) {
-        next = page_of(t + 2);
-        load_k(t + 1, page);
       }
+      // a lane's features (8 bits: 16; else 8 of each box) of tokens 2 c, 2 c + 1 and those 8 later
+      uint32_t vr[4][BOXES * VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = 2 * c + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+        for (int b = 0; b < BOXES; ++b) {
+          if constexpr (VW == 4) {
+            const uint4 w = ld_shared_16(vs + b * 16 * BOX + tok * BOX + (r ^ (tok & 7)) * 16);
+            vr[i][b * 4] = w.x; vr[i][b * 4 + 1] = w.y; vr[i][b * 4 + 2] = w.z; vr[i][b * 4 + 3] = w.w;
+          } else {
+            const uint2 w = ld_shared_8(vs + tok * BOX + ((r >> 1) ^ (tok >> 1 & 3)) * 16 + (r & 1) * 8);
+            vr[i][0] = w.x; vr[i][1] = w.y;
+          }
+        }
+      }
+      // tokens outside of the window: no weight, and no values (what lies there may be NaN)
+      const bool whole_step = p >= use.first && p + 16 <= use.last;
+      bool on[2] = {true, true};
+      if (!whole_step) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) on[h] = p + r + 8 * h >= use.first && p + r + 8 * h < use.last;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = 2 * c + (i & 1) + 8 * (i >> 1);
+          if (p + tok >= use.first && p + tok < use.last) continue;
+#pragma unroll
+          for (int e = 0; e < BOXES * VW; ++e) vr[i][e] = 0;
+        }
+      }
+      __syncwarp();
+      issue();                                           // (all of the slot is in registers)
       // scores; the maxima, where one passes them by 8
       bool raise = false;
       [[maybe_unused]] float y[NQ][4];
@@ -304,7 +397,7 @@ __global__ void __launch_bounds__(W * 32, PER_SM) paged_step_kernel(const __grid
           if (!on[e >> 1]) x[n][e] = -INFINITY;
           raise = raise || x[n][e] > m[n][e & 1] + 8.f;
           if constexpr (E4) {
-            y[n][e] = x[n][e] + vx[e >> 1];
+            y[n][e] = on[e >> 1] ? x[n][e] + vx[e >> 1] : -INFINITY;
             raise = raise || y[n][e] > M[n][e & 1] + 8.f;
           }
         }
@@ -384,10 +477,8 @@ __global__ void __launch_bounds__(W * 32, PER_SM) paged_step_kernel(const __grid
           }
         }
       }
-      if (t + 1 < t1) load_v(t + 1, page);
     }
-    // -------- the warps' sums: a lane holds features 16 j.. of r for columns 2 c, 2 c + 1
-    float* const mine = paged_smem + warp * ROWS * ROW;
+    // -------- the warps' sums (rows of D features, then m, l, M)
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -396,73 +487,96 @@ __global__ void __launch_bounds__(W * 32, PER_SM) paged_step_kernel(const __grid
         for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xFFFFFFFFu, l[n][e], o);
         const int row = n * 8 + 2 * c + e;
         if (row >= rows) continue;
-        float* const to = mine + row * ROW;
+        float* const to = sums + (warp * sum_rows + row) * ROW;
 #pragma unroll
-        for (int j = 0; j < MT; j += 2)
-          *reinterpret_cast<float4*>(to + r * (D / 8) + 2 * j) = make_float4(acc[n][j][e], acc[n][j][e + 2], acc[n][j + 1][e], acc[n][j + 1][e + 2]);
+        for (int j = 0; j < MT; j += 2) {
+          const int d = BOXES == 1 ? r * (D / 8) + 2 * j : j / 4 * 64 + r * 8 + j % 4 * 2;
+          *reinterpret_cast<float4*>(to + d) = make_float4(acc[n][j][e], acc[n][j][e + 2], acc[n][j + 1][e], acc[n][j + 1][e + 2]);
+        }
         if (r == 0) *reinterpret_cast<float4*>(to + D) = make_float4(m[n][e], l[n][e], E4 ? M[n][e] : m[n][e], 0.f);
       }
     __syncthreads();
-    const bool whole = t1 == span.tiles && t0 == 0;
-    const int64_t begin = run0 + done - t0;               // the unit's first tile among all
-    float* const piece = whole ? nullptr : a.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * ROWS * ROW;
+    const bool whole = use.t1 == use.tiles && t0 == 0;
+    const int64_t begin = run0 + done - t0;              // the unit's first tile among all
+    auto piece_of = [&](int64_t run, bool first) { return a.pieces + (run * 2 + (first ? 1 : 0)) * sum_rows * ROW; };
+    float* const piece = whole ? nullptr : piece_of(blockIdx.x, t0 == 0);
     bf16* const o = a.o + (static_cast<int64_t>(seq) * a.heads + static_cast<int64_t>(head) * a.share + row0) * D;
     for (int i = threadIdx.x; i < rows * D; i += THREADS) {
       const int row = i / D, d = i % D;
-      const float* const from = paged_smem + row * ROW;
+      const float* const from = sums + row * ROW;
       float tm = kLowest, tM = kLowest, sum = 0.f, tl = 0.f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        tm = fmaxf(tm, from[w * ROWS * ROW + D]);
-        tM = fmaxf(tM, from[w * ROWS * ROW + D + 2]);
+        tm = fmaxf(tm, from[w * sum_rows * ROW + D]);
+        tM = fmaxf(tM, from[w * sum_rows * ROW + D + 2]);
       }
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float* const f = from + w * ROWS * ROW;
+        const float* const f = from + w * sum_rows * ROW;
         sum += f[d] * exp2_ftz(f[D + 2] - tM);
         tl += f[D + 1] * exp2_ftz(f[D] - tm);
       }
       if (whole) {
-        o[i] = __float2bfloat16_rn(span.last > span.first ? sum * (exp2_ftz(tM - tm) / tl) : 0.f);
+        o[i] = __float2bfloat16_rn(use.last > use.first ? sum * (exp2_ftz(tM - tm) / tl) : 0.f);
       } else {
         piece[row * ROW + d] = sum;
-        if (d < 3) piece[row * ROW + D + d] = d == 0 ? tm : d == 1 ? tl : tM;
+        if (d < 4) piece[row * ROW + D + d] = d == 0 ? tm : d == 1 ? tl : d == 2 ? tM : 0.f;
       }
     }
     if (!whole) {
       // the run that leaves the last of the unit's pieces adds them up
-      const int first_run = static_cast<int>(begin / per), last_run = static_cast<int>((begin + span.tiles - 1) / per);
+      const int64_t first_run = begin / per, last_run = (begin + use.tiles - 1) / per;
+      const int count = static_cast<int>(last_run - first_run) + 1;
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
-        const uint32_t before = atomicAdd(a.counters + first_run, 1u);
-        arrived = before;
-        if (before == static_cast<uint32_t>(last_run - first_run)) a.counters[first_run] = 0;
+        arrived = atomicAdd(a.counters + first_run, 1u);
+        if (arrived == static_cast<uint32_t>(count - 1)) a.counters[first_run] = 0;
       }
       __syncthreads();
-      if (arrived == static_cast<uint32_t>(last_run - first_run)) {
+      if (arrived == static_cast<uint32_t>(count - 1)) {
         __threadfence();
-        for (int i = threadIdx.x; i < rows * D; i += THREADS) {
-          const int row = i / D, d = i % D;
-          auto of = [&](int run) { return a.pieces + (static_cast<int64_t>(run) * 2 + (run == first_run ? 1 : 0)) * ROWS * ROW + row * ROW; };
-          float tm = kLowest, tM = kLowest, sum = 0.f, tl = 0.f;
-          for (int run = first_run; run <= last_run; ++run) {
-            tm = fmaxf(tm, __ldcg(of(run) + D));
-            tM = fmaxf(tM, __ldcg(of(run) + D + 2));
+        // a warp a row: each piece's factor, and the row's
+        float* const factors = sums;                     // [rows][count] (at most as many runs as the sums of a row take)
+        for (int row = warp; row < rows; row += W) {
+          float tm = kLowest, tM = kLowest, tl = 0.f;
+          for (int i = lane; i < count; i += 32) {
+            const float4 s = __ldcg(reinterpret_cast<const float4*>(piece_of(first_run + i, i == 0) + row * ROW + D));
+            tm = fmaxf(tm, s.x);
+            tM = fmaxf(tM, s.z);
           }
-          for (int run = first_run; run <= last_run; ++run) {
-            const float* const f = of(run);
-            sum += __ldcg(f + d) * exp2_ftz(__ldcg(f + D + 2) - tM);
-            tl += __ldcg(f + D + 1) * exp2_ftz(__ldcg(f + D) - tm);
+#pragma unroll
+          for (int s = 16; s > 0; s >>= 1) {
+            tm = fmaxf(tm, __shfl_xor_sync(0xFFFFFFFFu, tm, s));
+            tM = fmaxf(tM, __shfl_xor_sync(0xFFFFFFFFu, tM, s));
           }
-          o[i] = __float2bfloat16_rn(sum * (exp2_ftz(tM - tm) / tl));
+          for (int i = lane; i < count; i += 32) {
+            const float4 s = __ldcg(reinterpret_cast<const float4*>(piece_of(first_run + i, i == 0) + row * ROW + D));
+            tl += s.y * exp2_ftz(s.x - tm);
+            factors[row * count + i] = exp2_ftz(s.z - tM);
+          }
+#pragma unroll
+          for (int s = 16; s > 0; s >>= 1) tl += __shfl_xor_sync(0xFFFFFFFFu, tl, s);
+          if (lane == 0) scales[row] = exp2_ftz(tM - tm) / tl;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
+          const int row = i / (D / 4), d = i % (D / 4) * 4;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int k = 0; k < count; ++k) {
+            const float4 s = __ldcg(reinterpret_cast<const float4*>(piece_of(first_run + k, k == 0) + row * ROW + d));
+            const float f = factors[row * count + k];
+            sum.x += s.x * f; sum.y += s.y * f; sum.z += s.z * f; sum.w += s.w * f;
+          }
+          const float f = scales[row];
+          *reinterpret_cast<uint2*>(o + row * D + d) = make_uint2(pack_bf16x2(sum.x * f, sum.y * f), pack_bf16x2(sum.z * f, sum.w * f));
         }
       }
     }
     __syncthreads();
-    done += t1 - t0;
-    left -= t1 - t0;
-    t0 = 0;
+    done += use.t1 - t0;
+    leave(use, t0);
   }
 }
 

@@ -66,9 +66,9 @@ def test_missing_rotary_pointers_are_refused(lib):
     assert lib.lact_rotary_axes(None, P, P, P, P, P, P, None) == -1
 
 
-def _step(lib, c, q=P, q_bs=256, q_hs=64, heads=4, window=0, scale=0.1, o=P, counters=P, room=P, nbytes=1 << 30):
+def _step(lib, c, q=P, q_bs=256, q_hs=64, heads=4, window=0, scale=0.1, o=P, counters=P, room=P, nbytes=1 << 30, status=P):
     return lib.lact_paged_attention_step(C.byref(c), q, C.c_int64(q_bs), C.c_int64(q_hs), C.c_int64(heads), C.c_int64(window), C.c_float(scale), o, counters, room,
-                                         C.c_size_t(nbytes), None)
+                                         C.c_size_t(nbytes), status, None)
 
 
 def _write(lib, c, k=P, v=P, strides=(128, 640, 64, 128, 640, 64), batch=2, tokens=5, cu=None):
@@ -84,7 +84,8 @@ def _read(lib, c, out=P, batch=2, tokens=5, cu=None):
     (dict(k=None), -1), (dict(v=None), -1), (dict(page_table=None), -1), (dict(lengths=None), -1), (dict(k_exponent=4096), -5), (dict(head_dim=96), -2),
     (dict(page_size=8), -2), (dict(page_size=24), -2), (dict(page_size=512), -2), (dict(pages=0), -2), (dict(pages=1 << 31), -2), (dict(kv_heads=0), -2),
     (dict(sequences=0), -2), (dict(table_cols=0), -2), (dict(table_cols=(1 << 26) + 1), -2), (dict(k=4112), -2), (dict(k_page_stride=2047), -2),
-    (dict(v_page_stride=2056), -2), (dict(k_exponent=1, v_exponent=1, ke_page_stride=31), -2)])
+    (dict(v_page_stride=2056), -2), (dict(k_exponent=4096, v_exponent=4096, ke_page_stride=31), -2),
+    (dict(k_exponent=4096, v_exponent=4100), -2), (dict(k_exponent=4096, v_exponent=4096, ve_page_stride=40), -2)])
 def test_bad_caches_are_refused(lib, over, code):
     c = _cache(**over)
     n, w = C.c_size_t(0), C.c_int64(0)
@@ -100,7 +101,7 @@ def test_bad_calls_on_a_cache_are_refused(lib):
     rc, nbytes, words = size(c=_cache(table_cols=4096))
     assert rc == 0 and nbytes > 0 and 0 < words <= 1024
     assert size(heads=3)[0] == -2 and size(heads=0)[0] == -2 and size(window=-1)[0] == -2
-    for over, code in [(dict(q=None), -1), (dict(o=None), -1), (dict(q=C.c_void_p(4104)), -2), (dict(q_bs=257), -2), (dict(q_hs=68), -2), (dict(heads=5), -2),
+    for over, code in [(dict(q=None), -1), (dict(o=None), -1), (dict(status=None), -1), (dict(o=C.c_void_p(4104)), -2), (dict(q=C.c_void_p(4104)), -2), (dict(q_bs=257), -2), (dict(q_hs=68), -2), (dict(heads=5), -2),
                        (dict(scale=float("nan")), -5), (dict(scale=float("inf")), -5)]:
         assert _step(lib, c, **over) == code
     for over in (dict(counters=None), dict(room=None), dict(nbytes=nbytes - 1), dict(room=C.c_void_p(4100))):
