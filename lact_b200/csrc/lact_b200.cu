@@ -2445,27 +2445,39 @@ int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t
 
 // How a call's tiles are dealt out.
 struct PagedStepPlan {
-  int nq, blocks, runs, stages;
+  int nq, blocks, runs, cluster, stages, long_stages;
   size_t bytes, smem;
 };
-constexpr int kPagedWarps = 4, kPagedPerSm = 2;
-constexpr int kPagedLeast = 2;   // tiles of a run at least
-constexpr int kPagedWhole = 4;   // tiles of a unit up to which a CTA takes a unit
+constexpr int kPagedWarps = 4;
+constexpr int kPagedLeast = 2;      // tiles of a run at least
+constexpr int kPagedWhole = 4;      // tiles of a unit up to which one CTA takes a unit, however many there are
+constexpr int kPagedClustered = 8;  // tiles of a CTA of a cluster at most
 int paged_step_plan(const lact_paged_cache* c, int64_t heads, int64_t window, PagedStepPlan* p) {
   if (heads < 1 || heads > 65535 || heads % c->kv_heads != 0 || window < 0) return LACT_ERR_SHAPE;
-  const int64_t share = heads / c->kv_heads, tile = 16 * kPagedWarps;
+  const int64_t row_bytes = c->head_dim * (c->k_exponent != nullptr ? 1 : 2), step = 16 * kPagedSub(static_cast<int>(row_bytes));
+  const int64_t share = heads / c->kv_heads, tile = step * kPagedWarps;
   p->nq = share > 8 ? 2 : 1;
   p->blocks = ceil_div(share, 8 * p->nq);
   const int64_t units = c->sequences * c->kv_heads * p->blocks, room = c->table_cols * c->page_size;
-  const int64_t most = (std::min(window > 0 ? window + 15 : room, room) + tile - 1) / tile;   // of a unit
+  const int64_t most = (std::min(window > 0 ? window + step - 1 : room, room) + tile - 1) / tile;   // of a unit
   if (units > 0x7FFFFFFF) return LACT_ERR_SHAPE;
+  const int per_sm = p->nq == 1 ? 3 : 2;   // (by the kernel's registers)
+  const int64_t ctas = static_cast<int64_t>(sm_count()) * per_sm;
+  p->runs = 0;
+  p->cluster = 1;
+  while (p->cluster < 8 && p->cluster < most && 2 * p->cluster * units <= ctas) p->cluster *= 2;
+  if (most > (p->cluster > 1 ? kPagedClustered * p->cluster : kPagedWhole)) {
+    p->cluster = 1;
+    p->runs = static_cast<int>(std::min(ctas, (units * most + kPagedLeast - 1) / kPagedLeast));
+  }
   const int64_t rows = std::min<int64_t>(share, 8 * p->nq), sums = rows * kPagedPieceRow(static_cast<int>(c->head_dim)) * 4;
-  p->runs = most <= kPagedWhole ? 0 : static_cast<int>(std::min<int64_t>(sm_count() * kPagedPerSm, (units * most + kPagedLeast - 1) / kPagedLeast));
   p->bytes = static_cast<size_t>(p->runs) * 2 * sums;
-  const int64_t stage = 32 * c->head_dim * (c->k_exponent != nullptr ? 1 : 2) + (c->k_exponent != nullptr ? 32 : 0);
-  // (the sums of a row hold the factors of all of a unit's pieces later on; 3 KB: alignment, and what the kernel has beside)
-  const int64_t room_cta = 227 * 1024 / kPagedPerSm - 3072, at_end = std::max<int64_t>(kPagedWarps * sums, rows * p->runs * 4);
+  const int64_t stage = 2 * step * (row_bytes + (c->k_exponent != nullptr ? 1 : 0));
+  // (the sums of a row hold the factors of all of a unit's pieces later on, a cluster's CTAs have their own added up; 3 KB: alignment,
+  // and what the kernel has beside)
+  const int64_t room_cta = 227 * 1024 / per_sm - 3072, at_end = std::max<int64_t>((kPagedWarps + (p->cluster > 1 ? 1 : 0)) * sums, rows * p->runs * 4);
   p->stages = static_cast<int>(std::min<int64_t>(kPagedStages, (room_cta - at_end) / (kPagedWarps * stage)));
+  p->long_stages = std::min<int>(p->stages, static_cast<int>(std::max<int64_t>(1, 8192 / stage)));
   p->smem = static_cast<size_t>(kPagedWarps * p->stages * stage + at_end) + 1024;
   return LACT_OK;
 }
@@ -2475,12 +2487,32 @@ int launch_paged_step(const lact_paged_cache* c, const PagedStepArgs& a, size_t 
   CUtensorMap k_map, v_map;
   constexpr int64_t cols = E4 ? D / 2 : D;   // of 16 bits
   const int64_t rows = c->kv_heads * c->page_size;
-  LACT_TRY(encode_map(&k_map, {c->k, rows, cols, cols, c->pages, a.c.k_ps / 2}, 16, cols < 64 ? 32 : 64));
-  LACT_TRY(encode_map(&v_map, {c->v, rows, cols, cols, c->pages, a.c.v_ps / 2}, 16, cols < 64 ? 32 : 64));
+  const uint32_t box = static_cast<uint32_t>(std::min<int64_t>(c->page_size, 16 * kPagedSub(2 * cols)));
+  LACT_TRY(encode_map(&k_map, {c->k, rows, cols, cols, c->pages, a.c.k_ps / 2}, box, cols < 64 ? 32 : 64));
+  LACT_TRY(encode_map(&v_map, {c->v, rows, cols, cols, c->pages, a.c.v_ps / 2}, box, cols < 64 ? 32 : 64));
   LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  const int64_t grid = a.runs > 0 ? a.runs : static_cast<int64_t>(a.c.sequences) * a.c.heads * a.blocks;
+  const int64_t grid = a.runs > 0 ? a.runs : static_cast<int64_t>(a.c.sequences) * a.c.heads * a.blocks * a.cluster;
+  if (grid > 0x7FFFFFFF) return LACT_ERR_SHAPE;
   KernelScope scope(kClsOther, st);
-  LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kPagedWarps * 32), smem, st, a, k_map, v_map));
+  if (a.cluster == 1) {
+    LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kPagedWarps * 32), smem, st, a, k_map, v_map));
+    return LACT_OK;
+  }
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kPagedWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(a.cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  LACT_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, k_map, v_map));
   return LACT_OK;
 }
 
@@ -3707,7 +3739,8 @@ int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t 
   a.counters = static_cast<uint32_t*>(counters);
   a.pieces = static_cast<float*>(workspace);
   a.status = status_word;
-  a.stages = p.stages;
+  a.stages = p.stages; a.long_stages = p.long_stages;
+  a.cluster = p.cluster;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int form = (c->head_dim == 128 ? 4 : 0) + (c->k_exponent != nullptr ? 2 : 0) + p.nq - 1;
   switch (form) {

@@ -14,13 +14,15 @@
 // Work: a unit is a (sequence, kv head, block of query heads), its tokens tiles of 16 a warp; lengths are known on the device alone.
 // All units' tiles, in order, are dealt out in even runs, one for each CTA, whatever the lengths are.  A run that holds all of a unit
 // writes its result; of a unit cut among runs each leaves a piece (sums, maxima), and the run that comes last adds the pieces in their
-// order.  Where a unit has few tiles at most (`runs` 0), each CTA takes one unit.
+// order.  Where units are few and have few tiles at most, or have very few (`runs` 0), a unit is a cluster of CTAs that share its tiles
+// evenly and read one another's sums from shared memory: no pieces, no counters.
 #pragma once
 #include "paged_cache.cuh"
 
 namespace lact {
 
 constexpr int kPagedStages = 8;   // at most
+constexpr int kPagedLong = 8;
 struct PagedStepArgs {
   PagedCache c;
   const bf16* q;                   // [sequences][heads][D], features adjacent, other strides in elements
@@ -30,10 +32,11 @@ struct PagedStepArgs {
   int32_t window;                  // 0: all
   float scale;                     // softmax scale * log2(e)
   int32_t runs, least;             // CTAs that share the tiles; tiles of a run at least
+  int32_t cluster;                 // runs 0: CTAs of a unit (1, 2, 4 or 8)
   uint32_t* counters;              // [runs], zero before and after
   float* pieces;                   // [runs][2][min(share, rows of a block)][D + 4]
   int32_t* status;
-  int32_t stages;                  // steps of 16 tokens that a warp has on their way or in work
+  int32_t stages, long_stages;     // steps that a warp has on their way or in work; the same in runs of more tiles than kPagedLong
 };
 
 __device__ __forceinline__ void mma_16x8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool halves) {
@@ -57,7 +60,7 @@ struct PagedSpan {
   int first, last;   // positions [first, last)
   int tiles;
 };
-template <int TILE>
+template <int STEP, int TILE>
 __device__ __forceinline__ PagedSpan paged_span(const PagedStepArgs& a, int seq) {
   PagedSpan s;
   const int64_t room = static_cast<int64_t>(a.c.cols) << a.c.shift;
@@ -65,19 +68,19 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedStepArgs& a, int seq)
   s.last = static_cast<int>(min(static_cast<int64_t>(len), room));
   s.first = a.window > 0 ? max(len - a.window, 0) : 0;
   s.first = min(s.first, s.last);
-  s.tiles = max((s.last - (s.first & ~15) + TILE - 1) / TILE, 1);
+  s.tiles = max((s.last - (s.first & ~(STEP - 1)) + TILE - 1) / TILE, 1);
   return s;
 }
 
 constexpr float kLowest = -3.402823466e38f;
 __host__ __device__ constexpr int kPagedPieceRow(int D) { return D + 4; }   // sums, then m, l, M
 
-// 2^4 bytes of exponents: an untiled copy (both addresses on 16 bytes)
-__device__ __forceinline__ void bulk_load_16_if(uint32_t leader, uint32_t smem_dst, const void* from, uint32_t bar) {
+// An untiled copy (both addresses on 16 bytes, a multiple of 16 bytes)
+__device__ __forceinline__ void bulk_load_if(uint32_t leader, uint32_t smem_dst, const void* from, uint32_t bytes, uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\t"
-      "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];\n\t}" ::"r"(smem_dst),
-      "l"(reinterpret_cast<uint64_t>(from)), "r"(bar), "r"(leader)
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+      "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(smem_dst),
+      "l"(reinterpret_cast<uint64_t>(from)), "r"(bytes), "r"(bar), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared_16(uint32_t at) {
@@ -98,32 +101,104 @@ struct PagedWalk {
   const int32_t* table;
 };
 
+__device__ __forceinline__ float4 ld_cluster_16(uint32_t at, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 p;\n\tmapa.shared::cluster.u32 p, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [p];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(at), "r"(rank)
+      : "memory");
+  return v;
+}
+// The sums of a cluster's CTAs, W of each in `sums`, as the unit's result.
+template <int D, int W, int ROW>
+__device__ __forceinline__ void paged_join_cluster(const PagedStepArgs& a, float* sums, int sum_rows, int rows, bool any, bf16* o) {
+  constexpr int THREADS = W * 32;
+  float* const mine = sums + W * sum_rows * ROW;
+  for (int i = threadIdx.x; i < rows * (D / 4 + 1); i += THREADS) {
+    const int row = i / (D / 4 + 1), d = i % (D / 4 + 1) * 4;
+    const float* const from = sums + row * ROW;
+    float tm = kLowest, tM = kLowest;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      tm = fmaxf(tm, from[w * sum_rows * ROW + D]);
+      tM = fmaxf(tM, from[w * sum_rows * ROW + D + 2]);
+    }
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float tl = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float* const f = from + w * sum_rows * ROW;
+      const float by = exp2_ftz(f[D + 2] - tM);
+      const float4 x = *reinterpret_cast<const float4*>(f + min(d, D - 4));
+      sum.x += x.x * by; sum.y += x.y * by; sum.z += x.z * by; sum.w += x.w * by;
+      tl += f[D + 1] * exp2_ftz(f[D] - tm);
+    }
+    *reinterpret_cast<float4*>(mine + row * ROW + d) = d < D ? sum : make_float4(tm, tl, tM, 0.f);
+  }
+  cluster_arrive();
+  cluster_wait();
+  const uint32_t at = smem_u32(mine);
+  for (int i = cluster_rank() * THREADS + threadIdx.x; i < rows * (D / 4); i += a.cluster * THREADS) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float4 s[8], x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      s[k] = make_float4(kLowest, 0.f, kLowest, 0.f);
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k >= a.cluster) continue;
+      s[k] = ld_cluster_16(at + (row * ROW + D) * 4, k);
+      x[k] = ld_cluster_16(at + (row * ROW + d) * 4, k);
+    }
+    float tm = kLowest, tM = kLowest, tl = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      tm = fmaxf(tm, s[k].x);
+      tM = fmaxf(tM, s[k].z);
+    }
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float by = exp2_ftz(s[k].z - tM);
+      sum.x += x[k].x * by; sum.y += x[k].y * by; sum.z += x[k].z * by; sum.w += x[k].w * by;
+      tl += s[k].y * exp2_ftz(s[k].x - tm);
+    }
+    const float f = any ? exp2_ftz(tM - tm) / tl : 0.f;
+    *reinterpret_cast<uint2*>(o + row * D + d) = make_uint2(pack_bf16x2(sum.x * f, sum.y * f), pack_bf16x2(sum.z * f, sum.w * f));
+  }
+  cluster_arrive();   // (nobody leaves while its sums are read)
+  cluster_wait();
+}
+
+// 16 tokens of a step times this
+__host__ __device__ constexpr int kPagedSub(int row_bytes) { return row_bytes > 128 ? 1 : 2; }
+
 template <int D, bool E4, int NQ, int W>
-__global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constant__ PagedStepArgs a, const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(W * 32, NQ == 2 ? 2 : D == 64 ? 4 : 3) paged_step_kernel(const __grid_constant__ PagedStepArgs a, const __grid_constant__ CUtensorMap k_map,
                                                             const __grid_constant__ CUtensorMap v_map) {
-  constexpr int ROWS = 8 * NQ, TILE = 16 * W, ROW = kPagedPieceRow(D), THREADS = W * 32;
   constexpr int BYTES = E4 ? D : 2 * D;                  // of a row
+  constexpr int SUB = kPagedSub(BYTES), STEP = 16 * SUB; // tokens of a step: 8 KB where rows allow
+  constexpr int ROWS = 8 * NQ, TILE = STEP * W, ROW = kPagedPieceRow(D), THREADS = W * 32;
   constexpr int BOX = BYTES >= 128 ? 128 : 64;           // bytes of a row in a box of 16 rows; swizzled over as many
   constexpr int BOXES = BYTES / BOX;
-  constexpr int KB = 16 * BYTES, STAGE = 2 * KB;
+  constexpr int KB = STEP * BYTES, EB = E4 ? 2 * STEP : 0, STAGE = 2 * KB;
   constexpr int KW = BOX / 16;                           // words of a box's K row that a lane has
   constexpr int VW = BOX / 32;                           // words of a box's V row that a lane has
   constexpr int MT = D / 16;                             // products of 16 features
   constexpr int QW = D / 8;                              // words of a lane's queries: two a step of 16 features
-  extern __shared__ uint8_t smem_raw[];   // [W][stages] of K and V, [W][stages][32] exponents, sums [W][rows][ROW]
+  extern __shared__ uint8_t smem_raw[];   // [W][stages] of K and V, [W][stages] of exponents, sums [W][rows][ROW]
   __shared__ uint64_t full[W * kPagedStages];
   __shared__ int plan[4];
   __shared__ int64_t warp_sum[W];
   __shared__ uint32_t arrived, gave_up;
   __shared__ float scales[ROWS];
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int stages = a.stages;
   const uint32_t leader = elect_leader();
   uint8_t* const paged_smem = smem_raw + ((smem_u32(smem_raw) + 1023u & ~1023u) - smem_u32(smem_raw));
-  const uint32_t ring = smem_u32(paged_smem) + warp * stages * STAGE, exp_ring = smem_u32(paged_smem) + W * stages * STAGE + warp * stages * 32;
-  float* const sums = reinterpret_cast<float*>(paged_smem + W * stages * (STAGE + (E4 ? 32 : 0)));
+  const uint32_t ring = smem_u32(paged_smem) + warp * a.stages * STAGE, exp_ring = smem_u32(paged_smem) + W * a.stages * STAGE + warp * a.stages * EB;
+  float* const sums = reinterpret_cast<float*>(paged_smem + W * a.stages * (STAGE + EB));
   if (lane == 0)
-    for (int i = 0; i < stages; ++i) mbar_init(&full[warp * kPagedStages + i], 1);
+    for (int i = 0; i < a.stages; ++i) mbar_init(&full[warp * kPagedStages + i], 1);
   if (threadIdx.x == 0) gave_up = 0;
   fence_mbar_init();
   griddep_launch_dependents();
@@ -134,15 +209,17 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
   PagedWalk make;                                        // (the copies run ahead of the products)
   int64_t run0 = 0, per = 0;
   if (a.runs == 0) {
-    make.seq = blockIdx.x / units;
-    make.unit = blockIdx.x - make.seq * units;
-    make.t = 0;
-    make.left = paged_span<TILE>(a, make.seq).tiles;
+    const int u = blockIdx.x / a.cluster, rank = blockIdx.x - u * a.cluster;
+    make.seq = u / units;
+    make.unit = u - make.seq * units;
+    const int tiles = paged_span<STEP, TILE>(a, make.seq).tiles, each = (tiles + a.cluster - 1) / a.cluster;
+    make.t = min(rank * each, tiles);
+    make.left = min(each, tiles - make.t);
     __syncthreads();
   } else {
     const int chunk = (a.c.sequences + THREADS - 1) / THREADS, s0 = min(static_cast<int>(threadIdx.x) * chunk, a.c.sequences), s1 = min(s0 + chunk, a.c.sequences);
     int64_t mine = 0;
-    for (int s = s0; s < s1; ++s) mine += paged_span<TILE>(a, s).tiles;
+    for (int s = s0; s < s1; ++s) mine += paged_span<STEP, TILE>(a, s).tiles;
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -165,7 +242,7 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
     int64_t at = (upto - mine) * units;
     if (run0 >= at && run0 < upto * units) {
       for (int s = s0; s < s1; ++s) {
-        const int64_t n = paged_span<TILE>(a, s).tiles;
+        const int64_t n = paged_span<STEP, TILE>(a, s).tiles;
         if (run0 < at + n * units) {
           plan[0] = s;
           plan[1] = static_cast<int>((run0 - at) / n);
@@ -181,9 +258,9 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
     make.t = plan[2];
   }
   auto enter = [&](PagedWalk& w) {                       // seq, unit, t and left are set
-    const PagedSpan span = paged_span<TILE>(a, w.seq);
+    const PagedSpan span = paged_span<STEP, TILE>(a, w.seq);
     w.first = span.first; w.last = span.last; w.tiles = span.tiles;
-    w.base = span.first & ~15;
+    w.base = span.first & ~(STEP - 1);
     w.t1 = min(span.tiles, w.t + w.left);
     w.head = w.unit / a.blocks;
     w.table = a.c.table + w.seq * a.c.table_rs;
@@ -196,34 +273,60 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
       ++w.seq;
     }
   };
-  auto position = [&](const PagedWalk& w) { return w.base + (w.t * W + warp) * 16; };
-  // (a step of 16 tokens lies in one page; past the end none is looked up)
-  auto page_of = [&](const PagedWalk& w) { return position(w) < w.last ? w.table[position(w) >> a.c.shift] : -1; };
+  auto position = [&](const PagedWalk& w) { return w.base + (w.t * W + warp) * STEP; };
+  // A step lies in one page, or (pages of 16, steps of 32) in two; past the end none is looked up.
+  const bool split = SUB == 2 && a.c.shift == 4;
+  auto pages_of = [&](const PagedWalk& w, int (&pg)[SUB]) {
+    const int p = position(w), at = p >> a.c.shift;
+    pg[0] = p < w.last ? w.table[at] : -1;
+    if constexpr (SUB == 2) pg[1] = split && p + 16 < w.last ? w.table[at + 1] : -1;
+  };
   enter(make);
+  const int stages = make.left > kPagedLong ? a.long_stages : a.stages;
   PagedWalk use = make;
-  int make_from = make.t, page = page_of(make), make_slot = 0, use_slot = 0;
-  uint32_t has = 0, phase = 0;                           // slots that hold a step; parities of their next waits
-  // the copies of this warp's 16 tokens of the next tile
+  int make_from = make.t, page[SUB], make_slot = 0, use_slot = 0;
+  pages_of(make, page);
+  uint32_t has = 0, half = 0, phase = 0;                 // slots that hold a step, half of one; parities of their next waits
+  // the copies of this warp's tokens of the next tile
   auto issue = [&]() {
     if (make.left <= 0) return;
-    const int p = position(make);
-    bool real = p < make.last;
-    if (real && static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.c.pages)) {
-      if (lane == 0) report_bad_page();
-      real = false;
-    }
-    has = real ? has | 1u << make_slot : has & ~(1u << make_slot);
-    if (real) {
-      const int row = (make.head << a.c.shift) + (p & ((1 << a.c.shift) - 1));
-      const uint32_t bar = smem_u32(&full[warp * kPagedStages + make_slot]), to = ring + make_slot * STAGE;
-      mbar_expect_tx_if(leader, bar, STAGE + (E4 ? 32 : 0));
+    const int p = position(make), row = (make.head << a.c.shift) + (p & ((1 << a.c.shift) - 1));
+    const uint32_t bar = smem_u32(&full[warp * kPagedStages + make_slot]), to = ring + make_slot * STAGE, exps = exp_ring + make_slot * EB;
+    auto copy = [&](int pg, int at, int rows, uint32_t on) {
 #pragma unroll
-      for (int i = 0; i < BOXES; ++i) tma_load_3d_if(leader, to + i * 16 * BOX, &k_map, bar, i * 64, row, page);
+      for (int i = 0; i < BOXES; ++i) tma_load_3d_if(on, to + i * STEP * BOX + at * BOX, &k_map, bar, i * 64, row, pg);
 #pragma unroll
-      for (int i = 0; i < BOXES; ++i) tma_load_3d_if(leader, to + KB + i * 16 * BOX, &v_map, bar, i * 64, row, page);
+      for (int i = 0; i < BOXES; ++i) tma_load_3d_if(on, to + KB + i * STEP * BOX + at * BOX, &v_map, bar, i * 64, row, pg);
       if constexpr (E4) {
-        bulk_load_16_if(leader, exp_ring + make_slot * 32, a.c.ke + page * a.c.ke_ps + row, bar);
-        bulk_load_16_if(leader, exp_ring + make_slot * 32 + 16, a.c.ve + page * a.c.ve_ps + row, bar);
+        bulk_load_if(on, exps + at, a.c.ke + pg * a.c.ke_ps + row, rows, bar);
+        bulk_load_if(on, exps + STEP + at, a.c.ve + pg * a.c.ve_ps + row, rows, bar);
+      }
+    };
+    auto there = [&](int pg, int at) {
+      const bool real = p + at < make.last;
+      if (real && static_cast<uint32_t>(pg) >= static_cast<uint32_t>(a.c.pages)) {
+        if (lane == 0) report_bad_page();
+        return false;
+      }
+      return real;
+    };
+    const uint32_t bit = 1u << make_slot;
+    const bool first = there(page[0], 0);
+    if (!split) {
+      has = first ? has | bit : has & ~bit;
+      if (first) {
+        mbar_expect_tx_if(leader, bar, STAGE + EB);
+        copy(page[0], 0, STEP, leader);
+      }
+    } else {
+      // (a half that is not there is left as it was, and counts as outside of the window)
+      const bool second = there(page[SUB - 1], 16);
+      has = first || second ? has | bit : has & ~bit;
+      half = (half & ~(bit | bit << 16)) | (first ? 0 : bit) | (second ? 0 : bit << 16);
+      if (first || second) {
+        mbar_expect_tx_if(leader, bar, first && second ? STAGE + EB : (STAGE + EB) / 2);
+        if (first) copy(page[0], 0, 16, leader);
+        if (second) copy(page[SUB - 1], 16, 16, leader);
       }
     }
     if (++make_slot == stages) make_slot = 0;
@@ -232,12 +335,12 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
       make_from = 0;
       if (make.left > 0) enter(make);
     }
-    if (make.left > 0) page = page_of(make);
+    if (make.left > 0) pages_of(make, page);
   };
   for (int i = 0; i < stages; ++i) issue();
   bool failed = false;
   // -------- its units
-  for (int64_t done = 0; use.left > 0;) {
+  for (int64_t done = 0; use.left > 0 || a.cluster > 1;) {   // (of a cluster every CTA has one turn, with tiles or without)
     if (done > 0) enter(use);
     const int t0 = use.t, seq = use.seq, head = use.head, row0 = (use.unit - head * a.blocks) * ROWS, rows = min(a.share - row0, ROWS);
     if (threadIdx.x == 0 && a.c.lengths[seq] > use.last && use.t1 == use.tiles) report_bad_page();
@@ -283,7 +386,7 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
         qm[n][1] = __shfl_sync(0xFFFFFFFFu, down, c * 8 + 4);
       }
     }
-    // -------- tiles: this warp's 16 tokens of each
+    // -------- tiles: this warp's step of each
     float acc[NQ][MT][4], m[NQ][2], l[NQ][2];
     [[maybe_unused]] float M[NQ][2];
 #pragma unroll
@@ -315,109 +418,138 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
         continue;
       }
       const uint32_t ks = ring + slot * STAGE, vs = ks + KB;
-      float x[NQ][4];
+      float x[SUB][NQ][4];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
+      for (int u = 0; u < SUB; ++u) {
+        float z[NQ][4];                                  // (two chains of products)
 #pragma unroll
-      for (int i = 0; i < BOXES; ++i) {
-        uint32_t kr[2][KW];                              // rows r, r + 8: a lane's BOX / 4 bytes
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int e = 0; e < 4; ++e) x[u][n][e] = z[n][e] = 0.f;
 #pragma unroll
-          for (int e = 0; e < KW / 4; ++e) {
-            const int row = r + 8 * h;
-            const uint4 w = ld_shared_16(ks + i * 16 * BOX + row * BOX + ((c * (KW / 4) + e) ^ (BOX == 128 ? r : r >> 1 & 3)) * 16);
-            kr[h][4 * e] = w.x; kr[h][4 * e + 1] = w.y; kr[h][4 * e + 2] = w.z; kr[h][4 * e + 3] = w.w;
+        for (int i = 0; i < BOXES; ++i) {
+          uint32_t kr[2][KW];                            // rows r, r + 8: a lane's BOX / 4 bytes
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < KW / 4; ++e) {
+              const uint4 w = ld_shared_16(ks + i * STEP * BOX + (16 * u + r + 8 * h) * BOX + ((c * (KW / 4) + e) ^ (BOX == 128 ? r : r >> 1 & 3)) * 16);
+              kr[h][4 * e] = w.x; kr[h][4 * e + 1] = w.y; kr[h][4 * e + 2] = w.z; kr[h][4 * e + 3] = w.w;
+            }
+#pragma unroll
+          for (int e = 0; e < KW; e += E4 ? 1 : 2) {
+            uint32_t a0, a1, a2, a3;
+            if constexpr (E4) {
+              halves_of_e4m3(kr[0][e], a0, a2);
+              halves_of_e4m3(kr[1][e], a1, a3);
+            } else {
+              a0 = kr[0][e]; a1 = kr[1][e]; a2 = kr[0][e + 1]; a3 = kr[1][e + 1];
+            }
+            const int s = E4 ? 2 * e : i * KW + e;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) mma_16x8(s / 2 % 2 ? z[n] : x[u][n], a0, a1, a2, a3, q[n][s], q[n][s + 1], E4);
           }
-#pragma unroll
-        for (int e = 0; e < KW; e += E4 ? 1 : 2) {
-          uint32_t a0, a1, a2, a3;
-          if constexpr (E4) {
-            a0 = halves_of_e4m3(kr[0][e] & 0xFFFFu); a1 = halves_of_e4m3(kr[1][e] & 0xFFFFu);
-            a2 = halves_of_e4m3(kr[0][e] >> 16); a3 = halves_of_e4m3(kr[1][e] >> 16);
-          } else {
-            a0 = kr[0][e]; a1 = kr[1][e]; a2 = kr[0][e + 1]; a3 = kr[1][e + 1];
-          }
-          const int s = E4 ? 2 * e : i * KW + e;
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) mma_16x8(x[n], a0, a1, a2, a3, q[n][s], q[n][s + 1], E4);
         }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][n][e] = (x[u][n][e] + z[n][e]) * qm[n][e & 1];
       }
-      [[maybe_unused]] float kx[2], vx[2];
+      [[maybe_unused]] float y[SUB][NQ][4];
       if constexpr (E4) {
-        const uint8_t* const exps = paged_smem + (exp_ring - smem_u32(paged_smem)) + slot * 32;
+        const uint8_t* const exps = paged_smem + (exp_ring - smem_u32(paged_smem)) + slot * EB;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t kb = exps[r + 8 * h], vb = exps[16 + r + 8 * h];
-          kx[h] = exponent_value(kb);
-          vx[h] = vb == 255 ? __uint_as_float(0x7FC00000u) : static_cast<float>(static_cast<int>(vb) - 127);
-        }
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // 2^(byte - 127) and byte - 127, NaN for 255 (infinity times zero)
+            const uint32_t kb = exps[16 * u + r + 8 * h], vb = exps[STEP + 16 * u + r + 8 * h];
+            const float kx = fmaf(__uint_as_float(kb << 23), 0.f, __uint_as_float(kb << 23));
+            const float vx = fmaf(__uint_as_float(vb << 23), 0.f, __uint_as_float(0x4B000000u | vb) - 8388735.f);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+              for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                x[u][n][e] *= kx;
+                y[u][n][e] = x[u][n][e] + vx;
+              }
+          }
       }
       // a lane's features (8 bits: 16; else 8 of each box) of tokens 2 c, 2 c + 1 and those 8 later
-      uint32_t vr[4][BOXES * VW];
+      uint32_t vr[SUB][4][BOXES * VW];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = 2 * c + (i & 1) + 8 * (i >> 1);
-#pragma unroll
-        for (int b = 0; b < BOXES; ++b) {
-          if constexpr (VW == 4) {
-            const uint4 w = ld_shared_16(vs + b * 16 * BOX + tok * BOX + (r ^ (tok & 7)) * 16);
-            vr[i][b * 4] = w.x; vr[i][b * 4 + 1] = w.y; vr[i][b * 4 + 2] = w.z; vr[i][b * 4 + 3] = w.w;
-          } else {
-            const uint2 w = ld_shared_8(vs + tok * BOX + ((r >> 1) ^ (tok >> 1 & 3)) * 16 + (r & 1) * 8);
-            vr[i][0] = w.x; vr[i][1] = w.y;
-          }
-        }
-      }
-      // tokens outside of the window: no weight, and no values (what lies there may be NaN)
-      const bool whole_step = p >= use.first && p + 16 <= use.last;
-      bool on[2] = {true, true};
-      if (!whole_step) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) on[h] = p + r + 8 * h >= use.first && p + r + 8 * h < use.last;
+      for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tok = 2 * c + (i & 1) + 8 * (i >> 1);
-          if (p + tok >= use.first && p + tok < use.last) continue;
 #pragma unroll
-          for (int e = 0; e < BOXES * VW; ++e) vr[i][e] = 0;
+          for (int b = 0; b < BOXES; ++b) {
+            if constexpr (VW == 4) {
+              const uint4 w = ld_shared_16(vs + b * STEP * BOX + (16 * u + tok) * BOX + (r ^ (tok & 7)) * 16);
+              vr[u][i][b * 4] = w.x; vr[u][i][b * 4 + 1] = w.y; vr[u][i][b * 4 + 2] = w.z; vr[u][i][b * 4 + 3] = w.w;
+            } else {
+              const uint2 w = ld_shared_8(vs + (16 * u + tok) * BOX + ((r >> 1) ^ (tok >> 1 & 3)) * 16 + (r & 1) * 8);
+              vr[u][i][0] = w.x; vr[u][i][1] = w.y;
+            }
+          }
+        }
+      // tokens outside of the window: no weight, and no values (what lies there may be NaN)
+      if (p < use.first || p + STEP > use.last || (half >> slot & 0x10001u) != 0) {
+        const bool gone[2] = {(half >> slot & 1) != 0, (half >> slot >> 16 & 1) != 0};
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int at = p + 16 * u + r + 8 * h;
+            if (!gone[u] && at >= use.first && at < use.last) continue;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+              for (int e = 2 * h; e < 2 * h + 2; ++e) x[u][n][e] = y[u][n][e] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = p + 16 * u + 2 * c + (i & 1) + 8 * (i >> 1);
+            if (!gone[u] && at >= use.first && at < use.last) continue;
+#pragma unroll
+            for (int e = 0; e < BOXES * VW; ++e) vr[u][i][e] = 0;
+          }
         }
       }
       __syncwarp();
       issue();                                           // (all of the slot is in registers)
-      // scores; the maxima, where one passes them by 8
+      // the maxima, where a score passes them by 8
+      float top[NQ][2], high[NQ][2];
       bool raise = false;
-      [[maybe_unused]] float y[NQ][4];
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[n][e] *= qm[n][e & 1];
-          if constexpr (E4) x[n][e] *= kx[e >> 1];
-          if (!on[e >> 1]) x[n][e] = -INFINITY;
-          raise = raise || x[n][e] > m[n][e & 1] + 8.f;
-          if constexpr (E4) {
-            y[n][e] = on[e >> 1] ? x[n][e] + vx[e >> 1] : -INFINITY;
-            raise = raise || y[n][e] > M[n][e & 1] + 8.f;
+        for (int e = 0; e < 2; ++e) {
+          top[n][e] = fmaxf(x[0][n][e], x[0][n][e + 2]);
+          if constexpr (E4) high[n][e] = fmaxf(y[0][n][e], y[0][n][e + 2]);
+          if constexpr (SUB == 2) {
+            top[n][e] = fmaxf(top[n][e], fmaxf(x[1][n][e], x[1][n][e + 2]));
+            if constexpr (E4) high[n][e] = fmaxf(high[n][e], fmaxf(y[1][n][e], y[1][n][e + 2]));
           }
+          raise = raise || top[n][e] > m[n][e] + 8.f;
+          if constexpr (E4) raise = raise || high[n][e] > M[n][e] + 8.f;
         }
       if (__any_sync(0xFFFFFFFFu, raise)) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            auto top = [&](float old, float u, float v) {
-              float z = fmaxf(u, v);
+            auto over_rows = [&](float old, float z) {
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) z = fmaxf(z, __shfl_xor_sync(0xFFFFFFFFu, z, o));
               return fmaxf(old, z);
             };
-            const float now = top(m[n][e], x[n][e], x[n][e + 2]);
+            const float now = over_rows(m[n][e], top[n][e]);
             float f = exp2_ftz(m[n][e] - now);
             l[n][e] *= f;
             m[n][e] = now;
             if constexpr (E4) {
-              const float big = top(M[n][e], y[n][e], y[n][e + 2]);
+              const float big = over_rows(M[n][e], high[n][e]);
               f = exp2_ftz(M[n][e] - big);
               M[n][e] = big;
             }
@@ -428,52 +560,56 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
             }
           }
       }
-      // weights, turned over so that their tokens are the inner axis
-      uint32_t hi[NQ][2];
-      [[maybe_unused]] uint32_t lo[NQ][2];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float w[4];
+      for (int u = 0; u < SUB; ++u) {
+        // weights, turned over so that their tokens are the inner axis
+        uint32_t hi[NQ][2];
+        [[maybe_unused]] uint32_t lo[NQ][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = exp2_ftz(x[n][e] - m[n][e & 1]);
-          l[n][e & 1] += w[e];
-          if constexpr (E4) w[e] = exp2_ftz(y[n][e] - M[n][e & 1]);
-        }
+        for (int n = 0; n < NQ; ++n) {
+          float w[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if constexpr (E4) {
-            const __half2 two = __floats2half2_rn(w[2 * h], w[2 * h + 1]);
-            hi[n][h] = transposed_8x8(*reinterpret_cast<const uint32_t*>(&two));
-          } else {
-            const uint32_t two = pack_bf16x2(w[2 * h], w[2 * h + 1]);
-            lo[n][h] = transposed_8x8(pack_bf16x2(w[2 * h] - __uint_as_float(two << 16), w[2 * h + 1] - __uint_as_float(two & 0xFFFF0000u)));
-            hi[n][h] = transposed_8x8(two);
+          for (int e = 0; e < 4; ++e) {
+            w[e] = exp2_ftz(x[u][n][e] - m[n][e & 1]);
+            l[n][e & 1] += w[e];
+            if constexpr (E4) w[e] = exp2_ftz(y[u][n][e] - M[n][e & 1]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if constexpr (E4) {
+              const __half2 two = __floats2half2_rn(w[2 * h], w[2 * h + 1]);
+              hi[n][h] = transposed_8x8(*reinterpret_cast<const uint32_t*>(&two));
+            } else {
+              const uint32_t two = pack_bf16x2(w[2 * h], w[2 * h + 1]);
+              lo[n][h] = transposed_8x8(pack_bf16x2(w[2 * h] - __uint_as_float(two << 16), w[2 * h + 1] - __uint_as_float(two & 0xFFFF0000u)));
+              hi[n][h] = transposed_8x8(two);
+            }
           }
         }
-      }
-      if constexpr (E4) {
+        if constexpr (E4) {
 #pragma unroll
-        for (int j = 0; j < MT; j += 2) {
-          const uint32_t t01 = __byte_perm(vr[0][j / 2], vr[1][j / 2], 0x5140), u01 = __byte_perm(vr[0][j / 2], vr[1][j / 2], 0x7362);
-          const uint32_t t23 = __byte_perm(vr[2][j / 2], vr[3][j / 2], 0x5140), u23 = __byte_perm(vr[2][j / 2], vr[3][j / 2], 0x7362);
-          const uint32_t a0 = halves_of_e4m3(t01 & 0xFFFFu), a1 = halves_of_e4m3(t01 >> 16), a2 = halves_of_e4m3(t23 & 0xFFFFu), a3 = halves_of_e4m3(t23 >> 16);
-          const uint32_t b0 = halves_of_e4m3(u01 & 0xFFFFu), b1 = halves_of_e4m3(u01 >> 16), b2 = halves_of_e4m3(u23 & 0xFFFFu), b3 = halves_of_e4m3(u23 >> 16);
+          for (int j = 0; j < MT; j += 2) {
+            uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+            halves_of_e4m3(__byte_perm(vr[u][0][j / 2], vr[u][1][j / 2], 0x5140), a0, a1);
+            halves_of_e4m3(__byte_perm(vr[u][2][j / 2], vr[u][3][j / 2], 0x5140), a2, a3);
+            halves_of_e4m3(__byte_perm(vr[u][0][j / 2], vr[u][1][j / 2], 0x7362), b0, b1);
+            halves_of_e4m3(__byte_perm(vr[u][2][j / 2], vr[u][3][j / 2], 0x7362), b2, b3);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-            mma_16x8(acc[n][j], a0, a1, a2, a3, hi[n][0], hi[n][1], true);
-            mma_16x8(acc[n][j + 1], b0, b1, b2, b3, hi[n][0], hi[n][1], true);
+            for (int n = 0; n < NQ; ++n) {
+              mma_16x8(acc[n][j], a0, a1, a2, a3, hi[n][0], hi[n][1], true);
+              mma_16x8(acc[n][j + 1], b0, b1, b2, b3, hi[n][0], hi[n][1], true);
+            }
           }
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const uint32_t a0 = __byte_perm(vr[0][j], vr[1][j], 0x5410), a1 = __byte_perm(vr[0][j], vr[1][j], 0x7632);
-          const uint32_t a2 = __byte_perm(vr[2][j], vr[3][j], 0x5410), a3 = __byte_perm(vr[2][j], vr[3][j], 0x7632);
+          for (int j = 0; j < MT; ++j) {
+            const uint32_t a0 = __byte_perm(vr[u][0][j], vr[u][1][j], 0x5410), a1 = __byte_perm(vr[u][0][j], vr[u][1][j], 0x7632);
+            const uint32_t a2 = __byte_perm(vr[u][2][j], vr[u][3][j], 0x5410), a3 = __byte_perm(vr[u][2][j], vr[u][3][j], 0x7632);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-            mma_16x8(acc[n][j], a0, a1, a2, a3, hi[n][0], hi[n][1], false);
-            mma_16x8(acc[n][j], a0, a1, a2, a3, lo[n][0], lo[n][1], false);
+            for (int n = 0; n < NQ; ++n) {
+              mma_16x8(acc[n][j], a0, a1, a2, a3, hi[n][0], hi[n][1], false);
+              mma_16x8(acc[n][j], a0, a1, a2, a3, lo[n][0], lo[n][1], false);
+            }
           }
         }
       }
@@ -496,6 +632,10 @@ __global__ void __launch_bounds__(W * 32) paged_step_kernel(const __grid_constan
         if (r == 0) *reinterpret_cast<float4*>(to + D) = make_float4(m[n][e], l[n][e], E4 ? M[n][e] : m[n][e], 0.f);
       }
     __syncthreads();
+    if (a.cluster > 1) {
+      paged_join_cluster<D, W, ROW>(a, sums, sum_rows, rows, use.last > use.first, a.o + (static_cast<int64_t>(seq) * a.heads + static_cast<int64_t>(head) * a.share + row0) * D);
+      return;
+    }
     const bool whole = use.t1 == use.tiles && t0 == 0;
     const int64_t begin = run0 + done - t0;              // the unit's first tile among all
     auto piece_of = [&](int64_t run, bool first) { return a.pieces + (run * 2 + (first ? 1 : 0)) * sum_rows * ROW; };

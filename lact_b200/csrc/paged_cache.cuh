@@ -46,11 +46,9 @@ __device__ __forceinline__ uint32_t exponent_byte(uint32_t top) {
   if (e == 255) return 255;
   return static_cast<uint32_t>(min(max(e - 8 + ((top & 0x7F) > 0x60 ? 1 : 0), 1), 246));
 }
-// Two e4m3 values (low byte first) as two halves, exactly
-__device__ __forceinline__ uint32_t halves_of_e4m3(uint32_t two) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two)));
-  return r;
+// Four e4m3 values as halves, exactly: the lower two and the upper two of a word
+__device__ __forceinline__ void halves_of_e4m3(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 // Two values in e4m3 (low byte: the first)
 __device__ __forceinline__ uint32_t e4m3_of(float lo, float hi) {
@@ -189,10 +187,14 @@ __global__ void __launch_bounds__(kPagedThreads) paged_rows_kernel(const __grid_
           const uint32_t w[2] = {raw[i].x, raw[i].y};
           uint32_t o[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t two = halves_of_e4m3(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
-            o[e] = pack_bf16x2(f.x * by, f.y * by);
+          for (int e = 0; e < 2; ++e) {
+            uint32_t two[2];
+            halves_of_e4m3(w[e], two[0], two[1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two[h]));
+              o[2 * e + h] = pack_bf16x2(f.x * by, f.y * by);
+            }
           }
           raw[i] = make_uint4(o[0], o[1], o[2], o[3]);
         }
