@@ -2352,18 +2352,19 @@ int norm_args(const lact_group_norm_config* c, const NormPlan& p, const void* x,
 // ------------------------------------------------------------------------------------------ rotary positions
 template <class T, int V>
 int launch_rotary(RotaryArgs a, bool halves, cudaStream_t st) {
-  // as many thread groups a token as give four blocks a SM, for each of which it has a head; the angles of a token are worked out once
+  // Thread groups that share a token: as many as leave each six heads (two turns of three: 65536 tokens of 24 heads of 128 in bf16 with
+  // 1, 2, 4 and 8 groups 137, 129, 125 and 135 us), more where there would be fewer than four blocks a SM, for each of which it has a head.
   const int64_t groups = kRotaryThreads / (a.d / (2 * V)), heads = a.heads[0] + a.heads[1];
   int64_t share = 1;
-  while (2 * share <= std::min(groups, heads) && a.tokens * share < groups * 4 * sm_count()) share *= 2;
+  while (2 * share <= std::min(groups, heads) && (heads >= 12 * share || a.tokens * share < groups * 4 * sm_count())) share *= 2;
   a.share = static_cast<int32_t>(share);
   a.per_block = static_cast<int32_t>(groups / share);
   const int64_t grid = (a.tokens + a.per_block - 1) / a.per_block;
   if (grid > 0x7FFFFFFF) return LACT_ERR_SHAPE;
   const size_t smem = static_cast<size_t>(a.per_block) * a.P * sizeof(float2);
   KernelScope scope(kClsOther, st);
-  if (halves) LACT_CUDA(launch_pdl(rotary_kernel<T, V, true>, dim3(static_cast<unsigned>(grid)), dim3(kRotaryThreads), smem, st, a));
-  else LACT_CUDA(launch_pdl(rotary_kernel<T, V, false>, dim3(static_cast<unsigned>(grid)), dim3(kRotaryThreads), smem, st, a));
+  if (halves) LACT_CUDA(launch_pdl(rotary_kernel<T, V, true, 3, 4>, dim3(static_cast<unsigned>(grid)), dim3(kRotaryThreads), smem, st, a));
+  else LACT_CUDA(launch_pdl(rotary_kernel<T, V, false, 3, 4>, dim3(static_cast<unsigned>(grid)), dim3(kRotaryThreads), smem, st, a));
   return LACT_OK;
 }
 int rotary_check(const lact_rotary_config* c) {
@@ -2419,7 +2420,7 @@ PagedCache paged_args(const lact_paged_cache* c) {
 template <int D, bool E4>
 int launch_paged_rows(const PagedRows& a, bool write, int64_t grid, cudaStream_t st) {
   KernelScope scope(kClsOther, st);
-  const dim3 blocks(static_cast<unsigned>(grid), 2);
+  const dim3 blocks(static_cast<unsigned>(grid));
   if (write) LACT_CUDA(launch_pdl(paged_rows_kernel<D, E4, true>, blocks, dim3(kPagedThreads), 0, st, a));
   else LACT_CUDA(launch_pdl(paged_rows_kernel<D, E4, false>, blocks, dim3(kPagedThreads), 0, st, a));
   return LACT_OK;
@@ -2431,11 +2432,12 @@ int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t
   a.cu = cu;
   a.tokens = entries * tokens;
   a.L = static_cast<int32_t>(tokens);
-  // tokens of a block: four blocks a SM, and at most four turns of four rows a thread
-  const int64_t rows_at_once = kPagedThreads / (c->head_dim / 8) * kPagedAhead;
-  int64_t n = 1;
-  while (2 * n <= kPagedTokens && 2 * n * c->kv_heads <= 4 * rows_at_once && a.tokens >= 2 * n * 2 * sm_count()) n *= 2;
-  a.per_block = static_cast<int32_t>(n);
+  // as many thread groups a token as leave each four heads at most, and more where the call is small
+  const int64_t groups = kPagedThreads / (c->head_dim / 8);
+  int64_t share = 1;
+  while (2 * share <= groups && (share * kPagedAhead < c->kv_heads || (share < c->kv_heads && a.tokens * share < groups * 2 * sm_count()))) share *= 2;
+  a.share = static_cast<int32_t>(share);
+  const int64_t n = groups / share;
   const int64_t grid = (a.tokens + n - 1) / n;
   if (grid > 0x7FFFFFFF) return LACT_ERR_SHAPE;
   const bool e4 = c->k_exponent != nullptr;
@@ -3650,11 +3652,11 @@ int lact_rotary_axes(const lact_rotary_config* c, const void* q, const void* k, 
   a.freq = frequencies;
   a.tokens = c->batch * c->tokens; a.L = static_cast<int32_t>(c->tokens); a.d = static_cast<int32_t>(c->head_dim); a.P = a.ends[c->axes - 1];
   a.sign = c->backwards ? -1.f : 1.f;
-  // whole accesses of up to 16 bytes: as many features as divide the pairs, half a head, the strides and the bases
+  // whole accesses of up to 16 bytes: as many features as divide what is turned, half a head, the strides and the bases
   const int size = c->dtype == LACT_F32 ? 4 : 2;
   int v = 16 / size;
   auto fits = [&](int n) {
-    if (a.P % n != 0 || a.d % (2 * n) != 0 || 256 / (a.d / (2 * n)) < 1) return false;
+    if ((c->interleaved != 0 && n > 1 ? 2 * a.P : a.P) % n != 0 || a.d % (2 * n) != 0 || kRotaryThreads / (a.d / (2 * n)) < 1) return false;
     for (int i = 0; i < (c->k_heads > 0 ? 2 : 1); ++i) {
       for (int64_t s : {c->batch > 1 ? a.bs[i] : 0, c->tokens > 1 ? a.ts[i] : 0, a.heads[i] > 1 ? a.hs[i] : 0})
         if (s % n != 0) return false;

@@ -64,7 +64,7 @@ struct PagedRows {
   bf16* out;                       // read: [2][entries][tokens][heads][D]
   const int32_t* cu;               // packed: [sequences + 1] bounds within the one entry
   int64_t tokens;                  // of all entries
-  int32_t L, per_block;            // of an entry; of a block
+  int32_t L, share;                // of an entry; thread groups that share a token's heads
 };
 
 // Where row `t` of the batch lies: its page (-1: nowhere) and row.
@@ -97,108 +97,113 @@ __device__ __forceinline__ int2 paged_place(const PagedRows& a, int64_t t) {
   return make_int2(page, static_cast<int>(pos & ((1 << a.c.shift) - 1)));
 }
 
-// Both directions are bound by memory.  A block finds the places of its tokens once; D / 8 threads hold a row of a head, 8 values each;
-// blockIdx.y says keys or values.  Four rows of a thread are fetched together.
-constexpr int kPagedThreads = 256, kPagedTokens = 64, kPagedAhead = 4;
+// Both directions are bound by memory.  D / 8 threads hold a row of a head, 8 values each; such a group takes one token, finds its place,
+// and goes through its share of the heads, keys and values of four at a time on their way together (writing, they are fetched before
+// the place is known).
+constexpr int kPagedThreads = 256, kPagedAhead = 4;
 template <int D, bool E4, bool WRITE>
 __global__ void __launch_bounds__(kPagedThreads) paged_rows_kernel(const __grid_constant__ PagedRows a) {
-  constexpr int LANES = D / 8, ROWS = kPagedThreads / LANES, N = kPagedAhead;
-  __shared__ int2 place[kPagedTokens];
+  constexpr int LANES = D / 8, GROUPS = kPagedThreads / LANES, N = kPagedAhead;
+  constexpr int BYTES = E4 ? 8 : 16;   // of the cache, a thread
   griddep_launch_dependents();
   griddep_wait();
-  const bool values = blockIdx.y != 0;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
-  const int here = static_cast<int>(min(static_cast<int64_t>(a.per_block), a.tokens - t0));
-  for (int i = threadIdx.x; i < here; i += kPagedThreads) place[i] = paged_place(a, t0 + i);
-  __syncthreads();
-  const int lane = threadIdx.x % LANES, rows = here * a.c.heads;
-  uint8_t* const pages = values ? a.c.v : a.c.k;
-  uint8_t* const exps = values ? a.c.ve : a.c.ke;
-  const int64_t ps = values ? a.c.v_ps : a.c.k_ps, eps = values ? a.c.ve_ps : a.c.ke_ps;
-  const bf16* const x = values ? a.xv : a.xk;
-  const int64_t bs = values ? a.v_bs : a.k_bs, ts = values ? a.v_ts : a.k_ts, hs = values ? a.v_hs : a.k_hs;
-  bf16* const out = a.out + (values ? a.tokens * a.c.heads * D : 0);
-  constexpr int BYTES = E4 ? 8 : 16;   // of the cache, a thread
-  // (every thread of a warp takes part in every turn: rows that are not there have no page)
-  for (int r0 = threadIdx.x / LANES; r0 - static_cast<int>(threadIdx.x / LANES) < rows; r0 += N * ROWS) {
-    uint4 raw[N];
-    [[maybe_unused]] uint32_t byte[N];
-    int2 at[N];
-    int64_t to[N];
-    int head[N], tok[N];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, tok = group / a.share, part = group - tok * a.share;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (GROUPS / a.share) + tok;
+  // (every thread of a warp takes part in every turn: tokens past the end have no place, and no heads)
+  const int heads = t < a.tokens ? a.c.heads : 0;
+  const int64_t b = t / a.L, l = t - b * a.L;
+  int2 at = make_int2(-1, 0);
+  for (int h0 = part; h0 - part < a.c.heads; h0 += N * a.share) {
+    uint4 raw[2][N];
+    [[maybe_unused]] uint32_t byte[2][N];
+    if constexpr (WRITE) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = r0 + i * ROWS;
-      tok[i] = r / a.c.heads;
-      head[i] = r - tok[i] * a.c.heads;
-      at[i] = r < rows ? place[tok[i]] : make_int2(-1, 0);
-      to[i] = (static_cast<int64_t>(head[i]) << a.c.shift) + at[i].y;   // row within the page
-      raw[i] = make_uint4(0, 0, 0, 0);
-      byte[i] = 127;
-      if (at[i].x < 0) continue;
-      if constexpr (WRITE) {
-        const int64_t t = t0 + tok[i], b = t / a.L;
-        raw[i] = *reinterpret_cast<const uint4*>(x + b * bs + (t - b * a.L) * ts + head[i] * hs + lane * 8);
-      } else {
-        const uint8_t* from = pages + at[i].x * ps + (to[i] * LANES + lane) * BYTES;
-        if constexpr (E4) {
-          const uint2 two = *reinterpret_cast<const uint2*>(from);
-          raw[i].x = two.x;
-          raw[i].y = two.y;
-          byte[i] = exps[at[i].x * eps + to[i]];
-        } else {
-          raw[i] = *reinterpret_cast<const uint4*>(from);
+      for (int i = 0; i < N; ++i) {
+        const int h = h0 + i * a.share;
+        raw[0][i] = raw[1][i] = make_uint4(0, 0, 0, 0);
+        if (h >= heads) continue;
+        raw[0][i] = *reinterpret_cast<const uint4*>(a.xk + b * a.k_bs + l * a.k_ts + h * a.k_hs + lane * 8);
+        raw[1][i] = *reinterpret_cast<const uint4*>(a.xv + b * a.v_bs + l * a.v_ts + h * a.v_hs + lane * 8);
+      }
+    }
+    if (h0 == part && heads > 0) at = paged_place(a, t);
+    const bool there = at.x >= 0;
+    if constexpr (!WRITE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int h = h0 + i * a.share;
+        raw[0][i] = raw[1][i] = make_uint4(0, 0, 0, 0);
+        byte[0][i] = byte[1][i] = 127;
+        if (h >= heads || !there) continue;
+        const int64_t row = (static_cast<int64_t>(h) << a.c.shift) + at.y;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const uint8_t* const from = (v ? a.c.v + at.x * a.c.v_ps : a.c.k + at.x * a.c.k_ps) + (row * LANES + lane) * BYTES;
+          if constexpr (E4) {
+            const uint2 two = *reinterpret_cast<const uint2*>(from);
+            raw[v][i].x = two.x;
+            raw[v][i].y = two.y;
+            byte[v][i] = v ? a.c.ve[at.x * a.c.ve_ps + row] : a.c.ke[at.x * a.c.ke_ps + row];
+          } else {
+            raw[v][i] = *reinterpret_cast<const uint4*>(from);
+          }
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if constexpr (WRITE) {
-        if constexpr (E4) {
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          uint32_t top = 0;
+      const int h = h0 + i * a.share;
+      const int64_t row = (static_cast<int64_t>(h) << a.c.shift) + at.y;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = __vmaxu2(top, w[e] & 0x7FFF7FFFu);
-          top = max(top & 0xFFFFu, top >> 16);
+      for (int v = 0; v < 2; ++v) {
+        if constexpr (WRITE) {
+          uint8_t* const to = (v ? a.c.v + at.x * a.c.v_ps : a.c.k + at.x * a.c.k_ps) + (row * LANES + lane) * BYTES;
+          if constexpr (E4) {
+            const uint32_t w[4] = {raw[v][i].x, raw[v][i].y, raw[v][i].z, raw[v][i].w};
+            uint32_t top = 0;
 #pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-          if (at[i].x < 0) continue;
-          const uint32_t b = exponent_byte(top);
-          const float by = __uint_as_float((254u - min(b, 253u)) << 23);   // 2^(127 - byte)
-          uint32_t q[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
-          if (b != 255) {
+            for (int e = 0; e < 4; ++e) top = __vmaxu2(top, w[e] & 0x7FFF7FFFu);
+            top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            if (h >= heads || !there) continue;
+            const uint32_t e8 = exponent_byte(top);
+            const float by = __uint_as_float((254u - min(e8, 253u)) << 23);   // 2^(127 - byte)
+            uint32_t q[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
+            if (e8 != 255) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t lo = w[2 * e], hi = w[2 * e + 1];
+                q[e] = e4m3_of(__uint_as_float(lo << 16) * by, __uint_as_float(lo & 0xFFFF0000u) * by) |
+                       e4m3_of(__uint_as_float(hi << 16) * by, __uint_as_float(hi & 0xFFFF0000u) * by) << 16;
+              }
+            }
+            *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[1]);
+            if (lane == 0) (v ? a.c.ve + at.x * a.c.ve_ps : a.c.ke + at.x * a.c.ke_ps)[row] = static_cast<uint8_t>(e8);
+          } else {
+            if (h >= heads || !there) continue;
+            *reinterpret_cast<uint4*>(to) = raw[v][i];
+          }
+        } else {
+          if (h >= heads) continue;
+          if constexpr (E4) {
+            const float by = exponent_value(byte[v][i]);
+            const uint32_t w[2] = {raw[v][i].x, raw[v][i].y};
+            uint32_t o[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint32_t lo = w[2 * e], hi = w[2 * e + 1];
-              q[e] = e4m3_of(__uint_as_float(lo << 16) * by, __uint_as_float(lo & 0xFFFF0000u) * by) |
-                     e4m3_of(__uint_as_float(hi << 16) * by, __uint_as_float(hi & 0xFFFF0000u) * by) << 16;
-            }
-          }
-          *reinterpret_cast<uint2*>(pages + at[i].x * ps + (to[i] * LANES + lane) * BYTES) = make_uint2(q[0], q[1]);
-          if (lane == 0) exps[at[i].x * eps + to[i]] = static_cast<uint8_t>(b);
-        } else {
-          if (at[i].x < 0) continue;
-          *reinterpret_cast<uint4*>(pages + at[i].x * ps + (to[i] * LANES + lane) * BYTES) = raw[i];
-        }
-      } else {
-        if (r0 + i * ROWS >= rows) continue;
-        if constexpr (E4) {
-          const float by = exponent_value(byte[i]);
-          const uint32_t w[2] = {raw[i].x, raw[i].y};
-          uint32_t o[4];
+              uint32_t two[2];
+              halves_of_e4m3(w[e], two[0], two[1]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t two[2];
-            halves_of_e4m3(w[e], two[0], two[1]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two[h]));
-              o[2 * e + h] = pack_bf16x2(f.x * by, f.y * by);
+              for (int s = 0; s < 2; ++s) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two[s]));
+                o[2 * e + s] = pack_bf16x2(f.x * by, f.y * by);
+              }
             }
+            raw[v][i] = make_uint4(o[0], o[1], o[2], o[3]);
           }
-          raw[i] = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(a.out + ((v ? a.tokens : 0) + t) * a.c.heads * D + h * D + lane * 8) = raw[v][i];
         }
-        *reinterpret_cast<uint4*>(out + ((t0 + tok[i]) * a.c.heads + head[i]) * D + lane * 8) = raw[i];
       }
     }
   }
