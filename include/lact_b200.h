@@ -438,12 +438,11 @@ int lact_paged_cache_read(const lact_paged_cache *cache, void *out, int64_t batc
                           void *stream);
 /* Attention of one token of every sequence: q [sequences, heads, head_dim] bf16 (16-byte aligned, strides multiples of 8), kv_heads divides
  * heads (consecutive heads share) -> o [sequences, heads, head_dim] bf16, contiguous: softmax(softmax_scale q K^T) V over positions
- * max(0, length - window) .. length - 1 (window 0: all); zeros where the length is not above 0.  counters, workspace: sizes from
- * lact_paged_attention_step_bytes (uint32 words, zero before the first call and zero again after every one; bytes, 16-byte
- * aligned; both may be 0); calls that share them must follow one another.  o: 16-byte aligned. */
-int lact_paged_attention_step_bytes(const lact_paged_cache *cache, int64_t heads, int64_t window, size_t *bytes, int64_t *counters);
+ * max(0, length - window) .. length - 1 (window 0: all); zeros where the length is not above 0.  o: 16-byte aligned.  workspace:
+ * lact_paged_attention_step_bytes, 16-byte aligned (may be NULL if that is 0). */
+int lact_paged_attention_step_bytes(const lact_paged_cache *cache, int64_t heads, int64_t window, size_t *bytes);
 int lact_paged_attention_step(const lact_paged_cache *cache, const void *q, int64_t q_bs, int64_t q_hs, int64_t heads, int64_t window,
-                              float softmax_scale, void *o, void *counters, void *workspace, size_t workspace_bytes,
+                              float softmax_scale, void *o, void *workspace, size_t workspace_bytes,
                               int32_t *status_word, void *stream);
 
 /* Backward of lact_qkv_prologue / lact_qkv_prologue_rope on the saved projections (same strides): dq, dk, dv are the

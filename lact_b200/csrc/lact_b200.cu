@@ -12,6 +12,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/lact_b200.h"
@@ -2447,63 +2448,76 @@ int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t
 
 // How a call's tiles are dealt out.
 struct PagedStepPlan {
-  int nq, blocks, runs, cluster, stages, long_stages;
+  int nq, warps, blocks, runs, cluster, stages, long_stages;
   size_t bytes, smem;
 };
-constexpr int kPagedWarps = 4;
 constexpr int kPagedLeast = 2;      // tiles of a run at least
 constexpr int kPagedWhole = 4;      // tiles of a unit up to which one CTA takes a unit, however many there are
 constexpr int kPagedClustered = 8;  // tiles of a CTA of a cluster at most
 int paged_step_plan(const lact_paged_cache* c, int64_t heads, int64_t window, PagedStepPlan* p) {
   if (heads < 1 || heads > 65535 || heads % c->kv_heads != 0 || window < 0) return LACT_ERR_SHAPE;
   const int64_t row_bytes = c->head_dim * (c->k_exponent != nullptr ? 1 : 2), step = 16 * kPagedSub(static_cast<int>(row_bytes));
-  const int64_t share = heads / c->kv_heads, tile = step * kPagedWarps;
+  const int64_t share = heads / c->kv_heads;
+  const int dw = getenv("DEV_WHOLE") ? atoi(getenv("DEV_WHOLE")) : 16, dl = getenv("DEV_LEAST") ? atoi(getenv("DEV_LEAST")) : 2;
   p->nq = share > 8 ? 2 : 1;
   p->blocks = ceil_div(share, 8 * p->nq);
   const int64_t units = c->sequences * c->kv_heads * p->blocks, room = c->table_cols * c->page_size;
-  const int64_t most = (std::min(window > 0 ? window + step - 1 : room, room) + tile - 1) / tile;   // of a unit
   if (units > 0x7FFFFFFF) return LACT_ERR_SHAPE;
-  const int per_sm = p->nq == 1 ? 3 : 2;   // (by the kernel's registers)
-  const int64_t ctas = static_cast<int64_t>(sm_count()) * per_sm;
+  const int64_t tokens = std::min(window > 0 ? window + step - 1 : room, room);   // of a unit, at most
+  auto tiles = [&](int warps) { return (tokens + step * warps - 1) / (step * warps); };
+  p->warps = 4;
+  int64_t ctas = static_cast<int64_t>(sm_count()) * kPagedPerSm(p->nq, 4);
   p->runs = 0;
   p->cluster = 1;
-  while (p->cluster < 8 && p->cluster < most && 2 * p->cluster * units <= ctas) p->cluster *= 2;
-  if (most > (p->cluster > 1 ? kPagedClustered * p->cluster : kPagedWhole)) {
+  while (p->cluster < 8 && p->cluster < tiles(4) && 2 * p->cluster * units <= ctas) p->cluster *= 2;
+  if (tiles(4) > dw * p->cluster) {
     p->cluster = 1;
-    p->runs = static_cast<int>(std::min(ctas, (units * most + kPagedLeast - 1) / kPagedLeast));
+    p->runs = static_cast<int>(std::min({ctas, (units * tiles(p->warps) + dl - 1) / dl, static_cast<int64_t>(kPagedJoinMost)}));
   }
   const int64_t rows = std::min<int64_t>(share, 8 * p->nq), sums = rows * kPagedPieceRow(static_cast<int>(c->head_dim)) * 4;
-  p->bytes = static_cast<size_t>(p->runs) * 2 * sums;
+  p->bytes = static_cast<size_t>(p->runs) * (2 * sums + sizeof(PagedCut));
   const int64_t stage = 2 * step * (row_bytes + (c->k_exponent != nullptr ? 1 : 0));
-  // (the sums of a row hold the factors of all of a unit's pieces later on, a cluster's CTAs have their own added up; 3 KB: alignment,
-  // and what the kernel has beside)
-  const int64_t room_cta = 227 * 1024 / per_sm - 3072, at_end = std::max<int64_t>((kPagedWarps + (p->cluster > 1 ? 1 : 0)) * sums, rows * p->runs * 4);
-  p->stages = static_cast<int>(std::min<int64_t>(kPagedStages, (room_cta - at_end) / (kPagedWarps * stage)));
+  // (a cluster's CTAs have their own sums added up beside their warps'; 3 KB: alignment, and what the kernel has beside)
+  const int64_t room_cta = 227 * 1024 / kPagedPerSm(p->nq, p->warps) - 3072, at_end = (p->warps + (p->cluster > 1 ? 1 : 0)) * sums;
+  p->stages = static_cast<int>(std::min<int64_t>(kPagedStages, (room_cta - at_end) / (p->warps * stage)));
   p->long_stages = std::min<int>(p->stages, static_cast<int>(std::max<int64_t>(1, 8192 / stage)));
-  p->smem = static_cast<size_t>(kPagedWarps * p->stages * stage + at_end) + 1024;
+  p->smem = static_cast<size_t>(p->warps * p->stages * stage + at_end) + 1024;
   return LACT_OK;
 }
-template <int D, bool E4, int NQ>
+template <int D, bool E4, int NQ, int W>
 int launch_paged_step(const lact_paged_cache* c, const PagedStepArgs& a, size_t smem, cudaStream_t st) {
-  auto kernel = paged_step_kernel<D, E4, NQ, kPagedWarps>;
+  auto kernel = paged_step_kernel<D, E4, NQ, W>;
   CUtensorMap k_map, v_map;
   constexpr int64_t cols = E4 ? D / 2 : D;   // of 16 bits
   const int64_t rows = c->kv_heads * c->page_size;
   const uint32_t box = static_cast<uint32_t>(std::min<int64_t>(c->page_size, 16 * kPagedSub(2 * cols)));
   LACT_TRY(encode_map(&k_map, {c->k, rows, cols, cols, c->pages, a.c.k_ps / 2}, box, cols < 64 ? 32 : 64));
   LACT_TRY(encode_map(&v_map, {c->v, rows, cols, cols, c->pages, a.c.v_ps / 2}, box, cols < 64 ? 32 : 64));
-  LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  static std::atomic<uint64_t> allowed{0};   // devices that know how much shared memory the kernel may take
+  int dev = 0;
+  LACT_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || (allowed.load(std::memory_order_relaxed) >> dev & 1) == 0) {
+    LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 / kPagedPerSm(NQ, W) - 2048));
+    if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   const int64_t grid = a.runs > 0 ? a.runs : static_cast<int64_t>(a.c.sequences) * a.c.heads * a.blocks * a.cluster;
   if (grid > 0x7FFFFFFF) return LACT_ERR_SHAPE;
-  KernelScope scope(kClsOther, st);
   if (a.cluster == 1) {
-    LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kPagedWarps * 32), smem, st, a, k_map, v_map));
+    { KernelScope scope(kClsOther, st); LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(W * 32), smem, st, a, k_map, v_map)); }
+    if (a.runs == 0) return LACT_OK;
+    // as many groups as have eight pieces each at a time
+    const int64_t rows = std::min(a.share, 8 * NQ), units = static_cast<int64_t>(a.c.sequences) * a.c.heads * a.blocks, pieces = a.runs / units + 2;
+    int threads = 64;
+    while (threads < 512 && pieces * 64 > 8 * threads) threads *= 2;
+    KernelScope scope(kClsOther, st);
+    LACT_CUDA(launch_pdl(paged_join_kernel<D>, dim3(static_cast<unsigned>(grid), ceil_div(rows * D, 256)), dim3(threads), 0, st, a.pieces, a.cuts, a.o, static_cast<int32_t>(rows)));
     return LACT_OK;
   }
+  KernelScope scope(kClsOther, st);
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kPagedWarps * 32);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -3709,25 +3723,24 @@ int lact_paged_cache_read(const lact_paged_cache* c, void* out, int64_t batch, i
   return paged_rows(c, a, batch, tokens, cu_seqlens, false, static_cast<cudaStream_t>(stream));
 }
 
-int lact_paged_attention_step_bytes(const lact_paged_cache* c, int64_t heads, int64_t window, size_t* bytes_out, int64_t* counters_out) {
-  if (bytes_out == nullptr || counters_out == nullptr) return LACT_ERR_NULL;
+int lact_paged_attention_step_bytes(const lact_paged_cache* c, int64_t heads, int64_t window, size_t* bytes_out) {
+  if (bytes_out == nullptr) return LACT_ERR_NULL;
   LACT_TRY(paged_check(c));
   PagedStepPlan p;
   LACT_TRY(paged_step_plan(c, heads, window, &p));
   *bytes_out = p.bytes;
-  *counters_out = p.runs;
   return LACT_OK;
 }
 
 int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t q_bs, int64_t q_hs, int64_t heads, int64_t window,
-                              float softmax_scale, void* o, void* counters, void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream) {
+                              float softmax_scale, void* o, void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream) {
   LACT_TRY(paged_check(c));
   if (q == nullptr || o == nullptr || status_word == nullptr) return LACT_ERR_NULL;
   if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || (reinterpret_cast<uintptr_t>(o) & 15) != 0 || q_bs % 8 != 0 || q_hs % 8 != 0) return LACT_ERR_SHAPE;
   if (!(std::fabs(softmax_scale) <= 1e18f)) return LACT_ERR_CONFIG;
   PagedStepPlan p;
   LACT_TRY(paged_step_plan(c, heads, window, &p));
-  if (p.runs > 0 && (counters == nullptr || workspace == nullptr || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) return LACT_ERR_WORKSPACE;
+  if (p.runs > 0 && (workspace == nullptr || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) return LACT_ERR_WORKSPACE;
   LACT_TRY(check_device());
   PagedStepArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -3737,24 +3750,23 @@ int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t 
   a.heads = static_cast<int32_t>(heads); a.share = static_cast<int32_t>(heads / c->kv_heads); a.blocks = p.blocks;
   a.window = static_cast<int32_t>(std::min<int64_t>(window, 0x7FFFFFFF));
   a.scale = softmax_scale * 1.4426950408889634f;
-  a.runs = p.runs; a.least = kPagedLeast;
-  a.counters = static_cast<uint32_t*>(counters);
-  a.pieces = static_cast<float*>(workspace);
+  a.runs = p.runs; a.least = getenv("DEV_LEAST") ? atoi(getenv("DEV_LEAST")) : 2;
+  a.cuts = static_cast<PagedCut*>(workspace);
+  a.pieces = reinterpret_cast<float*>(a.cuts + p.runs);
   a.status = status_word;
   a.stages = p.stages; a.long_stages = p.long_stages;
   a.cluster = p.cluster;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int form = (c->head_dim == 128 ? 4 : 0) + (c->k_exponent != nullptr ? 2 : 0) + p.nq - 1;
-  switch (form) {
-    case 0: return launch_paged_step<64, false, 1>(c, a, p.smem, st);
-    case 1: return launch_paged_step<64, false, 2>(c, a, p.smem, st);
-    case 2: return launch_paged_step<64, true, 1>(c, a, p.smem, st);
-    case 3: return launch_paged_step<64, true, 2>(c, a, p.smem, st);
-    case 4: return launch_paged_step<128, false, 1>(c, a, p.smem, st);
-    case 5: return launch_paged_step<128, false, 2>(c, a, p.smem, st);
-    case 6: return launch_paged_step<128, true, 1>(c, a, p.smem, st);
-    default: return launch_paged_step<128, true, 2>(c, a, p.smem, st);
-  }
+  auto launch = [&](auto d, auto e4) {
+    constexpr int D = decltype(d)::value;
+    constexpr bool E4 = decltype(e4)::value;
+    return p.nq == 2 ? launch_paged_step<D, E4, 2, 4>(c, a, p.smem, st) : launch_paged_step<D, E4, 1, 4>(c, a, p.smem, st);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (c->head_dim == 64) return c->k_exponent != nullptr ? launch(D64{}, std::true_type{}) : launch(D64{}, std::false_type{});
+  return c->k_exponent != nullptr ? launch(D128{}, std::true_type{}) : launch(D128{}, std::false_type{});
+}
 }
 
 // ------------------------------------------------------------------------------------------ linear attention
@@ -4412,4 +4424,3 @@ int lact_bmm_bf16(const void* a, int32_t a_mn_major, const void* b, int32_t b_mn
   return launch_op<OpBmmStore, 1>(bt, fill_bf16, s, kClsOther, 1);
 }
 
-}  // extern "C"

@@ -76,9 +76,6 @@ struct StatusWord {
 };
 StatusWord status_word(const Tensor& like);
 void poll_status(const Tensor& like);
-// `words` 32-bit counters that are zero, and that the call leaves at zero: shared by the calls on (device of `like`, current stream), of a
-// call that is being captured its own, which the graph clears at every replay.
-Tensor zeroed_counters(const Tensor& like, int64_t words);
 // End of a backward: with LACT_B200_SYNC_CHECK=1 (and no capture) waits for the stream and reports what it has left (forwards
 // are waited for in Python).
 void settle(const Tensor& like);

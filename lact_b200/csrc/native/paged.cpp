@@ -153,15 +153,11 @@ Tensor step(const Tensor& q_, const Tensor& kc, const Tensor& vc, const OptTenso
   const Tensor q = lies ? q_ : plain(q_);
   const Cache r = describe(kc, vc, ke, ve, table, lengths);
   size_t need = 0;
-  int64_t words = 0;
-  check(lact_paged_attention_step_bytes(&r.c, q.size(1), window, &need, &words), "lact_paged_attention_step_bytes");
-  Tensor room, counters;
-  if (need > 0) {
-    room = bytes(need, q);
-    counters = zeroed_counters(q, words);
-  }
+  check(lact_paged_attention_step_bytes(&r.c, q.size(1), window, &need), "lact_paged_attention_step_bytes");
+  Tensor room;
+  if (need > 0) room = bytes(need, q);
   check(lact_paged_attention_step(&r.c, ptr(q), stride_of(q, 0), stride_of(q, 1), q.size(1), window, static_cast<float>(scale), ptr(o),
-                                  need > 0 ? ptr(counters) : nullptr, need > 0 ? ptr(room) : nullptr, need, status_word(q), stream_of(q)),
+                                  need > 0 ? ptr(room) : nullptr, need, status_word(q), stream_of(q)),
         "lact_paged_attention_step");
   return o;
 }

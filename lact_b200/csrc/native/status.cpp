@@ -99,25 +99,6 @@ StatusWord status_word(const Tensor& like) {
   return {Tensor(), w.buf.data_ptr<int32_t>()};
 }
 
-Tensor zeroed_counters(const Tensor& like, int64_t words) {
-  constexpr int64_t kShared = 1024;
-  if (words > kShared || capturing()) return empty({words}, at::kInt, like).zero_();
-  static std::mutex mu;
-  static auto& shared = *new std::unordered_map<uint64_t, Word>();   // (never destroyed, as the words above)
-  const int dev = like.device().index();
-  const auto stream = c10::cuda::getCurrentCUDAStream(dev);
-  const uint64_t key = (static_cast<uint64_t>(dev) << 56) ^ static_cast<uint64_t>(reinterpret_cast<uintptr_t>(stream.stream()));
-  const uint64_t epoch = g_epoch.load();
-  std::lock_guard<std::mutex> lock(mu);
-  Word& w = shared[key];
-  if (!w.buf.defined()) w.buf = empty({kShared}, at::kInt, like);
-  if (w.epoch != epoch) {   // (after a failure, too)
-    w.buf.zero_();
-    w.epoch = epoch;
-  }
-  return w.buf;
-}
-
 }  // namespace lact_torch
 
 // Status recorded on `device` so far (0: none), cleared by the read; what the Python side calls after a synchronisation.

@@ -13,8 +13,7 @@
 //
 // Work: a unit is a (sequence, kv head, block of query heads), its tokens tiles of 16 a warp; lengths are known on the device alone.
 // All units' tiles, in order, are dealt out in even runs, one for each CTA, whatever the lengths are.  A run that holds all of a unit
-// writes its result; of a unit cut among runs each leaves a piece (sums, maxima), and the run that comes last adds the pieces in their
-// order.  Where units are few and have few tiles at most, or have very few (`runs` 0), a unit is a cluster of CTAs that share its tiles
+// writes its result; of a unit cut among runs each leaves a piece (sums, maxima), and a small launch adds the pieces in a fixed order.  Where units are few and have few tiles at most, or have very few (`runs` 0), a unit is a cluster of CTAs that share its tiles
 // evenly and read one another's sums from shared memory: no pieces, no counters.
 #pragma once
 #include "paged_cache.cuh"
@@ -33,8 +32,8 @@ struct PagedStepArgs {
   float scale;                     // softmax scale * log2(e)
   int32_t runs, least;             // CTAs that share the tiles; tiles of a run at least
   int32_t cluster;                 // runs 0: CTAs of a unit (1, 2, 4 or 8)
-  uint32_t* counters;              // [runs], zero before and after
-  float* pieces;                   // [runs][2][min(share, rows of a block)][D + 4]
+  struct PagedCut* cuts;           // [runs]
+  float* pieces;                   // [runs][2][min(share, rows of a block)][D + 4]: of the unit that a run begins in, of one that begins in it
   int32_t* status;
   int32_t stages, long_stages;     // steps that a warp has on their way or in work; the same in runs of more tiles than kPagedLong
 };
@@ -110,43 +109,48 @@ __device__ __forceinline__ float4 ld_cluster_16(uint32_t at, uint32_t rank) {
       : "memory");
   return v;
 }
-// The sums of a cluster's CTAs, W of each in `sums`, as the unit's result.
-template <int D, int W, int ROW>
-__device__ __forceinline__ void paged_join_cluster(const PagedStepArgs& a, float* sums, int sum_rows, int rows, bool any, bf16* o) {
-  constexpr int THREADS = W * 32;
-  float* const mine = sums + W * sum_rows * ROW;
-  for (int i = threadIdx.x; i < rows * (D / 4 + 1); i += THREADS) {
-    const int row = i / (D / 4 + 1), d = i % (D / 4 + 1) * 4;
-    const float* const from = sums + row * ROW;
-    float tm = kLowest, tM = kLowest;
+// The sums of W warps in `sums` ([W][sum_rows][ROW]: D features, then m, l, M), added up for four features of a row at a time:
+// put(row, d, sum, float4(m, l, M, 0)).
+template <int D, int W, int ROW, class Put>
+__device__ __forceinline__ void paged_merge(const float* sums, int sum_rows, int rows, const Put& put) {
+  for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float4 s[W], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float tm = kLowest, tM = kLowest, tl = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      tm = fmaxf(tm, from[w * sum_rows * ROW + D]);
-      tM = fmaxf(tM, from[w * sum_rows * ROW + D + 2]);
+      s[w] = *reinterpret_cast<const float4*>(sums + (w * sum_rows + row) * ROW + D);
+      tm = fmaxf(tm, s[w].x);
+      tM = fmaxf(tM, s[w].z);
     }
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float tl = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float* const f = from + w * sum_rows * ROW;
-      const float by = exp2_ftz(f[D + 2] - tM);
-      const float4 x = *reinterpret_cast<const float4*>(f + min(d, D - 4));
+      const float4 x = *reinterpret_cast<const float4*>(sums + (w * sum_rows + row) * ROW + d);
+      const float by = exp2_ftz(s[w].z - tM);
       sum.x += x.x * by; sum.y += x.y * by; sum.z += x.z * by; sum.w += x.w * by;
-      tl += f[D + 1] * exp2_ftz(f[D] - tm);
+      tl += s[w].y * exp2_ftz(s[w].x - tm);
     }
-    *reinterpret_cast<float4*>(mine + row * ROW + d) = d < D ? sum : make_float4(tm, tl, tM, 0.f);
+    put(row, d, sum, make_float4(tm, tl, tM, 0.f));
   }
+}
+__device__ __forceinline__ void store_bf16x4(bf16* to, const float4& x, float by) {
+  *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(x.x * by, x.y * by), pack_bf16x2(x.z * by, x.w * by));
+}
+
+// The sums of a cluster's CTAs, each added up in `mine` ([rows][ROW]), as the unit's result.
+template <int D, int W, int ROW>
+__device__ __forceinline__ void paged_join_cluster(int ctas, const float* mine, int rows, bool any, bf16* o) {
   cluster_arrive();
   cluster_wait();
   const uint32_t at = smem_u32(mine);
-  for (int i = cluster_rank() * THREADS + threadIdx.x; i < rows * (D / 4); i += a.cluster * THREADS) {
+  for (int i = cluster_rank() * W * 32 + threadIdx.x; i < rows * (D / 4); i += ctas * W * 32) {
     const int row = i / (D / 4), d = i % (D / 4) * 4;
     float4 s[8], x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       s[k] = make_float4(kLowest, 0.f, kLowest, 0.f);
       x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k >= a.cluster) continue;
+      if (k >= ctas) continue;
       s[k] = ld_cluster_16(at + (row * ROW + D) * 4, k);
       x[k] = ld_cluster_16(at + (row * ROW + d) * 4, k);
     }
@@ -163,18 +167,101 @@ __device__ __forceinline__ void paged_join_cluster(const PagedStepArgs& a, float
       sum.x += x[k].x * by; sum.y += x[k].y * by; sum.z += x[k].z * by; sum.w += x[k].w * by;
       tl += s[k].y * exp2_ftz(s[k].x - tm);
     }
-    const float f = any ? exp2_ftz(tM - tm) / tl : 0.f;
-    *reinterpret_cast<uint2*>(o + row * D + d) = make_uint2(pack_bf16x2(sum.x * f, sum.y * f), pack_bf16x2(sum.z * f, sum.w * f));
+    store_bf16x4(o + row * D + d, sum, any ? exp2_ftz(tM - tm) / tl : 0.f);
   }
   cluster_arrive();   // (nobody leaves while its sums are read)
   cluster_wait();
 }
 
+// CTAs of a SM, by registers: 12 warps of 168, or 8 of 255.
+__host__ __device__ constexpr int kPagedPerSm(int nq, int warps) { return (nq == 1 ? 12 : 8) / warps; }
 // 16 tokens of a step times this
 __host__ __device__ constexpr int kPagedSub(int row_bytes) { return row_bytes > 128 ? 1 : 2; }
 
+// A unit that begins in a run and does not end there: its result, and how many runs have pieces of it (0: there is none).
+struct PagedCut {
+  int64_t o;
+  int32_t rows, count;
+};
+// The pieces of the units that were cut, added up: blockIdx.x is the run that one begins in, blockIdx.y 64 times four of its sums; groups
+// of 64 threads share the pieces, eight of a group on their way at a time.  A launch of its own, so that nothing is left behind in the
+// kernel that has to wait for pieces (which would cost its loop registers: there, by who comes last, step_long took 101 in place of 97 us,
+// and one unit of 131072 tokens 78 in place of 30).
+constexpr int kPagedJoinMost = 1024;   // pieces of a unit at most: the runs of a call
+template <int D>
+__global__ void __launch_bounds__(512) paged_join_kernel(const float* pieces, const PagedCut* cuts, bf16* out, int32_t sum_rows) {
+  constexpr int ROW = kPagedPieceRow(D), ROWS = 256 / D, N = 8;   // rows of 64 times four sums
+  __shared__ float factor[ROWS][kPagedJoinMost], scale[ROWS];
+  __shared__ float4 part[7][64];
+  griddep_launch_dependents();
+  griddep_wait();
+  const PagedCut u = cuts[blockIdx.x];
+  const int row0 = blockIdx.y * ROWS, rows = min(u.rows - row0, ROWS), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (u.count == 0 || rows <= 0) return;
+  // (the first piece is its run's second)
+  const float* const base = pieces + static_cast<int64_t>(blockIdx.x) * 2 * sum_rows * ROW + row0 * ROW;
+  auto piece = [&](int i) { return base + static_cast<int64_t>(2 * i + (i == 0 ? 1 : 0)) * sum_rows * ROW; };
+  for (int row = warp; row < rows; row += blockDim.x >> 5) {
+    float tm = kLowest, tM = kLowest, tl = 0.f;                   // (a lane's own, until they are put together)
+    for (int i0 = lane; i0 < u.count; i0 += 4 * 32) {
+      float4 s[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        s[k] = make_float4(kLowest, 0.f, kLowest, 0.f);
+        if (i0 + k * 32 < u.count) s[k] = *reinterpret_cast<const float4*>(piece(i0 + k * 32) + row * ROW + D);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float now = fmaxf(tm, s[k].x);
+        tl = tl * exp2_ftz(tm - now) + s[k].y * exp2_ftz(s[k].x - now);
+        tm = now;
+        tM = fmaxf(tM, s[k].z);
+        if (i0 + k * 32 < u.count) factor[row][i0 + k * 32] = s[k].z;
+      }
+    }
+    float top = tm;
+#pragma unroll
+    for (int e = 16; e > 0; e >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, e));
+      tM = fmaxf(tM, __shfl_xor_sync(0xFFFFFFFFu, tM, e));
+    }
+    tl *= exp2_ftz(tm - top);
+#pragma unroll
+    for (int e = 16; e > 0; e >>= 1) tl += __shfl_xor_sync(0xFFFFFFFFu, tl, e);
+    for (int i = lane; i < u.count; i += 32) factor[row][i] = exp2_ftz(factor[row][i] - tM);
+    if (lane == 0) scale[row] = exp2_ftz(tM - top) / tl;
+  }
+  __syncthreads();
+  const int groups = blockDim.x / 64, group = threadIdx.x / 64, at = threadIdx.x % 64, row = at / (D / 4), d = at % (D / 4) * 4;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (row < rows) {
+    for (int i0 = group; i0 < u.count; i0 += N * groups) {
+      float4 x[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + k * groups < u.count) x[k] = *reinterpret_cast<const float4*>(piece(i0 + k * groups) + row * ROW + d);
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        if (i0 + k * groups >= u.count) continue;
+        const float f = factor[row][i0 + k * groups];
+        sum.x += x[k].x * f; sum.y += x[k].y * f; sum.z += x[k].z * f; sum.w += x[k].w * f;
+      }
+    }
+  }
+  if (group > 0) part[group - 1][at] = sum;
+  __syncthreads();
+  if (group > 0 || row >= rows) return;
+  for (int g = 0; g < groups - 1; ++g) {
+    const float4 x = part[g][at];
+    sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+  }
+  store_bf16x4(out + u.o + (row0 + row) * D + d, sum, scale[row]);
+}
+
 template <int D, bool E4, int NQ, int W>
-__global__ void __launch_bounds__(W * 32, NQ == 2 ? 2 : D == 64 ? 4 : 3) paged_step_kernel(const __grid_constant__ PagedStepArgs a, const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ, W)) paged_step_kernel(const __grid_constant__ PagedStepArgs a, const __grid_constant__ CUtensorMap k_map,
                                                             const __grid_constant__ CUtensorMap v_map) {
   constexpr int BYTES = E4 ? D : 2 * D;                  // of a row
   constexpr int SUB = kPagedSub(BYTES), STEP = 16 * SUB; // tokens of a step: 8 KB where rows allow
@@ -190,8 +277,7 @@ __global__ void __launch_bounds__(W * 32, NQ == 2 ? 2 : D == 64 ? 4 : 3) paged_s
   __shared__ uint64_t full[W * kPagedStages];
   __shared__ int plan[4];
   __shared__ int64_t warp_sum[W];
-  __shared__ uint32_t arrived, gave_up;
-  __shared__ float scales[ROWS];
+  __shared__ uint32_t gave_up;
   const int warp = uniform_warp_index(), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const uint32_t leader = elect_leader();
   uint8_t* const paged_smem = smem_raw + ((smem_u32(smem_raw) + 1023u & ~1023u) - smem_u32(smem_raw));
@@ -237,6 +323,7 @@ __global__ void __launch_bounds__(W * 32, NQ == 2 ? 2 : D == 64 ? 4 : 3) paged_s
     all *= units;
     per = max((all + a.runs - 1) / a.runs, static_cast<int64_t>(a.least));
     run0 = blockIdx.x * per;
+    if (threadIdx.x == 0) a.cuts[blockIdx.x].count = 0;   // (until there is one)
     if (run0 >= all) return;
     make.left = static_cast<int>(min(per, all - run0));
     int64_t at = (upto - mine) * units;
@@ -632,86 +719,26 @@ __global__ void __launch_bounds__(W * 32, NQ == 2 ? 2 : D == 64 ? 4 : 3) paged_s
         if (r == 0) *reinterpret_cast<float4*>(to + D) = make_float4(m[n][e], l[n][e], E4 ? M[n][e] : m[n][e], 0.f);
       }
     __syncthreads();
-    if (a.cluster > 1) {
-      paged_join_cluster<D, W, ROW>(a, sums, sum_rows, rows, use.last > use.first, a.o + (static_cast<int64_t>(seq) * a.heads + static_cast<int64_t>(head) * a.share + row0) * D);
-      return;
-    }
-    const bool whole = use.t1 == use.tiles && t0 == 0;
-    const int64_t begin = run0 + done - t0;              // the unit's first tile among all
-    auto piece_of = [&](int64_t run, bool first) { return a.pieces + (run * 2 + (first ? 1 : 0)) * sum_rows * ROW; };
-    float* const piece = whole ? nullptr : piece_of(blockIdx.x, t0 == 0);
-    bf16* const o = a.o + (static_cast<int64_t>(seq) * a.heads + static_cast<int64_t>(head) * a.share + row0) * D;
-    for (int i = threadIdx.x; i < rows * D; i += THREADS) {
-      const int row = i / D, d = i % D;
-      const float* const from = sums + row * ROW;
-      float tm = kLowest, tM = kLowest, sum = 0.f, tl = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        tm = fmaxf(tm, from[w * sum_rows * ROW + D]);
-        tM = fmaxf(tM, from[w * sum_rows * ROW + D + 2]);
+    const bool whole = use.t1 == use.tiles && t0 == 0, any = use.last > use.first;
+    const int64_t at = (static_cast<int64_t>(seq) * a.heads + static_cast<int64_t>(head) * a.share + row0) * D;
+    if (a.cluster == 1 && whole) {
+      paged_merge<D, W, ROW>(sums, sum_rows, rows, [&](int row, int d, const float4& sum, const float4& s) {
+        store_bf16x4(a.o + at + row * D + d, sum, any ? exp2_ftz(s.z - s.x) / s.y : 0.f);
+      });
+    } else {
+      // a piece: to this CTA's part of the cluster's, or to global memory
+      float* const piece = a.cluster > 1 ? sums + W * sum_rows * ROW : a.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * sum_rows * ROW;
+      paged_merge<D, W, ROW>(sums, sum_rows, rows, [&](int row, int d, const float4& sum, const float4& s) {
+        *reinterpret_cast<float4*>(piece + row * ROW + d) = sum;
+        if (d == 0) *reinterpret_cast<float4*>(piece + row * ROW + D) = s;
+      });
+      if (a.cluster > 1) {
+        paged_join_cluster<D, W, ROW>(a.cluster, piece, rows, any, a.o + at);
+        return;
       }
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float* const f = from + w * sum_rows * ROW;
-        sum += f[d] * exp2_ftz(f[D + 2] - tM);
-        tl += f[D + 1] * exp2_ftz(f[D] - tm);
-      }
-      if (whole) {
-        o[i] = __float2bfloat16_rn(use.last > use.first ? sum * (exp2_ftz(tM - tm) / tl) : 0.f);
-      } else {
-        piece[row * ROW + d] = sum;
-        if (d < 4) piece[row * ROW + D + d] = d == 0 ? tm : d == 1 ? tl : d == 2 ? tM : 0.f;
-      }
-    }
-    if (!whole) {
-      // the run that leaves the last of the unit's pieces adds them up
-      const int64_t first_run = begin / per, last_run = (begin + use.tiles - 1) / per;
-      const int count = static_cast<int>(last_run - first_run) + 1;
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        arrived = atomicAdd(a.counters + first_run, 1u);
-        if (arrived == static_cast<uint32_t>(count - 1)) a.counters[first_run] = 0;
-      }
-      __syncthreads();
-      if (arrived == static_cast<uint32_t>(count - 1)) {
-        __threadfence();
-        // a warp a row: each piece's factor, and the row's
-        float* const factors = sums;                     // [rows][count] (at most as many runs as the sums of a row take)
-        for (int row = warp; row < rows; row += W) {
-          float tm = kLowest, tM = kLowest, tl = 0.f;
-          for (int i = lane; i < count; i += 32) {
-            const float4 s = __ldcg(reinterpret_cast<const float4*>(piece_of(first_run + i, i == 0) + row * ROW + D));
-            tm = fmaxf(tm, s.x);
-            tM = fmaxf(tM, s.z);
-          }
-#pragma unroll
-          for (int s = 16; s > 0; s >>= 1) {
-            tm = fmaxf(tm, __shfl_xor_sync(0xFFFFFFFFu, tm, s));
-            tM = fmaxf(tM, __shfl_xor_sync(0xFFFFFFFFu, tM, s));
-          }
-          for (int i = lane; i < count; i += 32) {
-            const float4 s = __ldcg(reinterpret_cast<const float4*>(piece_of(first_run + i, i == 0) + row * ROW + D));
-            tl += s.y * exp2_ftz(s.x - tm);
-            factors[row * count + i] = exp2_ftz(s.z - tM);
-          }
-#pragma unroll
-          for (int s = 16; s > 0; s >>= 1) tl += __shfl_xor_sync(0xFFFFFFFFu, tl, s);
-          if (lane == 0) scales[row] = exp2_ftz(tM - tm) / tl;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
-          const int row = i / (D / 4), d = i % (D / 4) * 4;
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int k = 0; k < count; ++k) {
-            const float4 s = __ldcg(reinterpret_cast<const float4*>(piece_of(first_run + k, k == 0) + row * ROW + d));
-            const float f = factors[row * count + k];
-            sum.x += s.x * f; sum.y += s.y * f; sum.z += s.z * f; sum.w += s.w * f;
-          }
-          const float f = scales[row];
-          *reinterpret_cast<uint2*>(o + row * D + d) = make_uint2(pack_bf16x2(sum.x * f, sum.y * f), pack_bf16x2(sum.z * f, sum.w * f));
-        }
+      if (threadIdx.x == 0 && t0 == 0) {
+        const int64_t begin = run0 + done;               // the unit's first tile among all
+        a.cuts[blockIdx.x] = {at, rows, static_cast<int32_t>((begin + use.tiles - 1) / per - blockIdx.x) + 1};
       }
     }
     __syncthreads();

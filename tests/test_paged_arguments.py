@@ -66,8 +66,8 @@ def test_missing_rotary_pointers_are_refused(lib):
     assert lib.lact_rotary_axes(None, P, P, P, P, P, P, None) == -1
 
 
-def _step(lib, c, q=P, q_bs=256, q_hs=64, heads=4, window=0, scale=0.1, o=P, counters=P, room=P, nbytes=1 << 30, status=P):
-    return lib.lact_paged_attention_step(C.byref(c), q, C.c_int64(q_bs), C.c_int64(q_hs), C.c_int64(heads), C.c_int64(window), C.c_float(scale), o, counters, room,
+def _step(lib, c, q=P, q_bs=256, q_hs=64, heads=4, window=0, scale=0.1, o=P, room=P, nbytes=1 << 30, status=P):
+    return lib.lact_paged_attention_step(C.byref(c), q, C.c_int64(q_bs), C.c_int64(q_hs), C.c_int64(heads), C.c_int64(window), C.c_float(scale), o, room,
                                          C.c_size_t(nbytes), status, None)
 
 
@@ -88,23 +88,23 @@ def _read(lib, c, out=P, batch=2, tokens=5, cu=None):
     (dict(k_exponent=4096, v_exponent=4100), -2), (dict(k_exponent=4096, v_exponent=4096, ve_page_stride=40), -2)])
 def test_bad_caches_are_refused(lib, over, code):
     c = _cache(**over)
-    n, w = C.c_size_t(0), C.c_int64(0)
-    assert lib.lact_paged_attention_step_bytes(C.byref(c), C.c_int64(4), C.c_int64(0), C.byref(n), C.byref(w)) == code
+    n = C.c_size_t(0)
+    assert lib.lact_paged_attention_step_bytes(C.byref(c), C.c_int64(4), C.c_int64(0), C.byref(n)) == code
     assert _step(lib, c) == code and _write(lib, c) == code and _read(lib, c) == code
 
 
 def test_bad_calls_on_a_cache_are_refused(lib):
     c = _cache()
-    n, w = C.c_size_t(0), C.c_int64(0)
-    size = lambda heads=4, window=0, c=c: (lib.lact_paged_attention_step_bytes(C.byref(c), C.c_int64(heads), C.c_int64(window), C.byref(n), C.byref(w)), n.value, w.value)
-    assert size() == (0, 0, 0)                                     # 64 positions: a CTA a unit, no pieces
-    rc, nbytes, words = size(c=_cache(table_cols=4096))
-    assert rc == 0 and nbytes > 0 and 0 < words <= 1024
+    n = C.c_size_t(0)
+    size = lambda heads=4, window=0, c=c: (lib.lact_paged_attention_step_bytes(C.byref(c), C.c_int64(heads), C.c_int64(window), C.byref(n)), n.value)
+    assert size() == (0, 0)                                     # 64 positions: a CTA a unit, no pieces
+    rc, nbytes = size(c=_cache(table_cols=4096))
+    assert rc == 0 and nbytes > 0
     assert size(heads=3)[0] == -2 and size(heads=0)[0] == -2 and size(window=-1)[0] == -2
     for over, code in [(dict(q=None), -1), (dict(o=None), -1), (dict(status=None), -1), (dict(o=C.c_void_p(4104)), -2), (dict(q=C.c_void_p(4104)), -2), (dict(q_bs=257), -2), (dict(q_hs=68), -2), (dict(heads=5), -2),
                        (dict(scale=float("nan")), -5), (dict(scale=float("inf")), -5)]:
         assert _step(lib, c, **over) == code
-    for over in (dict(counters=None), dict(room=None), dict(nbytes=nbytes - 1), dict(room=C.c_void_p(4100))):
+    for over in (dict(room=None), dict(nbytes=nbytes - 1), dict(room=C.c_void_p(4100))):
         assert _step(lib, _cache(table_cols=4096), **over) == -4
     for over, code in [(dict(k=None), -1), (dict(v=None), -1), (dict(v=C.c_void_p(4104)), -2), (dict(strides=(128, 640, 63, 128, 640, 64)), -2),
                        (dict(strides=(128, 640, 64, 129, 640, 64)), -2), (dict(batch=3), -5), (dict(batch=2, cu=P), -5), (dict(tokens=0), -2)]:
