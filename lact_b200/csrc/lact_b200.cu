@@ -2448,45 +2448,50 @@ int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t
 
 // How a call's tiles are dealt out.
 struct PagedStepPlan {
-  int nq, warps, blocks, runs, cluster, stages, long_stages;
+  int nq, blocks, runs, cluster, stages, long_stages;
   size_t bytes, smem;
 };
-constexpr int kPagedLeast = 2;      // tiles of a run at least
-constexpr int kPagedWhole = 4;      // tiles of a unit up to which one CTA takes a unit, however many there are
-constexpr int kPagedClustered = 8;  // tiles of a CTA of a cluster at most
+// Measured as us of a call, bf16, 128 features unless stated:
+//   tiles of a run at least: one sequence, one kv head of 8 query heads, 32000 tokens with 1, 2, 4: 17.6, 16.4, 13.7; 8000 tokens 11.5, 10.6, 11.4;
+constexpr int kPagedLeast = 4;
+//   tiles of a unit up to which one CTA takes it: 64 sequences of 8 heads and up to 500 tokens (8 tiles) so 19.4, in even runs 25.6; 1000
+//   tokens (16 tiles) 30.1 and 33.3; 193 sequences of 4 heads, 158 tokens of 8 bits 11.6 and 16.8;
+constexpr int kPagedWhole = 16;
+//   tiles of each CTA of a cluster, where units are few: one sequence of 12 heads, 777 tokens (2 tiles) 6.9, in even runs 10.6; 4000 tokens (8)
+//   11.1 and 12.6; one kv head of 8 query heads, 8000 tokens (16) 17.1 and 10.6.
+constexpr int kPagedClustered = 8;
 int paged_step_plan(const lact_paged_cache* c, int64_t heads, int64_t window, PagedStepPlan* p) {
   if (heads < 1 || heads > 65535 || heads % c->kv_heads != 0 || window < 0) return LACT_ERR_SHAPE;
   const int64_t row_bytes = c->head_dim * (c->k_exponent != nullptr ? 1 : 2), step = 16 * kPagedSub(static_cast<int>(row_bytes));
   const int64_t share = heads / c->kv_heads;
-  const int dw = getenv("DEV_WHOLE") ? atoi(getenv("DEV_WHOLE")) : 16, dl = getenv("DEV_LEAST") ? atoi(getenv("DEV_LEAST")) : 2;
   p->nq = share > 8 ? 2 : 1;
   p->blocks = ceil_div(share, 8 * p->nq);
   const int64_t units = c->sequences * c->kv_heads * p->blocks, room = c->table_cols * c->page_size;
   if (units > 0x7FFFFFFF) return LACT_ERR_SHAPE;
   const int64_t tokens = std::min(window > 0 ? window + step - 1 : room, room);   // of a unit, at most
-  auto tiles = [&](int warps) { return (tokens + step * warps - 1) / (step * warps); };
-  p->warps = 4;
-  int64_t ctas = static_cast<int64_t>(sm_count()) * kPagedPerSm(p->nq, 4);
+  const int64_t tiles = (tokens + step * kPagedWarps - 1) / (step * kPagedWarps);
+  const int per_sm = kPagedPerSm(p->nq);
+  const int64_t ctas = static_cast<int64_t>(sm_count()) * per_sm;
   p->runs = 0;
   p->cluster = 1;
-  while (p->cluster < 8 && p->cluster < tiles(4) && 2 * p->cluster * units <= ctas) p->cluster *= 2;
-  if (tiles(4) > dw * p->cluster) {
+  while (p->cluster < 8 && p->cluster < tiles && 2 * p->cluster * units <= ctas) p->cluster *= 2;
+  if (tiles > (p->cluster > 1 ? kPagedClustered * p->cluster : kPagedWhole)) {
     p->cluster = 1;
-    p->runs = static_cast<int>(std::min({ctas, (units * tiles(p->warps) + dl - 1) / dl, static_cast<int64_t>(kPagedJoinMost)}));
+    p->runs = static_cast<int>(std::min({ctas, (units * tiles + kPagedLeast - 1) / kPagedLeast, static_cast<int64_t>(kPagedJoinMost)}));
   }
   const int64_t rows = std::min<int64_t>(share, 8 * p->nq), sums = rows * kPagedPieceRow(static_cast<int>(c->head_dim)) * 4;
   p->bytes = static_cast<size_t>(p->runs) * (2 * sums + sizeof(PagedCut));
   const int64_t stage = 2 * step * (row_bytes + (c->k_exponent != nullptr ? 1 : 0));
   // (a cluster's CTAs have their own sums added up beside their warps'; 3 KB: alignment, and what the kernel has beside)
-  const int64_t room_cta = 227 * 1024 / kPagedPerSm(p->nq, p->warps) - 3072, at_end = (p->warps + (p->cluster > 1 ? 1 : 0)) * sums;
-  p->stages = static_cast<int>(std::min<int64_t>(kPagedStages, (room_cta - at_end) / (p->warps * stage)));
+  const int64_t room_cta = 227 * 1024 / per_sm - 3072, at_end = (kPagedWarps + (p->cluster > 1 ? 1 : 0)) * sums;
+  p->stages = static_cast<int>(std::min<int64_t>(kPagedStages, (room_cta - at_end) / (kPagedWarps * stage)));
   p->long_stages = std::min<int>(p->stages, static_cast<int>(std::max<int64_t>(1, 8192 / stage)));
-  p->smem = static_cast<size_t>(p->warps * p->stages * stage + at_end) + 1024;
+  p->smem = static_cast<size_t>(kPagedWarps * p->stages * stage + at_end) + 1024;
   return LACT_OK;
 }
-template <int D, bool E4, int NQ, int W>
+template <int D, bool E4, int NQ>
 int launch_paged_step(const lact_paged_cache* c, const PagedStepArgs& a, size_t smem, cudaStream_t st) {
-  auto kernel = paged_step_kernel<D, E4, NQ, W>;
+  auto kernel = paged_step_kernel<D, E4, NQ, kPagedWarps>;
   CUtensorMap k_map, v_map;
   constexpr int64_t cols = E4 ? D / 2 : D;   // of 16 bits
   const int64_t rows = c->kv_heads * c->page_size;
@@ -2497,13 +2502,13 @@ int launch_paged_step(const lact_paged_cache* c, const PagedStepArgs& a, size_t 
   int dev = 0;
   LACT_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || (allowed.load(std::memory_order_relaxed) >> dev & 1) == 0) {
-    LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 / kPagedPerSm(NQ, W) - 2048));
+    LACT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 / kPagedPerSm(NQ) - 2048));
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   const int64_t grid = a.runs > 0 ? a.runs : static_cast<int64_t>(a.c.sequences) * a.c.heads * a.blocks * a.cluster;
   if (grid > 0x7FFFFFFF) return LACT_ERR_SHAPE;
   if (a.cluster == 1) {
-    { KernelScope scope(kClsOther, st); LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(W * 32), smem, st, a, k_map, v_map)); }
+    { KernelScope scope(kClsOther, st); LACT_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kPagedWarps * 32), smem, st, a, k_map, v_map)); }
     if (a.runs == 0) return LACT_OK;
     // as many groups as have eight pieces each at a time
     const int64_t rows = std::min(a.share, 8 * NQ), units = static_cast<int64_t>(a.c.sequences) * a.c.heads * a.blocks, pieces = a.runs / units + 2;
@@ -2517,7 +2522,7 @@ int launch_paged_step(const lact_paged_cache* c, const PagedStepArgs& a, size_t 
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(W * 32);
+  cfg.blockDim = dim3(kPagedWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -3750,7 +3755,7 @@ int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t 
   a.heads = static_cast<int32_t>(heads); a.share = static_cast<int32_t>(heads / c->kv_heads); a.blocks = p.blocks;
   a.window = static_cast<int32_t>(std::min<int64_t>(window, 0x7FFFFFFF));
   a.scale = softmax_scale * 1.4426950408889634f;
-  a.runs = p.runs; a.least = getenv("DEV_LEAST") ? atoi(getenv("DEV_LEAST")) : 2;
+  a.runs = p.runs; a.least = kPagedLeast;
   a.cuts = static_cast<PagedCut*>(workspace);
   a.pieces = reinterpret_cast<float*>(a.cuts + p.runs);
   a.status = status_word;
@@ -3760,7 +3765,7 @@ int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t 
   auto launch = [&](auto d, auto e4) {
     constexpr int D = decltype(d)::value;
     constexpr bool E4 = decltype(e4)::value;
-    return p.nq == 2 ? launch_paged_step<D, E4, 2, 4>(c, a, p.smem, st) : launch_paged_step<D, E4, 1, 4>(c, a, p.smem, st);
+    return p.nq == 2 ? launch_paged_step<D, E4, 2>(c, a, p.smem, st) : launch_paged_step<D, E4, 1>(c, a, p.smem, st);
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

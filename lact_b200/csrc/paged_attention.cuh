@@ -2,26 +2,37 @@
 //   o = sum_p w_p v_p / sum_p w_p,   w_p = 2^(x_p - m),  x_p = scale log2(e) q k_p,   p over the last `window` positions of the length.
 // Bound by memory: the window's keys and values once; the g query heads of a kv head make 2 g flops of a byte of bf16, 4 g of 8 bits.
 // Up to 8 (or 16) of them are the columns of m16n8k16 products with 16 tokens or 16 features as rows.  Those are warp products on
-// registers, not tcgen05: fragments come straight from global memory, since the order of a product's inner axis is free (K: a lane's
-// 32 bytes of a row are four (8 bits: eight) steps' pieces of that row; V: a lane holds the same features of four tokens, and byte
-// permutes pair the tokens), so nothing passes through shared memory, and 16 tokens of 128 take 16 products while 8 KB arrive.
-// The maximum m is raised only when a score passes it by 8 (weights up to 2^8 lose nothing), so that a step of 16 tokens needs one vote
-// in place of a reduction.  Weights are rounded for the product with V: in two bf16 pieces (2^-17 of each) with bf16 caches, to fp16
-// (2^-12) with 8 bits.  There, V is taken as e4m3, exact in fp16, and its powers of two multiply the weights: u_p = 2^(x_p + e_p - M)
-// with a maximum M of its own, against which small weights are rounded by 2^-25.  Queries become fp16 after scaling each by a power of
-// two, to a largest value of 2^14 (what is below 2^-38 of it is cut).  Sums are in fp32.
+// registers, not tcgen05, whose 128 rows are more tokens than a step has, and whose second product would want V turned over and the
+// weights written to tensor memory before it can begin: here a warp goes on by itself, and 16 tokens of 128 features take 24 products
+// while their 8 KB arrive (tensor pipe 15 to 17 % busy).  The order of a product's inner axis is free, so that no fragment is turned
+// over: of K a lane has 32 bytes of a row, four (8 bits: eight) steps' pieces of it; of V the same features of four tokens, which byte
+// permutes pair.
+// The maximum m is raised only when a score passes it by 8 (weights up to 2^8 lose nothing), so that a step needs one vote in place of a
+// reduction.  Weights are rounded for the product with V: in two bf16 pieces (2^-16 of each) with bf16 caches, to fp16 (2^-11) with 8
+// bits.  There, V is taken as e4m3, exact in fp16, and its powers of two multiply the weights: u_p = 2^(x_p + e_p - M) with a maximum M
+// of its own, against which small weights are rounded by 2^-25.  Queries become fp16 after scaling each by a power of two, to a largest
+// value of 2^14 (what is below 2^-38 of it is cut).  Sums are in fp32.
 //
-// Work: a unit is a (sequence, kv head, block of query heads), its tokens tiles of 16 a warp; lengths are known on the device alone.
-// All units' tiles, in order, are dealt out in even runs, one for each CTA, whatever the lengths are.  A run that holds all of a unit
-// writes its result; of a unit cut among runs each leaves a piece (sums, maxima), and a small launch adds the pieces in a fixed order.  Where units are few and have few tiles at most, or have very few (`runs` 0), a unit is a cluster of CTAs that share its tiles
-// evenly and read one another's sums from shared memory: no pieces, no counters.
+// Loads: every warp keeps a ring of steps of its own in shared memory (16 tokens of rows over 128 bytes, else 32), filled by tiled copies
+// with a swizzle that both kinds of fragment read without conflicts; a step's page number is looked up one step ahead.  A step is in
+// registers before its slot is filled again.  96 KB on their way in a SM is what bandwidth gains from (12 warps with one step of 8 KB; two
+// steps: step_window 170 in place of 162 us, step_long 103 and 100): longer runs use no more slots than that.
+//
+// Work: a unit is a (sequence, kv head, block of query heads), its tokens tiles of one step a warp; lengths are known on the device alone.
+// All units' tiles, in order, are dealt out in even runs, one for each CTA, whatever the lengths are (more runs than fit at once: two for
+// each place step_long 109 in place of 106 us, step_window 173 and 165).  A run that holds all of a unit writes its result; of a unit
+// cut among runs each leaves a piece (sums, maxima), and a small launch adds the pieces in a fixed order.  Where units are few and have few
+// tiles at most, or have very few (`runs` 0), a unit is a cluster of CTAs that share its tiles evenly and read one another's sums from
+// shared memory.
+// Measured (of the measured copy rate): 4 sequences of up to 131072 tokens, 16 heads on 4 of 128, bf16 95 us (94 %); 64 of up to 16384,
+// 32 on 8 of 128, 8 bits 184 us (96 %); 192 of up to 5000, a window of 2048, 12 heads of 64 159 us (97 %); one of 777, 12 heads 6.8 us.
 #pragma once
 #include "paged_cache.cuh"
 
 namespace lact {
 
-constexpr int kPagedStages = 8;   // at most
-constexpr int kPagedLong = 8;
+constexpr int kPagedStages = 8;   // slots of a warp at most
+constexpr int kPagedLong = 8;     // tiles up to which a run uses them all
 struct PagedStepArgs {
   PagedCache c;
   const bf16* q;                   // [sequences][heads][D], features adjacent, other strides in elements
@@ -173,8 +184,10 @@ __device__ __forceinline__ void paged_join_cluster(int ctas, const float* mine, 
   cluster_wait();
 }
 
-// CTAs of a SM, by registers: 12 warps of 168, or 8 of 255.
-__host__ __device__ constexpr int kPagedPerSm(int nq, int warps) { return (nq == 1 ? 12 : 8) / warps; }
+// CTAs of a SM, by registers: 12 warps of 168, or 8 of 255.  (One CTA of 12 warps: step_many 203 in place of 192 us, step_window 174 and 169:
+// nothing is computed while one adds up its warps' sums.)
+constexpr int kPagedWarps = 4;
+__host__ __device__ constexpr int kPagedPerSm(int nq) { return nq == 1 ? 3 : 2; }
 // 16 tokens of a step times this
 __host__ __device__ constexpr int kPagedSub(int row_bytes) { return row_bytes > 128 ? 1 : 2; }
 
@@ -193,7 +206,8 @@ __global__ void __launch_bounds__(512) paged_join_kernel(const float* pieces, co
   constexpr int ROW = kPagedPieceRow(D), ROWS = 256 / D, N = 8;   // rows of 64 times four sums
   __shared__ float factor[ROWS][kPagedJoinMost], scale[ROWS];
   __shared__ float4 part[7][64];
-  griddep_launch_dependents();
+  // (the next launch begins when this one ends: begun beside its blocks, which hold shared memory that three CTAs of the next call's kernel
+  // need, that finds fewer places: step_window 208 in place of 159 us, generate 62 and 48, call after call)
   griddep_wait();
   const PagedCut u = cuts[blockIdx.x];
   const int row0 = blockIdx.y * ROWS, rows = min(u.rows - row0, ROWS), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -261,7 +275,7 @@ __global__ void __launch_bounds__(512) paged_join_kernel(const float* pieces, co
 }
 
 template <int D, bool E4, int NQ, int W>
-__global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ, W)) paged_step_kernel(const __grid_constant__ PagedStepArgs a, const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(const __grid_constant__ PagedStepArgs a, const __grid_constant__ CUtensorMap k_map,
                                                             const __grid_constant__ CUtensorMap v_map) {
   constexpr int BYTES = E4 ? D : 2 * D;                  // of a row
   constexpr int SUB = kPagedSub(BYTES), STEP = 16 * SUB; // tokens of a step: 8 KB where rows allow
