@@ -69,6 +69,7 @@ __device__ __forceinline__ uint32_t transposed_8x8(uint32_t x) {
 struct PagedSpan {
   int first, last;   // positions [first, last)
   int tiles;
+  bool over;         // the length is past the table's end
 };
 template <int STEP, int TILE>
 __device__ __forceinline__ PagedSpan paged_span(const PagedStepArgs& a, int seq) {
@@ -76,6 +77,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedStepArgs& a, int seq)
   const int64_t room = static_cast<int64_t>(a.c.cols) << a.c.shift;
   const int len = max(a.c.lengths[seq], 0);
   s.last = static_cast<int>(min(static_cast<int64_t>(len), room));
+  s.over = len > room;
   s.first = a.window > 0 ? max(len - a.window, 0) : 0;
   s.first = min(s.first, s.last);
   s.tiles = max((s.last - (s.first & ~(STEP - 1)) + TILE - 1) / TILE, 1);
@@ -108,6 +110,7 @@ __device__ __forceinline__ uint2 ld_shared_8(uint32_t at) {
 struct PagedWalk {
   int seq, unit, t, t1, left;      // left: tiles of the run from this unit's first on
   int head, first, last, base, tiles;
+  bool over;                       // the length is past the table's end
   const int32_t* table;
 };
 
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
   }
   auto enter = [&](PagedWalk& w) {                       // seq, unit, t and left are set
     const PagedSpan span = paged_span<STEP, TILE>(a, w.seq);
-    w.first = span.first; w.last = span.last; w.tiles = span.tiles;
+    w.first = span.first; w.last = span.last; w.tiles = span.tiles; w.over = span.over;
     w.base = span.first & ~(STEP - 1);
     w.t1 = min(span.tiles, w.t + w.left);
     w.head = w.unit / a.blocks;
@@ -440,38 +443,32 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
   };
   for (int i = 0; i < stages; ++i) issue();
   bool failed = false;
-  // -------- its units
-  for (int64_t done = 0; use.left > 0 || a.cluster > 1;) {   // (of a cluster every CTA has one turn, with tiles or without)
-    if (done > 0) enter(use);
-    const int t0 = use.t, seq = use.seq, head = use.head, row0 = (use.unit - head * a.blocks) * ROWS, rows = min(a.share - row0, ROWS);
-    if (threadIdx.x == 0 && a.c.lengths[seq] > use.last && use.t1 == use.tiles) report_bad_page();
-    // queries: column r of a product is query head row0 + r (+ 8)
-    uint32_t q[NQ][QW];
-    float qm[NQ][2];                                     // what scores of columns 2 c, 2 c + 1 are multiplied by
+  // queries: column r of a product is query head row0 + r (+ 8); as they are, and as the products take them
+  uint32_t q[NQ][QW];
+  float qm[NQ][2];                                       // what scores of columns 2 c, 2 c + 1 are multiplied by
+  auto first_row = [&](const PagedWalk& w) { return (w.unit - w.head * a.blocks) * ROWS; };
+  auto load_q = [&](const PagedWalk& w) {
+    const int row0 = first_row(w), rows = min(a.share - row0, ROWS);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const bool on = n * 8 + r < rows;
-      const bf16* from = a.q + seq * a.q_bs + (static_cast<int64_t>(head) * a.share + row0 + n * 8 + r) * a.q_hs;
-      if constexpr (!E4) {
+      const bf16* from = a.q + w.seq * a.q_bs + (static_cast<int64_t>(w.head) * a.share + row0 + n * 8 + r) * a.q_hs;
 #pragma unroll
-        for (int i = 0; i < BOXES; ++i)
+      for (int e = 0; e < QW; e += 4) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        // (8 bits: QW words from c's on; else KW of each box)
+        if (n * 8 + r < rows) x = *reinterpret_cast<const uint4*>(from + (E4 ? c * (2 * QW) + e * 2 : e / KW * 64 + c * 16 + e % KW * 2));
+        q[n][e] = x.x; q[n][e + 1] = x.y; q[n][e + 2] = x.z; q[n][e + 3] = x.w;
+      }
+    }
+  };
+  auto ready_q = [&]() {
 #pragma unroll
-          for (int e = 0; e < KW; e += 4) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (on) w = *reinterpret_cast<const uint4*>(from + i * 64 + c * 16 + e * 2);
-            q[n][i * KW + e] = w.x; q[n][i * KW + e + 1] = w.y; q[n][i * KW + e + 2] = w.z; q[n][i * KW + e + 3] = w.w;
-          }
-        qm[n][0] = qm[n][1] = a.scale;
-      } else {
-        uint32_t raw[QW], top = 0;
+    for (int n = 0; n < NQ; ++n) {
+      qm[n][0] = qm[n][1] = a.scale;
+      if constexpr (E4) {
+        uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < QW; e += 4) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (on) w = *reinterpret_cast<const uint4*>(from + c * (2 * QW) + e * 2);
-          raw[e] = w.x; raw[e + 1] = w.y; raw[e + 2] = w.z; raw[e + 3] = w.w;
-        }
-#pragma unroll
-        for (int i = 0; i < QW; ++i) top = __vmaxu2(top, raw[i] & 0x7FFF7FFFu);
+        for (int i = 0; i < QW; ++i) top = __vmaxu2(top, q[n][i] & 0x7FFF7FFFu);
         top = max(top & 0xFFFFu, top >> 16);
         top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
         top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -480,13 +477,20 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
         const float up = __uint_as_float(static_cast<uint32_t>(127 + 141 - e) << 23), down = a.scale * __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
 #pragma unroll
         for (int i = 0; i < QW; ++i) {
-          const __half2 h = __floats2half2_rn(__uint_as_float(raw[i] << 16) * up, __uint_as_float(raw[i] & 0xFFFF0000u) * up);
+          const __half2 h = __floats2half2_rn(__uint_as_float(q[n][i] << 16) * up, __uint_as_float(q[n][i] & 0xFFFF0000u) * up);
           q[n][i] = *reinterpret_cast<const uint32_t*>(&h);
         }
         qm[n][0] = __shfl_sync(0xFFFFFFFFu, down, c * 8);
         qm[n][1] = __shfl_sync(0xFFFFFFFFu, down, c * 8 + 4);
       }
     }
+  };
+  load_q(use);
+  // -------- its units
+  for (int64_t done = 0; use.left > 0 || a.cluster > 1;) {   // (of a cluster every CTA has one turn, with tiles or without)
+    const int t0 = use.t, row0 = first_row(use), rows = min(a.share - row0, ROWS);
+    if (threadIdx.x == 0 && use.over && use.t1 == use.tiles) report_bad_page();
+    ready_q();
     // -------- tiles: this warp's step of each
     float acc[NQ][MT][4], m[NQ][2], l[NQ][2];
     [[maybe_unused]] float M[NQ][2];
@@ -732,9 +736,16 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
         }
         if (r == 0) *reinterpret_cast<float4*>(to + D) = make_float4(m[n][e], l[n][e], E4 ? M[n][e] : m[n][e], 0.f);
       }
-    __syncthreads();
     const bool whole = use.t1 == use.tiles && t0 == 0, any = use.last > use.first;
-    const int64_t at = (static_cast<int64_t>(seq) * a.heads + static_cast<int64_t>(head) * a.share + row0) * D;
+    const int64_t at = (static_cast<int64_t>(use.seq) * a.heads + static_cast<int64_t>(use.head) * a.share + row0) * D, begin = run0 + done;
+    const int tiles = use.tiles;
+    done += use.t1 - t0;
+    leave(use, t0);
+    if (use.left > 0) {   // (the next unit's queries are on their way while this one's sums are added up)
+      enter(use);
+      load_q(use);
+    }
+    __syncthreads();
     if (a.cluster == 1 && whole) {
       paged_merge<D, W, ROW>(sums, sum_rows, rows, [&](int row, int d, const float4& sum, const float4& s) {
         store_bf16x4(a.o + at + row * D + d, sum, any ? exp2_ftz(s.z - s.x) / s.y : 0.f);
@@ -750,14 +761,9 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
         paged_join_cluster<D, W, ROW>(a.cluster, piece, rows, any, a.o + at);
         return;
       }
-      if (threadIdx.x == 0 && t0 == 0) {
-        const int64_t begin = run0 + done;               // the unit's first tile among all
-        a.cuts[blockIdx.x] = {at, rows, static_cast<int32_t>((begin + use.tiles - 1) / per - blockIdx.x) + 1};
-      }
+      if (threadIdx.x == 0 && t0 == 0) a.cuts[blockIdx.x] = {at, rows, static_cast<int32_t>((begin + tiles - 1) / per - blockIdx.x) + 1};
     }
     __syncthreads();
-    done += use.t1 - t0;
-    leave(use, t0);
   }
 }
 
