@@ -432,7 +432,7 @@ typedef struct lact_paged_cache {
 int lact_paged_cache_write(const lact_paged_cache *cache, const void *k, int64_t k_ts, int64_t k_bs, int64_t k_hs, const void *v,
                            int64_t v_ts, int64_t v_bs, int64_t v_hs, int64_t batch, int64_t tokens, const int32_t *cu_seqlens,
                            void *stream);
-/* The same rows back: out [2, batch, tokens, kv_heads, head_dim] bf16 (keys, then values), 16-byte aligned; rows without a position
+/* The same rows back: out [2, batch, tokens, kv_heads, head_dim] bf16 (keys, then values), 32-byte aligned; rows without a position
  * are zeros. */
 int lact_paged_cache_read(const lact_paged_cache *cache, void *out, int64_t batch, int64_t tokens, const int32_t *cu_seqlens,
                           void *stream);

@@ -2422,8 +2422,8 @@ template <int D, bool E4>
 int launch_paged_rows(const PagedRows& a, bool write, int64_t grid, cudaStream_t st) {
   KernelScope scope(kClsOther, st);
   const dim3 blocks(static_cast<unsigned>(grid));
-  if (write) LACT_CUDA(launch_pdl(paged_rows_kernel<D, E4, true>, blocks, dim3(kPagedThreads), 0, st, a));
-  else LACT_CUDA(launch_pdl(paged_rows_kernel<D, E4, false>, blocks, dim3(kPagedThreads), 0, st, a));
+  if (write) LACT_CUDA(launch_pdl(paged_rows_kernel<D, E4, true, E4 ? 2 : 4, E4 ? 4 : 3>, blocks, dim3(kPagedThreads), 0, st, a));
+  else LACT_CUDA(launch_pdl(paged_rows_kernel<D, E4, false, E4 ? 2 : 4, E4 ? 5 : 4>, blocks, dim3(kPagedThreads), 0, st, a));
   return LACT_OK;
 }
 int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t tokens, const int32_t* cu, bool write, cudaStream_t st) {
@@ -2433,15 +2433,17 @@ int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t
   a.cu = cu;
   a.tokens = entries * tokens;
   a.L = static_cast<int32_t>(tokens);
-  // as many thread groups a token as leave each four heads at most, and more where the call is small
-  const int64_t groups = kPagedThreads / (c->head_dim / 8);
+  const bool e4 = c->k_exponent != nullptr;
+  // As many thread groups a token as leave each four heads at most (28080 tokens of 12 heads of 128, 1, 2 and 4 groups: bf16 written in 58.5, 56.4
+  // and 54.5 us, read in 59.1, 56.5 and 55.7), three where they are read in 8 bits (50.8, 46.2, 44.4), eight where they are written in 8 bits
+  // (48.4, 44.2, 48.1: the fewer, the more of a page's neighbouring rows a block writes); more where the call is small.
+  const int64_t groups = kPagedThreads / kPagedLanes(static_cast<int>(c->head_dim), e4), most = !e4 ? 4 : write ? 8 : 3;
   int64_t share = 1;
-  while (2 * share <= groups && (share * kPagedAhead < c->kv_heads || (share < c->kv_heads && a.tokens * share < groups * 2 * sm_count()))) share *= 2;
+  while (2 * share <= groups && (share * most < c->kv_heads || (share < c->kv_heads && a.tokens * share < groups * 2 * sm_count()))) share *= 2;
   a.share = static_cast<int32_t>(share);
   const int64_t n = groups / share;
   const int64_t grid = (a.tokens + n - 1) / n;
   if (grid > 0x7FFFFFFF) return LACT_ERR_SHAPE;
-  const bool e4 = c->k_exponent != nullptr;
   if (c->head_dim == 64) return e4 ? launch_paged_rows<64, true>(a, write, grid, st) : launch_paged_rows<64, false>(a, write, grid, st);
   return e4 ? launch_paged_rows<128, true>(a, write, grid, st) : launch_paged_rows<128, false>(a, write, grid, st);
 }
@@ -3721,7 +3723,7 @@ int lact_paged_cache_write(const lact_paged_cache* c, const void* k, int64_t k_t
 int lact_paged_cache_read(const lact_paged_cache* c, void* out, int64_t batch, int64_t tokens, const int32_t* cu_seqlens, void* stream) {
   LACT_TRY(paged_check(c));
   if (out == nullptr) return LACT_ERR_NULL;
-  if ((reinterpret_cast<uintptr_t>(out) & 15) != 0) return LACT_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(out) & 31) != 0) return LACT_ERR_SHAPE;
   PagedRows a;
   std::memset(&a, 0, sizeof(a));
   a.out = static_cast<bf16*>(out);

@@ -2,6 +2,7 @@
 // allocates through PyTorch, validates, and enqueues through the C ABI of liblact_b200.so; no kernel lives here.
 #pragma once
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -59,6 +60,8 @@ inline void no_tangents(const char* what, std::initializer_list<const Tensor*> t
 inline void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 inline Tensor empty(at::IntArrayRef shape, at::ScalarType dt, const Tensor& like) {
+  // (past the dispatcher: 0.6 us less of a call that waits for the host)
+  if (like.is_cuda() && like.layout() == at::kStrided) return Tensor(at::detail::empty_cuda(shape, dt, like.device(), std::nullopt));
   return at::empty(shape, like.options().dtype(dt).requires_grad(false));
 }
 inline Tensor bytes(size_t n, const Tensor& like) {

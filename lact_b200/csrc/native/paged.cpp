@@ -40,6 +40,9 @@ void check_cache(const char* what, const Tensor& k, const Tensor& v, const OptTe
   TORCH_CHECK_VALUE(!k.is_cpu(), what, " needs CUDA tensors (there is no CPU implementation)");
 }
 
+// Whole numbers as the kernels read them: what 31 bits do not hold stays past every end
+Tensor as_int(const Tensor& t) { return t.scalar_type() == at::kInt ? t : t.clamp(-1, INT32_MAX).to(at::kInt); }
+
 // What a call keeps alive of its arguments, and the description of the cache.
 struct Cache {
   lact_paged_cache c{};
@@ -47,9 +50,9 @@ struct Cache {
 };
 Cache describe(const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve, const Tensor& table, const Tensor& lengths) {
   Cache r;
-  r.table = table.to(at::kInt);
+  r.table = as_int(table);
   if (r.table.size(1) > 1 && r.table.stride(1) != 1) r.table = r.table.contiguous();
-  r.lengths = lengths.to(at::kInt).contiguous();
+  r.lengths = as_int(lengths).contiguous();
   r.c.k = ptr(k); r.c.v = ptr(v);
   r.c.k_exponent = ptr(ke); r.c.v_exponent = ptr(ve);
   r.c.pages = k.size(0); r.c.kv_heads = k.size(1); r.c.page_size = k.size(2); r.c.head_dim = k.size(3);
@@ -76,7 +79,7 @@ Tensor bounds(const OptTensor& cu, int64_t sequences, int64_t batch, const Tenso
   TORCH_CHECK_TYPE(whole_number(*cu), "cu_seqlens: whole numbers");
   TORCH_CHECK_VALUE(cu->dim() == 1 && cu->size(0) == sequences + 1, "cu_seqlens: [sequences + 1]");
   TORCH_CHECK_VALUE(cu->device() == like.device(), "all tensors must be on the same device");
-  return cu->to(at::kInt).contiguous();
+  return as_int(*cu).contiguous();
 }
 
 // The addresses that a tensor's elements lie between

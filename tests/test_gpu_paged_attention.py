@@ -123,6 +123,14 @@ def test_every_cut(lo, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,share", [(1, 12), (3, 16), (1, 40)])
+def test_cut_units_of_many_heads(lo, bits, d, heads, share):
+    _check(lo, [9999, 30, 0, 14000, 5000], heads, share, d, 32, bits)
+    _check(lo, [4000] * 20, heads, share, d, 16, bits, window=1500)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 5.0])
 def test_scales(lo, bits, scale):
     """Sharp weights, too: maxima that rise many times, weights that vanish."""

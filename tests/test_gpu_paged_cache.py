@@ -167,6 +167,25 @@ def test_a_page_that_is_not_there_is_left_out_and_told(lo):
         lo.L.synchronize_and_check()
 
 
+def test_numbers_of_64_bits_stay_out_of_range(lo):
+    """A page number or a length that 32 bits would make a valid one is left out and told."""
+    c = _filled(lo, 6, 16, 1, 64, 16)
+    x = _rn(2, 1, 1, 64).to(BF16)
+    table = torch.tensor([[(1 << 32) + 1], [2]], device="cuda")
+    lo.L.synchronize_and_check()
+    lo.paged_cache_write(c, x, x, table, torch.tensor([1, 1], device="cuda"))
+    with pytest.raises(lo.L.LactError):
+        lo.L.synchronize_and_check()
+    assert bool((_bytes(c.k)[1] == 0x31).all()) and torch.equal(c.k[2, 0, 0], x[1, 0, 0])
+    lo.paged_cache_write(c, x, x, table.clamp(max=3), torch.tensor([(1 << 32) + 1, 0], device="cuda"))
+    with pytest.raises(lo.L.LactError):
+        lo.L.synchronize_and_check()
+    assert bool((_bytes(c.k)[3] == 0x31).all())
+    lo.paged_cache_write(c, x, x, table.clamp(max=3), torch.tensor([-(1 << 40), 0], device="cuda"))
+    lo.L.synchronize_and_check()
+    assert bool((_bytes(c.k)[3] == 0x31).all())
+
+
 def test_bounds_that_fall_or_pass_the_end_stay_inside(lo):
     c = _filled(lo, 8, 16, 1, 64, 16)
     lengths = torch.tensor([16, 16, 16], dtype=I32, device="cuda")

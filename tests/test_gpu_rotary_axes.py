@@ -138,6 +138,22 @@ def test_what_is_not_turned_is_copied_and_stays_apart(lo):
     assert bool(y.isfinite()[~spoiled].all()) and not bool(y.isfinite()[spoiled].any())
 
 
+def test_frequencies_of_every_size(lo):
+    """Several turns a position, backwards, none; what is not finite makes its own pairs NaN."""
+    f = torch.tensor([0.0, -0.3, 7.0, -100.25, 1e6, 3.141592653589793, 1e-12, 2.5e9], device="cuda", dtype=torch.float64)
+    x, pos = _rn(1, 30, 2, 16), torch.randint(-9, 9, (30, 1), device="cuda")
+    for interleaved in (False, True):
+        y, _ = lo.rotary_axes(x, None, pos, f, [8], interleaved)
+        # (the formula's own angle, in 64 bits, is off by half a step of 2.25e10: 2^-19)
+        _near(y, orc.rotary_axes(x, pos, f, [8], interleaved), x, 8, interleaved, torch.float32, far=2.0 ** -18)
+    bad = f.clone()
+    bad[2], bad[5] = float("inf"), float("nan")
+    y, _ = lo.rotary_axes(x, None, pos, bad, [8])
+    lost = torch.zeros(16, dtype=torch.bool, device="cuda")
+    lost[[2, 5, 10, 13]] = True
+    assert torch.equal(y.isnan(), lost.expand_as(y))
+
+
 def test_gradients_against_differences(lo):
     """Linear: a difference over a step of any size is the derivative, up to the roundings of its two outputs (2^-24 of each, over the step)."""
     q, f = _rn(1, 5, 2, 16), lo.rotary_frequencies([5, 3], device="cuda")

@@ -109,7 +109,7 @@ def test_bad_calls_on_a_cache_are_refused(lib):
     for over, code in [(dict(k=None), -1), (dict(v=None), -1), (dict(v=C.c_void_p(4104)), -2), (dict(strides=(128, 640, 63, 128, 640, 64)), -2),
                        (dict(strides=(128, 640, 64, 129, 640, 64)), -2), (dict(batch=3), -5), (dict(batch=2, cu=P), -5), (dict(tokens=0), -2)]:
         assert _write(lib, c, **over) == code
-    for over, code in [(dict(out=None), -1), (dict(out=C.c_void_p(4104)), -2), (dict(batch=1), -5), (dict(tokens=0), -2)]:
+    for over, code in [(dict(out=None), -1), (dict(out=C.c_void_p(4112)), -2), (dict(batch=1), -5), (dict(tokens=0), -2)]:
         assert _read(lib, c, **over) == code
 
 
