@@ -2485,7 +2485,7 @@ int paged_step_plan(const lact_paged_cache* c, int64_t heads, int64_t window, Pa
   p->bytes = static_cast<size_t>(p->runs) * (2 * sums + sizeof(PagedCut));
   const int64_t stage = 2 * step * (row_bytes + (c->k_exponent != nullptr ? 1 : 0));
   // (a cluster's CTAs have their own sums added up beside their warps'; 3 KB: alignment, and what the kernel has beside)
-  const int64_t room_cta = 227 * 1024 / per_sm - 3072, at_end = (kPagedWarps + (p->cluster > 1 ? 1 : 0)) * sums;
+  const int64_t room_cta = 227 * 1024 / per_sm - 3 * 1024, at_end = (kPagedWarps + (p->cluster > 1 ? 1 : 0)) * sums;
   p->stages = static_cast<int>(std::min<int64_t>(kPagedStages, (room_cta - at_end) / (kPagedWarps * stage)));
   p->long_stages = std::min<int>(p->stages, static_cast<int>(std::max<int64_t>(1, 8192 / stage)));
   p->smem = static_cast<size_t>(kPagedWarps * p->stages * stage + at_end) + 1024;

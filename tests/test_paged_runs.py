@@ -51,7 +51,7 @@ def _plan(c):
     stage = 2 * step * (c["row_bytes"] + e4)
     sums = min(c["share"], 8 * nq) * (c["d"] + 4) * 4
     at_end = (WARPS + (cluster > 1)) * sums
-    stages = min(STAGES, (227 * 1024 // per_sm - 3072 - at_end) // (WARPS * stage))
+    stages = min(STAGES, (227 * 1024 // per_sm - 3 * 1024 - at_end) // (WARPS * stage))
     assert stages >= 1 and WARPS * stages * stage + at_end + 1024 <= 227 * 1024 // per_sm - 2048
     return runs, cluster, stages, min(stages, max(1, 8192 // stage)), blocks, step
 
