@@ -2353,11 +2353,12 @@ int norm_args(const lact_group_norm_config* c, const NormPlan& p, const void* x,
 // ------------------------------------------------------------------------------------------ rotary positions
 template <class T, int V>
 int launch_rotary(RotaryArgs a, bool halves, cudaStream_t st) {
-  // Thread groups that share a token: as many as leave each six heads (two turns of three: 65536 tokens of 24 heads of 128 in bf16 with
-  // 1, 2, 4 and 8 groups 137, 129, 125 and 135 us), more where there would be fewer than four blocks a SM, for each of which it has a head.
+  // Thread groups that share a token: as many as leave each three heads, one turn whose loads are on their way ahead of the angles (65536 tokens of
+  // 24 heads of 128 in bf16 with 1, 2, 4 and 8 groups 152, 139, 129 and 124 us), more where there would be fewer than four blocks a SM, for
+  // each of which it has a head.
   const int64_t groups = kRotaryThreads / (a.d / (2 * V)), heads = a.heads[0] + a.heads[1];
   int64_t share = 1;
-  while (2 * share <= std::min(groups, heads) && (heads >= 12 * share || a.tokens * share < groups * 4 * sm_count())) share *= 2;
+  while (2 * share <= std::min(groups, heads) && (heads > 3 * share || a.tokens * share < groups * 4 * sm_count())) share *= 2;
   a.share = static_cast<int32_t>(share);
   a.per_block = static_cast<int32_t>(groups / share);
   const int64_t grid = (a.tokens + a.per_block - 1) / a.per_block;
@@ -2429,6 +2430,7 @@ int launch_paged_rows(const PagedRows& a, bool write, int64_t grid, cudaStream_t
 int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t tokens, const int32_t* cu, bool write, cudaStream_t st) {
   if (entries < 1 || tokens < 1 || tokens > (1ll << 30) || entries * tokens > (1ll << 36)) return LACT_ERR_SHAPE;
   if (cu == nullptr ? entries != c->sequences : entries != 1) return LACT_ERR_CONFIG;
+  LACT_TRY(check_device());
   a.c = paged_args(c);
   a.cu = cu;
   a.tokens = entries * tokens;
@@ -2470,7 +2472,7 @@ int paged_step_plan(const lact_paged_cache* c, int64_t heads, int64_t window, Pa
   p->blocks = ceil_div(share, 8 * p->nq);
   const int64_t units = c->sequences * c->kv_heads * p->blocks, room = c->table_cols * c->page_size;
   if (units > 0x7FFFFFFF) return LACT_ERR_SHAPE;
-  const int64_t tokens = std::min(window > 0 ? window + step - 1 : room, room);   // of a unit, at most
+  const int64_t tokens = window > 0 && window < room ? std::min(window + step - 1, room) : room;   // of a unit, at most
   const int64_t tiles = (tokens + step * kPagedWarps - 1) / (step * kPagedWarps);
   const int per_sm = kPagedPerSm(p->nq);
   const int64_t ctas = static_cast<int64_t>(sm_count()) * per_sm;

@@ -3,7 +3,7 @@
 //   (x, y) -> (x cos t - y sin t,  y cos t + x sin t);   the gradient turns by -t (`sign`).
 // Pairs are (j, j + P) or neighbours (2j, 2j + 1); elements from 2 P on are copied.
 // Bound by memory: every element is read and written once.  A block takes several tokens, works out their cosines and sines once into
-// shared memory, and each thread keeps those of its V pairs in registers while it goes through its share of the token's heads (queries
+// shared memory, and each thread keeps those of its V pairs in registers for its share of the token's heads (queries
 // first, then keys).  Angles are whole numbers of 2^-64 turns, in which products with a position drop full turns by themselves: what a
 // position of 2^31 is off by is 2^-25 of a turn, from the frequency in fp64.
 #pragma once
@@ -65,6 +65,33 @@ __global__ void __launch_bounds__(kRotaryThreads, PER_SM) rotary_kernel(const __
       l %= a.L;
     }
   };
+  const int nc = a.d / (2 * V), c = threadIdx.x % nc, slot = threadIdx.x / nc;
+  const int tok = slot / a.share, part = slot - tok * a.share;
+  const int64_t t = t0 + tok;
+  const int all = tok < here ? a.heads[0] + a.heads[1] : 0;   // (behind the last token: none)
+  int64_t b;
+  int l;
+  token(tok, b, l);
+  // This thread's two accesses of V features: of halves, those of V pairs (or two that are copied); of neighbours one in each half of
+  // the head, V / 2 pairs each (accesses next to one another would leave every other one to a second instruction: 185 against 160 us
+  // for 32760 tokens of 24 heads of 128, forward and backward); single features are a pair's two.
+  constexpr bool APART = !HALVES && V > 1;
+  const bool turned[2] = {APART ? c * V < 2 * a.P : c * V < a.P, APART ? (c + nc) * V < 2 * a.P : c * V < a.P};
+  const int first = APART || (HALVES && turned[0]) ? c * V : 2 * c * V, second = APART ? (c + nc) * V : HALVES && turned[0] ? a.P + c * V : 2 * c * V + V;
+  using Raw = RawOf<T, V>;
+  Raw ra[N], rb[N];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int h = h0 + k * a.share;
+      if (h >= all) continue;
+      const int w = h >= a.heads[0];
+      const T* x = static_cast<const T*>(a.x[w]) + b * a.bs[w] + l * a.ts[w] + (w ? h - a.heads[0] : h) * a.hs[w];
+      ra[k] = load_raw<T, V>(x + first);
+      rb[k] = load_raw<T, V>(x + second);
+    }
+  };
+  fetch(part);   // (on their way while the angles are worked out: 12243 tokens of 8 heads of 64 in fp32 11.1 -> 10.4 us)
   {
     // a thread has one pair, of every so many tokens
     const int j = threadIdx.x % a.P, rows = kRotaryThreads / a.P;
@@ -86,19 +113,7 @@ __global__ void __launch_bounds__(kRotaryThreads, PER_SM) rotary_kernel(const __
     }
   }
   __syncthreads();
-  const int nc = a.d / (2 * V), c = threadIdx.x % nc, slot = threadIdx.x / nc;
-  const int tok = slot / a.share, part = slot - tok * a.share;
-  if (tok >= here) return;
-  const int64_t t = t0 + tok;
-  int64_t b;
-  int l;
-  token(tok, b, l);
-  // This thread's two accesses of V features: of halves, those of V pairs (or two that are copied); of neighbours one in each half of
-  // the head, V / 2 pairs each (accesses next to one another would leave every other one to a second instruction: 185 against 160 us
-  // for 32760 tokens of 24 heads of 128, forward and backward); single features are a pair's two.
-  constexpr bool APART = !HALVES && V > 1;
-  const bool turned[2] = {APART ? c * V < 2 * a.P : c * V < a.P, APART ? (c + nc) * V < 2 * a.P : c * V < a.P};
-  const int first = APART || (HALVES && turned[0]) ? c * V : 2 * c * V, second = APART ? (c + nc) * V : HALVES && turned[0] ? a.P + c * V : 2 * c * V + V;
+  if (all == 0) return;
   float co[V], si[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -109,19 +124,8 @@ __global__ void __launch_bounds__(kRotaryThreads, PER_SM) rotary_kernel(const __
     co[e] = rotary_smem[at];
     si[e] = rotary_smem[a.per_block * a.P + at];
   }
-  const int all = a.heads[0] + a.heads[1];
-  using Raw = RawOf<T, V>;
   for (int h0 = part; h0 < all; h0 += N * a.share) {
-    Raw ra[N], rb[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int h = h0 + k * a.share;
-      if (h >= all) continue;
-      const int w = h >= a.heads[0];
-      const T* x = static_cast<const T*>(a.x[w]) + b * a.bs[w] + l * a.ts[w] + (w ? h - a.heads[0] : h) * a.hs[w];
-      ra[k] = load_raw<T, V>(x + first);
-      rb[k] = load_raw<T, V>(x + second);
-    }
+    if (h0 != part) fetch(h0);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int h = h0 + k * a.share;

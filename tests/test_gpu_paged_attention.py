@@ -102,7 +102,7 @@ def test_heads(lo, bits, d, heads, share):
 
 @pytest.mark.parametrize("bits", [16, 8])
 @pytest.mark.parametrize("size", [16, 32, 64, 128, 256])
-@pytest.mark.parametrize("window", [None, 1, 15, 16, 17, 100, 383, 1024, 100000])
+@pytest.mark.parametrize("window", [None, 1, 15, 16, 17, 100, 383, 1024, 100000, 2 ** 63 - 1])
 def test_windows_and_pages(lo, bits, size, window):
     _check(lo, LENGTHS, 2, 4, 64 if size == 32 else 128, size, bits, window)
 

@@ -154,6 +154,44 @@ def test_frequencies_of_every_size(lo):
     assert torch.equal(y.isnan(), lost.expand_as(y))
 
 
+@pytest.mark.parametrize("h,hk,d", [(96, 12, 128), (40, 0, 96), (24, 24, 512), (7, 1, 6)])
+def test_many_heads(lo, h, hk, d):
+    q, k = _rn(2, 33, h, d).to(BF16), _rn(2, 33, hk, d, seed=1).to(BF16) if hk else None
+    _check(lo, q, k, torch.randint(0, 999, (33, 1), device="cuda"), [d // 2], True)
+    _check(lo, q, k, torch.randint(0, 999, (33, 1), device="cuda"), [d // 2 - 1], False)
+
+
+def test_shared_keys_get_the_sum_of_their_gradients(lo):
+    """Keys broadcast over heads and entries: the gradient of the one they come from."""
+    f, pos = lo.rotary_frequencies([32], device="cuda"), torch.arange(7, device="cuda")[:, None]
+    k, dy = _rn(1, 7, 1, 64).requires_grad_(), _rn(3, 7, 4, 64, seed=2)
+    y, _ = lo.rotary_axes(k.expand(3, 7, 4, 64), None, pos, f, [32])
+    dk, = torch.autograd.grad(y, k, dy)
+    ref = k.detach().double().requires_grad_()
+    want, = torch.autograd.grad(orc.rotary_axes(ref.expand(3, 7, 4, 64), pos, f, [32]), ref, dy.double())
+    # (twelve terms, each off by 2^-21.5 of its pair's size and rounded, and eleven sums in fp32)
+    size = (dy.abs().sum((0, 2), keepdim=True).double() * 2).reshape(1, 7, 1, 64)
+    size = size + size.roll(32, -1)
+    assert bool(((dk.double() - want).abs() <= 2.0 ** -20 * size).all())
+
+
+def test_more_than_2_to_31_elements(lo):
+    """Every batch entry holds the same values and has to give the same bits as the first."""
+    if torch.cuda.get_device_properties(0).total_memory < 100e9:
+        pytest.skip("needs 100 GB")
+    b, l, h, hk, d = 9, 30001, 64, 2, 128
+    one = [_rn(1, l, n, d, seed=i).to(BF16) for i, n in enumerate((h, hk))]
+    f, pos = lo.rotary_frequencies([64], device="cuda"), torch.arange(l, device="cuda")[:, None]
+    q, k = (t.expand(b, -1, -1, -1).contiguous() for t in one)
+    assert q.numel() > 2 ** 31
+    y, z = lo.rotary_axes(q, k, pos, f, [64])
+    want = lo.rotary_axes(*one, pos, f, [64])
+    assert all(torch.equal(y[i], want[0][0]) and torch.equal(z[i], want[1][0]) for i in range(b))
+    del y, z
+    y, _ = lo.rotary_axes(q.view(1, b * l, h, d), None, pos.repeat(b, 1), f, [64])
+    assert all(torch.equal(y[0, i * l:(i + 1) * l], want[0][0]) for i in range(b))
+
+
 def test_gradients_against_differences(lo):
     """Linear: a difference over a step of any size is the derivative, up to the roundings of its two outputs (2^-24 of each, over the step)."""
     q, f = _rn(1, 5, 2, 16), lo.rotary_frequencies([5, 3], device="cuda")

@@ -100,6 +100,7 @@ def test_bad_calls_on_a_cache_are_refused(lib):
     assert size() == (0, 0)                                     # 64 positions: a CTA a unit, no pieces
     rc, nbytes = size(c=_cache(table_cols=4096))
     assert rc == 0 and nbytes > 0
+    assert size(window=2 ** 63 - 1, c=_cache(table_cols=4096)) == (0, nbytes)   # (as no window)
     assert size(heads=3)[0] == -2 and size(heads=0)[0] == -2 and size(window=-1)[0] == -2
     for over, code in [(dict(q=None), -1), (dict(o=None), -1), (dict(status=None), -1), (dict(o=C.c_void_p(4104)), -2), (dict(q=C.c_void_p(4104)), -2), (dict(q_bs=257), -2), (dict(q_hs=68), -2), (dict(heads=5), -2),
                        (dict(scale=float("nan")), -5), (dict(scale=float("inf")), -5)]:

@@ -38,7 +38,7 @@ def _plan(c):
     blocks = -(-c["share"] // (8 * nq))
     units = len(c["lengths"]) * c["heads"] * blocks
     room = c["cols"] * c["page"]
-    tokens = min(c["window"] + step - 1 if c["window"] else room, room)
+    tokens = min(c["window"] + step - 1, room) if 0 < c["window"] < room else room
     tiles = -(-tokens // (step * WARPS))
     per_sm = 3 if nq == 1 else 2
     ctas = SMS * per_sm
