@@ -50,7 +50,7 @@ __device__ __forceinline__ void turned_pair(float x, float y, float c, float s, 
 }
 
 constexpr int kRotaryThreads = 256;
-template <class T, int V, bool HALVES, int N, int PER_SM>   // N heads of a thread are fetched together
+template <class T, int V, bool HALVES, bool AHEAD, int N, int PER_SM>   // N heads of a thread are fetched together; AHEAD: all it has, ahead of the angles
 __global__ void __launch_bounds__(kRotaryThreads, PER_SM) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   extern __shared__ float rotary_smem[];   // cosines [per_block][P], sines
   griddep_launch_dependents();
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kRotaryThreads, PER_SM) rotary_kernel(const __
       rb[k] = load_raw<T, V>(x + second);
     }
   };
-  fetch(part);   // (on their way while the angles are worked out: 12243 tokens of 8 heads of 64 in fp32 11.1 -> 10.4 us)
+  if constexpr (AHEAD) fetch(part);
   {
     // a thread has one pair, of every so many tokens
     const int j = threadIdx.x % a.P, rows = kRotaryThreads / a.P;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kRotaryThreads, PER_SM) rotary_kernel(const __
     si[e] = rotary_smem[a.per_block * a.P + at];
   }
   for (int h0 = part; h0 < all; h0 += N * a.share) {
-    if (h0 != part) fetch(h0);
+    if constexpr (!AHEAD) fetch(h0);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int h = h0 + k * a.share;
