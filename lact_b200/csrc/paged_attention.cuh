@@ -13,7 +13,7 @@
 // of its own, against which small weights are rounded by 2^-25.  Queries become fp16 after scaling each by a power of two, to a largest
 // value of 2^14 (what is below 2^-38 of it is cut).  Sums are in fp32.
 //
-// Loads: every warp keeps a ring of steps of its own in shared memory (16 tokens of rows over 128 bytes, else 32), filled by tiled copies
+// Loads: every warp keeps a ring of steps of its own in shared memory (16 tokens of rows of 256 bytes, 32 of 128, 64 of 64), filled by tiled copies
 // with a swizzle that both kinds of fragment read without conflicts; a step's page number is looked up one step ahead.  A step is in
 // registers before its slot is filled again.  96 KB on their way in a SM is what bandwidth gains from (12 warps with one step of 8 KB; two
 // steps: step_window 170 in place of 162 us, step_long 103 and 100): longer runs use no more slots than that.
@@ -192,7 +192,7 @@ __device__ __forceinline__ void paged_join_cluster(int ctas, const float* mine, 
 constexpr int kPagedWarps = 4;
 __host__ __device__ constexpr int kPagedPerSm(int nq) { return nq == 1 ? 3 : 2; }
 // 16 tokens of a step times this
-__host__ __device__ constexpr int kPagedSub(int row_bytes) { return row_bytes > 128 ? 1 : 2; }
+__host__ __device__ constexpr int kPagedSub(int row_bytes) { return row_bytes > 128 ? 1 : row_bytes > 64 ? 2 : 4; }
 
 // A unit that begins in a run and does not end there: its result, and how many runs have pieces of it (0: there is none).
 struct PagedCut {
@@ -378,19 +378,20 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
     }
   };
   auto position = [&](const PagedWalk& w) { return w.base + (w.t * W + warp) * STEP; };
-  // A step lies in one page, or (pages of 16, steps of 32) in two; past the end none is looked up.
-  const bool split = SUB == 2 && a.c.shift == 4;
+  // A step lies in one page, or in `parts` of smaller ones; past the end none is looked up.
+  const int parts = max(STEP >> a.c.shift, 1), part_rows = min(STEP, 1 << a.c.shift), part_bytes = (STAGE + EB) / parts;
   auto pages_of = [&](const PagedWalk& w, int (&pg)[SUB]) {
     const int p = position(w), at = p >> a.c.shift;
     pg[0] = p < w.last ? w.table[at] : -1;
-    if constexpr (SUB == 2) pg[1] = split && p + 16 < w.last ? w.table[at + 1] : -1;
+#pragma unroll
+    for (int i = 1; i < SUB; ++i) pg[i] = i < parts && p + i * part_rows < w.last ? w.table[at + i] : -1;
   };
   enter(make);
   const int stages = make.left > kPagedLong ? a.long_stages : a.stages;
   PagedWalk use = make;
   int make_from = make.t, page[SUB], make_slot = 0, use_slot = 0;
   pages_of(make, page);
-  uint32_t has = 0, half = 0, phase = 0;                 // slots that hold a step, half of one; parities of their next waits
+  uint32_t has = 0, gone = 0, phase = 0;                 // slots that hold something; 16 tokens that are not there, SUB bits a slot; parities of the next waits
   // the copies of this warp's tokens of the next tile
   auto issue = [&]() {
     if (make.left <= 0) return;
@@ -414,23 +415,30 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
       }
       return real;
     };
-    const uint32_t bit = 1u << make_slot;
-    const bool first = there(page[0], 0);
-    if (!split) {
-      has = first ? has | bit : has & ~bit;
-      if (first) {
+    if (SUB == 1 || parts == 1) {
+      const bool real = there(page[0], 0);
+      has = real ? has | 1u << make_slot : has & ~(1u << make_slot);
+      if (real) {
         mbar_expect_tx_if(leader, bar, STAGE + EB);
         copy(page[0], 0, STEP, leader);
       }
     } else {
-      // (a half that is not there is left as it was, and counts as outside of the window)
-      const bool second = there(page[SUB - 1], 16);
-      has = first || second ? has | bit : has & ~bit;
-      half = (half & ~(bit | bit << 16)) | (first ? 0 : bit) | (second ? 0 : bit << 16);
-      if (first || second) {
-        mbar_expect_tx_if(leader, bar, first && second ? STAGE + EB : (STAGE + EB) / 2);
-        if (first) copy(page[0], 0, 16, leader);
-        if (second) copy(page[SUB - 1], 16, 16, leader);
+      // (a part that is not there is left as it was, and counts as outside of the window)
+      uint32_t on = 0;
+#pragma unroll
+      for (int i = 0; i < SUB; ++i)
+        if (i < parts && there(page[i], i * part_rows)) on |= 1u << i;
+      has = on != 0 ? has | 1u << make_slot : has & ~(1u << make_slot);
+      uint32_t lost = 0;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+        if ((on >> (u * 16 >> a.c.shift) & 1) == 0) lost |= 1u << u;
+      gone = (gone & ~(((1u << SUB) - 1) << make_slot * SUB)) | lost << make_slot * SUB;
+      if (on != 0) {
+        mbar_expect_tx_if(leader, bar, __popc(on) * part_bytes);
+#pragma unroll
+        for (int i = 0; i < SUB; ++i)
+          if (on >> i & 1) copy(page[i], i * part_rows, part_rows, leader);
       }
     }
     if (++make_slot == stages) make_slot = 0;
@@ -599,14 +607,14 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
           }
         }
       // tokens outside of the window: no weight, and no values (what lies there may be NaN)
-      if (p < use.first || p + STEP > use.last || (half >> slot & 0x10001u) != 0) {
-        const bool gone[2] = {(half >> slot & 1) != 0, (half >> slot >> 16 & 1) != 0};
+      const uint32_t lost = gone >> slot * SUB & ((1u << SUB) - 1);
+      if (p < use.first || p + STEP > use.last || lost != 0) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int at = p + 16 * u + r + 8 * h;
-            if (!gone[u] && at >= use.first && at < use.last) continue;
+            if ((lost >> u & 1) == 0 && at >= use.first && at < use.last) continue;
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -615,7 +623,7 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int at = p + 16 * u + 2 * c + (i & 1) + 8 * (i >> 1);
-            if (!gone[u] && at >= use.first && at < use.last) continue;
+            if ((lost >> u & 1) == 0 && at >= use.first && at < use.last) continue;
 #pragma unroll
             for (int e = 0; e < BOXES * VW; ++e) vr[u][i][e] = 0;
           }
@@ -632,9 +640,10 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
         for (int e = 0; e < 2; ++e) {
           top[n][e] = fmaxf(x[0][n][e], x[0][n][e + 2]);
           if constexpr (E4) high[n][e] = fmaxf(y[0][n][e], y[0][n][e + 2]);
-          if constexpr (SUB == 2) {
-            top[n][e] = fmaxf(top[n][e], fmaxf(x[1][n][e], x[1][n][e + 2]));
-            if constexpr (E4) high[n][e] = fmaxf(high[n][e], fmaxf(y[1][n][e], y[1][n][e + 2]));
+#pragma unroll
+          for (int u = 1; u < SUB; ++u) {
+            top[n][e] = fmaxf(top[n][e], fmaxf(x[u][n][e], x[u][n][e + 2]));
+            if constexpr (E4) high[n][e] = fmaxf(high[n][e], fmaxf(y[u][n][e], y[u][n][e + 2]));
           }
           raise = raise || top[n][e] > m[n][e] + 8.f;
           if constexpr (E4) raise = raise || high[n][e] > M[n][e] + 8.f;

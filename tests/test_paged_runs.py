@@ -33,7 +33,7 @@ def _span(length, window, room, step):
 
 def _plan(c):
     """As paged_step_plan: (runs, CTAs of a cluster, slots, slots of long runs, query blocks)."""
-    step = 32 if c["row_bytes"] <= 128 else 16
+    step = {256: 16, 128: 32, 64: 64}[c["row_bytes"]]
     nq = 2 if c["share"] > 8 else 1
     blocks = -(-c["share"] // (8 * nq))
     units = len(c["lengths"]) * c["heads"] * blocks
@@ -145,7 +145,7 @@ def test_every_tile_once_and_every_piece_found(seed):
             for w in range(WARPS):
                 p = base + (t * WARPS + w) * step
                 if p < last:
-                    assert p // c["page"] < c["cols"] and p % c["page"] % 16 == 0 and (c["page"] == 16 or p % c["page"] + step <= c["page"])
+                    assert p // c["page"] < c["cols"] and p % c["page"] % 16 == 0 and (c["page"] < step or p % c["page"] + step <= c["page"])
                     covered |= set(range(p, min(p + step, last)))
         assert set(range(first, last)) <= covered
 
