@@ -259,8 +259,9 @@ class PagedCache(NamedTuple):
     [pages, kv_heads, page_size]): a row of a head stands for its values times 2 ** (byte - 127) (byte 255: NaN).  Pages are contiguous in
     themselves; page_size 16, 32, 64, 128 or 256, head_dim 64 or 128.  Which pages a sequence has says its row of a page table (int32
     [sequences, pages of the longest]): position p lies in page `page_table[i, p // page_size]`, row `p % page_size`; entries past its
-    length are not looked at.  An entry that the cache does not have, or a length past the table's end, is left out, and a later call
-    raises LactError.  Page tables and lengths are read on the device: a captured call follows what they hold at its replay."""
+    length are not looked at.  k and v begin on 32 bytes, exponents on 16, and page strides are multiples of as much.  An entry
+    that the cache does not have, or a length past the table's end, is left out, and a later call raises LactError (of a window with no
+    page at all, attention is NaN).  Page tables and lengths are read on the device: a captured call follows what they hold at its replay."""
     k: torch.Tensor
     v: torch.Tensor
     k_exponent: Optional[torch.Tensor] = None
