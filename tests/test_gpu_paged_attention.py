@@ -235,6 +235,20 @@ def test_pages_that_are_not_there(lo, bits):
     lo.L.synchronize_and_check()
 
 
+@pytest.mark.parametrize("lengths", [[90, 100], [90, 20000], [100] * 200])   # a cluster; cut units; one CTA a unit
+def test_a_window_without_a_page(lo, lengths):
+    c, table, n, _ = _cache(lo, lengths, 64, 2, 64, 16)
+    q = _rn(len(lengths), 4, 64).to(BF16)
+    want = lo.paged_attention_step(q, c, table, n)
+    bad = table.clone()
+    bad[1] = -1
+    lo.L.synchronize_and_check()
+    got = lo.paged_attention_step(q, c, bad, n)
+    with pytest.raises(lo.L.LactError, match="page number or a length"):
+        lo.L.synchronize_and_check()
+    assert bool(got[1].isnan().all()) and torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:])
+
+
 def test_layouts(lo):
     for bits in (16, 8):
         c, table, n, _ = _cache(lo, [600, 70, 0], 32, 2, 64, bits)
