@@ -378,13 +378,14 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
     }
   };
   auto position = [&](const PagedWalk& w) { return w.base + (w.t * W + warp) * STEP; };
-  // A step lies in one page, or in `parts` of smaller ones; past the end none is looked up.
+  // A step lies in one page, or in `parts` of smaller ones; those that hold nothing of the window are neither looked up nor copied (the
+  // user may have given them back).
   const int parts = max(STEP >> a.c.shift, 1), part_rows = min(STEP, 1 << a.c.shift), part_bytes = (STAGE + EB) / parts;
   auto pages_of = [&](const PagedWalk& w, int (&pg)[SUB]) {
     const int p = position(w), at = p >> a.c.shift;
-    pg[0] = p < w.last ? w.table[at] : -1;
+    pg[0] = p < w.last && p + part_rows > w.first ? w.table[at] : -1;
 #pragma unroll
-    for (int i = 1; i < SUB; ++i) pg[i] = i < parts && p + i * part_rows < w.last ? w.table[at + i] : -1;
+    for (int i = 1; i < SUB; ++i) pg[i] = i < parts && p + i * part_rows < w.last && p + (i + 1) * part_rows > w.first ? w.table[at + i] : -1;
   };
   enter(make);
   const int stages = make.left > kPagedLong ? a.long_stages : a.stages;
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
       }
     };
     auto there = [&](int pg, int at) {
-      const bool real = p + at < make.last;
+      const bool real = p + at < make.last && p + at + part_rows > make.first;
       if (real && static_cast<uint32_t>(pg) >= static_cast<uint32_t>(a.c.pages)) {
         if (lane == 0) report_bad_page();
         return false;

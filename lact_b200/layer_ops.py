@@ -258,8 +258,8 @@ class PagedCache(NamedTuple):
     """Keys and values in pages.  k, v [pages, kv_heads, page_size, head_dim]: bf16, or float8_e4m3fn with k_exponent, v_exponent (uint8
     [pages, kv_heads, page_size]): a row of a head stands for its values times 2 ** (byte - 127) (byte 255: NaN).  Pages are contiguous in
     themselves; page_size 16, 32, 64, 128 or 256, head_dim 64 or 128.  Which pages a sequence has says its row of a page table (int32
-    [sequences, pages of the longest]): position p lies in page `page_table[i, p // page_size]`, row `p % page_size`; entries past its
-    length are not looked at.  k and v begin on 32 bytes, exponents on 16, and page strides are multiples of as much.  An entry
+    [sequences, pages of the longest]): position p lies in page `page_table[i, p // page_size]`, row `p % page_size`; entries of pages without
+    a position that a call needs (past a sequence's length; in front of its window) are not looked at.  k and v begin on 32 bytes, exponents on 16, and page strides are multiples of as much.  An entry
     that the cache does not have, or a length past the table's end, is left out, and a later call raises LactError (of a window with no
     page at all, attention is NaN).  Page tables and lengths are read on the device: a captured call follows what they hold at its replay."""
     k: torch.Tensor
@@ -307,8 +307,9 @@ def paged_attention_step(q: torch.Tensor, cache: PagedCache, page_table: torch.T
     of positions `max(0, lengths[i] - window_size)` to `lengths[i] - 1` (`window_size` None: all; the new token's own are written before,
     and lengths count them).  The heads of the cache divide those of q (consecutive heads share).  softmax_scale: head_dim ** -0.5 by
     default.  Returns o [sequences, heads, head_dim] bf16; a sequence without tokens has zeros.  Scores, maxima and sums are float32; weights
-    are rounded to two bf16 pieces (bf16 cache) or to fp16 (8 bits) for their product with the values.  Rows outside of the window are not
-    read; a NaN within it makes its heads' outputs NaN.  No backward: a call with gradients raises."""
+    are rounded to two bf16 pieces (bf16 cache) or to fp16 (8 bits) for their product with the values.  Pages that hold
+    nothing of the window may have been given back (their entries are not looked at), and whatever other rows outside of it hold counts for
+    nothing; a NaN within it makes its heads' outputs NaN.  No backward: a call with gradients raises."""
     return L.call(_op("paged_attention_step"), q, *cache, page_table, lengths, int(window_size) if window_size else 0,
                   float(softmax_scale) if softmax_scale is not None else cache[0].shape[-1] ** -0.5)
 
