@@ -413,7 +413,7 @@ int lact_rotary_axes(const lact_rotary_config *cfg, const void *q, const void *k
  * bytes, 16-byte aligned, page strides multiples of 16) e4m3 values that stand for themselves times 2^(byte - 127), 255: NaN.  head_dim 64 or 128; page_size 16, 32, 64, 128 or 256.
  * Position p of sequence i lies in page page_table[i * table_stride + p / page_size], row p % page_size, for p below lengths[i];
  * table_cols * page_size at most 2^30.  Entries of the table whose page holds no position that a call needs (past a sequence's
- * length; in front of its window) are not looked at; a needed page or a position that the cache does not have is left out, and device status 102 goes to the host's word (lact_status_host_word).  No counterpart in the
+ * length; in front of its window) are not looked at; a needed page or a position that the cache does not have is left out, and device status 102 goes to the host's word (lact_status_host_word), if that holds nothing unread.  No counterpart in the
  * reference, whose cache is left to the attention library's caller (layer_lact_swiglu.py:328-343). */
 typedef struct lact_paged_cache {
   void *k, *v;

@@ -28,10 +28,11 @@ struct PagedCache {
   int32_t sequences;
 };
 
-// A page number or a length that the cache does not have is left out, and told to the host (which raises on its next call).
+// A page number or a length that the cache does not have is left out, and told to the host (which raises on its next call), unless something
+// is there already that the host has not read: a wait that ran out spoils more than the rows that are left out here.
 __device__ __forceinline__ void report_bad_page() {
   if (g_host_status != nullptr) {
-    *reinterpret_cast<volatile int32_t*>(g_host_status) = kStatusBadPage;
+    atomicCAS(g_host_status, static_cast<int32_t>(kStatusOk), static_cast<int32_t>(kStatusBadPage));
     __threadfence_system();
   }
 }
