@@ -3779,7 +3779,6 @@ int lact_paged_attention_step(const lact_paged_cache* c, const void* q, int64_t 
   if (c->head_dim == 64) return c->k_exponent != nullptr ? launch(D64{}, std::true_type{}) : launch(D64{}, std::false_type{});
   return c->k_exponent != nullptr ? launch(D128{}, std::true_type{}) : launch(D128{}, std::false_type{});
 }
-}
 
 // ------------------------------------------------------------------------------------------ linear attention
 int lact_linear_attention_workspace_bytes(const lact_linear_config* c, int32_t backward, size_t* bytes_out) {
@@ -4436,3 +4435,4 @@ int lact_bmm_bf16(const void* a, int32_t a_mn_major, const void* b, int32_t b_mn
   return launch_op<OpBmmStore, 1>(bt, fill_bf16, s, kClsOther, 1);
 }
 
+}  // extern "C"
