@@ -1,0 +1,35 @@
+"""Attention of single tokens where queries are very large and keys very small: scores of an ordinary size, whatever the factors that a kernel
+takes apart.  Tolerances: those of test_gpu_paged_attention (its docstring)."""
+import pytest
+import torch
+
+from oracle import lact_oracle as orc
+from test_gpu_paged_attention import BF16, _cache, _rn, _tolerance, lo  # noqa: F401  (a fixture)
+
+pytestmark = pytest.mark.gpu
+LENGTHS = [1, 40, 700, 5000]
+
+
+def _check(lo, c, table, n, stands, q, scale):  # noqa: F811
+    o = lo.paged_attention_step(q, c, table, n, None, scale)
+    lo.L.synchronize_and_check()
+    want, size, score = orc.paged_attention_step(q, *stands, table, LENGTHS, None, scale)
+    assert 0.5 < float(score.max()) < 1000.0                # (the softmax has something to do)
+    tol = _tolerance(q, want, size, score, LENGTHS, None, stands, table, c, scale)
+    assert bool(o.isfinite().all()) and bool(((o.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("share", [2, 12])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_large_queries_on_small_keys(lo, bits, d, share):  # noqa: F811
+    c, table, n, stands = _cache(lo, LENGTHS, 32, 2, d, bits)
+    small = 2.0 ** -118
+    if bits == 16:
+        c.k.mul_(small)
+    else:
+        c.k_exponent.copy_(torch.where(c.k_exponent == 255, c.k_exponent.int(), c.k_exponent.int() - 118))   # (bytes of 1 and 2)
+        assert int(c.k_exponent[c.k_exponent < 255].max()) < 4 and int(c.k_exponent.min()) > 0
+    k = stands[0] * small if bits == 8 else (stands[0].to(BF16) * small).double()
+    q = (_rn(len(LENGTHS), 2 * share, d) * 2.0 ** 118).to(BF16)
+    _check(lo, c, table, n, [k, stands[1]], q, d ** -0.5)
