@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
             // 2^(byte - 127) and byte - 127, NaN for 255 (infinity times zero).  The query's factor and the key's come together first: large
             // queries on small keys have scores of an ordinary size, the one or the other alone may not be there in fp32.
             const uint32_t kb = exps[16 * u + r + 8 * h], vb = exps[STEP + 16 * u + r + 8 * h];
-            const float k2 = __uint_as_float(kb << 23), kx = fmaf(k2, 0.f, k2);
+            const float k2 = __uint_as_float(max(kb << 23, 0x00400000u)), kx = fmaf(k2, 0.f, k2);
             const float vx = fmaf(__uint_as_float(vb << 23), 0.f, __uint_as_float(0x4B000000u | vb) - 8388735.f);
 #pragma unroll
             for (int n = 0; n < NQ; ++n)

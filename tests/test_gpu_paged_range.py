@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import lact_oracle as orc
-from test_gpu_paged_attention import BF16, _cache, _rn, _tolerance, lo  # noqa: F401  (a fixture)
+from test_gpu_paged_attention import BF16, E4M3, _cache, _rn, _tolerance, lo  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
 LENGTHS = [1, 40, 700, 5000]
@@ -33,3 +33,16 @@ def test_large_queries_on_small_keys(lo, bits, d, share):  # noqa: F811
     k = stands[0] * small if bits == 8 else (stands[0].to(BF16) * small).double()
     q = (_rn(len(LENGTHS), 2 * share, d) * 2.0 ** 118).to(BF16)
     _check(lo, c, table, n, [k, stands[1]], q, d ** -0.5)
+
+
+@pytest.mark.parametrize("share", [2, 12])
+@pytest.mark.parametrize("d", [64, 128])
+def test_the_smallest_power_of_two(lo, d, share):  # noqa: F811
+    """A byte of 0 stands for 2^-127 (the write has 1 at least; a cache may be filled by others)."""
+    c, table, n, stands = _cache(lo, LENGTHS, 32, 2, d, 8)
+    pages, heads, size, _ = c.k.shape
+    rows = (_rn(pages, heads, size, d, seed=5) * 16).clamp(-448, 448).to(E4M3)
+    c.k.view(torch.uint8).copy_(rows.view(torch.uint8))
+    c.k_exponent.zero_()
+    q = (_rn(len(LENGTHS), 2 * share, d) * 2.0 ** 118).to(BF16)
+    _check(lo, c, table, n, [rows.double() * 2.0 ** -127, stands[1]], q, 32 * d ** -0.5)
