@@ -65,9 +65,11 @@ __device__ __forceinline__ uint32_t transposed_8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// Tiles of a sequence (one at least: an empty sequence's zeros are a unit's result, too)
+// Tiles of a sequence (one at least: an empty sequence's zeros are a unit's result, too).  The first begins with the step that the window begins
+// in, or, where a step is several pages, with the page: pages in front of it may have been given back.
 struct PagedSpan {
   int first, last;   // positions [first, last)
+  int base;          // where the first tile begins
   int tiles;
   bool over;         // the length is past the table's end
 };
@@ -80,7 +82,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedStepArgs& a, int seq)
   s.over = len > room;
   s.first = a.window > 0 ? max(len - a.window, 0) : 0;
   s.first = min(s.first, s.last);
-  s.tiles = max((s.last - (s.first & ~(STEP - 1)) + TILE - 1) / TILE, 1);
+  s.base = s.first & -min(STEP, 1 << a.c.shift);
+  s.tiles = max((s.last - s.base + TILE - 1) / TILE, 1);
   return s;
 }
 
@@ -363,8 +366,7 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
   }
   auto enter = [&](PagedWalk& w) {                       // seq, unit, t and left are set
     const PagedSpan span = paged_span<STEP, TILE>(a, w.seq);
-    w.first = span.first; w.last = span.last; w.tiles = span.tiles; w.over = span.over;
-    w.base = span.first & ~(STEP - 1);
+    w.first = span.first; w.last = span.last; w.base = span.base; w.tiles = span.tiles; w.over = span.over;
     w.t1 = min(span.tiles, w.t + w.left);
     w.head = w.unit / a.blocks;
     w.table = a.c.table + w.seq * a.c.table_rs;
@@ -378,14 +380,13 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
     }
   };
   auto position = [&](const PagedWalk& w) { return w.base + (w.t * W + warp) * STEP; };
-  // A step lies in one page, or in `parts` of smaller ones; those that hold nothing of the window are neither looked up nor copied (the
-  // user may have given them back).
+  // A step lies in one page, or in `parts` of smaller ones; past the end none is looked up.
   const int parts = max(STEP >> a.c.shift, 1), part_rows = min(STEP, 1 << a.c.shift), part_bytes = (STAGE + EB) / parts;
   auto pages_of = [&](const PagedWalk& w, int (&pg)[SUB]) {
     const int p = position(w), at = p >> a.c.shift;
-    pg[0] = p < w.last && p + part_rows > w.first ? w.table[at] : -1;
+    pg[0] = p < w.last ? w.table[at] : -1;
 #pragma unroll
-    for (int i = 1; i < SUB; ++i) pg[i] = i < parts && p + i * part_rows < w.last && p + (i + 1) * part_rows > w.first ? w.table[at + i] : -1;
+    for (int i = 1; i < SUB; ++i) pg[i] = i < parts && p + i * part_rows < w.last ? w.table[at + i] : -1;
   };
   enter(make);
   const int stages = make.left > kPagedLong ? a.long_stages : a.stages;
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(W * 32, kPagedPerSm(NQ)) paged_step_kernel(con
       }
     };
     auto there = [&](int pg, int at) {
-      const bool real = p + at < make.last && p + at + part_rows > make.first;
+      const bool real = p + at < make.last;
       if (real && static_cast<uint32_t>(pg) >= static_cast<uint32_t>(a.c.pages)) {
         if (lane == 0) report_bad_page();
         return false;
