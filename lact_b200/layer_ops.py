@@ -307,9 +307,10 @@ def paged_attention_step(q: torch.Tensor, cache: PagedCache, page_table: torch.T
     of positions `max(0, lengths[i] - window_size)` to `lengths[i] - 1` (`window_size` None: all; the new token's own are written before,
     and lengths count them).  The heads of the cache divide those of q (consecutive heads share).  softmax_scale: head_dim ** -0.5 by
     default.  Returns o [sequences, heads, head_dim] bf16; a sequence without tokens has zeros.  Scores, maxima and sums are float32; weights
-    are rounded to two bf16 pieces (bf16 cache) or to fp16 (8 bits) for their product with the values.  Pages that hold
-    nothing of the window may have been given back (their entries are not looked at), and whatever other rows outside of it hold counts for
-    nothing; a NaN within it makes its heads' outputs NaN.  No backward: a call with gradients raises."""
+    are rounded to two bf16 pieces (bf16 cache) or to fp16 (8 bits) for their product with the values.  Pages that hold nothing of the
+    window may have been given back (their entries are not looked at), and whatever other rows outside of it hold counts for nothing.  Within
+    it a NaN among the keys makes its heads' outputs NaN, one among the values their outputs of that feature; an infinite value makes these
+    infinite or NaN (both pieces of its weight meet it, and the second may be 0 or negative).  No backward: a call with gradients raises."""
     return L.call(_op("paged_attention_step"), q, *cache, page_table, lengths, int(window_size) if window_size else 0,
                   float(softmax_scale) if softmax_scale is not None else cache[0].shape[-1] ** -0.5)
 

@@ -46,3 +46,24 @@ def test_the_smallest_power_of_two(lo, d, share):  # noqa: F811
     c.k_exponent.zero_()
     q = (_rn(len(LENGTHS), 2 * share, d) * 2.0 ** 118).to(BF16)
     _check(lo, c, table, n, [rows.double() * 2.0 ** -127, stands[1]], q, 32 * d ** -0.5)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("length", [40, 700, 30000])           # one CTA or a cluster; cut units
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_a_value_that_is_not_finite_spoils_its_feature_alone(lo, d, length, value):  # noqa: F811
+    """The outputs of that feature, of the heads that share the row; all others keep their bits.  A weight w meets an infinity in two pieces, hi =
+    bf16(w) > 0 and lo = bf16(w - hi): hi inf + lo inf is infinite for lo > 0 and NaN for lo <= 0, so that either is right."""
+    lengths = [length, length + 3, 17]
+    c, table, n, _ = _cache(lo, lengths, 64, 3, d, 16)
+    q = _rn(3, 6, d).to(BF16)
+    want = lo.paged_attention_step(q, c, table, n)
+    for p in (0, length // 2, length - 1):
+        held = c.v.clone()
+        c.v[int(table[0, p // 64]), 1, p % 64, 5] = value
+        got = lo.paged_attention_step(q, c, table, n)
+        bad = torch.zeros_like(got, dtype=torch.bool)
+        bad[0, 2:4, 5] = True
+        wrong = got[bad].isnan() if value != value else got[bad].isnan() | (got[bad] == value)
+        assert bool(wrong.all()) and torch.equal(got[~bad], want[~bad])
+        c.v.copy_(held)
