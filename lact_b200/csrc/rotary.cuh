@@ -5,7 +5,7 @@
 // Bound by memory: every element is read and written once.  A block takes several tokens, works out their cosines and sines once into
 // shared memory, and each thread keeps those of its V pairs in registers for its share of the token's heads (queries
 // first, then keys).  Angles are whole numbers of 2^-64 turns, in which products with a position drop full turns by themselves: what a
-// position of 2^31 is off by is 2^-25 of a turn, from the frequency in fp64.
+// position of 2^31 is off by is 2^-24 of a turn at a frequency of 1 (2^-56 each from the frequency's product in fp64 and its constant).
 #pragma once
 #include "group_norm.cuh"
 

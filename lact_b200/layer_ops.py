@@ -247,8 +247,10 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     positions (int32 or int64) [l, axes], or [b, l, axes].  The first 2 P features of a head are P = sum(sections) pairs, (j, j + P) or, with
     `interleaved`, (2j, 2j + 1); pairs go to the axes in sections (at most 8), and pair j turns by `positions[axis] * frequencies[j]`
     (float64 [P], `rotary_frequencies`): (x, y) -> (x cos - y sin, y cos + x sin).  Features from 2 P on are copied.  Returns the turned q
-    and k, contiguous.  Differentiable with respect to q and k, any number of times.  Angles are taken in float64 and reduced before
-    they become float32, so that far positions are as exact as near ones; the results are rounded once."""
+    and k, contiguous.  Differentiable with respect to q and k, any number of times.  Angles are whole numbers of 2^-64 turns, from the
+    float64 frequencies, in which full turns drop out by themselves (what float64 leaves of a position of 2^31 is 2^-24 of a turn at a frequency of
+    1); of a turn they keep 32 bits and then float32 (2^-26 of a turn) for their cosines and sines, which bf16 results take from the
+    hardware's approximations (2^-20.9).  The results are rounded once."""
     r = L.call(_op("rotary_axes"), q, k, positions, frequencies, sections, interleaved)
     return r[0], r[1] if k is not None else None
 
@@ -297,7 +299,8 @@ def paged_cache_read(cache: PagedCache, page_table: torch.Tensor, lengths: torch
     sequences and then their values (what `sliding_window_attention_inference` takes as `kv_cache`).  Row j is position
     `lengths[i] - num_tokens + j`, zeros where that is negative.  `cu_seqlens` (int32 [sequences + 1]): [2, num_tokens, kv_heads, head_dim], of
     sequence i the last cu_seqlens[i + 1] - cu_seqlens[i] tokens; rows outside of them are zeros.  8 bits become the bf16 values that
-    they stand for, exactly.  No backward."""
+    they stand for: exactly, as `paged_cache_write` leaves them (bytes of 0 to 2 and above 246 can stand for values that bf16 does not have; those of a
+    cache that others filled are rounded).  No backward."""
     return L.call(_op("paged_cache_read"), *cache, page_table, lengths, num_tokens, cu_seqlens)
 
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import lact_oracle as orc
-from test_gpu_paged_attention import BF16, E4M3, _cache, _rn, _tolerance, lo  # noqa: F401  (a fixture)
+from test_gpu_paged_attention import BF16, E4M3, I32, _cache, _rn, _tolerance, lo  # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
 LENGTHS = [1, 40, 700, 5000]
@@ -67,3 +67,23 @@ def test_a_value_that_is_not_finite_spoils_its_feature_alone(lo, d, length, valu
         wrong = got[bad].isnan() if value != value else got[bad].isnan() | (got[bad] == value)
         assert bool(wrong.all()) and torch.equal(got[~bad], want[~bad])
         c.v.copy_(held)
+
+
+def test_every_value_of_8_bits_read_back(lo):  # noqa: F811
+    """All codes under all bytes, as bf16 rounds what they stand for: exact from byte 3 to 246 (2^-9 2^-124 is bf16's smallest number, 448 2^119 below its largest)."""
+    c = lo.paged_cache(16, 256, 1, 64, E4M3, "cuda")
+    code = torch.arange(256, device="cuda", dtype=torch.uint8)
+    c.k.view(torch.uint8).copy_(code.reshape(4, 1, 1, 64).repeat(4, 1, 256, 1))       # page p: codes 64 (p % 4) on; row r: byte r
+    c.v.view(torch.uint8).copy_(code.flip(0).reshape(4, 1, 1, 64).repeat(4, 1, 256, 1))
+    for e in c[2:]:
+        e.copy_(code.expand(16, 1, 256))
+    table, n = torch.arange(16, device="cuda", dtype=I32)[None], torch.tensor([4096], dtype=I32, device="cuda")
+    got = lo.paged_cache_read(c, table, n, 4096).reshape(2, 16, 256, 64)
+    power = torch.exp2(code.double() - 127)
+    power[255] = float("nan")
+    for x, y in zip(got, (c.k, c.v)):
+        stands = y.double()[:, 0] * power[:, None]
+        want = stands.to(BF16)
+        assert torch.equal(x.isnan(), want.isnan()) and torch.equal(x.nan_to_num(0.0, 1e38, -1e38), want.nan_to_num(0.0, 1e38, -1e38))
+        fine = stands[:, 3:247].nan_to_num()
+        assert torch.equal(x[:, 3:247].double().nan_to_num(), fine)
