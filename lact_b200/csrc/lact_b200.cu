@@ -2453,7 +2453,8 @@ int paged_rows(const lact_paged_cache* c, PagedRows& a, int64_t entries, int64_t
   return e4 ? launch_paged_rows<128, true>(a, write, grid, st) : launch_paged_rows<128, false>(a, write, grid, st);
 }
 
-// How a call's tiles are dealt out.
+// How a call's tiles are dealt out.  Lengths are on the device, so that the rules go by the page table's width: they are the right ones where it
+// is near the longest sequence's pages (one sequence of 777 tokens, 12 heads: 6.4 us under a table of its 13 pages, 11.6 under one of 2048).
 struct PagedStepPlan {
   int nq, blocks, runs, cluster, stages, long_stages;
   size_t bytes, smem;

@@ -313,7 +313,10 @@ def paged_attention_step(q: torch.Tensor, cache: PagedCache, page_table: torch.T
     are rounded to two bf16 pieces (bf16 cache) or to fp16 (8 bits) for their product with the values.  Pages that hold nothing of the
     window may have been given back (their entries are not looked at), and whatever other rows outside of it hold counts for nothing.  Within
     it a NaN among the keys makes its heads' outputs NaN, one among the values their outputs of that feature; an infinite value makes these
-    infinite or NaN (both pieces of its weight meet it, and the second may be 0 or negative).  No backward: a call with gradients raises."""
+    infinite or NaN (both pieces of its weight meet it, and the second may be 0 or negative).  How the work is split is chosen on the host, by the
+    page table's width (lengths are on the device): short texts under a wide table take longer (one of 777 tokens, 12 heads of 128: 6.4 us with the
+    13 columns that it needs, 11.6 with 2048), so that a caller who knows a bound of the lengths passes `page_table[:, :columns]`.  No backward: a
+    call with gradients raises."""
     return L.call(_op("paged_attention_step"), q, *cache, page_table, lengths, int(window_size) if window_size else 0,
                   float(softmax_scale) if softmax_scale is not None else cache[0].shape[-1] ** -0.5)
 
