@@ -9,14 +9,17 @@
 // permutes pair.
 // The maximum m is raised only when a score passes it by 8 (weights up to 2^8 lose nothing), so that a step needs one vote in place of a
 // reduction.  Weights are rounded for the product with V: in two bf16 pieces (2^-16 of each) with bf16 caches, to fp16 (2^-11) with 8
-// bits.  There, V is taken as e4m3, exact in fp16, and its powers of two multiply the weights: u_p = 2^(x_p + e_p - M) with a maximum M
-// of its own, against which small weights are rounded by 2^-25.  Queries become fp16 after scaling each by a power of two, to a largest
-// value of 2^14 (what is below 2^-38 of it is cut).  Sums are in fp32.
+// bits.  (A second piece there could bring results from 1.68e-3 off 64 bits to the 1.66e-3 of their own rounding, and takes 198 us in place of
+// 192 with 64 sequences of up to 16384 tokens, 58 in place of 52 with 40 heads on one.)  V is then taken as e4m3, exact in fp16, and its
+// powers of two multiply the weights: u_p = 2^(x_p + e_p - M) with a maximum M of its own, against which a warp's small weights are rounded
+// by 2^-25.  Queries become fp16 after scaling each by a power of two, to a largest value of 2^14 (what is below 2^-38 of it is cut).
+// Sums are in fp32.
 //
 // Loads: every warp keeps a ring of steps of its own in shared memory (16 tokens of rows of 256 bytes, 32 of 128, 64 of 64), filled by tiled copies
 // with a swizzle that both kinds of fragment read without conflicts; a step's page number is looked up one step ahead.  A step is in
 // registers before its slot is filled again.  96 KB on their way in a SM is what bandwidth gains from (12 warps with one step of 8 KB; two
-// steps: step_window 170 in place of 162 us, step_long 103 and 100): longer runs use no more slots than that.
+// steps: step_window 170 in place of 162 us, step_long 103 and 100): longer runs use no more slots than that (with more than 8 query heads a kv
+// head, of which 8 warps are on a SM, that is 64 KB: 16 heads 84 % in bf16).
 //
 // Work: a unit is a (sequence, kv head, block of query heads), its tokens tiles of one step a warp; lengths are known on the device alone.
 // All units' tiles, in order, are dealt out in even runs, one for each CTA, whatever the lengths are (more runs than fit at once: two for
@@ -24,8 +27,10 @@
 // cut among runs each leaves a piece (sums, maxima), and a small launch adds the pieces in a fixed order.  Where units are few and have few
 // tiles at most, or have very few (`runs` 0), a unit is a cluster of CTAs that share its tiles evenly and read one another's sums from
 // shared memory.
-// Measured (of the measured copy rate): 4 sequences of up to 131072 tokens, 16 heads on 4 of 128, bf16 95 us (94 %); 64 of up to 16384,
-// 32 on 8 of 128, 8 bits 184 us (96 %); 192 of up to 5000, a window of 2048, 12 heads of 64 159 us (97 %); one of 777, 12 heads 6.8 us.
+// Measured (of the measured copy rate; from one GPU to another): 4 sequences of up to 131072 tokens, 16 heads on 4 of 128, bf16 94 to 96 us (94 %); 64 of
+// up to 16384, 32 on 8 of 128, 8 bits 185 to 193 us (92 to 95 %); 192 of up to 5000, a window of 2048, 12 heads of 64 156 to 160 us (96 to 98 %); one
+// of 777, 12 heads 6.4 to 7.2 us.  Less near it: 82 of up to 4000, 12 heads of 64 in 8 bits 59 us (70 %); 64 of up to 8192, 64 heads on 4 of 128
+// 105 us (84 %), in 8 bits 70 (64 %); 80 on 4 181 (the cache is read twice: 49 %); 40 on 1 in 8 bits 52 (read three times: 22 %).
 #pragma once
 #include "paged_cache.cuh"
 
@@ -204,8 +209,7 @@ struct PagedCut {
 };
 // The pieces of the units that were cut, added up: blockIdx.x is the run that one begins in, blockIdx.y 64 times four of its sums; groups
 // of 64 threads share the pieces, eight of a group on their way at a time.  A launch of its own, so that nothing is left behind in the
-// kernel that has to wait for pieces (which would cost its loop registers: there, by who comes last, step_long took 101 in place of 97 us,
-// and one unit of 131072 tokens 78 in place of 30).
+// kernel that has to wait for pieces (which would cost its loop registers: there, by who comes last, step_long took 101 in place of 97 us).
 constexpr int kPagedJoinMost = 1024;   // pieces of a unit at most: the runs of a call
 template <int D>
 __global__ void __launch_bounds__(512) paged_join_kernel(const float* pieces, const PagedCut* cuts, bf16* out, int32_t sum_rows) {
