@@ -140,8 +140,9 @@ int64_t lact_stream_sync_count(void);
  * the call) holds 101 once the kernel has run.  No counterpart in the reference. */
 int lact_set_wait_limit_ns(uint64_t limit_ns);
 /* A word of pinned host memory (one per device, made at the first call) in which every kernel that records a non-zero
- * device status also leaves it: a host that reads it now and then learns of a failure without copies or waits.  The
- * host clears it.  May be called while a stream is being captured.  No counterpart in the reference. */
+ * device status also leaves it: a host that reads it now and then learns of a failure without copies or waits.  A
+ * missing page of a paged cache (102) goes to its second byte, everything else to the first: neither hides the other, and
+ * lact_error_string of the whole word names the first.  The host clears it.  May be called while a stream is being captured.  No counterpart in the reference. */
 int lact_status_host_word(int32_t **word_out);
 int lact_debug_wait_timeout(int32_t *status_word, void *stream);
 
@@ -413,7 +414,8 @@ int lact_rotary_axes(const lact_rotary_config *cfg, const void *q, const void *k
  * bytes, 16-byte aligned, page strides multiples of 16) e4m3 values that stand for themselves times 2^(byte - 127), 255: NaN.  head_dim 64 or 128; page_size 16, 32, 64, 128 or 256.
  * Position p of sequence i lies in page page_table[i * table_stride + p / page_size], row p % page_size, for p below lengths[i];
  * table_cols * page_size at most 2^30.  Entries of the table whose page holds no position that a call needs (past a sequence's
- * length; in front of its window) are not looked at; a needed page or a position that the cache does not have is left out, and device status 102 goes to the host's word (lact_status_host_word), if that holds nothing unread.  No counterpart in the
+ * length; in front of its window) are not looked at; a needed page or a position that the cache does not have is left
+ * out, and device status 102 goes to the second byte of the host's word (lact_status_host_word).  No counterpart in the
  * reference, whose cache is left to the attention library's caller (layer_lact_swiglu.py:328-343). */
 typedef struct lact_paged_cache {
   void *k, *v;

@@ -2558,6 +2558,7 @@ extern "C" {
 int lact_version(void) { return 1004; }
 
 const char* lact_error_string(int code) {
+  if (code > 255) code = (code & 255) != 0 ? code & 255 : code >> 8 & 255;   // the host's word as it is
   switch (code) {
     case LACT_OK: return "ok";
     case LACT_ERR_NULL: return "a required pointer is NULL";

@@ -41,6 +41,9 @@ std::mutex g_mu;
 // 256 bytes per (device, stream) in use; never destroyed (the CUDA context may be gone before static destructors run)
 std::unordered_map<uint64_t, Word>& g_words = *new std::unordered_map<uint64_t, Word>();
 
+// The code in a host's word: a wait that ran out (first byte) before a missing page (second).
+int32_t code_of(int32_t word) { return (word & 255) != 0 ? word & 255 : word >> 8 & 255; }
+
 volatile int32_t* host_word(int dev) {
   int32_t* w = g_host[dev].load(std::memory_order_acquire);
   if (w == nullptr) {
@@ -58,7 +61,7 @@ void poll_status(const Tensor& like) {
   const int dev = like.device().index();
   TORCH_CHECK(dev >= 0 && dev < kMaxDevices, "unsupported device index");
   volatile int32_t* w = host_word(dev);
-  const int32_t st = *w;
+  const int32_t st = code_of(*w);
   if (st == 0) return;
   *w = 0;
   g_epoch.fetch_add(1);
@@ -106,7 +109,7 @@ extern "C" int lact_torch_take_status(int device) {
   if (device < 0 || device >= lact_torch::kMaxDevices) return 0;
   int32_t* w = lact_torch::g_host[device].load(std::memory_order_acquire);
   if (w == nullptr) return 0;
-  const int32_t st = *reinterpret_cast<volatile int32_t*>(w);
+  const int32_t st = lact_torch::code_of(*reinterpret_cast<volatile int32_t*>(w));
   if (st != 0) {
     *reinterpret_cast<volatile int32_t*>(w) = 0;
     lact_torch::g_epoch.fetch_add(1);

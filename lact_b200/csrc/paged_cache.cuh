@@ -28,11 +28,12 @@ struct PagedCache {
   int32_t sequences;
 };
 
-// A page number or a length that the cache does not have is left out, and told to the host (which raises on its next call), unless something
-// is there already that the host has not read: a wait that ran out spoils more than the rows that are left out here.
+// A page number or a length that the cache does not have is left out, and told to the host (which raises on its next call): in the second
+// byte of its word, so that a wait that ran out (the first byte), which spoils more than the rows left out here, stays to be read.  (A
+// compare-and-swap of the whole word would do it too, at 7 us each, one after the other: 2.4 s for 80000 rows without a page in place of 80 us.)
 __device__ __forceinline__ void report_bad_page() {
   if (g_host_status != nullptr) {
-    atomicCAS(g_host_status, static_cast<int32_t>(kStatusOk), static_cast<int32_t>(kStatusBadPage));
+    reinterpret_cast<volatile uint8_t*>(g_host_status)[1] = kStatusBadPage;
     __threadfence_system();
   }
 }

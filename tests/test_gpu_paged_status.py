@@ -35,8 +35,30 @@ def test_a_missing_page_does_not_replace_a_wait_that_ran_out(lo, call):  # noqa:
         word[0] = before
         graph.replay()
         torch.cuda.synchronize()
-        assert word[0] == after
+        assert word[0] == (before | 102 << 8)             # (a byte for each)
+        text = lo.L.lib().lact_error_string(word[0])
+        assert text == lo.L.lib().lact_error_string(after) and b"unknown" not in text
         with pytest.raises(lo.L.LactError, match=str(after)):
             lo.L.synchronize_and_check()
         assert word[0] == 0
     lo.L.synchronize_and_check()
+
+
+def test_many_missing_pages_are_told_quickly(lo):  # noqa: F811
+    """80000 rows without a page (80 us where a store tells it, 2.4 s where every one is an atomic operation on the host's memory)."""
+    c = lo.paged_cache(2, 64, 8, 128, device="cuda")
+    table, n = torch.full((8, 157), -1, dtype=I32, device="cuda"), torch.full((8,), 10000, dtype=I32, device="cuda")
+    lo.paged_cache_read(c, table, n, 10)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(lo.L.LactError, match="102"):
+        lo.L.synchronize_and_check()
+    with torch.cuda.graph(graph):
+        lo.paged_cache_read(c, table, n, 10000)
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    a.record()
+    graph.replay()
+    b.record()
+    torch.cuda.synchronize()
+    with pytest.raises(lo.L.LactError, match="102"):
+        lo.L.synchronize_and_check()
+    assert a.elapsed_time(b) < 100
